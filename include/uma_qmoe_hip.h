@@ -282,6 +282,57 @@ int uqm_rmsnorm(const void* input, int64_t rows, int64_t hidden_size, const void
 int uqm_dequantize(int32_t encoding, const void* data, const float* scales, int64_t elements,
                    int64_t group_size, void* output, void* stream);
 
+/* ---- 8-bit floats with scales ----
+ * Matrices of e4m3 codes (OCP, largest value 448) with FP32 scales, value =
+ * code * scale. A scale covers a block of 1 x 128 (row, columns: activations)
+ * or 128 x 128 (weights); the last block of a row, or of the rows, may be
+ * smaller. Codes [rows, cols] and scales [ceil(rows / block_rows),
+ * ceil(cols / 128)] are row-major and contiguous.
+ *   d = max|v| / 448, at least 2^-126; 1 for a block of zeros
+ *   code = e4m3(v / d), to nearest even
+ * A block that holds a NaN or an infinity gets a scale that is one too, and
+ * codes that are NaN or 0; a product with it is NaN. None of these entry points
+ * needs a workspace, and every result is the same for the same inputs. rows = 0
+ * does nothing. No counterpart in the reference, whose dense layers are BF16. */
+
+/* Residual addition and RMSNorm:
+ *   s = bf16(input + residual) -> sum      (residual and sum NULL: s = input)
+ *   n = s * rsqrt(mean(s^2) + eps)
+ *   output = bf16(weight * bf16(n))        (as uqm_rmsnorm; NULL: not wanted)
+ *   codes, scales = weight * n in blocks of 1 x 128, not rounded to BF16
+ *                                          in between (both NULL: not wanted)
+ * bf16 [rows, hidden_size], any hidden_size; weight bf16 [hidden_size] or NULL
+ * for ones. sum may be input or residual itself; outputs must not overlap
+ * otherwise. Rows of a multiple of 8 elements on 16-byte aligned tensors (codes:
+ * 8-byte) are the fast case. */
+int uqm_add_rmsnorm(const void* input, const void* residual, int64_t rows, int64_t hidden_size, const void* weight,
+                    float eps, void* sum, void* output, void* codes, float* scales, void* stream);
+
+/* y = silu(g) * u of gate_up bf16 [rows, 2 * features], g the first and u the
+ * second half of a row, silu(g) = g / (1 + exp(-g)), in FP32:
+ * output = bf16(y), codes and scales = y in blocks of 1 x 128; either kind may
+ * be NULL. */
+int uqm_silu_mul(const void* gate_up, int64_t rows, int64_t features, void* output, void* codes, float* scales,
+                 void* stream);
+
+/* Codes and scales of bf16 [rows, cols] in blocks of block_rows x 128,
+ * block_rows 1 or 128. */
+int uqm_fp8_quantize(const void* input, int64_t rows, int64_t cols, int64_t block_rows, void* codes, float* scales,
+                     void* stream);
+
+/* output bf16 [rows, out_features]:
+ *   output[t, n] = bf16(bias[n] + sum over blocks b of 128 columns of
+ *       scales[t, b] * weight_scales[n / 128, b] * sum over k in b of codes[t, k] * weight_codes[n, k])
+ * in FP32, but for the matrix cores' own sums of eight neighbouring products,
+ * each cut towards zero at 2^-13 of the largest one's power of two. codes [rows, in_features] in blocks of 1 x 128, weight_codes
+ * [out_features, in_features] in blocks of 128 x 128, both 16-byte aligned;
+ * in_features a multiple of 16; bias bf16 [out_features] or NULL. The product of
+ * two scales must stay within FP32's range. Calls of few and of many rows sum in
+ * different orders, so a row's result may differ in its last bit between them. */
+int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const void* weight_codes,
+                   const float* weight_scales, int64_t out_features, int64_t in_features, const void* bias,
+                   void* output, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

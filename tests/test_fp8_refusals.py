@@ -1,0 +1,167 @@
+"""What the 8-bit operators refuse, without a GPU: the library's entry points
+check their arguments before they look at the device, the wrappers before they
+call the library."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from uma_qmoe_amd import _native
+from uma_qmoe_amd.native_backend import Fp8Matrix, HipExtension
+
+A, B, C, D, E = (1 << 20, 2 << 20, 3 << 20, 4 << 20, 5 << 20)  # addresses that nothing reads
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _native.library()
+
+
+def refused(lib, name, args, words):
+    rc = getattr(lib, name)(*args, None)
+    message = lib.uqm_last_error().decode()
+    assert rc == 1, (rc, message)  # UQM_ERR_ARGUMENT
+    assert words in message, message
+
+
+@pytest.mark.parametrize("args,words", [
+    ((A, None, -1, 128, None, 1e-6, None, B, None, None), "rows"),
+    ((A, None, 1 << 31, 128, None, 1e-6, None, B, None, None), "rows"),
+    ((A, None, 4, 0, None, 1e-6, None, B, None, None), "columns"),
+    ((A, None, 4, 128, None, -1e-6, None, B, None, None), "eps"),
+    ((A, None, 4, 128, None, float("nan"), None, B, None, None), "eps"),
+    ((A, C, 4, 128, None, 1e-6, None, B, None, None), "residual and sum"),
+    ((A, None, 4, 128, None, 1e-6, C, B, None, None), "residual and sum"),
+    ((A, None, 4, 128, None, 1e-6, None, None, None, None), "no output"),
+    ((A, None, 4, 128, None, 1e-6, None, B, D, None), "together"),
+    ((A, None, 4, 128, None, 1e-6, None, B, None, D), "together"),
+    ((None, None, 4, 128, None, 1e-6, None, B, None, None), "required"),
+    ((A + 1, None, 4, 128, None, 1e-6, None, B, None, None), "aligned"),
+    ((A, None, 4, 128, None, 1e-6, None, B, D, E + 2), "aligned"),
+    ((A, None, 4, 128, None, 1e-6, None, A, None, None), "overlaps an input"),
+    ((A, B, 4, 128, None, 1e-6, A + 2, C, None, None), "overlaps an input"),
+    ((A, B, 4, 128, C, 1e-6, B, C + 254, None, None), "overlaps an input"),
+    ((A, B, 4, 128, None, 1e-6, C, C + 1022, None, None), "outputs overlap"),
+    ((A, None, 4, 128, None, 1e-6, None, B, B + 1020, D), "outputs overlap"),
+])
+def test_add_rmsnorm(lib, args, words):
+    refused(lib, "uqm_add_rmsnorm", args, words)
+
+
+@pytest.mark.parametrize("args,words", [
+    ((A, -1, 128, B, None, None), "rows"),
+    ((A, 4, 0, B, None, None), "columns"),
+    ((A, 4, 128, None, None, None), "no output"),
+    ((A, 4, 128, None, B, None), "together"),
+    ((None, 4, 128, B, None, None), "required"),
+    ((A, 4, 128, A + 2046, None, None), "overlaps an input"),
+])
+def test_silu_mul(lib, args, words):
+    refused(lib, "uqm_silu_mul", args, words)
+
+
+@pytest.mark.parametrize("args,words", [
+    ((A, 4, 128, 2, B, C), "blocks"),
+    ((A, 4, 128, 0, B, C), "blocks"),
+    ((A, -4, 128, 1, B, C), "rows"),
+    ((A, 4, 128, 1, None, None), "no output"),
+    ((A, 4, 128, 1, B, None), "together"),
+    ((None, 4, 128, 1, B, C), "required"),
+    ((A, 4, 128, 1, A + 100, C), "overlaps an input"),
+])
+def test_fp8_quantize(lib, args, words):
+    refused(lib, "uqm_fp8_quantize", args, words)
+
+
+@pytest.mark.parametrize("args,words", [
+    ((A, B, -1, C, D, 64, 128, None, E), "rows"),
+    ((A, B, 4, C, D, 0, 128, None, E), "features"),
+    ((A, B, 4, C, D, 64, 0, None, E), "multiple of 16"),
+    ((A, B, 4, C, D, 64, 120, None, E), "multiple of 16"),
+    ((A, B, 4, None, D, 64, 128, None, E), "required"),
+    ((A, B, 4, C, None, 64, 128, None, E), "required"),
+    ((None, B, 4, C, D, 64, 128, None, E), "required"),
+    ((A, None, 4, C, D, 64, 128, None, E), "required"),
+    ((A, B, 4, C, D, 64, 128, None, None), "required"),
+    ((A + 8, B, 4, C, D, 64, 128, None, E), "aligned"),
+    ((A, B, 4, C + 8, D, 64, 128, None, E), "aligned"),
+    ((A, B + 2, 4, C, D, 64, 128, None, E), "aligned"),
+    ((A, B, 4, C, D, 64, 128, A + 4097, E), "aligned"),
+    ((A, B, 4, C, D, 64, 128, None, E + 1), "aligned"),
+    ((A, B, 4, C, D, 64, 128, None, A + 510), "overlaps"),
+    ((A, B, 4, C, D, 64, 128, E + 2, E), "overlaps"),
+])
+def test_fp8_linear(lib, args, words):
+    refused(lib, "uqm_fp8_linear", args, words)
+
+
+def test_no_rows_is_no_work(lib):
+    assert lib.uqm_add_rmsnorm(None, None, 0, 128, None, 1e-6, None, None, None, None, None) == 0
+    assert lib.uqm_silu_mul(None, 0, 128, None, None, None, None) == 0
+    assert lib.uqm_fp8_quantize(None, 0, 128, 1, None, None, None) == 0
+    assert lib.uqm_fp8_linear(None, None, 0, A, B, 64, 128, None, None, None) == 0
+
+
+# ------------------------------------------------------------- wrappers --
+@pytest.fixture(scope="module")
+def ext():
+    return HipExtension()
+
+
+def bf(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+def fp8(rows, cols, block_rows=1, scales=None):
+    groups = -(-cols // 128)
+    codes = torch.zeros(rows, cols, dtype=torch.float8_e4m3fn)
+    return Fp8Matrix(codes, torch.ones(-(-rows // block_rows), groups) if scales is None else scales, block_rows)
+
+
+@pytest.mark.parametrize("call,words", [
+    (lambda e: e.add_rmsnorm(bf(2, 8).float()), "BF16"),
+    (lambda e: e.add_rmsnorm(bf(2, 0)), "column"),
+    (lambda e: e.add_rmsnorm(bf(2, 8)), "device tensors"),
+    (lambda e: e.add_rmsnorm(bf(2, 8), bf16=False), "at least one"),
+    (lambda e: e.add_rmsnorm(bf(2, 8), bf(3, 8)), "hidden's shape"),
+    (lambda e: e.add_rmsnorm(bf(2, 8), bf(2, 8).float()), "hidden's shape"),
+    (lambda e: e.add_rmsnorm(bf(2, 8), inplace=True), "requires a residual"),
+    (lambda e: e.add_rmsnorm(bf(2, 8), bf(8, 2).t(), inplace=True), "contiguous"),
+    (lambda e: e.add_rmsnorm(bf(2, 8), weight=bf(7)), "weight"),
+    (lambda e: e.add_rmsnorm(bf(2, 8), weight=bf(8).float()), "weight"),
+    (lambda e: e.silu_mul(bf(2, 7)), "even"),
+    (lambda e: e.silu_mul(bf(2, 8).half()), "BF16"),
+    (lambda e: e.silu_mul(bf(2, 8), bf16=False), "at least one"),
+    (lambda e: e.silu_mul(bf(2, 8)), "device tensors"),
+    (lambda e: e.fp8_quantize(bf(2, 8), block_rows=64), "blocks of 1 or 128"),
+    (lambda e: e.fp8_quantize(bf(2, 2, 8), block_rows=128), "matrix"),
+    (lambda e: e.fp8_quantize(bf(2, 8).float()), "BF16"),
+    (lambda e: e.fp8_linear(fp8(2, 32), fp8(8, 32, 128)), "device tensors"),
+    (lambda e: e.fp8_linear(fp8(2, 48), fp8(8, 32, 128)), "input features"),
+    (lambda e: e.fp8_linear(bf(2, 48), fp8(8, 32, 128)), "input features"),
+    (lambda e: e.fp8_linear(fp8(2, 24), fp8(8, 24, 128)), "multiple of 16"),
+    (lambda e: e.fp8_linear(fp8(2, 32), fp8(0, 32, 128)), "at least one row"),
+    (lambda e: e.fp8_linear(fp8(2, 32), fp8(8, 32, 1)), "blocks of 128"),
+    (lambda e: e.fp8_linear(fp8(128, 32, 128), fp8(8, 32, 128)), "blocks of 1 "),
+    (lambda e: e.fp8_linear(fp8(2, 32), fp8(200, 32, 128, torch.ones(1, 1))), "scales"),
+    (lambda e: e.fp8_linear(fp8(2, 32, 1, torch.ones(2, 2)), fp8(8, 32, 128)), "scales"),
+    (lambda e: e.fp8_linear(fp8(2, 32, 1, torch.ones(2, 1).double()), fp8(8, 32, 128)), "float32 scales"),
+    (lambda e: e.fp8_linear(Fp8Matrix(torch.zeros(2, 32, dtype=torch.uint8), torch.ones(2, 1)), fp8(8, 32, 128)),
+     "float8_e4m3fn"),
+    (lambda e: e.fp8_linear(fp8(2, 32), fp8(8, 32, 128), bf(7)), "bias"),
+    (lambda e: e.fp8_linear(fp8(2, 32), fp8(8, 32, 128), bf(8).float()), "bias"),
+])
+def test_wrappers(ext, call, words):
+    with pytest.raises(RuntimeError, match=words):
+        call(ext)
+
+
+def test_dequantize_of_a_matrix():
+    m = Fp8Matrix(torch.ones(130, 130).to(torch.float8_e4m3fn), torch.tensor([[1.0, 2.0], [3.0, 4.0]]), 128)
+    v = m.dequantize()
+    assert v.shape == (130, 130) and v[0, 0] == 1 and v[127, 128] == 2 and v[128, 0] == 3 and v[129, 129] == 4
+    a = Fp8Matrix(torch.ones(2, 3, 130).to(torch.float8_e4m3fn), torch.arange(12.0).view(2, 3, 2))
+    assert a.dequantize()[1, 2, 127] == 10 and a.dequantize()[1, 2, 129] == 11

@@ -6,12 +6,14 @@
 #include <string.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <unordered_map>
 
 #include "../../include/uma_qmoe_hip.h"
 #include "uqm_dense.h"
+#include "uqm_fp8.h"
 #include "uqm_internal.h"
 #include "uqm_prefill.h"
 #include "uqm_route.h"
@@ -1299,6 +1301,147 @@ int uqm_dequantize(int32_t encoding, const void* data, const float* scales, int6
   return hip_check(launch_dequantize(encoding == UQM_Q4, data, scales, elements, group_size, output,
                                      static_cast<hipStream_t>(stream)),
                    "dequantize launch");
+}
+
+}  // extern "C"
+
+namespace {
+
+constexpr int64_t kMaxExtent = 0x7FFFFFFF;  // rows and columns of the 8-bit operators
+
+bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
+  if (p == nullptr || q == nullptr) return false;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + static_cast<uintptr_t>(m) && b < a + static_cast<uintptr_t>(n);
+}
+
+bool misaligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+// The checks that the row operators share: extents, the wanted outputs
+// (`codes` and `scales` together, at least one kind), element alignment, and
+// that no output overlaps an input or another output.
+struct Span {
+  const void* p;
+  int64_t bytes;
+};
+int check_rows(const char* what, int64_t rows, int64_t cols, std::initializer_list<Span> inputs, const void* output,
+               const void* codes, const float* scales, Span also) {
+  if (rows < 0 || rows > kMaxExtent || cols <= 0 || cols > kMaxExtent)
+    return fail(UQM_ERR_ARGUMENT, "%s: rows must be in [0, 2^31) and columns in [1, 2^31)", what);
+  if (rows == 0) return UQM_OK;  // (pointers of empty tensors may be NULL)
+  if ((codes == nullptr) != (scales == nullptr))
+    return fail(UQM_ERR_ARGUMENT, "%s: codes and scales must be given together", what);
+  if (output == nullptr && codes == nullptr) return fail(UQM_ERR_ARGUMENT, "%s: no output is wanted", what);
+  if (misaligned(output, 2) || misaligned(scales, 4)) return fail(UQM_ERR_ARGUMENT, "%s: outputs must be aligned to their elements", what);
+  const Span outs[] = {{output, 2 * rows * cols}, {codes, rows * cols},
+                       {scales, 4 * rows * ((cols + uqm::kFp8Group - 1) / uqm::kFp8Group)}, also};
+  for (size_t i = 0; i < sizeof(outs) / sizeof(outs[0]); ++i) {
+    for (const Span& in : inputs) {
+      if (in.p != nullptr && misaligned(in.p, 2)) return fail(UQM_ERR_ARGUMENT, "%s: inputs must be 2-byte aligned", what);
+      // (the sum may take an input's place element by element)
+      if (i == 3 && in.p == outs[i].p && in.bytes == outs[i].bytes) continue;
+      if (overlap(outs[i].p, outs[i].bytes, in.p, in.bytes)) return fail(UQM_ERR_ARGUMENT, "%s: an output overlaps an input", what);
+    }
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes))
+        return fail(UQM_ERR_ARGUMENT, "%s: two outputs overlap", what);
+  }
+  return UQM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int uqm_add_rmsnorm(const void* input, const void* residual, int64_t rows, int64_t hidden_size, const void* weight,
+                    float eps, void* sum, void* output, void* codes, float* scales, void* stream) {
+  using namespace uqm;
+  if (!(eps >= 0.f)) return fail(UQM_ERR_ARGUMENT, "add_rmsnorm: eps must be >= 0");
+  if ((residual == nullptr) != (sum == nullptr))
+    return fail(UQM_ERR_ARGUMENT, "add_rmsnorm: residual and sum must be given together");
+  const int64_t bytes = rows >= 0 && rows <= kMaxExtent && hidden_size > 0 && hidden_size <= kMaxExtent ? 2 * rows * hidden_size : 0;
+  int rc = check_rows("add_rmsnorm", rows, hidden_size, {{input, bytes}, {residual, bytes}, {weight, 2 * hidden_size}},
+                      output, codes, scales, {sum, bytes});
+  if (rc) return rc;
+  if (misaligned(sum, 2)) return fail(UQM_ERR_ARGUMENT, "add_rmsnorm: outputs must be aligned to their elements");
+  if (rows == 0) return UQM_OK;
+  if (input == nullptr) return fail(UQM_ERR_ARGUMENT, "add_rmsnorm: input is required");
+  if ((rc = check_device())) return rc;
+  return hip_check(launch_add_rmsnorm(static_cast<const uint16_t*>(input), static_cast<const uint16_t*>(residual), rows,
+                                      hidden_size, static_cast<const uint16_t*>(weight), eps,
+                                      static_cast<uint16_t*>(sum),
+                                      {static_cast<uint16_t*>(output), static_cast<uint8_t*>(codes), scales},
+                                      static_cast<hipStream_t>(stream)),
+                   "add_rmsnorm launch");
+}
+
+int uqm_silu_mul(const void* gate_up, int64_t rows, int64_t features, void* output, void* codes, float* scales,
+                 void* stream) {
+  using namespace uqm;
+  const int64_t bytes = rows >= 0 && rows <= kMaxExtent && features > 0 && features <= kMaxExtent ? 4 * rows * features : 0;
+  int rc = check_rows("silu_mul", rows, features, {{gate_up, bytes}}, output, codes, scales, {nullptr, 0});
+  if (rc) return rc;
+  if (rows == 0) return UQM_OK;
+  if (gate_up == nullptr) return fail(UQM_ERR_ARGUMENT, "silu_mul: gate_up is required");
+  if ((rc = check_device())) return rc;
+  return hip_check(launch_silu_mul(static_cast<const uint16_t*>(gate_up), rows, features,
+                                   {static_cast<uint16_t*>(output), static_cast<uint8_t*>(codes), scales},
+                                   static_cast<hipStream_t>(stream)),
+                   "silu_mul launch");
+}
+
+int uqm_fp8_quantize(const void* input, int64_t rows, int64_t cols, int64_t block_rows, void* codes, float* scales,
+                     void* stream) {
+  using namespace uqm;
+  if (block_rows != 1 && block_rows != kFp8Group)
+    return fail(UQM_ERR_ARGUMENT, "fp8_quantize: blocks have 1 or %d rows, not %lld", kFp8Group, (long long)block_rows);
+  const int64_t bytes = rows >= 0 && rows <= kMaxExtent && cols > 0 && cols <= kMaxExtent ? 2 * rows * cols : 0;
+  int rc = check_rows("fp8_quantize", rows, cols, {{input, bytes}}, nullptr, codes, scales, {nullptr, 0});
+  if (rc) return rc;
+  if (rows == 0) return UQM_OK;
+  if (input == nullptr) return fail(UQM_ERR_ARGUMENT, "fp8_quantize: input is required");
+  if ((rc = check_device())) return rc;
+  return hip_check(launch_fp8_quantize(static_cast<const uint16_t*>(input), rows, cols, static_cast<int>(block_rows),
+                                       static_cast<uint8_t*>(codes), scales, static_cast<hipStream_t>(stream)),
+                   "fp8_quantize launch");
+}
+
+int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const void* weight_codes,
+                   const float* weight_scales, int64_t out_features, int64_t in_features, const void* bias,
+                   void* output, void* stream) {
+  using namespace uqm;
+  if (rows < 0 || rows > kMaxExtent || out_features <= 0 || out_features > kMaxExtent || in_features > kMaxExtent)
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: rows must be in [0, 2^31) and features in [1, 2^31)");
+  if (in_features <= 0 || in_features % 16 != 0)
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: input features %lld must be a positive multiple of 16", (long long)in_features);
+  if (weight_codes == nullptr || weight_scales == nullptr)
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: weight codes and scales are required");
+  if (misaligned(weight_codes, 16) || misaligned(weight_scales, 4) || misaligned(bias, 2))
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: weight codes must be 16-byte aligned, scales and bias to their elements");
+  if (rows == 0) return UQM_OK;
+  if (codes == nullptr || scales == nullptr || output == nullptr)
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: codes, scales and output are required");
+  if (misaligned(codes, 16) || misaligned(scales, 4) || misaligned(output, 2))
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: codes must be 16-byte aligned, scales and output to their elements");
+  const int64_t groups = (in_features + kFp8Group - 1) / kFp8Group, out_bytes = 2 * rows * out_features;
+  if (overlap(output, out_bytes, codes, rows * in_features) || overlap(output, out_bytes, scales, 4 * rows * groups) ||
+      overlap(output, out_bytes, weight_codes, out_features * in_features) ||
+      overlap(output, out_bytes, weight_scales, 4 * ((out_features + kFp8Group - 1) / kFp8Group) * groups) ||
+      overlap(output, out_bytes, bias, 2 * out_features))
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: the output overlaps an input");
+  const int rc = check_device();
+  if (rc) return rc;
+  Fp8LinearArgs a{};
+  a.x = static_cast<const uint8_t*>(codes);
+  a.xs = scales;
+  a.w = static_cast<const uint8_t*>(weight_codes);
+  a.ws = weight_scales;
+  a.bias = static_cast<const uint16_t*>(bias);
+  a.out = static_cast<uint16_t*>(output);
+  a.T = rows;
+  a.N = out_features;
+  a.K = in_features;
+  return hip_check(launch_fp8_linear(a, device_cus(), static_cast<hipStream_t>(stream)), "fp8_linear launch");
 }
 
 }  // extern "C"

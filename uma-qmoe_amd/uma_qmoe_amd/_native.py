@@ -137,6 +137,10 @@ SIGNATURES = {
     "uqm_moe_layer_plan": (ctypes.c_int, (ctypes.POINTER(LayerWeights), _i64, ctypes.POINTER(LayerPlan))),
     "uqm_rmsnorm": (ctypes.c_int, (_vp, _i64, _i64, _vp, ctypes.c_float, _vp, _vp)),
     "uqm_dequantize": (ctypes.c_int, (_i32, _vp, _vp, _i64, _i64, _vp, _vp)),
+    "uqm_add_rmsnorm": (ctypes.c_int, (_vp, _vp, _i64, _i64, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp)),
+    "uqm_silu_mul": (ctypes.c_int, (_vp, _i64, _i64, _vp, _vp, _vp, _vp)),
+    "uqm_fp8_quantize": (ctypes.c_int, (_vp, _i64, _i64, _i64, _vp, _vp, _vp)),
+    "uqm_fp8_linear": (ctypes.c_int, (_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp)),
     "uqm_set_option": (ctypes.c_int, (ctypes.c_int, _i64)),
     "uqm_workspace_status": (ctypes.c_int, (_vp, ctypes.c_size_t, _vp)),
     "uqm_noalloc_status": (ctypes.c_int, (_vp,)),

@@ -38,6 +38,7 @@ from .formats import ENCODINGS, ContractError
 EXPERT_NAME = "model.layers.{layer}.mlp.experts.{expert}.{proj}.weight"
 PROJECTIONS = ("gate_proj", "up_proj", "down_proj")
 PLATFORM = "hip_gfx950"
+FP8_GROUP = 128  # columns (and, for weights, rows) that share a scale of an Fp8Matrix
 
 _EXTENSIONS: dict[str, Any] = {}
 _BUILD_LOCK = threading.Lock()
@@ -138,6 +139,29 @@ class DenseBlock:
     @property
     def has_shared(self) -> bool:
         return self.shared_gate is not None
+
+
+@dataclass(frozen=True)
+class Fp8Matrix:
+    """A matrix in 8-bit floats: ``codes`` float8_e4m3fn [..., cols] and
+    ``scales`` float32, one per ``block_rows`` x 128 block (value = code *
+    scale). Activations have blocks of one row (scales [..., ceil(cols / 128)]),
+    weights of 128 (codes [rows, cols], scales [ceil(rows / 128), ceil(cols / 128)])."""
+
+    codes: Any
+    scales: Any
+    block_rows: int = 1
+
+    @property
+    def shape(self) -> Any:
+        return self.codes.shape
+
+    def dequantize(self) -> Any:
+        """The float32 values (torch operations; for checks, not for products)."""
+        rows, cols = self.codes.reshape(-1, self.codes.shape[-1]).shape
+        scales = self.scales.reshape(-1, self.scales.shape[-1])
+        each = scales.repeat_interleave(self.block_rows, 0)[:rows].repeat_interleave(FP8_GROUP, 1)[:, :cols]
+        return self.codes.float() * each.reshape(self.codes.shape)
 
 
 class HipExtension:
@@ -414,6 +438,150 @@ class HipExtension:
                                   _stream_handle(torch, x.device))
         _native.check(rc, "uqm_rmsnorm")
         return out.reshape(hidden.shape)
+
+    # ------------------------------------------- 8-bit floats with scales --
+    def _launch(self, name, device, *args):
+        """Calls entry point ``name`` on the device's current stream, with the
+        device made current (a kernel runs on the current device's context)."""
+        torch = self.torch
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                rc = getattr(self.lib, name)(*args, _stream_handle(torch, device))
+        else:
+            rc = getattr(self.lib, name)(*args, _stream_handle(torch, device))
+        if rc:
+            _native.check(rc, name)
+
+    def _fp8_outputs(self, shape, device, block_rows=1):
+        torch = self.torch
+        cols = shape[-1]
+        groups = -(-cols // FP8_GROUP)
+        codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
+        scale_shape = (*shape[:-1], groups) if block_rows == 1 else (-(-shape[0] // block_rows), groups)
+        return Fp8Matrix(codes, torch.empty(scale_shape, dtype=torch.float32, device=device), block_rows)
+
+    def _rows_of(self, x, what):
+        """(contiguous x, rows, columns) of a BF16 tensor [..., columns]."""
+        if x.dtype != self.torch.bfloat16:
+            raise RuntimeError(f"{what} requires BF16 tensors")
+        if x.ndim < 1 or x.shape[-1] == 0:
+            raise RuntimeError(f"{what} requires a tensor with at least one column")
+        x = x.contiguous()
+        return x, x.numel() // x.shape[-1], x.shape[-1]
+
+    @staticmethod
+    def _on_device(what, first, *others):
+        for t in others:
+            if t is not None and t.device != first.device:
+                raise RuntimeError(f"{what} requires all tensors on one device")
+        if not first.is_cuda:
+            raise RuntimeError(f"{what} requires device tensors")
+
+    def add_rmsnorm(self, hidden, residual=None, eps=1e-6, weight=None, *, bf16=True, fp8=False, inplace=False):
+        """s = hidden + residual (BF16) and RMSNorm(s): (s, the norm in BF16 or
+        None, the norm as an ``Fp8Matrix`` or None). The BF16 norm rounds as
+        ``rmsnorm`` does; the 8-bit one is taken before any rounding to BF16.
+        Without a residual s is ``hidden`` itself. ``inplace`` writes s over
+        ``residual``."""
+        if not (bf16 or fp8):
+            raise RuntimeError("add_rmsnorm requires at least one of bf16 and fp8")
+        torch = self.torch
+        x, rows, cols = self._rows_of(hidden, "add_rmsnorm")
+        r = total = None
+        if residual is not None:
+            if residual.dtype != torch.bfloat16 or residual.shape != hidden.shape:
+                raise RuntimeError("add_rmsnorm requires a BF16 residual of hidden's shape")
+            if inplace and not residual.is_contiguous():
+                raise RuntimeError("add_rmsnorm(inplace=True) requires a contiguous residual")
+            r = residual.contiguous()
+        elif inplace:
+            raise RuntimeError("add_rmsnorm(inplace=True) requires a residual")
+        if weight is not None:
+            if weight.dtype != torch.bfloat16 or weight.ndim != 1 or weight.shape[0] != cols:
+                raise RuntimeError(f"add_rmsnorm requires a BF16 weight [{cols}]")
+            weight = weight.contiguous()
+        self._on_device("add_rmsnorm", x, r, weight)
+        if r is not None:
+            total = r if inplace else torch.empty_like(x)
+        out = torch.empty_like(x) if bf16 else None
+        q = self._fp8_outputs(x.shape, x.device) if fp8 else None
+        self._launch("uqm_add_rmsnorm", x.device, x.data_ptr(), _ptr(r), rows, cols, _ptr(weight), float(eps),
+                     _ptr(total), _ptr(out), q and q.codes.data_ptr(), q and q.scales.data_ptr())
+        return (hidden if total is None else total), out, q
+
+    def silu_mul(self, gate_up, *, bf16=True, fp8=False):
+        """silu(gate) * up of ``gate_up`` [..., 2 * features] (gate first):
+        (BF16 [..., features] or None, ``Fp8Matrix`` or None)."""
+        if not (bf16 or fp8):
+            raise RuntimeError("silu_mul requires at least one of bf16 and fp8")
+        torch = self.torch
+        x, rows, cols = self._rows_of(gate_up, "silu_mul")
+        if cols % 2:
+            raise RuntimeError("silu_mul requires an even number of columns")
+        self._on_device("silu_mul", x)
+        shape = (*x.shape[:-1], cols // 2)
+        out = torch.empty(shape, dtype=torch.bfloat16, device=x.device) if bf16 else None
+        q = self._fp8_outputs(shape, x.device) if fp8 else None
+        self._launch("uqm_silu_mul", x.device, x.data_ptr(), rows, cols // 2, _ptr(out),
+                     q and q.codes.data_ptr(), q and q.scales.data_ptr())
+        return out, q
+
+    def fp8_quantize(self, x, *, block_rows=1):
+        """``x`` (BF16) as an ``Fp8Matrix``: ``block_rows`` 1 for activations
+        [..., cols], 128 for a weight [rows, cols]."""
+        if block_rows not in (1, FP8_GROUP):
+            raise RuntimeError(f"fp8_quantize takes blocks of 1 or {FP8_GROUP} rows")
+        x, rows, cols = self._rows_of(x, "fp8_quantize")
+        if block_rows != 1 and x.ndim != 2:
+            raise RuntimeError("fp8_quantize takes blocks of rows of a matrix only")
+        self._on_device("fp8_quantize", x)
+        q = self._fp8_outputs(x.shape, x.device, block_rows)
+        self._launch("uqm_fp8_quantize", x.device, x.data_ptr(), rows, cols, block_rows, q.codes.data_ptr(),
+                     q.scales.data_ptr())
+        return q
+
+    def _check_fp8(self, m, block_rows, what):
+        torch = self.torch
+        codes, scales = m.codes, m.scales
+        if m.block_rows != block_rows:
+            raise RuntimeError(f"fp8_linear requires {what} in blocks of {block_rows} x {FP8_GROUP}")
+        if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+            raise RuntimeError(f"fp8_linear requires {what} as float8_e4m3fn codes and float32 scales")
+        shape = codes.shape
+        groups = -(-shape[-1] // FP8_GROUP)
+        want = (*shape[:-1], groups) if block_rows == 1 else (-(-shape[0] // block_rows), groups)
+        if tuple(scales.shape) != want:
+            raise RuntimeError(f"fp8_linear: {what} of shape {tuple(shape)} need scales {want}, not {tuple(scales.shape)}")
+        return codes.contiguous(), scales.contiguous()
+
+    def fp8_linear(self, x, weight: Fp8Matrix, bias=None):
+        """BF16 [..., out_features] = x @ weight^T + bias in FP32 sums. ``x`` is
+        an ``Fp8Matrix`` of activations, or a BF16 tensor that is quantised
+        first; ``weight`` an ``Fp8Matrix`` [out_features, in_features] in blocks
+        of 128 x 128, in_features a multiple of 16; ``bias`` BF16."""
+        torch = self.torch
+        if weight.codes.ndim != 2:
+            raise RuntimeError("fp8_linear requires a weight matrix")
+        w, ws = self._check_fp8(weight, FP8_GROUP, "weights")
+        n, k = w.shape
+        if n == 0 or k == 0 or k % 16:
+            raise RuntimeError(f"fp8_linear requires a weight of at least one row and a multiple of 16 columns, not {n} x {k}")
+        if not isinstance(x, Fp8Matrix):
+            if x.ndim < 1 or x.shape[-1] != k:
+                raise RuntimeError(f"fp8_linear requires {k} input features")
+            x = self.fp8_quantize(x)
+        elif x.codes.ndim < 1 or x.codes.shape[-1] != k:
+            raise RuntimeError(f"fp8_linear requires {k} input features")
+        codes, scales = self._check_fp8(x, 1, "activations")
+        if bias is not None:
+            if bias.dtype != torch.bfloat16 or bias.ndim != 1 or bias.shape[0] != n:
+                raise RuntimeError(f"fp8_linear requires a BF16 bias [{n}]")
+            bias = bias.contiguous()
+        self._on_device("fp8_linear", codes, scales, w, ws, bias)
+        out = torch.empty((*codes.shape[:-1], n), dtype=torch.bfloat16, device=codes.device)
+        self._launch("uqm_fp8_linear", codes.device, codes.data_ptr(), scales.data_ptr(), codes.numel() // k,
+                     w.data_ptr(), ws.data_ptr(), n, k, _ptr(bias), out.data_ptr())
+        return out
 
     # ------------------------------------- reference binding signatures --
     def _fixed(self, encoding, hidden, indices, weights, gate, gate_scales, up, up_scales, down, down_scales,
@@ -907,6 +1075,8 @@ def install_mixed_target_backend(*, build_directory: str | Path | None = None, v
 __all__ = [
     "DenseBlock",
     "DeviceExperts",
+    "FP8_GROUP",
+    "Fp8Matrix",
     "HipExtension",
     "MixedTargetNativeBackend",
     "PackedQ4NativeBackend",
