@@ -216,7 +216,9 @@ def product(ext, codes, scales, w, ws, b):
 LINEAR = [(1, 1, 16), (1, 16, 128), (1, 17, 144), (2, 200, 112), (1, 384, 2048), (15, 129, 272), (16, 64, 128),
           (17, 15, 256), (31, 256, 1040), (33, 127, 384), (64, 300, 512), (65, 96, 640), (100, 1000, 2000),
           (127, 257, 528), (128, 256, 1024), (129, 130, 1152), (255, 513, 384), (256, 256, 256), (300, 640, 2048),
-          (513, 384, 144), (777, 1410, 656), (1, 2048, 5632), (5, 11264, 256), (32, 2048, 2816)]
+          (513, 384, 144), (777, 1410, 656), (1, 2048, 5632), (5, 11264, 256), (32, 2048, 2816),
+          # tiles of the large-tile kernel: whole and ragged in each direction, one block of columns, a short last one
+          (2048, 2048, 128), (2049, 2049, 384), (2100, 2300, 272), (4200, 1100, 1040), (1030, 4100, 16)]
 
 
 @pytest.mark.parametrize("t,n,k", LINEAR)
@@ -232,7 +234,7 @@ def test_linear(hip_ext, t, n, k, bias):
     assert torch.equal(product(hip_ext, *args), got)  # no order of sums that changes
 
 
-@pytest.mark.parametrize("t,n,k", [(3, 40, 144), (40, 300, 272), (200, 300, 400), (600, 520, 272)])
+@pytest.mark.parametrize("t,n,k", [(3, 40, 144), (40, 300, 272), (200, 300, 400), (600, 520, 272), (2100, 2100, 400)])
 def test_linear_confines_nan(hip_ext, t, n, k):
     """A row of NaN codes or scales (a neighbour's last, short block reads up to
     it) changes its own results only."""
@@ -251,7 +253,7 @@ def test_linear_confines_nan(hip_ext, t, n, k):
     assert ((got - y).abs() <= tol)[keep].all()
 
 
-@pytest.mark.parametrize("t,n,k", [(1, 33, 128), (20, 33, 128), (130, 250, 256), (300, 515, 256)])
+@pytest.mark.parametrize("t,n,k", [(1, 33, 128), (20, 33, 128), (130, 250, 256), (300, 515, 256), (2050, 2050, 256)])
 def test_linear_leaves_its_surroundings(hip_ext, t, n, k):
     """Nothing is written before or behind the output."""
     note(f"fp8_linear surroundings {t}x{n}x{k}")

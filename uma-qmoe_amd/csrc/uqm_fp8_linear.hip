@@ -18,17 +18,23 @@
 // times finer than the codes' own steps, and the scaled sums here are FP32.
 #include "uqm_device.h"
 #include "uqm_fp8.h"
+#include "uqm_stage.h"
 
 namespace uqm {
 namespace {
 
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ f32x4_t mfma_fp8(const uint4& a0, const uint4& a1, const uint4& b0, const uint4& b1) {
-  const i32x8_t a = {(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
-  const i32x8_t b = {(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w, (int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w};
+__device__ __forceinline__ f32x4_t mfma_fp8(i32x8_t a, i32x8_t b) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 }
+// A lane's operand from its two pieces (one value: as two the compiler would
+// keep copies of them where they live across a loop).
+__device__ __forceinline__ i32x8_t operand(i32x4_t lo, i32x4_t hi) {
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ i32x4_t load16(const uint8_t* p) { return *reinterpret_cast<const i32x4_t*>(p); }
 
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
@@ -55,15 +61,15 @@ __global__ __launch_bounds__(kThreads) void fp8_rows_kernel(Fp8LinearArgs a) {
     xs[i] = a.xs + t * KB;
     acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const i32x4_t zero = {0, 0, 0, 0};
   for (int64_t b = wave; b < KB; b += kWaves) {
     const int64_t k0 = b * kFp8Group + 16 * q, k1 = k0 + 64;
     const bool in0 = k0 < a.K, in1 = k1 < a.K;  // (K is a multiple of 16)
-    const uint4 w0 = in0 ? ldg16(w + k0) : zero, w1 = in1 ? ldg16(w + k1) : zero;
+    const i32x8_t wv = operand(in0 ? load16(w + k0) : zero, in1 ? load16(w + k1) : zero);
     const float s = ws[b];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const f32x4_t d = mfma_fp8(w0, w1, in0 ? ldg16(x[i] + k0) : zero, in1 ? ldg16(x[i] + k1) : zero);
+      const f32x4_t d = mfma_fp8(wv, operand(in0 ? load16(x[i] + k0) : zero, in1 ? load16(x[i] + k1) : zero));
       const float f = s * xs[i][b];
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(f, d[e], acc[i][e]);
@@ -86,11 +92,285 @@ __global__ __launch_bounds__(kThreads) void fp8_rows_kernel(Fp8LinearArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- tiles --
+// Many tokens: 16 * TN * WN weight rows x 16 * TT * WT tokens per workgroup of
+// WN x WT waves, the column blocks in a ring of two stages in LDS (rows of 128
+// bytes, loaded by the address unit straight into LDS).
+//
+// Position of a row's 16-byte piece p in LDS is p ^ ((row >> 1) & 7): the LDS
+// serves a 16-byte read of 64 lanes in four turns of 16 rows, 256 bytes each, rows
+// 0-3 and 12-15 from one quadrant of lanes and rows 4-11 from its neighbour; two
+// rows make 256 bytes, so the eight even (and odd) rows of a turn have to be at
+// eight different positions, which this gives for pieces p and p ^ 1. Four
+// neighbouring lanes of a load still take 64 contiguous bytes.
+constexpr int kScaleBlocks = 8;
+
+template <int TN, int TT, int WN, int WT>
+struct Tile {
+  static constexpr int kWaves = WN * WT;
+  static constexpr int kRowsN = 16 * TN * WN, kRowsT = 16 * TT * WT;
+  static constexpr int kPanelN = kRowsN * kFp8Group, kPanelT = kRowsT * kFp8Group;  // bytes of a block in LDS
+  static constexpr int kScalePanel = kRowsT * kScaleBlocks * 4;  // bytes of the tokens' scales of kScaleBlocks blocks
+  static constexpr int kLds = 2 * (kPanelN + kPanelT + kScalePanel);
+  static constexpr int kLoadsN = kRowsN / 8 / kWaves, kLoadsT = kRowsT / 8 / kWaves;  // per wave and block, 8 rows each
+  static constexpr int kLoadsS = kRowsT / 8 / kWaves;  // per wave and scale panel, 8 tokens each
+};
+
+__device__ __align__(16) const uint8_t kZeroPiece[16] = {};
+
+__device__ __forceinline__ int token_position(int piece, int row) { return piece ^ ((row >> 1) & 7); }
+// The weight's rows go to the tiles of a wave in another order: row 4 * i + e of
+// tile n is row 32 * (n / 2) + 8 * i + 4 * (n % 2) + e, so that a lane's results of
+// two tiles are 8 neighbours (16 bytes) and the four lanes of a token's fill 64
+// bytes. Bits 1 to 3 of the tile's row are then bits 1, 3 and 4 of the row.
+__device__ __forceinline__ int weight_position(int piece, int row) {
+  return piece ^ (((row >> 1) & 1) | ((row >> 2) & 6));
+}
+
+template <int TN, int TT, int WN, int WT, bool TAIL>
+__global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs a, int tiles_n, int tiles_t) {
+  using G = Tile<TN, TT, WN, WT>;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int q = lane >> 4, r = lane & 15;
+  const int wn = wave % WN, wt = wave / WN;
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((stage_lds_t*)(lds)));
+  const uint32_t K = static_cast<uint32_t>(a.K);
+  const int KB = static_cast<int>((a.K + kFp8Group - 1) / kFp8Group);
+
+  // ---- work: 8 contiguous ranges of tiles, one per XCD, dealt out to its
+  // workgroups; in a range 4 row tiles side by side walk through the tokens, so
+  // that what an XCD works on at a time shares both sides
+  const int64_t n_items = static_cast<int64_t>(tiles_n) * tiles_t;
+  const int xcd = static_cast<int>(blockIdx.x & 7u);
+  const int item = static_cast<int>(n_items * xcd / 8) + static_cast<int>(blockIdx.x >> 3);
+  if (item >= static_cast<int>(n_items * (xcd + 1) / 8)) return;
+  constexpr int kSide = 8;
+  const int band = item / (kSide * tiles_t), in_band = item - band * kSide * tiles_t;
+  const int side = min(kSide, tiles_n - band * kSide);
+  const int64_t n0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(band * kSide + in_band % side)) * G::kRowsN;
+  const int64_t t0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(in_band / side)) * G::kRowsT;
+  // last row and token of the tile that exist
+  const int last_n = static_cast<int>(min(a.N - n0, static_cast<int64_t>(G::kRowsN))) - 1;
+  const int last_t = static_cast<int>(min(a.T - t0, static_cast<int64_t>(G::kRowsT))) - 1;
+
+  // ---- loads into LDS, 8 rows each: wave w's j-th of the weight and of the tokens.
+  // Columns behind the last, and blocks behind the last one, come from a piece of
+  // zeros: no branch, which would part the block's products from the folding of
+  // their sums (the compiler then moves all of that behind it, at a register per
+  // product), and no mask on the operands.
+  static_assert(G::kLoadsN * 8 * G::kWaves == G::kRowsN && G::kLoadsT * 8 * G::kWaves == G::kRowsT, "whole loads");
+  const uint8_t* zeros = kZeroPiece;
+  auto setup = [&](bool weight, int loads, int j, int last, uint32_t& off, uint32_t& column) {
+    const int row = 8 * (wave * loads + j) + (lane >> 3);
+    column = 16u * static_cast<uint32_t>(weight ? weight_position(lane & 7, row) : token_position(lane & 7, row));
+    off = static_cast<uint32_t>(min(row, last)) * K + column;  // (rows behind the last repeat it)
+  };
+  uint32_t off_n[G::kLoadsN], off_t[G::kLoadsT], col_n[G::kLoadsN], col_t[G::kLoadsT];
+#pragma unroll
+  for (int j = 0; j < G::kLoadsN; ++j) setup(true, G::kLoadsN, j, last_n, off_n[j], col_n[j]);
+#pragma unroll
+  for (int j = 0; j < G::kLoadsT; ++j) setup(false, G::kLoadsT, j, last_t, off_t[j], col_t[j]);
+  auto load = [&](const uint8_t* base, int b, uint32_t off, uint32_t column, uint32_t to) {
+    const bool in = b < KB;
+    const uint8_t* from = in ? base + static_cast<int64_t>(b) * kFp8Group : zeros;
+    uint32_t o = in ? off : 0u;
+    if constexpr (TAIL) {
+      from += o;
+      if (b == KB - 1 && column >= K % kFp8Group) from = zeros;
+      dma16_to(from, __builtin_amdgcn_readfirstlane(lds_base + to));
+    } else {
+      asm("" : "+v"(o));  // (extended to 64 bits by the load itself, not kept extended)
+      dma16_to(from + o, __builtin_amdgcn_readfirstlane(lds_base + to));
+    }
+  };
+  const uint8_t *wsrc = a.w + n0 * a.K, *xsrc = a.x + t0 * a.K;
+  auto n_panel = [&](int slot) { return static_cast<uint32_t>(slot * G::kPanelN); };
+  auto t_panel = [&](int slot) { return static_cast<uint32_t>(2 * G::kPanelN + slot * G::kPanelT); };
+  auto load_n = [&](int j, int b, int slot) {
+    load(wsrc, b, off_n[j], col_n[j], n_panel(slot) + (wave * G::kLoadsN + j) * (8 * kFp8Group));
+  };
+  auto load_t = [&](int j, int b, int slot) {
+    load(xsrc, b, off_t[j], col_t[j], t_panel(slot) + (wave * G::kLoadsT + j) * (8 * kFp8Group));
+  };
+
+  constexpr int kLoads = G::kLoadsN + G::kLoadsT;
+  auto load_any = [&](int j, int b, int slot) {
+    if (j < G::kLoadsN) load_n(j, b, slot);
+    else load_t(j - G::kLoadsN, b, slot);
+  };
+
+  // ---- operands of a block in LDS
+  // (read as a vector type: the compiler would wait for all loads into LDS
+  // before a read whose type tells it nothing)
+  auto read = [&](uint32_t at, uint32_t p0, uint32_t p1) { return operand(load16(lds + at + p0), load16(lds + at + p1)); };
+  const int w_row = 8 * (r >> 2) + (r & 3);
+  const uint32_t w0 = w_row * kFp8Group + 16u * weight_position(q, w_row);
+  const uint32_t w1 = w_row * kFp8Group + 16u * weight_position(q + 4, w_row);
+  const uint32_t x0 = r * kFp8Group + 16u * token_position(q, r), x1 = r * kFp8Group + 16u * token_position(q + 4, r);
+  auto read_w = [&](int slot, int n) {
+    return read(n_panel(slot) + (wn * (16 * TN) + 32 * (n / 2) + 4 * (n % 2)) * kFp8Group, w0, w1);
+  };
+  auto read_x = [&](int slot, int t) { return read(t_panel(slot) + (wt * TT + t) * (16 * kFp8Group), x0, x1); };
+
+  // ---- factors. The tokens' scales of 8 blocks come through LDS, too, [token][block]:
+  // a load takes 8 tokens' 32 bytes. (One float per token and block, straight into
+  // registers, were 16 cache lines a load, fetched again for every block: with
+  // them 8192 x 8192 x 8192 took 622 us, without any 482.)
+  static_assert((G::kLoadsS & (G::kLoadsS - 1)) == 0 && G::kLoadsS <= kScaleBlocks, "one load a block");
+  const float* xs = a.xs + t0 * KB;
+  auto s_panel = [&](int slot) { return static_cast<uint32_t>(2 * (G::kPanelN + G::kPanelT) + slot * G::kScalePanel); };
+  auto load_scales = [&](int j, int panel) {
+    const int row = min(8 * (wave * G::kLoadsS + j) + (lane >> 3), last_t);
+    const int b = min(panel * kScaleBlocks + (lane & 7), KB - 1);
+    dma4_to(xs + static_cast<uint32_t>(row * KB + b),
+            __builtin_amdgcn_readfirstlane(lds_base + s_panel(panel & 1) + (wave * G::kLoadsS + j) * 256));
+  };
+  const float* ws = a.ws + min((n0 + 16 * TN * wn) / kFp8Group, (a.N - 1) / kFp8Group) * KB;
+  float fw, fx[TT];  // of the next block
+  auto read_scales = [&](int b) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+      fx[t] = *reinterpret_cast<const float*>(lds + s_panel((b / kScaleBlocks) & 1) +
+                                              4 * ((16 * (TT * wt + t) + r) * kScaleBlocks + b % kScaleBlocks));
+  };
+
+  f32x4_t acc[TN][TT], d[TT];
+  i32x8_t x[TT], w[2];
+  float f[TT], f_last[TT];
+
+#pragma unroll
+  for (int n = 0; n < TN; ++n)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    d[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    f_last[t] = 0.f;
+  }
+  fw = ws[0];
+#pragma unroll
+  for (int j = 0; j < G::kLoadsS; ++j) load_scales(j, 0);
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) load_any(j, 0, 0);
+#pragma unroll
+  for (int j = 0; j < kLoads / 2; ++j) load_any(j, 1, 1);
+  wait_loads<kLoads / 2>();
+  stage_barrier();
+  w[0] = read_w(0, 0);
+#pragma unroll
+  for (int t = 0; t < TT; ++t) x[t] = read_x(0, t);
+  read_scales(0);
+
+  static_assert(TN % 2 == 0, "w alternates");
+  // A block's loads are spread over its first rows of products (the address unit
+  // takes 16 cycles for each).
+  for (int b = 0; b < KB; ++b) {
+    const int slot = b & 1;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) f[t] = fw * fx[t];
+    fw = ws[min(b + 1, KB - 1)];
+#pragma unroll
+      for (int n = 0; n < TN; ++n) {
+        // (a panel's loads twice over; the second time they write what is there)
+        if (n == TN / 2) {
+          load_scales(b % G::kLoadsS, b / kScaleBlocks + 1);
+          read_scales(min(b + 1, KB - 1));
+        }
+        if (n == TN - 1) {
+          // This block's operands are all in registers: the next block's panels
+          // must have landed, and this one's are free. The products of the last
+          // row hide the first reads from them.
+          wait_loads<0>();
+          stage_barrier();
+          w[0] = read_w(slot ^ 1, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          // the sums of the row before, TT products ago
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int m = n == 0 ? TN - 1 : n - 1;
+            acc[m][t][e] = fmaf(n == 0 ? f_last[t] : f[t], d[t][e], acc[m][t][e]);
+          }
+          d[t] = mfma_fp8(w[n & 1], x[t]);
+          // The compiler takes loads into LDS for accesses through LDS's own
+          // counter, too, and waits for all reads where it needs one: so a row's
+          // operand is read behind the first product of the row before.
+          if (n == TN - 1) x[t] = read_x(slot ^ 1, t);
+          else if (t == 0) w[(n + 1) & 1] = read_w(slot, n + 1);
+          // half of the loads right behind the barrier that freed their panels, the
+          // others in the next row (eight at once hold up the products)
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j) {
+            if (n == TN - 1 && j < kLoads / 2 && j * TT * 2 / kLoads == t) load_any(j, b + 2, slot);
+            if (n == 0 && j >= kLoads / 2 && (j - kLoads / 2) * TT * 2 / kLoads == t) load_any(j, b + 1, slot ^ 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) f_last[t] = f[t];
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[TN - 1][t][e] = fmaf(f_last[t], d[t][e], acc[TN - 1][t][e]);
+
+  // ---- outputs: 8 neighbouring rows a lane, of two tiles
+  const bool vec = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
+#pragma unroll
+  for (int n = 0; n < TN; n += 2) {
+    const int64_t row = n0 + 16 * (TN * wn + n) + 8 * q;
+    if (row >= a.N) continue;
+    float bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bias[e] = a.bias != nullptr && row + e < a.N ? bf16_to_f32(a.bias[row + e]) : 0.f;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const int tok = 16 * (TT * wt + t) + r;
+      if (tok > last_t) continue;
+      uint32_t h[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4_t v = acc[n + e / 2][t];
+        h[e] = pack_bf16x2(v[2 * (e & 1)] + bias[2 * e], v[2 * (e & 1) + 1] + bias[2 * e + 1]);
+      }
+      uint16_t* o = a.out + (t0 + tok) * a.N + row;
+      if (vec) {
+        *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (row + e < a.N) o[e] = static_cast<uint16_t>(h[e / 2] >> (16 * (e & 1)));
+      }
+    }
+  }
+  wait_loads<0>();  // no load into LDS outlives the workgroup
+}
+
+template <int TN, int TT, int WN, int WT>
+hipError_t launch_tiles(const Fp8LinearArgs& a, hipStream_t stream) {
+  using G = Tile<TN, TT, WN, WT>;
+  const int64_t tiles_n = (a.N + G::kRowsN - 1) / G::kRowsN, tiles_t = (a.T + G::kRowsT - 1) / G::kRowsT;
+  if (tiles_n * tiles_t > 0x7FFFFFF) return hipErrorInvalidValue;
+  const int64_t grid = (tiles_n * tiles_t + 7) / 8 * 8;
+  auto* k = a.K % kFp8Group == 0 ? fp8_tile_kernel<TN, TT, WN, WT, false> : fp8_tile_kernel<TN, TT, WN, WT, true>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(64 * G::kWaves), G::kLds, stream, a,
+                     static_cast<int>(tiles_n), static_cast<int>(tiles_t));
+  return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream) {
-  (void)cus;
   if (a.T <= 0) return hipSuccess;
+  // Tiles where there are enough of them for the card (32-bit offsets within a tile's rows).
+  if ((a.N + 255) / 256 * ((a.T + 255) / 256) >= cus / 4 && a.K < (int64_t{1} << 23)) return launch_tiles<8, 4, 2, 4>(a, stream);
   const int nt = a.T <= 16 ? 1 : 4;
   const int64_t grid = (a.N + 15) / 16 * ((a.T + 16 * nt - 1) / (16 * nt));
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
