@@ -39,6 +39,7 @@ hipError_t launch_fp8_quantize(const uint16_t* x, int64_t rows, int64_t cols, in
 
 // out[t, n] = bf16(bias[n] + sum over blocks b of 128 columns of
 //                  xs[t, b] ws[n / 128, b] sum over k in b of x[t, k] w[n, k])
+constexpr int64_t kFp8MaxK = int64_t{1} << 26;  // 64 rows within 32 bits
 struct Fp8LinearArgs {
   const uint8_t* x;       // codes [T, K]
   const float* xs;        // scales [T, ceil(K / 128)]
@@ -46,7 +47,7 @@ struct Fp8LinearArgs {
   const float* ws;        // scales [ceil(N / 128), ceil(K / 128)]
   const uint16_t* bias;   // bf16 [N] or NULL
   uint16_t* out;          // bf16 [T, N]
-  int64_t T, N, K;        // K a multiple of 16
+  int64_t T, N, K;        // K a multiple of 16 below kFp8MaxK
 };
 hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream);
 

@@ -35,75 +35,212 @@ __device__ __forceinline__ i32x8_t operand(i32x4_t lo, i32x4_t hi) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 __device__ __forceinline__ i32x4_t load16(const uint8_t* p) { return *reinterpret_cast<const i32x4_t*>(p); }
-
-constexpr int kWaves = 8;
-constexpr int kThreads = 64 * kWaves;
-
-// 16 weight rows x 16 * NT tokens per workgroup, the column blocks dealt out to
-// its waves, whose sums are added in wave order.
-template <int NT>
-__global__ __launch_bounds__(kThreads) void fp8_rows_kernel(Fp8LinearArgs a) {
-  __shared__ f32x4_t part[kWaves][NT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int q = lane >> 4, r = lane & 15;
-  const int64_t blocks_n = (a.N + 15) / 16;
-  const int64_t n0 = blockIdx.x % blocks_n * 16, t0 = blockIdx.x / blocks_n * (16 * NT);
-  const int64_t KB = (a.K + kFp8Group - 1) / kFp8Group;
-  const uint8_t* w = a.w + min(n0 + r, a.N - 1) * a.K;
-  const float* ws = a.ws + n0 / kFp8Group * KB;
-  const uint8_t* x[NT];
-  const float* xs[NT];
-  f32x4_t acc[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int64_t t = min(t0 + 16 * i + r, a.T - 1);  // (rows behind the last repeat it)
-    x[i] = a.x + t * a.K;
-    xs[i] = a.xs + t * KB;
-    acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-  const i32x4_t zero = {0, 0, 0, 0};
-  for (int64_t b = wave; b < KB; b += kWaves) {
-    const int64_t k0 = b * kFp8Group + 16 * q, k1 = k0 + 64;
-    const bool in0 = k0 < a.K, in1 = k1 < a.K;  // (K is a multiple of 16)
-    const i32x8_t wv = operand(in0 ? load16(w + k0) : zero, in1 ? load16(w + k1) : zero);
-    const float s = ws[b];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const f32x4_t d = mfma_fp8(wv, operand(in0 ? load16(x[i] + k0) : zero, in1 ? load16(x[i] + k1) : zero));
-      const float f = s * xs[i][b];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(f, d[e], acc[i][e]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) part[wave][i][lane] = acc[i];
-  __syncthreads();
-  for (int o = threadIdx.x; o < NT * 64; o += kThreads) {
-    const int i = o >> 6, l = o & 63;
-    f32x4_t v = part[0][i][l];
-#pragma unroll
-    for (int g = 1; g < kWaves; ++g) v += part[g][i][l];
-    const int64_t t = t0 + 16 * i + (l & 15), n = n0 + 4 * (l >> 4);
-    if (t >= a.T) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < a.N)
-        a.out[t * a.N + n + e] = f32_to_bf16(v[e] + (a.bias != nullptr ? bf16_to_f32(a.bias[n + e]) : 0.f));
-  }
+// Keeps reads of LDS behind the wait before it.
+__device__ __forceinline__ void reads_follow() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// ---------------------------------------------------------------- tiles --
-// Many tokens: 16 * TN * WN weight rows x 16 * TT * WT tokens per workgroup of
-// WN x WT waves, the column blocks in a ring of two stages in LDS (rows of 128
-// bytes, loaded by the address unit straight into LDS).
-//
+// What stands in the place of columns behind the last.
+__device__ __align__(16) const uint8_t kZeroPiece[16] = {};
+
 // Position of a row's 16-byte piece p in LDS is p ^ ((row >> 1) & 7): the LDS
 // serves a 16-byte read of 64 lanes in four turns of 16 rows, 256 bytes each, rows
 // 0-3 and 12-15 from one quadrant of lanes and rows 4-11 from its neighbour; two
 // rows make 256 bytes, so the eight even (and odd) rows of a turn have to be at
 // eight different positions, which this gives for pieces p and p ^ 1. Four
 // neighbouring lanes of a load still take 64 contiguous bytes.
+__device__ __forceinline__ int token_position(int piece, int row) { return piece ^ ((row >> 1) & 7); }
+// The weight's rows go to the tiles of a wave in another order: row 4 * i + e of
+// tile n is row 32 * (n / 2) + 8 * i + 4 * (n % 2) + e, so that a lane's results of
+// two tiles are 8 neighbours (16 bytes) and the four lanes of a token's fill 64
+// bytes. Bits 1 to 3 of the tile's row are then bits 1, 3 and 4 of the row.
+__device__ __forceinline__ int weight_position(int piece, int row) {
+  return piece ^ (((row >> 1) & 1) | ((row >> 2) & 6));
+}
+
+// ---------------------------------------------------------------- split --
+// Few tokens: 16 * TN weight rows x 16 * TT tokens per workgroup, the column
+// blocks dealt out to its W waves. Each wave loads its blocks into a ring of its
+// own in LDS, S blocks ahead, and waits for nobody until the sums of all waves are
+// added, in wave order.
+template <int TN, int TT, int W, int S>
+struct Split {
+  static constexpr int kBlock = (TN + TT) * 16 * kFp8Group;  // bytes of a block's operands
+  static constexpr int kStage = kBlock + 512;                // ... and the scales of tokens and rows (64 floats each)
+  static constexpr int kRing = S * kStage;                   // of a wave
+  static constexpr int kLds = W * kRing;
+  static constexpr int kLoads = 2 * (TN + TT) + 2;           // per block
+  static_assert(kRing >= TN * TT * 1024, "a wave's sums take its ring's place");
+  static_assert((S - 1) * kLoads <= 63 && kLds <= 160 * 1024, "");
+};
+
+template <int TN, int TT, int W, int S>
+__global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int blocks_n, int blocks_t) {
+  using G = Split<TN, TT, W, S>;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int q = lane >> 4, r = lane & 15;
+  const uint32_t ring = wave * G::kRing;
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((stage_lds_t*)(lds))) + ring;
+  // (8 contiguous ranges of workgroups, one per XCD; token blocks of the same rows
+  // next to each other)
+  const int64_t n_items = static_cast<int64_t>(blocks_n) * blocks_t;
+  const int xcd = static_cast<int>(blockIdx.x & 7u);
+  const int item = static_cast<int>(n_items * xcd / 8) + static_cast<int>(blockIdx.x >> 3);
+  if (item >= static_cast<int>(n_items * (xcd + 1) / 8)) return;
+  const int64_t n0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(item / blocks_t)) * (16 * TN);
+  const int64_t t0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(item % blocks_t)) * (16 * TT);
+  const int last_n = static_cast<int>(min(a.N - n0, static_cast<int64_t>(16 * TN))) - 1;
+  const int last_t = static_cast<int>(min(a.T - t0, static_cast<int64_t>(16 * TT))) - 1;
+  const uint32_t K = static_cast<uint32_t>(a.K);
+  const int KB = static_cast<int>((a.K + kFp8Group - 1) / kFp8Group);
+  const int mine = KB > wave ? (KB - wave + W - 1) / W : 0;
+
+  // ---- loads of this wave's i-th block: 8 rows at a time, then the scales
+  const uint8_t* zeros = kZeroPiece;
+  const uint8_t *wsrc = a.w + n0 * a.K, *xsrc = a.x + t0 * a.K;
+  const float* xs = a.xs + (t0 + min(lane, last_t)) * KB;
+  const float* ws = a.ws + n0 / kFp8Group * KB;
+  auto issue = [&](int i, int slot) {
+    const int b = wave + i * W;
+    const bool in = i < mine;
+    const uint32_t limit = in ? K - static_cast<uint32_t>(b) * kFp8Group : 0u;
+    const uint32_t to = lds_base + slot * G::kStage;
+#pragma unroll
+    for (int j = 0; j < 2 * (TN + TT); ++j) {
+      const bool weight = j < 2 * TN;
+      const int row = 8 * (weight ? j : j - 2 * TN) + (lane >> 3);
+      const uint32_t column =
+          16u * static_cast<uint32_t>(weight && TN > 1 ? weight_position(lane & 7, row) : token_position(lane & 7, row));
+      const uint8_t* from = (weight ? wsrc : xsrc) + (static_cast<uint32_t>(min(row, weight ? last_n : last_t)) * K +
+                                                      static_cast<uint32_t>(b) * kFp8Group + column);
+      dma16_to(column < limit ? from : zeros, __builtin_amdgcn_readfirstlane(to + j * (8 * kFp8Group)));
+    }
+    const int sb = min(b, KB - 1);
+    dma4_to(xs + sb, __builtin_amdgcn_readfirstlane(to + G::kBlock));
+    dma4_to(ws + sb, __builtin_amdgcn_readfirstlane(to + G::kBlock + 256));
+  };
+
+  const int w_row = TN > 1 ? 8 * (r >> 2) + (r & 3) : r;
+  auto w_at = [&](int piece) {
+    return w_row * kFp8Group + 16u * (TN > 1 ? weight_position(piece, w_row) : token_position(piece, w_row));
+  };
+  const uint32_t w0 = w_at(q), w1 = w_at(q + 4);
+  const uint32_t x0 = r * kFp8Group + 16u * token_position(q, r), x1 = r * kFp8Group + 16u * token_position(q + 4, r);
+
+  f32x4_t acc[TN][TT];
+#pragma unroll
+  for (int n = 0; n < TN; ++n)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < S; ++i) issue(i, i);
+  int slot = 0;
+  for (int i = 0; i < mine; ++i) {
+    wait_loads<(S - 1) * G::kLoads>();
+    reads_follow();
+    const unsigned char* at = lds + ring + slot * G::kStage;
+    i32x8_t w[TN], x[TT];
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+      const unsigned char* p = at + (32 * (n / 2) + 4 * (n % 2)) * kFp8Group;
+      w[n] = operand(load16(p + w0), load16(p + w1));
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const unsigned char* p = at + (TN + t) * (16 * kFp8Group);
+      x[t] = operand(load16(p + x0), load16(p + x1));
+    }
+    float f[TT];
+    const float* sc = reinterpret_cast<const float*>(at + G::kBlock);
+    const float fw = sc[64];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) f[t] = fw * sc[16 * t + r];
+    // the reads are done: the block's place takes the one S further on
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+    issue(i + S, slot);
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const f32x4_t d = mfma_fp8(w[n], x[t]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][t][e] = fmaf(f[t], d[e], acc[n][t][e]);
+      }
+    slot = slot + 1 == S ? 0 : slot + 1;
+  }
+
+  // ---- sums of the waves
+  wait_loads<0>();
+  reads_follow();
+#pragma unroll
+  for (int n = 0; n < TN; ++n)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4_t*>(lds + ring + (n * TT + t) * 1024 + 16 * lane) = acc[n][t];
+  __syncthreads();
+  constexpr int kPair = TN > 1 ? 2 : 1;  // tiles whose rows a thread puts together
+  const bool vec = a.N % (4 * kPair) == 0 && (reinterpret_cast<uintptr_t>(a.out) & (8u * kPair - 1)) == 0;
+  for (int o = threadIdx.x; o < TN / kPair * TT * 64; o += 64 * W) {
+    const int l = o & 63, nt = o >> 6, n = nt / TT * kPair, t = nt % TT;
+    f32x4_t v[kPair];
+#pragma unroll
+    for (int p = 0; p < kPair; ++p) {
+      const unsigned char* from = lds + ((n + p) * TT + t) * 1024 + 16 * l;
+      v[p] = *reinterpret_cast<const f32x4_t*>(from);
+#pragma unroll
+      for (int g = 1; g < W; ++g) v[p] += *reinterpret_cast<const f32x4_t*>(from + g * G::kRing);
+    }
+    const int tok = 16 * t + (l & 15);
+    const int64_t row = n0 + 16 * n + 4 * kPair * (l >> 4);
+    if (tok > last_t || row >= a.N) continue;
+    uint16_t* out = a.out + (t0 + tok) * a.N + row;
+    uint32_t h[2 * kPair];
+#pragma unroll
+    for (int e = 0; e < 2 * kPair; ++e) {
+      float y[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int64_t at = row + 2 * e + u;
+        y[u] = v[e / 2][2 * (e & 1) + u] + (a.bias != nullptr && at < a.N ? bf16_to_f32(a.bias[at]) : 0.f);
+      }
+      h[e] = pack_bf16x2(y[0], y[1]);
+    }
+    if (vec) {
+      if constexpr (kPair == 2) *reinterpret_cast<uint4*>(out) = make_uint4(h[0], h[1], h[2], h[3]);
+      else *reinterpret_cast<uint2*>(out) = make_uint2(h[0], h[1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4 * kPair; ++e)
+        if (row + e < a.N) out[e] = static_cast<uint16_t>(h[e / 2] >> (16 * (e & 1)));
+    }
+  }
+}
+
+template <int TN, int TT, int W, int S>
+hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
+  using G = Split<TN, TT, W, S>;
+  const int64_t blocks_n = (a.N + 16 * TN - 1) / (16 * TN), blocks_t = (a.T + 16 * TT - 1) / (16 * TT);
+  if (blocks_n * blocks_t > 0x7FFFFFF) return hipErrorInvalidValue;
+  const int64_t grid = (blocks_n * blocks_t + 7) / 8 * 8;
+  auto* k = fp8_split_kernel<TN, TT, W, S>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(64 * W), G::kLds, stream, a,
+                     static_cast<int>(blocks_n), static_cast<int>(blocks_t));
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- tiles --
+// Many tokens: 16 * TN * WN weight rows x 16 * TT * WT tokens per workgroup of
+// WN x WT waves, the column blocks in a ring of two stages in LDS (rows of 128
+// bytes, loaded by the address unit straight into LDS).
 constexpr int kScaleBlocks = 8;
+constexpr uint32_t kOutside = 0x80000000u;       // an offset behind every tile's bytes
+constexpr int64_t kFp8TileMaxK = int64_t{1} << 23;  // 256 rows of fewer bytes stay below it
 
 template <int TN, int TT, int WN, int WT>
 struct Tile {
@@ -115,17 +252,6 @@ struct Tile {
   static constexpr int kLoadsN = kRowsN / 8 / kWaves, kLoadsT = kRowsT / 8 / kWaves;  // per wave and block, 8 rows each
   static constexpr int kLoadsS = kRowsT / 8 / kWaves;  // per wave and scale panel, 8 tokens each
 };
-
-__device__ __align__(16) const uint8_t kZeroPiece[16] = {};
-
-__device__ __forceinline__ int token_position(int piece, int row) { return piece ^ ((row >> 1) & 7); }
-// The weight's rows go to the tiles of a wave in another order: row 4 * i + e of
-// tile n is row 32 * (n / 2) + 8 * i + 4 * (n % 2) + e, so that a lane's results of
-// two tiles are 8 neighbours (16 bytes) and the four lanes of a token's fill 64
-// bytes. Bits 1 to 3 of the tile's row are then bits 1, 3 and 4 of the row.
-__device__ __forceinline__ int weight_position(int piece, int row) {
-  return piece ^ (((row >> 1) & 1) | ((row >> 2) & 6));
-}
 
 template <int TN, int TT, int WN, int WT, bool TAIL>
 __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs a, int tiles_n, int tiles_t) {
@@ -140,7 +266,7 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
   const int KB = static_cast<int>((a.K + kFp8Group - 1) / kFp8Group);
 
   // ---- work: 8 contiguous ranges of tiles, one per XCD, dealt out to its
-  // workgroups; in a range 4 row tiles side by side walk through the tokens, so
+  // workgroups; in a range 8 row tiles side by side walk through the tokens, so
   // that what an XCD works on at a time shares both sides
   const int64_t n_items = static_cast<int64_t>(tiles_n) * tiles_t;
   const int xcd = static_cast<int>(blockIdx.x & 7u);
@@ -156,45 +282,35 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
   const int last_t = static_cast<int>(min(a.T - t0, static_cast<int64_t>(G::kRowsT))) - 1;
 
   // ---- loads into LDS, 8 rows each: wave w's j-th of the weight and of the tokens.
-  // Columns behind the last, and blocks behind the last one, come from a piece of
-  // zeros: no branch, which would part the block's products from the folding of
-  // their sums (the compiler then moves all of that behind it, at a register per
-  // product), and no mask on the operands.
+  // Rows behind the last lie outside the buffers and read as zeros; so do columns
+  // behind the last and blocks behind the last one, by an offset outside. (No
+  // branch: it would part the block's products from the folding of their sums,
+  // and the compiler moves all of that behind it, at a register per product.)
   static_assert(G::kLoadsN * 8 * G::kWaves == G::kRowsN && G::kLoadsT * 8 * G::kWaves == G::kRowsT, "whole loads");
-  const uint8_t* zeros = kZeroPiece;
-  auto setup = [&](bool weight, int loads, int j, int last, uint32_t& off, uint32_t& column) {
-    const int row = 8 * (wave * loads + j) + (lane >> 3);
-    column = 16u * static_cast<uint32_t>(weight ? weight_position(lane & 7, row) : token_position(lane & 7, row));
-    off = static_cast<uint32_t>(min(row, last)) * K + column;  // (rows behind the last repeat it)
-  };
-  uint32_t off_n[G::kLoadsN], off_t[G::kLoadsT], col_n[G::kLoadsN], col_t[G::kLoadsT];
+  const auto wbuf = stage_buffer(a.w + n0 * a.K, static_cast<uint32_t>(last_n + 1) * K);
+  const auto xbuf = stage_buffer(a.x + t0 * a.K, static_cast<uint32_t>(last_t + 1) * K);
+  uint32_t off_n[G::kLoadsN], off_t[G::kLoadsT];
+  auto n_row = [&](int j) { return 8 * (wave * G::kLoadsN + j) + (lane >> 3); };
+  auto t_row = [&](int j) { return 8 * (wave * G::kLoadsT + j) + (lane >> 3); };
+  auto n_column = [&](int j) { return 16u * static_cast<uint32_t>(weight_position(lane & 7, n_row(j))); };
+  auto t_column = [&](int j) { return 16u * static_cast<uint32_t>(token_position(lane & 7, t_row(j))); };
 #pragma unroll
-  for (int j = 0; j < G::kLoadsN; ++j) setup(true, G::kLoadsN, j, last_n, off_n[j], col_n[j]);
+  for (int j = 0; j < G::kLoadsN; ++j) off_n[j] = n_row(j) * K + n_column(j);
 #pragma unroll
-  for (int j = 0; j < G::kLoadsT; ++j) setup(false, G::kLoadsT, j, last_t, off_t[j], col_t[j]);
-  auto load = [&](const uint8_t* base, int b, uint32_t off, uint32_t column, uint32_t to) {
-    const bool in = b < KB;
-    const uint8_t* from = in ? base + static_cast<int64_t>(b) * kFp8Group : zeros;
-    uint32_t o = in ? off : 0u;
-    if constexpr (TAIL) {
-      from += o;
-      if (b == KB - 1 && column >= K % kFp8Group) from = zeros;
-      dma16_to(from, __builtin_amdgcn_readfirstlane(lds_base + to));
-    } else {
-      asm("" : "+v"(o));  // (extended to 64 bits by the load itself, not kept extended)
-      dma16_to(from + o, __builtin_amdgcn_readfirstlane(lds_base + to));
-    }
+  for (int j = 0; j < G::kLoadsT; ++j) off_t[j] = t_row(j) * K + t_column(j);
+  auto load = [&](__amdgpu_buffer_rsrc_t buf, int b, uint32_t off, uint32_t column, uint32_t to) {
+    const bool in = b < KB && !(TAIL && b == KB - 1 && column >= K % kFp8Group);
+    buffer16_to(buf, in ? off : kOutside, static_cast<uint32_t>(b) * kFp8Group,
+                __builtin_amdgcn_readfirstlane(lds_base + to));
   };
-  const uint8_t *wsrc = a.w + n0 * a.K, *xsrc = a.x + t0 * a.K;
   auto n_panel = [&](int slot) { return static_cast<uint32_t>(slot * G::kPanelN); };
   auto t_panel = [&](int slot) { return static_cast<uint32_t>(2 * G::kPanelN + slot * G::kPanelT); };
   auto load_n = [&](int j, int b, int slot) {
-    load(wsrc, b, off_n[j], col_n[j], n_panel(slot) + (wave * G::kLoadsN + j) * (8 * kFp8Group));
+    load(wbuf, b, off_n[j], n_column(j), n_panel(slot) + (wave * G::kLoadsN + j) * (8 * kFp8Group));
   };
   auto load_t = [&](int j, int b, int slot) {
-    load(xsrc, b, off_t[j], col_t[j], t_panel(slot) + (wave * G::kLoadsT + j) * (8 * kFp8Group));
+    load(xbuf, b, off_t[j], t_column(j), t_panel(slot) + (wave * G::kLoadsT + j) * (8 * kFp8Group));
   };
-
   constexpr int kLoads = G::kLoadsN + G::kLoadsT;
   auto load_any = [&](int j, int b, int slot) {
     if (j < G::kLoadsN) load_n(j, b, slot);
@@ -219,13 +335,12 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
   // registers, were 16 cache lines a load, fetched again for every block: with
   // them 8192 x 8192 x 8192 took 622 us, without any 482.)
   static_assert((G::kLoadsS & (G::kLoadsS - 1)) == 0 && G::kLoadsS <= kScaleBlocks, "one load a block");
-  const float* xs = a.xs + t0 * KB;
+  const auto sbuf = stage_buffer(a.xs + t0 * KB, static_cast<uint32_t>(last_t + 1) * (4 * KB));
   auto s_panel = [&](int slot) { return static_cast<uint32_t>(2 * (G::kPanelN + G::kPanelT) + slot * G::kScalePanel); };
   auto load_scales = [&](int j, int panel) {
-    const int row = min(8 * (wave * G::kLoadsS + j) + (lane >> 3), last_t);
-    const int b = min(panel * kScaleBlocks + (lane & 7), KB - 1);
-    dma4_to(xs + static_cast<uint32_t>(row * KB + b),
-            __builtin_amdgcn_readfirstlane(lds_base + s_panel(panel & 1) + (wave * G::kLoadsS + j) * 256));
+    const int row = 8 * (wave * G::kLoadsS + j) + (lane >> 3);
+    buffer4_to(sbuf, static_cast<uint32_t>(row * KB + (lane & 7)) * 4u, static_cast<uint32_t>(panel * kScaleBlocks) * 4u,
+               __builtin_amdgcn_readfirstlane(lds_base + s_panel(panel & 1) + (wave * G::kLoadsS + j) * 256));
   };
   const float* ws = a.ws + min((n0 + 16 * TN * wn) / kFp8Group, (a.N - 1) / kFp8Group) * KB;
   float fw, fx[TT];  // of the next block
@@ -258,6 +373,7 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
   for (int j = 0; j < kLoads / 2; ++j) load_any(j, 1, 1);
   wait_loads<kLoads / 2>();
   stage_barrier();
+  reads_follow();
   w[0] = read_w(0, 0);
 #pragma unroll
   for (int t = 0; t < TT; ++t) x[t] = read_x(0, t);
@@ -284,8 +400,11 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
           // row hide the first reads from them.
           wait_loads<0>();
           stage_barrier();
+          reads_follow();
           w[0] = read_w(slot ^ 1, 0);
         }
+        if (n < TN - 1) w[(n + 1) & 1] = read_w(slot, n + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
           // the sums of the row before, TT products ago
@@ -295,11 +414,7 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
             acc[m][t][e] = fmaf(n == 0 ? f_last[t] : f[t], d[t][e], acc[m][t][e]);
           }
           d[t] = mfma_fp8(w[n & 1], x[t]);
-          // The compiler takes loads into LDS for accesses through LDS's own
-          // counter, too, and waits for all reads where it needs one: so a row's
-          // operand is read behind the first product of the row before.
           if (n == TN - 1) x[t] = read_x(slot ^ 1, t);
-          else if (t == 0) w[(n + 1) & 1] = read_w(slot, n + 1);
           // half of the loads right behind the barrier that freed their panels, the
           // others in the next row (eight at once hold up the products)
 #pragma unroll
@@ -365,18 +480,63 @@ hipError_t launch_tiles(const Fp8LinearArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// ------------------------------------------------------------------- plan --
+// What a call takes with each kernel: a fixed time (launch, first loads, last
+// stores), and for every round of workgroups that the CUs hold a part of its own
+// and one for each block of 128 columns, which grows with the share of the card
+// that works (L2 and the clock are shared): `empty` for one workgroup, `full` for
+// all. Fitted to 1750 products (T 1 to 8191, N 128 to 11264, K 128 to 8192; 5 to
+// 11% off in the mean square); the kernel taken is 1.8% slower in the mean than
+// the best of the eight, over 10% in 119 of them (at most 33%, calls of 5 to 12
+// us). Without one of the eight the best of the others is slower by 7.3, 1.4,
+// 1.2, 1.5, 0.8, 0.3, 0.1 and 1.0% in the mean (in their order below); the ends:
+//   1 x 11264 x 2048       16 x 16 rows and tokens 7.5 us, 32 x 32 9.8
+//   137 x 1400 x 2000      32 x 32 5.3, 64 x 64 8.9, 128 x 64 12
+//   512 x 2048 x 5632      64 x 64 14.7, 64 x 32 19.0, 128 x 64 31.9
+//   1024 x 2048 x 2048     128 x 64 14.1, 64 x 64 15.2, 256 x 256 26.1
+//   4096 x 2048 x 5632     128 x 256 51.2, 128 x 128 54.8, 256 x 256 61.4
+//   8191 x 11264 x 2048    256 x 256 196, 128 x 256 234, 128 x 64 285
+struct Kernel {
+  int rows, tokens, per_cu;
+  float fixed, round, full, empty;  // us
+  hipError_t (*launch)(const Fp8LinearArgs&, hipStream_t);
+};
+constexpr Kernel kKernels[] = {
+    {16, 16, 4, 1.99f, 1.35f, 0.209f, 0.018f, launch_split<1, 1, 8, 1>},
+    {32, 32, 2, 2.19f, 1.59f, 0.225f, 0.050f, launch_split<2, 2, 8, 1>},
+    {64, 32, 1, 2.19f, 2.01f, 0.173f, 0.106f, launch_split<4, 2, 8, 1>},
+    {64, 64, 1, 2.30f, 2.58f, 0.268f, 0.162f, launch_split<4, 4, 8, 1>},
+    {128, 64, 2, 2.18f, 1.67f, 0.728f, 0.502f, launch_tiles<4, 2, 2, 2>},
+    {128, 128, 2, 0.32f, 4.00f, 1.148f, 0.527f, launch_tiles<4, 2, 2, 4>},
+    {128, 256, 1, 0.70f, 4.73f, 1.021f, 0.778f, launch_tiles<4, 4, 2, 4>},
+    {256, 256, 1, 1.49f, 7.46f, 1.531f, 0.992f, launch_tiles<8, 4, 2, 4>},
+};
+
+float estimate(const Kernel& k, const Fp8LinearArgs& a, int cus) {
+  const int64_t items = (a.N + k.rows - 1) / k.rows * ((a.T + k.tokens - 1) / k.tokens);
+  const int64_t slots = static_cast<int64_t>(cus) * k.per_cu, rounds = items / slots, rest = items % slots;
+  const float blocks = static_cast<float>((a.K + kFp8Group - 1) / kFp8Group);
+  float us = k.fixed + static_cast<float>(rounds) * (k.round + k.full * blocks);
+  if (rest > 0)
+    us += k.round + blocks * (k.empty + (k.full - k.empty) * static_cast<float>(rest) / static_cast<float>(slots));
+  return us;
+}
+
 }  // namespace
 
 hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream) {
   if (a.T <= 0) return hipSuccess;
-  // Tiles where there are enough of them for the card (32-bit offsets within a tile's rows).
-  if ((a.N + 255) / 256 * ((a.T + 255) / 256) >= cus / 4 && a.K < (int64_t{1} << 23)) return launch_tiles<8, 4, 2, 4>(a, stream);
-  const int nt = a.T <= 16 ? 1 : 4;
-  const int64_t grid = (a.N + 15) / 16 * ((a.T + 16 * nt - 1) / (16 * nt));
-  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-  auto* k = nt == 1 ? fp8_rows_kernel<1> : fp8_rows_kernel<4>;
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
-  return hipGetLastError();
+  const Kernel* best = nullptr;
+  float least = 0.f;
+  for (const Kernel& k : kKernels) {
+    if (k.rows >= 128 && a.K >= kFp8TileMaxK) continue;
+    const float us = estimate(k, a, cus);
+    if (best == nullptr || us < least) {
+      best = &k;
+      least = us;
+    }
+  }
+  return best->launch(a, stream);
 }
 
 }  // namespace uqm

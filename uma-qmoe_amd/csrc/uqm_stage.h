@@ -37,4 +37,22 @@ __device__ __forceinline__ void dma4_to(const void* src, uint32_t lds_addr) {
   __builtin_amdgcn_global_load_lds(src, reinterpret_cast<stage_lds_t*>(static_cast<uintptr_t>(lds_addr)), 4, 0, 0);
 }
 
+// The same through a buffer of `bytes` bytes: bytes from there on read as zeros,
+// and the address is a scalar base plus the lane's 32-bit offset plus a scalar
+// one. (Unlike the loads above, which the compiler takes for accesses that also
+// count as LDS reads, so that it waits for all of these where it needs one.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t stage_buffer(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ void buffer16_to(__amdgpu_buffer_rsrc_t from, uint32_t lane_offset, uint32_t offset,
+                                            uint32_t lds_addr) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, reinterpret_cast<stage_lds_t*>(static_cast<uintptr_t>(lds_addr)), 16,
+                                           lane_offset, offset, 0, 0);
+}
+__device__ __forceinline__ void buffer4_to(__amdgpu_buffer_rsrc_t from, uint32_t lane_offset, uint32_t offset,
+                                           uint32_t lds_addr) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, reinterpret_cast<stage_lds_t*>(static_cast<uintptr_t>(lds_addr)), 4,
+                                           lane_offset, offset, 0, 0);
+}
+
 }  // namespace uqm

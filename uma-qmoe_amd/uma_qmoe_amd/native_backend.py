@@ -440,41 +440,35 @@ class HipExtension:
         return out.reshape(hidden.shape)
 
     # ------------------------------------------- 8-bit floats with scales --
-    def _launch(self, name, device, *args):
-        """Calls entry point ``name`` on the device's current stream, with the
-        device made current (a kernel runs on the current device's context)."""
+    # (A call of few rows takes as long on the host as on the GPU: the checks
+    # below cost 1 to 2 us a call, an allocation 1.3, the launch 3.)
+    def _launch(self, fn, index, *args):
+        """Calls entry point ``fn`` on the current stream of device ``index``,
+        which is made current if it is not."""
         torch = self.torch
-        if device.index != torch.cuda.current_device():
-            with torch.cuda.device(device):
-                rc = getattr(self.lib, name)(*args, _stream_handle(torch, device))
+        if torch._C._cuda_getDevice() == index:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
-            rc = getattr(self.lib, name)(*args, _stream_handle(torch, device))
+            with torch.cuda.device(index):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         if rc:
-            _native.check(rc, name)
-
-    def _fp8_outputs(self, shape, device, block_rows=1):
-        torch = self.torch
-        cols = shape[-1]
-        groups = -(-cols // FP8_GROUP)
-        codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
-        scale_shape = (*shape[:-1], groups) if block_rows == 1 else (-(-shape[0] // block_rows), groups)
-        return Fp8Matrix(codes, torch.empty(scale_shape, dtype=torch.float32, device=device), block_rows)
+            _native.check(rc, fn.__name__)
 
     def _rows_of(self, x, what):
-        """(contiguous x, rows, columns) of a BF16 tensor [..., columns]."""
-        if x.dtype != self.torch.bfloat16:
+        """(contiguous x, its device's index, rows, columns) of a BF16 tensor [..., columns]."""
+        if x.dtype is not self.torch.bfloat16:
             raise RuntimeError(f"{what} requires BF16 tensors")
-        if x.ndim < 1 or x.shape[-1] == 0:
+        cols = x.shape[-1] if x.ndim else 0
+        if cols == 0:
             raise RuntimeError(f"{what} requires a tensor with at least one column")
-        x = x.contiguous()
-        return x, x.numel() // x.shape[-1], x.shape[-1]
+        return x.contiguous(), x.get_device(), x.numel() // cols, cols
 
     @staticmethod
-    def _on_device(what, first, *others):
+    def _check_devices(what, index, *others):
         for t in others:
-            if t is not None and t.device != first.device:
+            if t is not None and t.get_device() != index:
                 raise RuntimeError(f"{what} requires all tensors on one device")
-        if not first.is_cuda:
+        if index < 0:
             raise RuntimeError(f"{what} requires device tensors")
 
     def add_rmsnorm(self, hidden, residual=None, eps=1e-6, weight=None, *, bf16=True, fp8=False, inplace=False):
@@ -483,13 +477,13 @@ class HipExtension:
         ``rmsnorm`` does; the 8-bit one is taken before any rounding to BF16.
         Without a residual s is ``hidden`` itself. ``inplace`` writes s over
         ``residual``."""
+        torch = self.torch
+        x, index, rows, cols = self._rows_of(hidden, "add_rmsnorm")
         if not (bf16 or fp8):
             raise RuntimeError("add_rmsnorm requires at least one of bf16 and fp8")
-        torch = self.torch
-        x, rows, cols = self._rows_of(hidden, "add_rmsnorm")
-        r = total = None
+        r = total = out = q = None
         if residual is not None:
-            if residual.dtype != torch.bfloat16 or residual.shape != hidden.shape:
+            if residual.dtype is not torch.bfloat16 or residual.shape != hidden.shape:
                 raise RuntimeError("add_rmsnorm requires a BF16 residual of hidden's shape")
             if inplace and not residual.is_contiguous():
                 raise RuntimeError("add_rmsnorm(inplace=True) requires a contiguous residual")
@@ -497,60 +491,72 @@ class HipExtension:
         elif inplace:
             raise RuntimeError("add_rmsnorm(inplace=True) requires a residual")
         if weight is not None:
-            if weight.dtype != torch.bfloat16 or weight.ndim != 1 or weight.shape[0] != cols:
+            if weight.dtype is not torch.bfloat16 or weight.ndim != 1 or weight.shape[0] != cols:
                 raise RuntimeError(f"add_rmsnorm requires a BF16 weight [{cols}]")
             weight = weight.contiguous()
-        self._on_device("add_rmsnorm", x, r, weight)
+        self._check_devices("add_rmsnorm", index, r, weight)
         if r is not None:
             total = r if inplace else torch.empty_like(x)
-        out = torch.empty_like(x) if bf16 else None
-        q = self._fp8_outputs(x.shape, x.device) if fp8 else None
-        self._launch("uqm_add_rmsnorm", x.device, x.data_ptr(), _ptr(r), rows, cols, _ptr(weight), float(eps),
+        if bf16:
+            out = torch.empty_like(x)
+        if fp8:
+            q = Fp8Matrix(torch.empty_like(x, dtype=torch.float8_e4m3fn),
+                          torch.empty(*x.shape[:-1], -(-cols // FP8_GROUP), dtype=torch.float32, device=x.device))
+        self._launch(self.lib.uqm_add_rmsnorm, index, x.data_ptr(), _ptr(r), rows, cols, _ptr(weight), eps,
                      _ptr(total), _ptr(out), q and q.codes.data_ptr(), q and q.scales.data_ptr())
         return (hidden if total is None else total), out, q
 
     def silu_mul(self, gate_up, *, bf16=True, fp8=False):
         """silu(gate) * up of ``gate_up`` [..., 2 * features] (gate first):
         (BF16 [..., features] or None, ``Fp8Matrix`` or None)."""
+        torch = self.torch
+        x, index, rows, cols = self._rows_of(gate_up, "silu_mul")
         if not (bf16 or fp8):
             raise RuntimeError("silu_mul requires at least one of bf16 and fp8")
-        torch = self.torch
-        x, rows, cols = self._rows_of(gate_up, "silu_mul")
         if cols % 2:
             raise RuntimeError("silu_mul requires an even number of columns")
-        self._on_device("silu_mul", x)
-        shape = (*x.shape[:-1], cols // 2)
-        out = torch.empty(shape, dtype=torch.bfloat16, device=x.device) if bf16 else None
-        q = self._fp8_outputs(shape, x.device) if fp8 else None
-        self._launch("uqm_silu_mul", x.device, x.data_ptr(), rows, cols // 2, _ptr(out),
+        self._check_devices("silu_mul", index)
+        lead, features, device = x.shape[:-1], cols // 2, x.device
+        out = torch.empty(*lead, features, dtype=torch.bfloat16, device=device) if bf16 else None
+        q = None
+        if fp8:
+            q = Fp8Matrix(torch.empty(*lead, features, dtype=torch.float8_e4m3fn, device=device),
+                          torch.empty(*lead, -(-features // FP8_GROUP), dtype=torch.float32, device=device))
+        self._launch(self.lib.uqm_silu_mul, index, x.data_ptr(), rows, features, _ptr(out),
                      q and q.codes.data_ptr(), q and q.scales.data_ptr())
         return out, q
 
     def fp8_quantize(self, x, *, block_rows=1):
         """``x`` (BF16) as an ``Fp8Matrix``: ``block_rows`` 1 for activations
         [..., cols], 128 for a weight [rows, cols]."""
-        if block_rows not in (1, FP8_GROUP):
+        torch = self.torch
+        x, index, rows, cols = self._rows_of(x, "fp8_quantize")
+        if block_rows == 1:
+            lead = x.shape[:-1]
+        elif block_rows != FP8_GROUP:
             raise RuntimeError(f"fp8_quantize takes blocks of 1 or {FP8_GROUP} rows")
-        x, rows, cols = self._rows_of(x, "fp8_quantize")
-        if block_rows != 1 and x.ndim != 2:
+        elif x.ndim != 2:
             raise RuntimeError("fp8_quantize takes blocks of rows of a matrix only")
-        self._on_device("fp8_quantize", x)
-        q = self._fp8_outputs(x.shape, x.device, block_rows)
-        self._launch("uqm_fp8_quantize", x.device, x.data_ptr(), rows, cols, block_rows, q.codes.data_ptr(),
-                     q.scales.data_ptr())
-        return q
+        else:
+            lead = (-(-rows // FP8_GROUP),)
+        self._check_devices("fp8_quantize", index)
+        codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+        scales = torch.empty(*lead, -(-cols // FP8_GROUP), dtype=torch.float32, device=x.device)
+        self._launch(self.lib.uqm_fp8_quantize, index, x.data_ptr(), rows, cols, block_rows, codes.data_ptr(),
+                     scales.data_ptr())
+        return Fp8Matrix(codes, scales, block_rows)
 
     def _check_fp8(self, m, block_rows, what):
         torch = self.torch
         codes, scales = m.codes, m.scales
         if m.block_rows != block_rows:
             raise RuntimeError(f"fp8_linear requires {what} in blocks of {block_rows} x {FP8_GROUP}")
-        if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        if codes.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32:
             raise RuntimeError(f"fp8_linear requires {what} as float8_e4m3fn codes and float32 scales")
         shape = codes.shape
         groups = -(-shape[-1] // FP8_GROUP)
         want = (*shape[:-1], groups) if block_rows == 1 else (-(-shape[0] // block_rows), groups)
-        if tuple(scales.shape) != want:
+        if scales.shape != want:
             raise RuntimeError(f"fp8_linear: {what} of shape {tuple(shape)} need scales {want}, not {tuple(scales.shape)}")
         return codes.contiguous(), scales.contiguous()
 
@@ -566,20 +572,20 @@ class HipExtension:
         n, k = w.shape
         if n == 0 or k == 0 or k % 16:
             raise RuntimeError(f"fp8_linear requires a weight of at least one row and a multiple of 16 columns, not {n} x {k}")
-        if not isinstance(x, Fp8Matrix):
-            if x.ndim < 1 or x.shape[-1] != k:
-                raise RuntimeError(f"fp8_linear requires {k} input features")
-            x = self.fp8_quantize(x)
-        elif x.codes.ndim < 1 or x.codes.shape[-1] != k:
+        ndim = x.codes.ndim if isinstance(x, Fp8Matrix) else x.ndim
+        if ndim < 1 or x.shape[-1] != k:
             raise RuntimeError(f"fp8_linear requires {k} input features")
+        if not isinstance(x, Fp8Matrix):
+            x = self.fp8_quantize(x)
         codes, scales = self._check_fp8(x, 1, "activations")
         if bias is not None:
-            if bias.dtype != torch.bfloat16 or bias.ndim != 1 or bias.shape[0] != n:
+            if bias.dtype is not torch.bfloat16 or bias.ndim != 1 or bias.shape[0] != n:
                 raise RuntimeError(f"fp8_linear requires a BF16 bias [{n}]")
             bias = bias.contiguous()
-        self._on_device("fp8_linear", codes, scales, w, ws, bias)
-        out = torch.empty((*codes.shape[:-1], n), dtype=torch.bfloat16, device=codes.device)
-        self._launch("uqm_fp8_linear", codes.device, codes.data_ptr(), scales.data_ptr(), codes.numel() // k,
+        index = codes.get_device()
+        self._check_devices("fp8_linear", index, scales, w, ws, bias)
+        out = torch.empty(*codes.shape[:-1], n, dtype=torch.bfloat16, device=codes.device)
+        self._launch(self.lib.uqm_fp8_linear, index, codes.data_ptr(), scales.data_ptr(), codes.numel() // k,
                      w.data_ptr(), ws.data_ptr(), n, k, _ptr(bias), out.data_ptr())
         return out
 
