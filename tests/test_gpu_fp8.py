@@ -35,11 +35,11 @@ def on_gpu(t, offset=0):
 
 # ------------------------------------------------------------- row operators --
 # one group, its ends, several; the 1-, 2- and 4-pass rows and longer ones; not multiples of 8
-COLS = [1, 7, 8, 120, 127, 128, 129, 136, 1400, 2047, 2048, 2056, 4104, 8192, 8200, 8201, 20000]
+COLS = [1, 7, 8, 120, 127, 128, 129, 136, 511, 512, 520, 1400, 2047, 2048, 2056, 4104, 5632, 8192, 8200, 8201, 20000]
 
 
 @pytest.mark.parametrize("cols", COLS)
-@pytest.mark.parametrize("rows,offset", [(1, 0), (5, 0), (3, 1)])
+@pytest.mark.parametrize("rows,offset", [(1, 0), (5, 0), (3, 1), (37, 3)])
 @pytest.mark.parametrize("residual", [False, True])
 def test_add_rmsnorm(hip_ext, rows, cols, offset, residual):
     note(f"add_rmsnorm {rows}x{cols}+{offset} residual={residual}")
@@ -159,6 +159,23 @@ def test_quantize_ends(hip_ext, block):
     at[4][0, 6] = 0
     assert (at[4] == 0).all()
     ref.check_fp8(c[:, 128:], s[:, 1:], x[:, 128:].double(), block, 0.0)
+
+
+def test_quantize_with_scales_next_to_the_input(hip_ext):
+    """Blocks of 128 rows have few scales: the ones of 4095 x 128 right before the
+    input, or right behind the codes, overlap nothing."""
+    note("fp8_quantize scales next to the input")
+    rows, cols = 4095, 128
+    groups = -(-rows // 128)
+    room = torch.zeros(4 * 4096 + 2 * rows * cols, dtype=torch.uint8, device=DEV)
+    scales = room[4 * 4096 - 4 * groups:4 * 4096].view(torch.float32)
+    x = room[4 * 4096:].view(torch.bfloat16).view(rows, cols)
+    x.copy_(normal(gen(2), rows, cols))
+    codes = torch.empty(rows, cols, dtype=torch.uint8, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert hip_ext.lib.uqm_fp8_quantize(x.data_ptr(), rows, cols, 128, codes.data_ptr(), scales.data_ptr(), stream) == 0
+    want = hip_ext.fp8_quantize(x, block_rows=128)
+    assert torch.equal(codes, want.codes.view(torch.uint8)) and torch.equal(scales, want.scales.flatten())
 
 
 def test_norm_and_sum_keep_nan_and_infinity(hip_ext):

@@ -1325,7 +1325,7 @@ struct Span {
   int64_t bytes;
 };
 int check_rows(const char* what, int64_t rows, int64_t cols, std::initializer_list<Span> inputs, const void* output,
-               const void* codes, const float* scales, Span also) {
+               const void* codes, const float* scales, Span also, int64_t block_rows = 1) {
   if (rows < 0 || rows > kMaxExtent || cols <= 0 || cols > kMaxExtent)
     return fail(UQM_ERR_ARGUMENT, "%s: rows must be in [0, 2^31) and columns in [1, 2^31)", what);
   if (rows == 0) return UQM_OK;  // (pointers of empty tensors may be NULL)
@@ -1334,7 +1334,8 @@ int check_rows(const char* what, int64_t rows, int64_t cols, std::initializer_li
   if (output == nullptr && codes == nullptr) return fail(UQM_ERR_ARGUMENT, "%s: no output is wanted", what);
   if (misaligned(output, 2) || misaligned(scales, 4)) return fail(UQM_ERR_ARGUMENT, "%s: outputs must be aligned to their elements", what);
   const Span outs[] = {{output, 2 * rows * cols}, {codes, rows * cols},
-                       {scales, 4 * rows * ((cols + uqm::kFp8Group - 1) / uqm::kFp8Group)}, also};
+                       {scales, 4 * ((rows + block_rows - 1) / block_rows) * ((cols + uqm::kFp8Group - 1) / uqm::kFp8Group)},
+                       also};
   for (size_t i = 0; i < sizeof(outs) / sizeof(outs[0]); ++i) {
     for (const Span& in : inputs) {
       if (in.p != nullptr && misaligned(in.p, 2)) return fail(UQM_ERR_ARGUMENT, "%s: inputs must be 2-byte aligned", what);
@@ -1396,7 +1397,7 @@ int uqm_fp8_quantize(const void* input, int64_t rows, int64_t cols, int64_t bloc
   if (block_rows != 1 && block_rows != kFp8Group)
     return fail(UQM_ERR_ARGUMENT, "fp8_quantize: blocks have 1 or %d rows, not %lld", kFp8Group, (long long)block_rows);
   const int64_t bytes = rows >= 0 && rows <= kMaxExtent && cols > 0 && cols <= kMaxExtent ? 2 * rows * cols : 0;
-  int rc = check_rows("fp8_quantize", rows, cols, {{input, bytes}}, nullptr, codes, scales, {nullptr, 0});
+  int rc = check_rows("fp8_quantize", rows, cols, {{input, bytes}}, nullptr, codes, scales, {nullptr, 0}, block_rows);
   if (rc) return rc;
   if (rows == 0) return UQM_OK;
   if (input == nullptr) return fail(UQM_ERR_ARGUMENT, "fp8_quantize: input is required");

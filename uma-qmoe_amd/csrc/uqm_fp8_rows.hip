@@ -17,33 +17,50 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kFp8Max = 448.0f;
 
-// Columns c .. c+7 of a row as FP32, zeros from `cols` on.
+// 16 and 8 bytes at any alignment of their elements: one access each (the memory
+// takes them at twice the cost or less; one per element was 3 to 4 times slower, 4000
+// rows of 5475 with both outputs 118.6 us).
+typedef uint32_t loose16_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t loose8_t __attribute__((ext_vector_type(2), aligned(1)));
+
+// Columns c .. c+7 of a row as FP32, zeros from `cols` on. VEC: rows of a multiple
+// of 8 columns, aligned.
 template <bool VEC>
 __device__ __forceinline__ void load8(const uint16_t* row, int64_t c, int64_t cols, float (&v)[8]) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
   if constexpr (VEC) {
-    const uint4 q = c < cols ? ldg16(row + c) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = bf16lo(w[j]);
-      v[2 * j + 1] = bf16hi(w[j]);
+    if (c < cols) {
+      const uint4 q = ldg16(row + c);
+      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
     }
+  } else if (c + 8 <= cols) {
+    const loose16_t q = *reinterpret_cast<const loose16_t*>(row + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = q[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? bf16_to_f32(row[c + j]) : 0.f;
+    for (int j = 0; j < 7; ++j)
+      if (c + j < cols) w[j / 2] |= static_cast<uint32_t>(row[c + j]) << (16 * (j & 1));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = bf16lo(w[j]);
+    v[2 * j + 1] = bf16hi(w[j]);
   }
 }
 
 template <bool VEC>
 __device__ __forceinline__ void store8_bf16(uint16_t* row, int64_t c, int64_t cols, const float (&v)[8]) {
+  const uint32_t w[4] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                         pack_bf16x2(v[6], v[7])};
   if constexpr (VEC) {
-    if (c < cols)
-      *reinterpret_cast<uint4*>(row + c) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                      pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    if (c < cols) *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if (c + 8 <= cols) {
+    *reinterpret_cast<loose16_t*>(row + c) = loose16_t{w[0], w[1], w[2], w[3]};
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < cols) row[c + j] = f32_to_bf16(v[j]);
+    for (int j = 0; j < 7; ++j)
+      if (c + j < cols) row[c + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
   }
 }
 
@@ -59,9 +76,11 @@ __device__ __forceinline__ void store8_fp8(uint8_t* row, int64_t c, int64_t cols
   const uint32_t hi = pack_fp8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
   if constexpr (VEC) {
     if (c < cols) *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+  } else if (c + 8 <= cols) {
+    *reinterpret_cast<loose8_t*>(row + c) = loose8_t{lo, hi};
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 7; ++j)
       if (c + j < cols) row[c + j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
   }
 }
@@ -93,11 +112,11 @@ __device__ __forceinline__ float scale_of(uint32_t bits) {
 // Codes and scale of the group that this lane's 8 columns belong to.
 template <bool VEC>
 __device__ __forceinline__ void write_fp8(const RowOutputs& out, int64_t row, int64_t c, int64_t cols,
-                                          const float (&v)[8]) {
+                                          int64_t all_cols, const float (&v)[8]) {
   const float d = scale_of(group_max(magnitude8(v)));
-  store8_fp8<VEC>(out.codes + row * cols, c, cols, v, 1.0f / d);
+  store8_fp8<VEC>(out.codes + row * all_cols, c, cols, v, 1.0f / d);
   if ((threadIdx.x & 15u) == 0 && c < cols)
-    out.scales[row * ((cols + kFp8Group - 1) / kFp8Group) + c / kFp8Group] = d;
+    out.scales[row * ((all_cols + kFp8Group - 1) / kFp8Group) + c / kFp8Group] = d;
 }
 
 // Sum over the workgroup of 4 waves.
@@ -108,17 +127,20 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return part[0] + part[1] + part[2] + part[3];
 }
 
-// One workgroup per row. Rows beyond 8 * kThreads * PASSES columns are read
+// LANES lanes per row: 16 for rows of a group, 64 (a wave, no barrier) up to 512
+// columns, a workgroup beyond. Rows beyond 8 * kThreads * PASSES columns are read
 // again in the second part (PASSES 0), each thread its own columns: the sum from
 // where it wrote it.
-template <int PASSES, bool VEC>
-__global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const uint16_t* x, const uint16_t* r, int64_t cols,
-                                                               const uint16_t* __restrict__ weight, float eps,
-                                                               uint16_t* sum, RowOutputs out) {
+template <int LANES, int PASSES, bool VEC>
+__global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const uint16_t* x, const uint16_t* r, int64_t rows,
+                                                               int64_t all_cols, const uint16_t* __restrict__ weight,
+                                                               float eps, uint16_t* sum, RowOutputs out) {
   __shared__ float part[kThreads / 64];
-  const int64_t row = blockIdx.x;
-  const int64_t at = row * cols;
-  const int64_t first = 8 * threadIdx.x;  // this thread's columns of pass p: first + 8 * kThreads * p
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / LANES) + threadIdx.x / LANES;
+  // (lanes behind the last row stay, with no columns: a wave's exchanges take them all)
+  const int64_t cols = row < rows ? all_cols : 0;
+  const int64_t at = row * all_cols;
+  const int64_t first = 8 * (threadIdx.x % LANES);  // this thread's columns of pass p: first + 8 * LANES * p
   auto load = [&](int64_t c, float (&s)[8]) {  // s = bf16(x + r), kept in `sum`
     load8<VEC>(x + at, c, cols, s);
     if (r != nullptr) {
@@ -142,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const uint16_t* x
     if (out.codes != nullptr) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = w[j] * (s[j] * rstd);
-      write_fp8<VEC>(out, row, c, cols, y);
+      write_fp8<VEC>(out, row, c, cols, all_cols, y);
     }
   };
   float ss = 0.f;
@@ -150,17 +172,28 @@ __global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const uint16_t* x
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = fmaf(s[j], s[j], ss);
   };
-  auto rstd = [&]() { return rsqrtf(block_sum(ss, part) / static_cast<float>(cols) + eps); };
+  auto rstd = [&]() {
+    if constexpr (LANES == 16) {
+      ss += xor_partner<8>(ss);
+      ss += xor_partner<4>(ss);
+      ss += xor_partner<2>(ss);
+      ss += xor_partner<1>(ss);
+    } else {
+      ss = LANES == 64 ? wave_sum(ss) : block_sum(ss, part);
+    }
+    return rsqrtf(ss / static_cast<float>(all_cols) + eps);
+  };
   if constexpr (PASSES > 0) {
     float v[PASSES][8];
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) load(first + 8 * kThreads * p, v[p]);
+    for (int p = 0; p < PASSES; ++p) load(first + 8 * LANES * p, v[p]);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) add(v[p]);
     const float f = rstd();
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) finish(first + 8 * kThreads * p, v[p], f);
+    for (int p = 0; p < PASSES; ++p) finish(first + 8 * LANES * p, v[p], f);
   } else {
+    static_assert(LANES == kThreads, "a workgroup per row");
     // (rounds in whole workgroups, so that a group's 16 lanes stay together)
     const int64_t rounds = (cols + 8 * kThreads - 1) / (8 * kThreads);
     float s[8];
@@ -199,6 +232,28 @@ int64_t place_grid(int64_t rows, int64_t chunks) {
 }
 __host__ __device__ int64_t chunks_of(int64_t cols) { return (cols + kFp8Group - 1) / kFp8Group * (kFp8Group / 8); }
 
+// g / (1 + exp(-g)): the reciprocal with one Newton step, as near as the division
+// at half its instructions. It flushes subnormal results to 0, so a wave with a
+// gate below -87.3 (1 + exp(-g) from 2^126 on) divides.
+__device__ __forceinline__ void silu8(float (&g)[8]) {
+  float d[8], most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    d[j] = 1.0f + __expf(-g[j]);
+    most = fmaxf(most, d[j]);
+  }
+  if (__builtin_expect(__any(most > 0x1p126f), 0)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] /= d[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = __builtin_amdgcn_rcpf(d[j]);
+      g[j] *= fmaf(fmaf(-d[j], r, 1.0f), r, r);
+    }
+  }
+}
+
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void silu_mul_kernel(const uint16_t* __restrict__ x, int64_t rows, int64_t cols,
                                                             RowOutputs out) {
@@ -208,10 +263,11 @@ __global__ __launch_bounds__(kThreads) void silu_mul_kernel(const uint16_t* __re
   float g[8], u[8];
   load8<VEC>(g_row, at.c, cols, g);
   load8<VEC>(g_row + cols, at.c, cols, u);
+  silu8(g);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) g[j] = silu(g[j]) * u[j];
+  for (int j = 0; j < 8; ++j) g[j] *= u[j];
   if (out.bf16 != nullptr) store8_bf16<VEC>(out.bf16 + at.row * cols, at.c, cols, g);
-  if (out.codes != nullptr) write_fp8<VEC>(out, at.row, at.c, cols, g);
+  if (out.codes != nullptr) write_fp8<VEC>(out, at.row, at.c, cols, cols, g);
 }
 
 template <bool VEC>
@@ -221,7 +277,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const uint16_t*
   if (at.row >= rows) return;
   float v[8];
   load8<VEC>(x + at.row * cols, at.c, cols, v);
-  write_fp8<VEC>(out, at.row, at.c, cols, v);
+  write_fp8<VEC>(out, at.row, at.c, cols, cols, v);
 }
 
 // One workgroup per 128 x 128 block: 16 lanes a row of it, 16 rows at a time, all
@@ -271,12 +327,17 @@ hipError_t launch_add_rmsnorm(const uint16_t* x, const uint16_t* r, int64_t rows
   if (rows > kMaxGrid) return hipErrorInvalidValue;
   const bool vec = aligned(cols, {x, r, weight, sum, out.bf16}, out.codes);
   const int64_t passes = (cols + 8 * kThreads - 1) / (8 * kThreads);
-  auto* k = passes <= 1   ? (vec ? add_rmsnorm_kernel<1, true> : add_rmsnorm_kernel<1, false>)
-            : passes <= 2 ? (vec ? add_rmsnorm_kernel<2, true> : add_rmsnorm_kernel<2, false>)
-            : passes <= 4 ? (vec ? add_rmsnorm_kernel<4, true> : add_rmsnorm_kernel<4, false>)
-                          : (vec ? add_rmsnorm_kernel<0, true> : add_rmsnorm_kernel<0, false>);
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, stream, x, r, cols, weight, eps, sum,
-                     out);
+  const int lanes = cols <= kFp8Group ? 16 : cols <= 512 ? 64 : kThreads;
+  auto* k = lanes == 16   ? (vec ? add_rmsnorm_kernel<16, 1, true> : add_rmsnorm_kernel<16, 1, false>)
+            : lanes == 64 ? (vec ? add_rmsnorm_kernel<64, 1, true> : add_rmsnorm_kernel<64, 1, false>)
+            : passes <= 1 ? (vec ? add_rmsnorm_kernel<kThreads, 1, true> : add_rmsnorm_kernel<kThreads, 1, false>)
+            : passes <= 2 ? (vec ? add_rmsnorm_kernel<kThreads, 2, true> : add_rmsnorm_kernel<kThreads, 2, false>)
+            : passes <= 3 ? (vec ? add_rmsnorm_kernel<kThreads, 3, true> : add_rmsnorm_kernel<kThreads, 3, false>)
+            : passes <= 4 ? (vec ? add_rmsnorm_kernel<kThreads, 4, true> : add_rmsnorm_kernel<kThreads, 4, false>)
+                          : (vec ? add_rmsnorm_kernel<kThreads, 0, true> : add_rmsnorm_kernel<kThreads, 0, false>);
+  const int64_t per = kThreads / lanes;
+  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kThreads), 0, stream, x, r, rows, cols,
+                     weight, eps, sum, out);
   return hipGetLastError();
 }
 

@@ -28,7 +28,7 @@ from dataclasses import dataclass
 import hashlib
 from pathlib import Path
 import threading
-from typing import Any
+from typing import Any, NamedTuple
 
 from . import _native
 from .build import CSRC
@@ -141,8 +141,7 @@ class DenseBlock:
         return self.shared_gate is not None
 
 
-@dataclass(frozen=True)
-class Fp8Matrix:
+class Fp8Matrix(NamedTuple):
     """A matrix in 8-bit floats: ``codes`` float8_e4m3fn [..., cols] and
     ``scales`` float32, one per ``block_rows`` x 128 block (value = code *
     scale). Activations have blocks of one row (scales [..., ceil(cols / 128)]),
@@ -440,28 +439,29 @@ class HipExtension:
         return out.reshape(hidden.shape)
 
     # ------------------------------------------- 8-bit floats with scales --
-    # (A call of few rows takes as long on the host as on the GPU: the checks
-    # below cost 1 to 2 us a call, an allocation 1.3, the launch 3.)
+    # (A call of few rows takes longer on the host than on the GPU, so what a
+    # call checks is kept short: one condition where all is well, and the words
+    # for a refusal only behind it.)
     def _launch(self, fn, index, *args):
         """Calls entry point ``fn`` on the current stream of device ``index``,
         which is made current if it is not."""
-        torch = self.torch
-        if torch._C._cuda_getDevice() == index:
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        c = self.torch._C
+        if c._cuda_getDevice() == index:
+            rc = fn(*args, c._cuda_getCurrentRawStream(index))
         else:
-            with torch.cuda.device(index):
-                rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            with self.torch.cuda.device(index):
+                rc = fn(*args, c._cuda_getCurrentRawStream(index))
         if rc:
             _native.check(rc, fn.__name__)
 
-    def _rows_of(self, x, what):
-        """(contiguous x, its device's index, rows, columns) of a BF16 tensor [..., columns]."""
+    def _columns(self, x, what):
+        """Columns of a BF16 device tensor [..., columns]."""
         if x.dtype is not self.torch.bfloat16:
             raise RuntimeError(f"{what} requires BF16 tensors")
         cols = x.shape[-1] if x.ndim else 0
         if cols == 0:
             raise RuntimeError(f"{what} requires a tensor with at least one column")
-        return x.contiguous(), x.get_device(), x.numel() // cols, cols
+        return cols
 
     @staticmethod
     def _check_devices(what, index, *others):
@@ -478,7 +478,8 @@ class HipExtension:
         Without a residual s is ``hidden`` itself. ``inplace`` writes s over
         ``residual``."""
         torch = self.torch
-        x, index, rows, cols = self._rows_of(hidden, "add_rmsnorm")
+        cols = self._columns(hidden, "add_rmsnorm")
+        x, index = hidden.contiguous(), hidden.get_device()
         if not (bf16 or fp8):
             raise RuntimeError("add_rmsnorm requires at least one of bf16 and fp8")
         r = total = out = q = None
@@ -491,7 +492,7 @@ class HipExtension:
         elif inplace:
             raise RuntimeError("add_rmsnorm(inplace=True) requires a residual")
         if weight is not None:
-            if weight.dtype is not torch.bfloat16 or weight.ndim != 1 or weight.shape[0] != cols:
+            if weight.dtype is not torch.bfloat16 or weight.shape != (cols,):
                 raise RuntimeError(f"add_rmsnorm requires a BF16 weight [{cols}]")
             weight = weight.contiguous()
         self._check_devices("add_rmsnorm", index, r, weight)
@@ -502,15 +503,16 @@ class HipExtension:
         if fp8:
             q = Fp8Matrix(torch.empty_like(x, dtype=torch.float8_e4m3fn),
                           torch.empty(*x.shape[:-1], -(-cols // FP8_GROUP), dtype=torch.float32, device=x.device))
-        self._launch(self.lib.uqm_add_rmsnorm, index, x.data_ptr(), _ptr(r), rows, cols, _ptr(weight), eps,
-                     _ptr(total), _ptr(out), q and q.codes.data_ptr(), q and q.scales.data_ptr())
+        self._launch(self.lib.uqm_add_rmsnorm, index, x.data_ptr(), _ptr(r), x.numel() // cols, cols, _ptr(weight),
+                     eps, _ptr(total), _ptr(out), q and q.codes.data_ptr(), q and q.scales.data_ptr())
         return (hidden if total is None else total), out, q
 
     def silu_mul(self, gate_up, *, bf16=True, fp8=False):
         """silu(gate) * up of ``gate_up`` [..., 2 * features] (gate first):
         (BF16 [..., features] or None, ``Fp8Matrix`` or None)."""
         torch = self.torch
-        x, index, rows, cols = self._rows_of(gate_up, "silu_mul")
+        cols = self._columns(gate_up, "silu_mul")
+        x, index = gate_up.contiguous(), gate_up.get_device()
         if not (bf16 or fp8):
             raise RuntimeError("silu_mul requires at least one of bf16 and fp8")
         if cols % 2:
@@ -522,7 +524,7 @@ class HipExtension:
         if fp8:
             q = Fp8Matrix(torch.empty(*lead, features, dtype=torch.float8_e4m3fn, device=device),
                           torch.empty(*lead, -(-features // FP8_GROUP), dtype=torch.float32, device=device))
-        self._launch(self.lib.uqm_silu_mul, index, x.data_ptr(), rows, features, _ptr(out),
+        self._launch(self.lib.uqm_silu_mul, index, x.data_ptr(), x.numel() // cols, features, _ptr(out),
                      q and q.codes.data_ptr(), q and q.scales.data_ptr())
         return out, q
 
@@ -530,7 +532,9 @@ class HipExtension:
         """``x`` (BF16) as an ``Fp8Matrix``: ``block_rows`` 1 for activations
         [..., cols], 128 for a weight [rows, cols]."""
         torch = self.torch
-        x, index, rows, cols = self._rows_of(x, "fp8_quantize")
+        cols = self._columns(x, "fp8_quantize")
+        x, index = x.contiguous(), x.get_device()
+        rows = x.numel() // cols
         if block_rows == 1:
             lead = x.shape[:-1]
         elif block_rows != FP8_GROUP:
@@ -547,18 +551,32 @@ class HipExtension:
         return Fp8Matrix(codes, scales, block_rows)
 
     def _check_fp8(self, m, block_rows, what):
+        """The words of a refusal of an ``Fp8Matrix``."""
         torch = self.torch
-        codes, scales = m.codes, m.scales
-        if m.block_rows != block_rows:
+        codes, scales, block = m
+        if block != block_rows:
             raise RuntimeError(f"fp8_linear requires {what} in blocks of {block_rows} x {FP8_GROUP}")
         if codes.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32:
             raise RuntimeError(f"fp8_linear requires {what} as float8_e4m3fn codes and float32 scales")
         shape = codes.shape
-        groups = -(-shape[-1] // FP8_GROUP)
-        want = (*shape[:-1], groups) if block_rows == 1 else (-(-shape[0] // block_rows), groups)
+        lead = shape[:-1] if block_rows == 1 else (-(-shape[0] // block_rows),)
+        want = (*lead, -(-shape[-1] // FP8_GROUP))
         if scales.shape != want:
             raise RuntimeError(f"fp8_linear: {what} of shape {tuple(shape)} need scales {want}, not {tuple(scales.shape)}")
-        return codes.contiguous(), scales.contiguous()
+
+    def _check_linear(self, x, weight, bias):
+        """The words of a refusal of fp8_linear's operands."""
+        if weight.codes.ndim != 2:
+            raise RuntimeError("fp8_linear requires a weight matrix")
+        n, k = weight.shape
+        if n == 0 or k == 0 or k % 16:
+            raise RuntimeError(f"fp8_linear requires a weight of at least one row and a multiple of 16 columns, not {n} x {k}")
+        if x.codes.ndim < 1 or x.shape[-1] != k:
+            raise RuntimeError(f"fp8_linear requires {k} input features")
+        self._check_fp8(weight, FP8_GROUP, "weights")
+        self._check_fp8(x, 1, "activations")
+        if bias is not None and (bias.dtype is not self.torch.bfloat16 or bias.shape != (n,)):
+            raise RuntimeError(f"fp8_linear requires a BF16 bias [{n}]")
 
     def fp8_linear(self, x, weight: Fp8Matrix, bias=None):
         """BF16 [..., out_features] = x @ weight^T + bias in FP32 sums. ``x`` is
@@ -566,27 +584,30 @@ class HipExtension:
         first; ``weight`` an ``Fp8Matrix`` [out_features, in_features] in blocks
         of 128 x 128, in_features a multiple of 16; ``bias`` BF16."""
         torch = self.torch
-        if weight.codes.ndim != 2:
-            raise RuntimeError("fp8_linear requires a weight matrix")
-        w, ws = self._check_fp8(weight, FP8_GROUP, "weights")
-        n, k = w.shape
-        if n == 0 or k == 0 or k % 16:
-            raise RuntimeError(f"fp8_linear requires a weight of at least one row and a multiple of 16 columns, not {n} x {k}")
-        ndim = x.codes.ndim if isinstance(x, Fp8Matrix) else x.ndim
-        if ndim < 1 or x.shape[-1] != k:
-            raise RuntimeError(f"fp8_linear requires {k} input features")
+        f8, f32 = torch.float8_e4m3fn, torch.float32
         if not isinstance(x, Fp8Matrix):
+            if x.ndim < 1 or x.shape[-1] != weight.shape[-1]:
+                raise RuntimeError(f"fp8_linear requires {weight.shape[-1]} input features")
             x = self.fp8_quantize(x)
-        codes, scales = self._check_fp8(x, 1, "activations")
-        if bias is not None:
-            if bias.dtype is not torch.bfloat16 or bias.ndim != 1 or bias.shape[0] != n:
-                raise RuntimeError(f"fp8_linear requires a BF16 bias [{n}]")
-            bias = bias.contiguous()
+        codes, scales, block = x
+        w, ws, w_block = weight
+        shape, w_shape = codes.shape, w.shape
+        n, k = w_shape if len(w_shape) == 2 else (0, 0)
+        groups = -(-k // FP8_GROUP)
+        if not (n > 0 and k > 0 and k % 16 == 0 and block == 1 and w_block == FP8_GROUP and len(shape) > 0
+                and shape[-1] == k and codes.dtype is f8 and w.dtype is f8 and scales.dtype is f32 and ws.dtype is f32
+                and ws.shape == (-(-n // FP8_GROUP), groups)
+                and scales.shape == ((shape[0], groups) if len(shape) == 2 else (*shape[:-1], groups))
+                and (bias is None or bias.dtype is torch.bfloat16 and bias.shape == (n,))):
+            self._check_linear(x, weight, bias)
         index = codes.get_device()
         self._check_devices("fp8_linear", index, scales, w, ws, bias)
-        out = torch.empty(*codes.shape[:-1], n, dtype=torch.bfloat16, device=codes.device)
+        codes, scales, w, ws = codes.contiguous(), scales.contiguous(), w.contiguous(), ws.contiguous()
+        if bias is not None:
+            bias = bias.contiguous()
+        out = torch.empty(*shape[:-1], n, dtype=torch.bfloat16, device=codes.device)
         self._launch(self.lib.uqm_fp8_linear, index, codes.data_ptr(), scales.data_ptr(), codes.numel() // k,
-                     w.data_ptr(), ws.data_ptr(), n, k, _ptr(bias), out.data_ptr())
+                     w.data_ptr(), ws.data_ptr(), n, k, bias if bias is None else bias.data_ptr(), out.data_ptr())
         return out
 
     # ------------------------------------- reference binding signatures --
