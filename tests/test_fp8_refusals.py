@@ -81,7 +81,7 @@ def test_fp8_quantize(lib, args, words):
     ((A, B, 4, C, D, 0, 128, None, E), "features"),
     ((A, B, 4, C, D, 64, 0, None, E), "multiple of 16"),
     ((A, B, 4, C, D, 64, 120, None, E), "multiple of 16"),
-    ((A, B, 4, C, D, 64, 1 << 26, None, E), "below 2^26"),
+    ((A, B, 4, C, D, 64, 1 << 25, None, E), "below 2^25"),
     ((A, B, 4, None, D, 64, 128, None, E), "required"),
     ((A, B, 4, C, None, 64, 128, None, E), "required"),
     ((None, B, 4, C, D, 64, 128, None, E), "required"),

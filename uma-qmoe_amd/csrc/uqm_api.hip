@@ -1414,7 +1414,7 @@ int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const v
   if (rows < 0 || rows > kMaxExtent || out_features <= 0 || out_features > kMaxExtent)
     return fail(UQM_ERR_ARGUMENT, "fp8_linear: rows must be in [0, 2^31) and features in [1, 2^31)");
   if (in_features <= 0 || in_features % 16 != 0 || in_features >= kFp8MaxK)
-    return fail(UQM_ERR_ARGUMENT, "fp8_linear: input features %lld must be a positive multiple of 16 below 2^26", (long long)in_features);
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: input features %lld must be a positive multiple of 16 below 2^25", (long long)in_features);
   if (weight_codes == nullptr || weight_scales == nullptr)
     return fail(UQM_ERR_ARGUMENT, "fp8_linear: weight codes and scales are required");
   if (misaligned(weight_codes, 16) || misaligned(weight_scales, 4) || misaligned(bias, 2))

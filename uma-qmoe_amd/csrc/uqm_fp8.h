@@ -39,7 +39,7 @@ hipError_t launch_fp8_quantize(const uint16_t* x, int64_t rows, int64_t cols, in
 
 // out[t, n] = bf16(bias[n] + sum over blocks b of 128 columns of
 //                  xs[t, b] ws[n / 128, b] sum over k in b of x[t, k] w[n, k])
-constexpr int64_t kFp8MaxK = int64_t{1} << 26;  // 64 rows within 32 bits
+constexpr int64_t kFp8MaxK = int64_t{1} << 25;  // 64 rows below 2^31 bytes
 struct Fp8LinearArgs {
   const uint8_t* x;       // codes [T, K]
   const float* xs;        // scales [T, ceil(K / 128)]

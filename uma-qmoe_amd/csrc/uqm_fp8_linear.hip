@@ -41,9 +41,6 @@ __device__ __forceinline__ void reads_follow() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// What stands in the place of columns behind the last.
-__device__ __align__(16) const uint8_t kZeroPiece[16] = {};
-
 // Position of a row's 16-byte piece p in LDS is p ^ ((row >> 1) & 7): the LDS
 // serves a 16-byte read of 64 lanes in four turns of 16 rows, 256 bytes each, rows
 // 0-3 and 12-15 from one quadrant of lanes and rows 4-11 from its neighbour; two
@@ -59,31 +56,36 @@ __device__ __forceinline__ int weight_position(int piece, int row) {
   return piece ^ (((row >> 1) & 1) | ((row >> 2) & 6));
 }
 
+constexpr uint32_t kOutside = 0x80000000u;  // an offset behind every buffer's bytes
+constexpr int kScaleBlocks = 8;             // blocks whose scales are loaded together
+
 // ---------------------------------------------------------------- split --
 // Few tokens: 16 * TN weight rows x 16 * TT tokens per workgroup, the column
-// blocks dealt out to its W waves. Each wave loads its blocks into a ring of its
-// own in LDS, S blocks ahead, and waits for nobody until the sums of all waves are
-// added, in wave order.
-template <int TN, int TT, int W, int S>
+// blocks split over its W waves. Each wave loads its blocks into a place of its
+// own in LDS, the next one while it multiplies, and waits for nobody until the
+// sums of all waves are added, in wave order.
+// The address unit bounds it (64 bytes a cycle, 16 cycles a load): 512 x 2048 x
+// 5632 is 704 KB a CU, 5 us. The scales therefore come for 8 blocks at a time, 32
+// bytes of 8 tokens a load: a load per block took 64 cache lines each time.
+template <int TN, int TT, int W>
 struct Split {
   static constexpr int kBlock = (TN + TT) * 16 * kFp8Group;  // bytes of a block's operands
-  static constexpr int kStage = kBlock + 512;                // ... and the scales of tokens and rows (64 floats each)
-  static constexpr int kRing = S * kStage;                   // of a wave
-  static constexpr int kLds = W * kRing;
-  static constexpr int kLoads = 2 * (TN + TT) + 2;           // per block
-  static_assert(kRing >= TN * TT * 1024, "a wave's sums take its ring's place");
-  static_assert((S - 1) * kLoads <= 63 && kLds <= 160 * 1024, "");
+  static constexpr int kScales = 2 * TT * 256 + 256;         // of 8 blocks: tokens, then the row block
+  static constexpr int kSums = TN * TT * 1024;               // of a wave, in its operands' place
+  static constexpr int kPlace = kBlock + kScales > kSums ? kBlock + kScales : kSums;
+  static constexpr int kLds = W * kPlace;
+  static_assert(kLds <= 160 * 1024, "");
 };
 
-template <int TN, int TT, int W, int S>
+template <int TN, int TT, int W>
 __global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int blocks_n, int blocks_t) {
-  using G = Split<TN, TT, W, S>;
+  using G = Split<TN, TT, W>;
   extern __shared__ __align__(16) unsigned char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int q = lane >> 4, r = lane & 15;
-  const uint32_t ring = wave * G::kRing;
-  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((stage_lds_t*)(lds))) + ring;
+  const uint32_t place = wave * G::kPlace;
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((stage_lds_t*)(lds))) + place;
   // (8 contiguous ranges of workgroups, one per XCD; token blocks of the same rows
   // next to each other)
   const int64_t n_items = static_cast<int64_t>(blocks_n) * blocks_t;
@@ -96,31 +98,38 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int 
   const int last_t = static_cast<int>(min(a.T - t0, static_cast<int64_t>(16 * TT))) - 1;
   const uint32_t K = static_cast<uint32_t>(a.K);
   const int KB = static_cast<int>((a.K + kFp8Group - 1) / kFp8Group);
-  const int mine = KB > wave ? (KB - wave + W - 1) / W : 0;
+  const int first = static_cast<int>(static_cast<int64_t>(KB) * wave / W);
+  const int mine = static_cast<int>(static_cast<int64_t>(KB) * (wave + 1) / W) - first;
 
-  // ---- loads of this wave's i-th block: 8 rows at a time, then the scales
-  const uint8_t* zeros = kZeroPiece;
-  const uint8_t *wsrc = a.w + n0 * a.K, *xsrc = a.x + t0 * a.K;
-  const float* xs = a.xs + (t0 + min(lane, last_t)) * KB;
-  const float* ws = a.ws + n0 / kFp8Group * KB;
-  auto issue = [&](int i, int slot) {
-    const int b = wave + i * W;
-    const bool in = i < mine;
-    const uint32_t limit = in ? K - static_cast<uint32_t>(b) * kFp8Group : 0u;
-    const uint32_t to = lds_base + slot * G::kStage;
+  // ---- loads of this wave's i-th block, 8 rows at a time: rows and tokens behind
+  // the last, and columns behind the last, lie outside the buffers and read as zeros
+  const auto wbuf = stage_buffer(a.w + n0 * a.K, static_cast<uint32_t>(last_n + 1) * K);
+  const auto xbuf = stage_buffer(a.x + t0 * a.K, static_cast<uint32_t>(last_t + 1) * K);
+  const auto sbuf = stage_buffer(a.xs + t0 * KB, static_cast<uint32_t>(last_t + 1) * (4u * KB));
+  const auto rbuf = stage_buffer(a.ws + n0 / kFp8Group * KB, 4u * KB);
+  auto column = [&](int j) {
+    const bool weight = j < 2 * TN;
+    const int row = 8 * (weight ? j : j - 2 * TN) + (lane >> 3);
+    return 16u * static_cast<uint32_t>(weight && TN > 1 ? weight_position(lane & 7, row) : token_position(lane & 7, row));
+  };
+  uint32_t off[2 * (TN + TT)];
 #pragma unroll
-    for (int j = 0; j < 2 * (TN + TT); ++j) {
-      const bool weight = j < 2 * TN;
-      const int row = 8 * (weight ? j : j - 2 * TN) + (lane >> 3);
-      const uint32_t column =
-          16u * static_cast<uint32_t>(weight && TN > 1 ? weight_position(lane & 7, row) : token_position(lane & 7, row));
-      const uint8_t* from = (weight ? wsrc : xsrc) + (static_cast<uint32_t>(min(row, weight ? last_n : last_t)) * K +
-                                                      static_cast<uint32_t>(b) * kFp8Group + column);
-      dma16_to(column < limit ? from : zeros, __builtin_amdgcn_readfirstlane(to + j * (8 * kFp8Group)));
+  for (int j = 0; j < 2 * (TN + TT); ++j)
+    off[j] = static_cast<uint32_t>(8 * (j < 2 * TN ? j : j - 2 * TN) + (lane >> 3)) * K + column(j);
+  auto issue = [&](int i) {
+    const uint32_t b = first + i;
+    if (i % kScaleBlocks == 0) {
+#pragma unroll
+      for (int j = 0; j < 2 * TT; ++j)
+        buffer4_to(sbuf, 4u * static_cast<uint32_t>((8 * j + (lane >> 3)) * KB + (lane & 7)), 4u * b,
+                   __builtin_amdgcn_readfirstlane(lds_base + G::kBlock + 256 * j));
+      buffer4_to(rbuf, 4u * (lane & 7), 4u * b, __builtin_amdgcn_readfirstlane(lds_base + G::kBlock + 512 * TT));
     }
-    const int sb = min(b, KB - 1);
-    dma4_to(xs + sb, __builtin_amdgcn_readfirstlane(to + G::kBlock));
-    dma4_to(ws + sb, __builtin_amdgcn_readfirstlane(to + G::kBlock + 256));
+    const uint32_t limit = K - b * kFp8Group;
+#pragma unroll
+    for (int j = 0; j < 2 * (TN + TT); ++j)
+      buffer16_to(j < 2 * TN ? wbuf : xbuf, column(j) < limit ? off[j] : kOutside, b * kFp8Group,
+                  __builtin_amdgcn_readfirstlane(lds_base + j * (8 * kFp8Group)));
   };
 
   const int w_row = TN > 1 ? 8 * (r >> 2) + (r & 3) : r;
@@ -135,13 +144,11 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int 
   for (int n = 0; n < TN; ++n)
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[n][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < S; ++i) issue(i, i);
-  int slot = 0;
+  if (mine > 0) issue(0);
   for (int i = 0; i < mine; ++i) {
-    wait_loads<(S - 1) * G::kLoads>();
+    wait_loads<0>();
     reads_follow();
-    const unsigned char* at = lds + ring + slot * G::kStage;
+    const unsigned char* at = lds + place;
     i32x8_t w[TN], x[TT];
 #pragma unroll
     for (int n = 0; n < TN; ++n) {
@@ -154,14 +161,14 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int 
       x[t] = operand(load16(p + x0), load16(p + x1));
     }
     float f[TT];
-    const float* sc = reinterpret_cast<const float*>(at + G::kBlock);
-    const float fw = sc[64];
+    const float* sc = reinterpret_cast<const float*>(at + G::kBlock) + i % kScaleBlocks;
+    const float fw = sc[128 * TT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) f[t] = fw * sc[16 * t + r];
-    // the reads are done: the block's place takes the one S further on
+    for (int t = 0; t < TT; ++t) f[t] = fw * sc[8 * (16 * t + r)];
+    // the reads are done: the block's place takes the next one
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-    __builtin_amdgcn_sched_barrier(0);
-    issue(i + S, slot);
+    reads_follow();
+    if (i + 1 < mine) issue(i + 1);
 #pragma unroll
     for (int n = 0; n < TN; ++n)
 #pragma unroll
@@ -170,16 +177,13 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int 
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][t][e] = fmaf(f[t], d[e], acc[n][t][e]);
       }
-    slot = slot + 1 == S ? 0 : slot + 1;
   }
 
   // ---- sums of the waves
-  wait_loads<0>();
-  reads_follow();
 #pragma unroll
   for (int n = 0; n < TN; ++n)
 #pragma unroll
-    for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4_t*>(lds + ring + (n * TT + t) * 1024 + 16 * lane) = acc[n][t];
+    for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4_t*>(lds + place + (n * TT + t) * 1024 + 16 * lane) = acc[n][t];
   __syncthreads();
   constexpr int kPair = TN > 1 ? 2 : 1;  // tiles whose rows a thread puts together
   const bool vec = a.N % (4 * kPair) == 0 && (reinterpret_cast<uintptr_t>(a.out) & (8u * kPair - 1)) == 0;
@@ -191,7 +195,7 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int 
       const unsigned char* from = lds + ((n + p) * TT + t) * 1024 + 16 * l;
       v[p] = *reinterpret_cast<const f32x4_t*>(from);
 #pragma unroll
-      for (int g = 1; g < W; ++g) v[p] += *reinterpret_cast<const f32x4_t*>(from + g * G::kRing);
+      for (int g = 1; g < W; ++g) v[p] += *reinterpret_cast<const f32x4_t*>(from + g * G::kPlace);
     }
     const int tok = 16 * t + (l & 15);
     const int64_t row = n0 + 16 * n + 4 * kPair * (l >> 4);
@@ -219,13 +223,13 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(Fp8LinearArgs a, int 
   }
 }
 
-template <int TN, int TT, int W, int S>
+template <int TN, int TT, int W>
 hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
-  using G = Split<TN, TT, W, S>;
+  using G = Split<TN, TT, W>;
   const int64_t blocks_n = (a.N + 16 * TN - 1) / (16 * TN), blocks_t = (a.T + 16 * TT - 1) / (16 * TT);
   if (blocks_n * blocks_t > 0x7FFFFFF) return hipErrorInvalidValue;
   const int64_t grid = (blocks_n * blocks_t + 7) / 8 * 8;
-  auto* k = fp8_split_kernel<TN, TT, W, S>;
+  auto* k = fp8_split_kernel<TN, TT, W>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
   if (e != hipSuccess) return e;
@@ -238,8 +242,6 @@ hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
 // Many tokens: 16 * TN * WN weight rows x 16 * TT * WT tokens per workgroup of
 // WN x WT waves, the column blocks in a ring of two stages in LDS (rows of 128
 // bytes, loaded by the address unit straight into LDS).
-constexpr int kScaleBlocks = 8;
-constexpr uint32_t kOutside = 0x80000000u;       // an offset behind every tile's bytes
 constexpr int64_t kFp8TileMaxK = int64_t{1} << 23;  // 256 rows of fewer bytes stay below it
 
 template <int TN, int TT, int WN, int WT>
@@ -502,14 +504,16 @@ struct Kernel {
   hipError_t (*launch)(const Fp8LinearArgs&, hipStream_t);
 };
 constexpr Kernel kKernels[] = {
-    {16, 16, 4, 1.99f, 1.35f, 0.209f, 0.018f, launch_split<1, 1, 8, 1>},
-    {32, 32, 2, 2.19f, 1.59f, 0.225f, 0.050f, launch_split<2, 2, 8, 1>},
-    {64, 32, 1, 2.19f, 2.01f, 0.173f, 0.106f, launch_split<4, 2, 8, 1>},
-    {64, 64, 1, 2.30f, 2.58f, 0.268f, 0.162f, launch_split<4, 4, 8, 1>},
-    {128, 64, 2, 2.18f, 1.67f, 0.728f, 0.502f, launch_tiles<4, 2, 2, 2>},
-    {128, 128, 2, 0.32f, 4.00f, 1.148f, 0.527f, launch_tiles<4, 2, 2, 4>},
-    {128, 256, 1, 0.70f, 4.73f, 1.021f, 0.778f, launch_tiles<4, 4, 2, 4>},
-    {256, 256, 1, 1.49f, 7.46f, 1.531f, 0.992f, launch_tiles<8, 4, 2, 4>},
+    {16, 16, 8, 1.48f, 1.28f, 0.323f, 0.044f, launch_split<1, 1, 4>},
+    {16, 16, 4, 1.94f, 1.01f, 0.182f, 0.015f, launch_split<1, 1, 8>},
+    {32, 32, 4, 1.67f, 1.42f, 0.354f, 0.081f, launch_split<2, 2, 4>},
+    {32, 32, 2, 1.85f, 1.44f, 0.191f, 0.045f, launch_split<2, 2, 8>},
+    {64, 32, 1, 1.74f, 1.76f, 0.154f, 0.100f, launch_split<4, 2, 8>},
+    {64, 64, 2, 2.17f, 2.25f, 0.442f, 0.178f, launch_split<4, 4, 4>},
+    {64, 64, 1, 1.61f, 2.43f, 0.234f, 0.150f, launch_split<4, 4, 8>},
+    {128, 128, 2, 0.36f, 3.95f, 1.161f, 0.494f, launch_tiles<4, 2, 2, 4>},
+    {128, 256, 1, 1.02f, 4.61f, 1.023f, 0.740f, launch_tiles<4, 4, 2, 4>},
+    {256, 256, 1, 1.35f, 7.64f, 1.547f, 0.950f, launch_tiles<8, 4, 2, 4>},
 };
 
 float estimate(const Kernel& k, const Fp8LinearArgs& a, int cus) {
