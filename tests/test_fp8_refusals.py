@@ -166,3 +166,15 @@ def test_dequantize_of_a_matrix():
     assert v.shape == (130, 130) and v[0, 0] == 1 and v[127, 128] == 2 and v[128, 0] == 3 and v[129, 129] == 4
     a = Fp8Matrix(torch.ones(2, 3, 130).to(torch.float8_e4m3fn), torch.arange(12.0).view(2, 3, 2))
     assert a.dequantize()[1, 2, 127] == 10 and a.dequantize()[1, 2, 129] == 11
+
+
+def test_dense_layers_of_the_host():
+    """8-bit dense layers need a HIP device and blocks that run the shared expert
+    as a module."""
+    from uma_qmoe_amd.formats import ContractError
+    from uma_qmoe_amd.qwen_host import load_fixed_qwen, quantize_dense_fp8
+
+    with pytest.raises(ContractError, match="HIP device"):
+        load_fixed_qwen("nowhere", "nothing", model_manifest_sha256="0" * 64, device="cpu", fp8_dense=True)
+    with pytest.raises(ContractError, match="HIP device"):
+        quantize_dense_fp8(torch.nn.Linear(16, 16))

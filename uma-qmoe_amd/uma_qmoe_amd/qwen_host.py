@@ -114,6 +114,71 @@ def replace_moe_blocks(model: Any, pack_handle: int, *, performance_mode: bool, 
     return n
 
 
+def _fp8_classes():
+    torch = _torch()
+    from .native_backend import FP8_GROUP, Fp8Matrix, load_native_extension
+
+    class Fp8Linear(torch.nn.Module):
+        """A Linear with its weight in 8-bit floats (a scale per 128 x 128
+        block): BF16 in and out, the input quantised per token and 128
+        columns. ``weight`` BF16 [out, in] on the device, in a multiple of 16."""
+
+        def __init__(self, weight: Any, bias: Any = None) -> None:
+            super().__init__()
+            self.extension = load_native_extension()[1]
+            q = self.extension.fp8_quantize(weight.detach(), block_rows=FP8_GROUP)
+            self.register_buffer("codes", q.codes)
+            self.register_buffer("scales", q.scales)
+            self.register_buffer("bias", None if bias is None else bias.detach())
+
+        def forward(self, x: Any) -> Any:
+            return self.extension.fp8_linear(x, Fp8Matrix(self.codes, self.scales, FP8_GROUP), self.bias)
+
+    class Fp8SharedExpert(torch.nn.Module):
+        """The shared expert in 8-bit floats: gate and up as one product, its
+        activation straight into the down projection's 8-bit input."""
+
+        def __init__(self, shared_expert: Any) -> None:
+            super().__init__()
+            self.gate_up = Fp8Linear(torch.cat([shared_expert.gate_proj.weight.detach(),
+                                                shared_expert.up_proj.weight.detach()]))
+            self.down = Fp8Linear(shared_expert.down_proj.weight)
+
+        def forward(self, x: Any) -> Any:
+            _y, q = self.gate_up.extension.silu_mul(self.gate_up(x), bf16=False, fp8=True)
+            return self.down(q)
+
+    return Fp8Linear, Fp8SharedExpert
+
+
+_FP8_CLASSES = None
+
+
+def quantize_dense_fp8(model: Any) -> int:
+    """Puts the dense projections of every layer into 8-bit floats: attention's
+    q, k, v and o, and the shared expert of its quantized block, which must run
+    it as a module of its own (``fused_block=False``). The BF16 weights are
+    dropped. Returns the number of weights replaced. No counterpart in the
+    reference, whose dense layers are BF16."""
+    global _FP8_CLASSES
+    if next(model.parameters()).device.type != "cuda":
+        raise ContractError("8-bit dense layers require a HIP device")
+    layers = model.model.layers
+    if any(getattr(layer.mlp, "fused_block", True) for layer in layers):
+        raise ContractError("8-bit dense layers require blocks with fused_block=False")
+    if _FP8_CLASSES is None:
+        _FP8_CLASSES = _fp8_classes()
+    linear, shared = _FP8_CLASSES
+    count = 0
+    for layer in layers:
+        for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
+            old = getattr(layer.self_attn, name)
+            setattr(layer.self_attn, name, linear(old.weight, old.bias))
+        layer.mlp.shared_expert = shared(layer.mlp.shared_expert)
+        count += 7
+    return count
+
+
 def restore_nonpersistent_buffers(model: Any, config: Any, device: Any) -> None:
     """Rebuilds the rotary embedding, whose frequencies are not in the
     state dict and so are uninitialised after ``to_empty``
@@ -320,7 +385,7 @@ def _fill_dense(model: Any, index: QwenCheckpointIndex, device: Any) -> tuple[in
 
 def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_manifest_sha256: str,
                     device: str = "cuda:0", performance_mode: bool = False, target_policy_id: str | None = None,
-                    fused_block: bool = True, architecture: tuple = QWEN_ARCHITECTURE,
+                    fused_block: bool = True, fp8_dense: bool = False, architecture: tuple = QWEN_ARCHITECTURE,
                     model_id: str = QWEN_MODEL_ID, model_revision: str = QWEN_MODEL_REVISION) -> FixedQwenHost:
     """A Qwen MoE host: the dense BF16 tensors of a local checkpoint directory
     in a Transformers model whose MoE blocks run the HIP operator over one
@@ -328,6 +393,9 @@ def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_mani
     with the same refusals and evidence keys). ``expert_pack`` is a pack file
     or an open reader; ``architecture`` is the (model_type, layers, experts,
     top-k) the checkpoint must have, the fixed model's by default.
+    ``fp8_dense`` puts the attention projections and shared experts into 8-bit
+    floats once they are loaded (``quantize_dense_fp8``; HIP devices only) and
+    runs the blocks with ``fused_block=False``.
 
     The pack is checked before anything is built: one mapping (one VMA when
     its file is known) and, for a TargetPack, exactly the model's routed
@@ -338,6 +406,10 @@ def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_mani
     torch = _torch()
     from transformers import AutoConfig
 
+    if fp8_dense:
+        if not str(device).startswith("cuda"):
+            raise ContractError("8-bit dense layers require a HIP device")
+        fused_block = False
     from .custom_op import register_expert_pack, register_moe_forward, unregister_expert_pack
     from .packfile import MemoryTargetPack, TargetPackReader
 
@@ -382,6 +454,7 @@ def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_mani
         for failed, message in failures:
             if failed:
                 raise ContractError(message)
+        fp8_weights = quantize_dense_fp8(model) if fp8_dense else 0
         model.eval()
         evidence = {
             "model_id": model_id,
@@ -389,6 +462,7 @@ def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_mani
             "device": str(device),
             "performance_mode": performance_mode,
             "fused_block": fused_block,
+            "fp8_dense_weight_count": fp8_weights,
             "dense_tensor_count": dense_count,
             "dense_tensor_bytes": dense_bytes,
             "skipped_expert_tensor_count": len(index.experts),
@@ -533,6 +607,7 @@ __all__ = [
     "QWEN_MODEL_REVISION",
     "is_qwen_expert_tensor_name",
     "load_fixed_qwen",
+    "quantize_dense_fp8",
     "quantized_block",
     "replace_moe_blocks",
     "restore_nonpersistent_buffers",
