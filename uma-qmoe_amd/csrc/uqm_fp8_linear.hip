@@ -241,7 +241,22 @@ hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
 // ---------------------------------------------------------------- tiles --
 // Many tokens: 16 * TN * WN weight rows x 16 * TT * WT tokens per workgroup of
 // WN x WT waves, the column blocks in a ring of two stages in LDS (rows of 128
-// bytes, loaded by the address unit straight into LDS).
+// bytes, loaded by the address unit straight into LDS), each wave 16 * TN rows x 16
+// * TT tokens in registers. A block of a wave is TN * TT products of 32 cycles and
+// four FMAs each, which run under the products (the two waves of a SIMD in turn
+// reach 4.2 PFLOP/s with nothing else to do).
+// What bounds it: 8191 x 11264 x 2048 takes 191 us (1.97 PFLOP/s; a library product
+// with one scale for a whole matrix 201 us, its best rate, at 8192^3, 2.74; this
+// kernel there 2.44). The matrix cores work 44% of its cycles at 2.07 GHz. Timed
+// with parts left out (8192^3, 459 us): without the loads 387, without the reads
+// of LDS as well 292, so the operands' way through LDS costs the most, the loads'
+// latency next; the barrier costs 2%, four operands of the weight in flight
+// instead of two nothing. A quarter of the time at K = 2048 is the start and end of
+// a tile (7.6 us of 32); workgroups that walk over their tiles, with the next one's
+// loads under the last one's stores, took 214 us instead of 196.
+// Steps (8191 x 11264 x 2048, us): loads behind one wait per block 251, a wait only
+// where a stage is needed and loads in two halves 225 with the scales in panels,
+// results of two tiles side by side (64-byte stores) 196, loads through buffers 192.
 constexpr int64_t kFp8TileMaxK = int64_t{1} << 23;  // 256 rows of fewer bytes stay below it
 
 template <int TN, int TT, int WN, int WT>
@@ -382,53 +397,51 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
   read_scales(0);
 
   static_assert(TN % 2 == 0, "w alternates");
-  // A block's loads are spread over its first rows of products (the address unit
-  // takes 16 cycles for each).
   for (int b = 0; b < KB; ++b) {
     const int slot = b & 1;
 #pragma unroll
     for (int t = 0; t < TT; ++t) f[t] = fw * fx[t];
     fw = ws[min(b + 1, KB - 1)];
 #pragma unroll
-      for (int n = 0; n < TN; ++n) {
-        // (a panel's loads twice over; the second time they write what is there)
-        if (n == TN / 2) {
-          load_scales(b % G::kLoadsS, b / kScaleBlocks + 1);
-          read_scales(min(b + 1, KB - 1));
-        }
-        if (n == TN - 1) {
-          // This block's operands are all in registers: the next block's panels
-          // must have landed, and this one's are free. The products of the last
-          // row hide the first reads from them.
-          wait_loads<0>();
-          stage_barrier();
-          reads_follow();
-          w[0] = read_w(slot ^ 1, 0);
-        }
-        if (n < TN - 1) w[(n + 1) & 1] = read_w(slot, n + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          // the sums of the row before, TT products ago
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int m = n == 0 ? TN - 1 : n - 1;
-            acc[m][t][e] = fmaf(n == 0 ? f_last[t] : f[t], d[t][e], acc[m][t][e]);
-          }
-          d[t] = mfma_fp8(w[n & 1], x[t]);
-          if (n == TN - 1) x[t] = read_x(slot ^ 1, t);
-          // half of the loads right behind the barrier that freed their panels, the
-          // others in the next row (eight at once hold up the products)
-#pragma unroll
-          for (int j = 0; j < kLoads; ++j) {
-            if (n == TN - 1 && j < kLoads / 2 && j * TT * 2 / kLoads == t) load_any(j, b + 2, slot);
-            if (n == 0 && j >= kLoads / 2 && (j - kLoads / 2) * TT * 2 / kLoads == t) load_any(j, b + 1, slot ^ 1);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+    for (int n = 0; n < TN; ++n) {
+      // (a panel's loads twice over; the second time they write what is there)
+      if (n == TN / 2) {
+        load_scales(b % G::kLoadsS, b / kScaleBlocks + 1);
+        read_scales(min(b + 1, KB - 1));
       }
+      if (n == TN - 1) {
+        // This block's operands are all in registers: the next block's panels
+        // must have landed, and this one's are free. The products of the last
+        // row hide the first reads from them.
+        wait_loads<0>();
+        stage_barrier();
+        reads_follow();
+        w[0] = read_w(slot ^ 1, 0);
+      }
+      if (n < TN - 1) w[(n + 1) & 1] = read_w(slot, n + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < TT; ++t) f_last[t] = f[t];
+      for (int t = 0; t < TT; ++t) {
+        // the sums of the row before, TT products ago
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = n == 0 ? TN - 1 : n - 1;
+          acc[m][t][e] = fmaf(n == 0 ? f_last[t] : f[t], d[t][e], acc[m][t][e]);
+        }
+        d[t] = mfma_fp8(w[n & 1], x[t]);
+        if (n == TN - 1) x[t] = read_x(slot ^ 1, t);
+        // half of the loads right behind the barrier that freed their panels, the
+        // others in the next row (eight at once hold up the products)
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          if (n == TN - 1 && j < kLoads / 2 && j * TT * 2 / kLoads == t) load_any(j, b + 2, slot);
+          if (n == 0 && j >= kLoads / 2 && (j - kLoads / 2) * TT * 2 / kLoads == t) load_any(j, b + 1, slot ^ 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) f_last[t] = f[t];
   }
 #pragma unroll
   for (int t = 0; t < TT; ++t)
@@ -488,16 +501,18 @@ hipError_t launch_tiles(const Fp8LinearArgs& a, hipStream_t stream) {
 // and one for each block of 128 columns, which grows with the share of the card
 // that works (L2 and the clock are shared): `empty` for one workgroup, `full` for
 // all. Fitted to 1750 products (T 1 to 8191, N 128 to 11264, K 128 to 8192; 5 to
-// 11% off in the mean square); the kernel taken is 1.8% slower in the mean than
-// the best of the eight, over 10% in 119 of them (at most 33%, calls of 5 to 12
-// us). Without one of the eight the best of the others is slower by 7.3, 1.4,
-// 1.2, 1.5, 0.8, 0.3, 0.1 and 1.0% in the mean (in their order below); the ends:
-//   1 x 11264 x 2048       16 x 16 rows and tokens 7.5 us, 32 x 32 9.8
-//   137 x 1400 x 2000      32 x 32 5.3, 64 x 64 8.9, 128 x 64 12
-//   512 x 2048 x 5632      64 x 64 14.7, 64 x 32 19.0, 128 x 64 31.9
-//   1024 x 2048 x 2048     128 x 64 14.1, 64 x 64 15.2, 256 x 256 26.1
-//   4096 x 2048 x 5632     128 x 256 51.2, 128 x 128 54.8, 256 x 256 61.4
-//   8191 x 11264 x 2048    256 x 256 196, 128 x 256 234, 128 x 64 285
+// 10% off in the mean square); the kernel taken is 2.3% slower in the mean than the
+// best of eighteen that were timed, over 10% in 168 of them (at most 40%, calls of
+// 3 to 7 us). Without one of the ten the best of the others is slower by 1.0, 3.3,
+// 0.6, 0.7, 0.5, 0.7, 0.6, 1.2, 0.2 and 1.1% in the mean (in their order below);
+// some of them (us, launches back to back; 16 x 16 means rows and tokens, W waves):
+//   1 x 11264 x 2048       16 x 16 W 4 5.8, W 8 5.9, 32 x 32 W 4 6.5, 64 x 32 6.7
+//   128 x 1408 x 2048      32 x 32 W 8 4.3, 16 x 16 W 4 4.7, 64 x 64 W 8 6.7, 128 x 128 12.5
+//   512 x 2048 x 5632      64 x 64 W 8 13.7, W 4 16.5, 64 x 32 18.0, 128 x 128 35.2
+//   4096 x 128 x 8192      64 x 32 14.2, 64 x 64 W 8 16.8, 32 x 32 22.0, 128 x 128 50.0
+//   1024 x 2048 x 2048     64 x 64 W 4 11.5, W 8 13.2, 128 x 128 15.4, 256 x 256 25.8
+//   4096 x 2048 x 5632     128 x 256 49.9, 128 x 128 54.5, 256 x 256 62.9, 64 x 64 111
+//   8191 x 11264 x 2048    256 x 256 185, 128 x 256 225, 128 x 128 230
 struct Kernel {
   int rows, tokens, per_cu;
   float fixed, round, full, empty;  // us

@@ -454,22 +454,13 @@ class HipExtension:
         if rc:
             _native.check(rc, fn.__name__)
 
-    def _columns(self, x, what):
-        """Columns of a BF16 device tensor [..., columns]."""
+    def _check_rows(self, x, what):
+        """The words of a refusal of a row operator's input."""
         if x.dtype is not self.torch.bfloat16:
             raise RuntimeError(f"{what} requires BF16 tensors")
-        cols = x.shape[-1] if x.ndim else 0
-        if cols == 0:
+        if not x.ndim or x.shape[-1] == 0:
             raise RuntimeError(f"{what} requires a tensor with at least one column")
-        return cols
-
-    @staticmethod
-    def _check_devices(what, index, *others):
-        for t in others:
-            if t is not None and t.get_device() != index:
-                raise RuntimeError(f"{what} requires all tensors on one device")
-        if index < 0:
-            raise RuntimeError(f"{what} requires device tensors")
+        raise RuntimeError(f"{what} requires device tensors")
 
     def add_rmsnorm(self, hidden, residual=None, eps=1e-6, weight=None, *, bf16=True, fp8=False, inplace=False):
         """s = hidden + residual (BF16) and RMSNorm(s): (s, the norm in BF16 or
@@ -478,76 +469,95 @@ class HipExtension:
         Without a residual s is ``hidden`` itself. ``inplace`` writes s over
         ``residual``."""
         torch = self.torch
-        cols = self._columns(hidden, "add_rmsnorm")
-        x, index = hidden.contiguous(), hidden.get_device()
+        half, index, shape = torch.bfloat16, hidden.get_device(), hidden.shape
+        cols = shape[-1] if shape else 0
         if not (bf16 or fp8):
             raise RuntimeError("add_rmsnorm requires at least one of bf16 and fp8")
-        r = total = out = q = None
+        if hidden.dtype is not half or cols == 0:
+            self._check_rows(hidden, "add_rmsnorm")
+        total = out = q = r = w = None
         if residual is not None:
-            if residual.dtype is not torch.bfloat16 or residual.shape != hidden.shape:
+            if residual.dtype is not half or residual.shape != shape:
                 raise RuntimeError("add_rmsnorm requires a BF16 residual of hidden's shape")
             if inplace and not residual.is_contiguous():
                 raise RuntimeError("add_rmsnorm(inplace=True) requires a contiguous residual")
-            r = residual.contiguous()
+            if residual.get_device() != index:
+                raise RuntimeError("add_rmsnorm requires all tensors on one device")
+            residual = residual.contiguous()
+            r = residual.data_ptr()
         elif inplace:
             raise RuntimeError("add_rmsnorm(inplace=True) requires a residual")
         if weight is not None:
-            if weight.dtype is not torch.bfloat16 or weight.shape != (cols,):
+            if weight.dtype is not half or weight.shape != (cols,):
                 raise RuntimeError(f"add_rmsnorm requires a BF16 weight [{cols}]")
+            if weight.get_device() != index:
+                raise RuntimeError("add_rmsnorm requires all tensors on one device")
             weight = weight.contiguous()
-        self._check_devices("add_rmsnorm", index, r, weight)
-        if r is not None:
-            total = r if inplace else torch.empty_like(x)
+            w = weight.data_ptr()
+        if index < 0:
+            self._check_rows(hidden, "add_rmsnorm")
+        x = hidden.contiguous()
+        if residual is not None:
+            total = residual if inplace else torch.empty_like(x)
         if bf16:
             out = torch.empty_like(x)
         if fp8:
             q = Fp8Matrix(torch.empty_like(x, dtype=torch.float8_e4m3fn),
-                          torch.empty(*x.shape[:-1], -(-cols // FP8_GROUP), dtype=torch.float32, device=x.device))
-        self._launch(self.lib.uqm_add_rmsnorm, index, x.data_ptr(), _ptr(r), x.numel() // cols, cols, _ptr(weight),
-                     eps, _ptr(total), _ptr(out), q and q.codes.data_ptr(), q and q.scales.data_ptr())
+                          torch.empty(*shape[:-1], -(-cols // FP8_GROUP), dtype=torch.float32, device=x.device))
+        self._launch(self.lib.uqm_add_rmsnorm, index, x.data_ptr(), r, x.numel() // cols, cols, w, eps,
+                     None if total is None else total.data_ptr(), out.data_ptr() if bf16 else None,
+                     q[0].data_ptr() if fp8 else None, q[1].data_ptr() if fp8 else None)
         return (hidden if total is None else total), out, q
 
     def silu_mul(self, gate_up, *, bf16=True, fp8=False):
         """silu(gate) * up of ``gate_up`` [..., 2 * features] (gate first):
         (BF16 [..., features] or None, ``Fp8Matrix`` or None)."""
         torch = self.torch
-        cols = self._columns(gate_up, "silu_mul")
-        x, index = gate_up.contiguous(), gate_up.get_device()
+        index, shape = gate_up.get_device(), gate_up.shape
+        cols = shape[-1] if shape else 0
         if not (bf16 or fp8):
             raise RuntimeError("silu_mul requires at least one of bf16 and fp8")
+        if gate_up.dtype is not torch.bfloat16 or cols == 0:
+            self._check_rows(gate_up, "silu_mul")
         if cols % 2:
             raise RuntimeError("silu_mul requires an even number of columns")
-        self._check_devices("silu_mul", index)
-        lead, features, device = x.shape[:-1], cols // 2, x.device
+        if index < 0:
+            self._check_rows(gate_up, "silu_mul")
+        x = gate_up.contiguous()
+        lead, features, device = shape[:-1], cols // 2, x.device
         out = torch.empty(*lead, features, dtype=torch.bfloat16, device=device) if bf16 else None
         q = None
         if fp8:
             q = Fp8Matrix(torch.empty(*lead, features, dtype=torch.float8_e4m3fn, device=device),
                           torch.empty(*lead, -(-features // FP8_GROUP), dtype=torch.float32, device=device))
-        self._launch(self.lib.uqm_silu_mul, index, x.data_ptr(), x.numel() // cols, features, _ptr(out),
-                     q and q.codes.data_ptr(), q and q.scales.data_ptr())
+        self._launch(self.lib.uqm_silu_mul, index, x.data_ptr(), x.numel() // cols, features,
+                     out.data_ptr() if bf16 else None, q[0].data_ptr() if fp8 else None,
+                     q[1].data_ptr() if fp8 else None)
         return out, q
 
     def fp8_quantize(self, x, *, block_rows=1):
         """``x`` (BF16) as an ``Fp8Matrix``: ``block_rows`` 1 for activations
         [..., cols], 128 for a weight [rows, cols]."""
         torch = self.torch
-        cols = self._columns(x, "fp8_quantize")
-        x, index = x.contiguous(), x.get_device()
-        rows = x.numel() // cols
+        index, shape = x.get_device(), x.shape
+        cols = shape[-1] if shape else 0
+        if x.dtype is not torch.bfloat16 or cols == 0:
+            self._check_rows(x, "fp8_quantize")
         if block_rows == 1:
-            lead = x.shape[:-1]
+            lead = shape[:-1]
         elif block_rows != FP8_GROUP:
             raise RuntimeError(f"fp8_quantize takes blocks of 1 or {FP8_GROUP} rows")
-        elif x.ndim != 2:
+        elif len(shape) != 2:
             raise RuntimeError("fp8_quantize takes blocks of rows of a matrix only")
         else:
-            lead = (-(-rows // FP8_GROUP),)
-        self._check_devices("fp8_quantize", index)
+            lead = (-(-shape[0] // FP8_GROUP),)
+        if index < 0:
+            self._check_rows(x, "fp8_quantize")
+        x = x.contiguous()
         codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
         scales = torch.empty(*lead, -(-cols // FP8_GROUP), dtype=torch.float32, device=x.device)
-        self._launch(self.lib.uqm_fp8_quantize, index, x.data_ptr(), rows, cols, block_rows, codes.data_ptr(),
-                     scales.data_ptr())
+        self._launch(self.lib.uqm_fp8_quantize, index, x.data_ptr(), x.numel() // cols, cols, block_rows,
+                     codes.data_ptr(), scales.data_ptr())
         return Fp8Matrix(codes, scales, block_rows)
 
     def _check_fp8(self, m, block_rows, what):
@@ -601,7 +611,9 @@ class HipExtension:
                 and (bias is None or bias.dtype is torch.bfloat16 and bias.shape == (n,))):
             self._check_linear(x, weight, bias)
         index = codes.get_device()
-        self._check_devices("fp8_linear", index, scales, w, ws, bias)
+        if not (index >= 0 and index == scales.get_device() == w.get_device() == ws.get_device()
+                and (bias is None or bias.get_device() == index)):
+            raise RuntimeError("fp8_linear requires device tensors, all on one device")
         codes, scales, w, ws = codes.contiguous(), scales.contiguous(), w.contiguous(), ws.contiguous()
         if bias is not None:
             bias = bias.contiguous()
