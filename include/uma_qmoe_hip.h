@@ -333,6 +333,13 @@ int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const v
                    const float* weight_scales, int64_t out_features, int64_t in_features, const void* bias,
                    void* output, void* stream);
 
+/* Reports the kernel that uqm_fp8_linear takes for these sizes: weight rows and
+ * tokens per workgroup and its waves (host pointers). Host only: without a device
+ * it plans for 256 compute units. For tests and measurements that mean a
+ * particular kernel. */
+int uqm_fp8_linear_plan(int64_t rows, int64_t out_features, int64_t in_features, int32_t* tile_rows,
+                        int32_t* tile_tokens, int32_t* waves);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ import ctypes
 import pytest
 import torch
 
+import fp8_cases
 from uma_qmoe_amd import _native
 from uma_qmoe_amd.native_backend import Fp8Matrix, HipExtension
 
@@ -97,6 +98,22 @@ def test_fp8_quantize(lib, args, words):
 ])
 def test_fp8_linear(lib, args, words):
     refused(lib, "uqm_fp8_linear", args, words)
+
+
+@pytest.mark.parametrize("args,words", [((-1, 64, 128), "rows"), ((4, 0, 128), "features"), ((4, 64, 8), "multiple of 16")])
+def test_fp8_linear_plan(lib, args, words):
+    out = [ctypes.byref(ctypes.c_int32()) for _ in range(3)]
+    assert lib.uqm_fp8_linear_plan(*args, *out) == 1 and words in lib.uqm_last_error().decode()
+    assert lib.uqm_fp8_linear_plan(4, 64, 128, None, *out[1:]) == 1
+
+
+def test_cases_reach_every_kernel(lib):
+    """The GPU tests' sizes (planned for 256 compute units) take the kernels that
+    they say, and no size takes another one."""
+    assert all(fp8_cases.plan(t, n, k) == kernel for kernel, t, n, k in fp8_cases.PLANNED)
+    known = {kernel for kernel, *_ in fp8_cases.PLANNED}
+    sizes = [1, 3, 16, 33, 100, 300, 777, 1500, 4000, 9000, 40000]
+    assert {fp8_cases.plan(t, n, 16 * k) for t in sizes for n in sizes for k in (1, 8, 40, 128, 600, 600000)} == known
 
 
 def test_no_rows_is_no_work(lib):

@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import fp8_cases
 import fp8_reference as ref
 from uma_qmoe_amd.native_backend import Fp8Matrix
 
@@ -290,6 +291,39 @@ def test_linear_leaves_its_surroundings(hip_ext, t, n, k):
     assert torch.equal(shifted.view(t, n), want)
 
 
+@pytest.mark.parametrize("kernel,t,n,k", fp8_cases.PLANNED)
+def test_linear_kernels(hip_ext, kernel, t, n, k):
+    """Every kernel, at whole and at ragged sizes: the product, again with the
+    same bits, with rows lost to NaN that the others must not see, and at an
+    output that is aligned to its elements only, with nothing written around it."""
+    note(f"fp8_linear kernel {kernel} {t}x{n}x{k}")
+    assert fp8_cases.plan(t, n, k) == kernel
+    codes, scales, w, ws, b = (v.to(DEV) for v in operands(t, n, k, t + n + k))
+    x, weight = Fp8Matrix(codes, scales), Fp8Matrix(w, ws, 128)
+    y, tol = ref.linear64(codes, scales, w, ws, b, device=DEV)
+    got = hip_ext.fp8_linear(x, weight, b)
+    assert ((got.double() - y).abs() <= tol).all()
+    assert torch.equal(hip_ext.fp8_linear(x, weight, b), got)
+    room = torch.full((t * n + 2048,), 7.0, dtype=torch.bfloat16, device=DEV)
+    for at in (1024, 1025):
+        room.fill_(7.0)
+        out = room[at:at + t * n]
+        assert hip_ext.lib.uqm_fp8_linear(codes.data_ptr(), scales.data_ptr(), t, w.data_ptr(), ws.data_ptr(), n, k,
+                                          b.data_ptr(), out.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out.view(t, n), got)
+        assert (room[:at] == 7).all() and (room[at + t * n:] == 7).all()
+    bad_t, bad_s, bad_n = t // 2, t - 1, n // 3
+    codes.view(torch.uint8)[bad_t] = 0x7F
+    w.view(torch.uint8)[bad_n] = 0x7F
+    scales[bad_s] = float("inf")
+    lost = hip_ext.fp8_linear(x, weight, b)
+    assert lost[bad_t].isnan().all() and lost[:, bad_n].isnan().all() and not lost[bad_s].isfinite().any()
+    keep = torch.ones(t, n, dtype=torch.bool, device=DEV)
+    keep[bad_t] = keep[bad_s] = False
+    keep[:, bad_n] = False
+    assert torch.equal(lost[keep], got[keep])
+
+
 def test_linear_of_bf16_and_batches(hip_ext):
     note("fp8_linear of BF16 input")
     g = gen(8)
@@ -374,3 +408,46 @@ def test_dense_layer_in_a_graph_and_on_streams(hip_ext, rows):
         s.synchronize()
     for (total, y), (total_w, y_w) in zip(got, want):
         assert torch.equal(total, total_w) and torch.equal(y, y_w)
+
+
+# ------------------------------------------------------- offsets past 32 bits --
+def repeated(rows, cols, seed):
+    """[rows, cols] BF16 on the device whose rows differ, made from 127 of them."""
+    base = normal(gen(seed), 127, cols).to(DEV)
+    return base.repeat(-(-rows // 127), 1)[:rows]
+
+
+def test_rows_past_32_bits(hip_ext):
+    """4.6 GB of BF16: the last rows are those of a small call."""
+    note("row operators past 32 bits")
+    rows, cols = 70001, 32768
+    x = repeated(rows, cols, 1)
+    last = x[-130:].clone()
+    for fn in (lambda v: hip_ext.add_rmsnorm(v, None, bf16=False, fp8=True)[2], lambda v: hip_ext.silu_mul(v, bf16=False, fp8=True)[1],
+               lambda v: hip_ext.fp8_quantize(v)):
+        big, small = fn(x), fn(last)
+        assert torch.equal(big.codes[-130:].view(torch.uint8), small.codes.view(torch.uint8))
+        assert torch.equal(big.scales[-130:], small.scales)
+        del big
+    big = hip_ext.fp8_quantize(x, block_rows=128)
+    small = hip_ext.fp8_quantize(x[70001 // 128 * 128:], block_rows=128)
+    assert torch.equal(big.codes[70001 // 128 * 128:].view(torch.uint8), small.codes.view(torch.uint8))
+    assert torch.equal(big.scales[-1:], small.scales)
+    del big
+    total, n, _ = hip_ext.add_rmsnorm(x, x)
+    want = hip_ext.add_rmsnorm(last, last)
+    assert torch.equal(total[-130:], want[0]) and torch.equal(n[-130:], want[1])
+
+
+@pytest.mark.parametrize("t,n,k", [(3, 140001, 32768), (140001, 17, 32768), (70001, 32776, 16), (300, 16777, 262144)])
+def test_linear_past_32_bits(hip_ext, t, n, k):
+    """Weight, activations or output of over 4 GB; the last results in 64 bits."""
+    note(f"fp8_linear past 32 bits {t}x{n}x{k}")
+    x = hip_ext.fp8_quantize(repeated(t, k, 2))
+    w = hip_ext.fp8_quantize(repeated(n, k, 3), block_rows=128)
+    got = hip_ext.fp8_linear(x, w)[-40:, -200:]
+    n0 = n // 128 * 128 if n % 128 >= 100 or n < 256 else (n // 128 - 1) * 128  # a block border before the last 200 rows
+    n0 = max(0, n0 - 128)
+    y, tol = ref.linear64(x.codes[-40:], x.scales[-40:], w.codes[n0:], w.scales[n0 // 128:], None)
+    y, tol = y[:, -200:], tol[:, -200:]
+    assert ((got.double().cpu() - y).abs() <= tol).all()

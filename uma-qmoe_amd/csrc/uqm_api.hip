@@ -1407,14 +1407,20 @@ int uqm_fp8_quantize(const void* input, int64_t rows, int64_t cols, int64_t bloc
                    "fp8_quantize launch");
 }
 
+static int check_linear_extents(int64_t rows, int64_t out_features, int64_t in_features) {
+  if (rows < 0 || rows > kMaxExtent || out_features <= 0 || out_features > kMaxExtent)
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: rows must be in [0, 2^31) and features in [1, 2^31)");
+  if (in_features <= 0 || in_features % 16 != 0 || in_features >= uqm::kFp8MaxK)
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: input features %lld must be a positive multiple of 16 below 2^25", (long long)in_features);
+  return UQM_OK;
+}
+
 int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const void* weight_codes,
                    const float* weight_scales, int64_t out_features, int64_t in_features, const void* bias,
                    void* output, void* stream) {
   using namespace uqm;
-  if (rows < 0 || rows > kMaxExtent || out_features <= 0 || out_features > kMaxExtent)
-    return fail(UQM_ERR_ARGUMENT, "fp8_linear: rows must be in [0, 2^31) and features in [1, 2^31)");
-  if (in_features <= 0 || in_features % 16 != 0 || in_features >= kFp8MaxK)
-    return fail(UQM_ERR_ARGUMENT, "fp8_linear: input features %lld must be a positive multiple of 16 below 2^25", (long long)in_features);
+  int rc = check_linear_extents(rows, out_features, in_features);
+  if (rc) return rc;
   if (weight_codes == nullptr || weight_scales == nullptr)
     return fail(UQM_ERR_ARGUMENT, "fp8_linear: weight codes and scales are required");
   if (misaligned(weight_codes, 16) || misaligned(weight_scales, 4) || misaligned(bias, 2))
@@ -1430,8 +1436,7 @@ int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const v
       overlap(output, out_bytes, weight_scales, 4 * ((out_features + kFp8Group - 1) / kFp8Group) * groups) ||
       overlap(output, out_bytes, bias, 2 * out_features))
     return fail(UQM_ERR_ARGUMENT, "fp8_linear: the output overlaps an input");
-  const int rc = check_device();
-  if (rc) return rc;
+  if ((rc = check_device())) return rc;
   Fp8LinearArgs a{};
   a.x = static_cast<const uint8_t*>(codes);
   a.xs = scales;
@@ -1443,6 +1448,24 @@ int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const v
   a.N = out_features;
   a.K = in_features;
   return hip_check(launch_fp8_linear(a, device_cus(), static_cast<hipStream_t>(stream)), "fp8_linear launch");
+}
+
+int uqm_fp8_linear_plan(int64_t rows, int64_t out_features, int64_t in_features, int32_t* tile_rows,
+                        int32_t* tile_tokens, int32_t* waves) {
+  using namespace uqm;
+  const int rc = check_linear_extents(rows, out_features, in_features);
+  if (rc) return rc;
+  if (tile_rows == nullptr || tile_tokens == nullptr || waves == nullptr)
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear_plan: tile_rows, tile_tokens and waves are required");
+  Fp8LinearArgs a{};
+  a.T = rows;
+  a.N = out_features;
+  a.K = in_features;
+  const Fp8LinearPlan p = plan_fp8_linear(a, device_cus());
+  *tile_rows = p.rows;
+  *tile_tokens = p.tokens;
+  *waves = p.waves;
+  return UQM_OK;
 }
 
 }  // extern "C"

@@ -49,6 +49,11 @@ struct Fp8LinearArgs {
   uint16_t* out;          // bf16 [T, N]
   int64_t T, N, K;        // K a multiple of 16 below kFp8MaxK
 };
+// Rows and tokens of a workgroup, and its waves, that the call takes.
+struct Fp8LinearPlan {
+  int rows, tokens, waves;
+};
+Fp8LinearPlan plan_fp8_linear(const Fp8LinearArgs& a, int cus);
 hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream);
 
 }  // namespace uqm

@@ -514,21 +514,21 @@ hipError_t launch_tiles(const Fp8LinearArgs& a, hipStream_t stream) {
 //   4096 x 2048 x 5632     128 x 256 49.9, 128 x 128 54.5, 256 x 256 62.9, 64 x 64 111
 //   8191 x 11264 x 2048    256 x 256 185, 128 x 256 225, 128 x 128 230
 struct Kernel {
-  int rows, tokens, per_cu;
+  int rows, tokens, waves, per_cu;
   float fixed, round, full, empty;  // us
   hipError_t (*launch)(const Fp8LinearArgs&, hipStream_t);
 };
 constexpr Kernel kKernels[] = {
-    {16, 16, 8, 1.48f, 1.28f, 0.323f, 0.044f, launch_split<1, 1, 4>},
-    {16, 16, 4, 1.94f, 1.01f, 0.182f, 0.015f, launch_split<1, 1, 8>},
-    {32, 32, 4, 1.67f, 1.42f, 0.354f, 0.081f, launch_split<2, 2, 4>},
-    {32, 32, 2, 1.85f, 1.44f, 0.191f, 0.045f, launch_split<2, 2, 8>},
-    {64, 32, 1, 1.74f, 1.76f, 0.154f, 0.100f, launch_split<4, 2, 8>},
-    {64, 64, 2, 2.17f, 2.25f, 0.442f, 0.178f, launch_split<4, 4, 4>},
-    {64, 64, 1, 1.61f, 2.43f, 0.234f, 0.150f, launch_split<4, 4, 8>},
-    {128, 128, 2, 0.36f, 3.95f, 1.161f, 0.494f, launch_tiles<4, 2, 2, 4>},
-    {128, 256, 1, 1.02f, 4.61f, 1.023f, 0.740f, launch_tiles<4, 4, 2, 4>},
-    {256, 256, 1, 1.35f, 7.64f, 1.547f, 0.950f, launch_tiles<8, 4, 2, 4>},
+    {16, 16, 4, 8, 1.48f, 1.28f, 0.323f, 0.044f, launch_split<1, 1, 4>},
+    {16, 16, 8, 4, 1.94f, 1.01f, 0.182f, 0.015f, launch_split<1, 1, 8>},
+    {32, 32, 4, 4, 1.67f, 1.42f, 0.354f, 0.081f, launch_split<2, 2, 4>},
+    {32, 32, 8, 2, 1.85f, 1.44f, 0.191f, 0.045f, launch_split<2, 2, 8>},
+    {64, 32, 8, 1, 1.74f, 1.76f, 0.154f, 0.100f, launch_split<4, 2, 8>},
+    {64, 64, 4, 2, 2.17f, 2.25f, 0.442f, 0.178f, launch_split<4, 4, 4>},
+    {64, 64, 8, 1, 1.61f, 2.43f, 0.234f, 0.150f, launch_split<4, 4, 8>},
+    {128, 128, 8, 2, 0.36f, 3.95f, 1.161f, 0.494f, launch_tiles<4, 2, 2, 4>},
+    {128, 256, 8, 1, 1.02f, 4.61f, 1.023f, 0.740f, launch_tiles<4, 4, 2, 4>},
+    {256, 256, 8, 1, 1.35f, 7.64f, 1.547f, 0.950f, launch_tiles<8, 4, 2, 4>},
 };
 
 float estimate(const Kernel& k, const Fp8LinearArgs& a, int cus) {
@@ -541,10 +541,7 @@ float estimate(const Kernel& k, const Fp8LinearArgs& a, int cus) {
   return us;
 }
 
-}  // namespace
-
-hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream) {
-  if (a.T <= 0) return hipSuccess;
+const Kernel& choose(const Fp8LinearArgs& a, int cus) {
   const Kernel* best = nullptr;
   float least = 0.f;
   for (const Kernel& k : kKernels) {
@@ -555,7 +552,18 @@ hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream
       least = us;
     }
   }
-  return best->launch(a, stream);
+  return *best;
+}
+
+}  // namespace
+
+Fp8LinearPlan plan_fp8_linear(const Fp8LinearArgs& a, int cus) {
+  const Kernel& k = choose(a, cus);
+  return {k.rows, k.tokens, k.waves};
+}
+
+hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream) {
+  return a.T <= 0 ? hipSuccess : choose(a, cus).launch(a, stream);
 }
 
 }  // namespace uqm

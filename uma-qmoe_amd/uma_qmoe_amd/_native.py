@@ -141,6 +141,7 @@ SIGNATURES = {
     "uqm_silu_mul": (ctypes.c_int, (_vp, _i64, _i64, _vp, _vp, _vp, _vp)),
     "uqm_fp8_quantize": (ctypes.c_int, (_vp, _i64, _i64, _i64, _vp, _vp, _vp)),
     "uqm_fp8_linear": (ctypes.c_int, (_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp)),
+    "uqm_fp8_linear_plan": (ctypes.c_int, (_i64, _i64, _i64, *[ctypes.POINTER(_i32)] * 3)),
     "uqm_set_option": (ctypes.c_int, (ctypes.c_int, _i64)),
     "uqm_workspace_status": (ctypes.c_int, (_vp, ctypes.c_size_t, _vp)),
     "uqm_noalloc_status": (ctypes.c_int, (_vp,)),
