@@ -64,9 +64,11 @@ constexpr int kScaleBlocks = 8;             // blocks whose scales are loaded to
 // blocks split over its W waves. Each wave loads its blocks into a place of its
 // own in LDS, the next one while it multiplies, and waits for nobody until the
 // sums of all waves are added, in wave order.
-// The address unit bounds it (64 bytes a cycle, 16 cycles a load): 512 x 2048 x
-// 5632 is 704 KB a CU, 5 us. The scales therefore come for 8 blocks at a time, 32
-// bytes of 8 tokens a load: a load per block took 64 cache lines each time.
+// 512 x 2048 x 5632 (13 us) loads 704 KB a CU, at 64 bytes a cycle 5 us; the address
+// unit is busy for half of the time, the waves wait for loads 38% of theirs. The
+// scales come for 8 blocks at a time, 32 bytes of 8 tokens a load: a load per
+// block took 64 cache lines each time (14.5 us). Fewer tokens are bound by what the
+// memory gives: 1 x 11264 x 2048 6.2 us, 23 MB, 3.7 TB/s with the launch.
 template <int TN, int TT, int W>
 struct Split {
   static constexpr int kBlock = (TN + TT) * 16 * kFp8Group;  // bytes of a block's operands
@@ -245,18 +247,19 @@ hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
 // * TT tokens in registers. A block of a wave is TN * TT products of 32 cycles and
 // four FMAs each, which run under the products (the two waves of a SIMD in turn
 // reach 4.2 PFLOP/s with nothing else to do).
-// What bounds it: 8191 x 11264 x 2048 takes 191 us (1.97 PFLOP/s; a library product
+// What bounds it: 8191 x 11264 x 2048 takes 194 us (1.95 PFLOP/s; a library product
 // with one scale for a whole matrix 201 us, its best rate, at 8192^3, 2.74; this
-// kernel there 2.44). The matrix cores work 44% of its cycles at 2.07 GHz. Timed
-// with parts left out (8192^3, 459 us): without the loads 387, without the reads
-// of LDS as well 292, so the operands' way through LDS costs the most, the loads'
-// latency next; the barrier costs 2%, four operands of the weight in flight
-// instead of two nothing. A quarter of the time at K = 2048 is the start and end of
-// a tile (7.6 us of 32); workgroups that walk over their tiles, with the next one's
-// loads under the last one's stores, took 214 us instead of 196.
-// Steps (8191 x 11264 x 2048, us): loads behind one wait per block 251, a wait only
-// where a stage is needed and loads in two halves 225 with the scales in panels,
-// results of two tiles side by side (64-byte stores) 196, loads through buffers 192.
+// kernel there 2.40). The matrix cores work 46% of its cycles at 2.05 GHz. Timed
+// with parts left out (8192^3, 458 us): without the operands' loads 384, without
+// the scales as well 363, without the reads of LDS as well 317, which leaves the
+// products, the FMAs and the barrier; so the loads cost the most, the reads next.
+// Four operands of the weight in flight instead of two gave nothing. A quarter of
+// the time at K = 2048 is the start and end of a tile (7.6 us of 32, from the fit
+// below); workgroups that walk over their tiles, with the next one's loads under
+// the last one's stores, took 214 us instead of 196.
+// Steps (8191 x 11264 x 2048, us): one float of scales per token and block straight
+// into registers 251, scales in panels 233, loads in two halves 225, results of two
+// tiles side by side (64-byte stores) 202, loads through buffers 196.
 constexpr int64_t kFp8TileMaxK = int64_t{1} << 23;  // 256 rows of fewer bytes stay below it
 
 template <int TN, int TT, int WN, int WT>
