@@ -293,7 +293,9 @@ int uqm_dequantize(int32_t encoding, const void* data, const float* scales, int6
  * A block that holds a NaN or an infinity gets a scale that is one too, and
  * codes that are NaN or 0; a product with it is NaN. None of these entry points
  * needs a workspace, and every result is the same for the same inputs. rows = 0
- * does nothing. No counterpart in the reference, whose dense layers are BF16. */
+ * does nothing. Row operators of more rows than a launch has room for (2^32
+ * threads) take several launches; a product of so many outputs (some 2^31 rows
+ * or features of one) is refused. No counterpart in the reference, whose dense layers are BF16. */
 
 /* Residual addition and RMSNorm:
  *   s = bf16(input + residual) -> sum      (residual and sum NULL: s = input)

@@ -177,6 +177,24 @@ def test_wrappers(ext, call, words):
         call(ext)
 
 
+@pytest.mark.parametrize("t,n,k", [(1 << 28, 1, 16), ((1 << 31) - 1 - 4096, 1, 16), (1 << 24, 2048, 128), (1, (1 << 31) - 4096, 16),
+                                   (1 << 20, 11264, 1 << 23), (1 << 24, 256, (1 << 25) - 16)])
+def test_launches_have_room(t, n, k):
+    """A launch has less than 2^32 threads."""
+    rows, tokens, waves = fp8_cases.plan(t, n, k)
+    groups = -(-n // rows) * -(-t // tokens)
+    assert -(-groups // 8) * 8 * 64 * waves < 1 << 32
+
+
+@pytest.mark.parametrize("t,n,k", [((1 << 31) - 1, (1 << 31) - 1, 16), (1, (1 << 31) - 1, 16), ((1 << 31) - 1, 1, 16)])
+def test_more_outputs_than_a_launch_has_room_for(lib, t, n, k):
+    """2^31 - 1 rows in the largest workgroups: 2^23 of 512 threads, 2^32 threads."""
+    got = [ctypes.c_int32() for _ in range(3)]
+    assert lib.uqm_fp8_linear_plan(t, n, k, *map(ctypes.byref, got)) == 1
+    assert "room" in lib.uqm_last_error().decode()
+    refused(lib, "uqm_fp8_linear", (A, B, t, C, D, n, k, None, E), "room")
+
+
 def test_dequantize_of_a_matrix():
     m = Fp8Matrix(torch.ones(130, 130).to(torch.float8_e4m3fn), torch.tensor([[1.0, 2.0], [3.0, 4.0]]), 128)
     v = m.dequantize()

@@ -451,3 +451,38 @@ def test_linear_past_32_bits(hip_ext, t, n, k):
     y, tol = ref.linear64(x.codes[-40:], x.scales[-40:], w.codes[n0:], w.scales[n0 // 128:], None)
     y, tol = y[:, -200:], tol[:, -200:]
     assert ((got.double().cpu() - y).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("op,cols", [("norm", 513), ("quantize", 1025), ("silu", 1025)])
+def test_more_rows_than_a_launch_has_room_for(hip_ext, op, cols):
+    """2^24 workgroups of a row each are 2^32 threads."""
+    note(f"{op} of more rows than a launch has room for")
+    fn = {"norm": lambda v: hip_ext.add_rmsnorm(v, None, bf16=False, fp8=True)[2],
+          "quantize": hip_ext.fp8_quantize,
+          "silu": lambda v: hip_ext.silu_mul(v, bf16=False, fp8=True)[1]}[op]
+    part = normal(gen(4), 4099, cols * (2 if op == "silu" else 1)).to(DEV)
+    repeats = ((1 << 24) + 4098) // 4099 + 1
+    x = part.repeat(repeats, 1)
+    big, small = fn(x), fn(part)
+    del x
+    for i in (0, repeats // 2, repeats - 2, repeats - 1):  # the last two hold the second launch's rows
+        rows = slice(4099 * i, 4099 * (i + 1))
+        assert torch.equal(big.codes[rows].view(torch.uint8), small.codes.view(torch.uint8))
+        assert torch.equal(big.scales[rows], small.scales)
+
+
+def test_more_blocks_than_a_launch_has_room_for(hip_ext):
+    """2^24 blocks; the last, in a launch of its own, has 127 rows."""
+    note("blocks of more rows than a launch has room for")
+    rows = (1 << 31) - 1
+    part = normal(gen(5), 1024, 1).to(DEV)
+    x = part.repeat(1 << 21, 1)[:rows]
+    big, small = hip_ext.fp8_quantize(x, block_rows=128), hip_ext.fp8_quantize(part, block_rows=128)
+    last = hip_ext.fp8_quantize(part[-128:-1], block_rows=128)
+    del x
+    assert big.scales.shape == (1 << 24, 1)
+    for first in (0, rows // 2048 * 1024, rows - 2047):
+        assert torch.equal(big.codes[first:first + 1024].view(torch.uint8), small.codes.view(torch.uint8))
+        assert torch.equal(big.scales[first // 128:first // 128 + 8], small.scales)
+    assert torch.equal(big.codes[-127:].view(torch.uint8), last.codes.view(torch.uint8))
+    assert torch.equal(big.scales[-1:], last.scales)

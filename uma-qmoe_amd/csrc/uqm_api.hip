@@ -1412,6 +1412,12 @@ static int check_linear_extents(int64_t rows, int64_t out_features, int64_t in_f
     return fail(UQM_ERR_ARGUMENT, "fp8_linear: rows must be in [0, 2^31) and features in [1, 2^31)");
   if (in_features <= 0 || in_features % 16 != 0 || in_features >= uqm::kFp8MaxK)
     return fail(UQM_ERR_ARGUMENT, "fp8_linear: input features %lld must be a positive multiple of 16 below 2^25", (long long)in_features);
+  uqm::Fp8LinearArgs a{};
+  a.T = rows;
+  a.N = out_features;
+  a.K = in_features;
+  if (!uqm::fp8_linear_fits(a))
+    return fail(UQM_ERR_ARGUMENT, "fp8_linear: %lld x %lld outputs are more than a launch has room for", (long long)rows, (long long)out_features);
   return UQM_OK;
 }
 

@@ -49,7 +49,9 @@ struct Fp8LinearArgs {
   uint16_t* out;          // bf16 [T, N]
   int64_t T, N, K;        // K a multiple of 16 below kFp8MaxK
 };
-// Rows and tokens of a workgroup, and its waves, that the call takes.
+// Whether a launch has room for the outputs (2^31 of one token are the first without).
+bool fp8_linear_fits(const Fp8LinearArgs& a);
+// Rows and tokens of a workgroup, and its waves, that the call takes (zeros if it does not fit).
 struct Fp8LinearPlan {
   int rows, tokens, waves;
 };

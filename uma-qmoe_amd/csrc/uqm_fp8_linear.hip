@@ -229,7 +229,6 @@ template <int TN, int TT, int W>
 hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
   using G = Split<TN, TT, W>;
   const int64_t blocks_n = (a.N + 16 * TN - 1) / (16 * TN), blocks_t = (a.T + 16 * TT - 1) / (16 * TT);
-  if (blocks_n * blocks_t > 0x7FFFFFF) return hipErrorInvalidValue;
   const int64_t grid = (blocks_n * blocks_t + 7) / 8 * 8;
   auto* k = fp8_split_kernel<TN, TT, W>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
@@ -487,7 +486,6 @@ template <int TN, int TT, int WN, int WT>
 hipError_t launch_tiles(const Fp8LinearArgs& a, hipStream_t stream) {
   using G = Tile<TN, TT, WN, WT>;
   const int64_t tiles_n = (a.N + G::kRowsN - 1) / G::kRowsN, tiles_t = (a.T + G::kRowsT - 1) / G::kRowsT;
-  if (tiles_n * tiles_t > 0x7FFFFFF) return hipErrorInvalidValue;
   const int64_t grid = (tiles_n * tiles_t + 7) / 8 * 8;
   auto* k = a.K % kFp8Group == 0 ? fp8_tile_kernel<TN, TT, WN, WT, false> : fp8_tile_kernel<TN, TT, WN, WT, true>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
@@ -544,29 +542,45 @@ float estimate(const Kernel& k, const Fp8LinearArgs& a, int cus) {
   return us;
 }
 
-const Kernel& choose(const Fp8LinearArgs& a, int cus) {
+// Whether a kernel takes the columns, and a launch, which has less than 2^32
+// threads, has room for the call (whole eights of workgroups).
+bool fits(const Kernel& k, const Fp8LinearArgs& a) {
+  if (k.rows >= 128 && a.K >= kFp8TileMaxK) return false;
+  const int64_t items = (a.N + k.rows - 1) / k.rows * ((a.T + k.tokens - 1) / k.tokens);
+  return (items + 7) / 8 * 8 <= 0xFFFFFFFF / (64 * k.waves);
+}
+
+const Kernel* choose(const Fp8LinearArgs& a, int cus) {
   const Kernel* best = nullptr;
   float least = 0.f;
   for (const Kernel& k : kKernels) {
-    if (k.rows >= 128 && a.K >= kFp8TileMaxK) continue;
+    if (!fits(k, a)) continue;
     const float us = estimate(k, a, cus);
     if (best == nullptr || us < least) {
       best = &k;
       least = us;
     }
   }
-  return *best;
+  return best;
 }
 
 }  // namespace
 
+bool fp8_linear_fits(const Fp8LinearArgs& a) {
+  for (const Kernel& k : kKernels)
+    if (fits(k, a)) return true;
+  return false;
+}
+
 Fp8LinearPlan plan_fp8_linear(const Fp8LinearArgs& a, int cus) {
-  const Kernel& k = choose(a, cus);
-  return {k.rows, k.tokens, k.waves};
+  const Kernel* k = choose(a, cus);
+  return k == nullptr ? Fp8LinearPlan{} : Fp8LinearPlan{k->rows, k->tokens, k->waves};
 }
 
 hipError_t launch_fp8_linear(const Fp8LinearArgs& a, int cus, hipStream_t stream) {
-  return a.T <= 0 ? hipSuccess : choose(a, cus).launch(a, stream);
+  if (a.T <= 0) return hipSuccess;
+  const Kernel* k = choose(a, cus);
+  return k == nullptr ? hipErrorInvalidValue : k->launch(a, stream);
 }
 
 }  // namespace uqm

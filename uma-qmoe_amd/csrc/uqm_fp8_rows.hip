@@ -10,6 +10,7 @@
 #include "uqm_device.h"
 #include "uqm_fp8.h"
 
+#include <algorithm>
 #include <initializer_list>
 
 namespace uqm {
@@ -318,14 +319,28 @@ bool aligned(int64_t cols, std::initializer_list<const void*> wide, const void* 
   return cols % 8 == 0 && (bits & 15u) == 0 && (reinterpret_cast<uintptr_t>(codes) & 7u) == 0;
 }
 
-constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+// A launch has less than 2^32 threads, so more workgroups than these take several
+// launches, each of whole rows.
+constexpr int64_t kMaxGrid = 0xFFFFFFFF / kThreads;
+
+template <typename T>
+T* behind(T* p, int64_t elements) {
+  return p == nullptr ? nullptr : p + elements;
+}
+RowOutputs behind(const RowOutputs& out, int64_t rows, int64_t cols) {
+  return {behind(out.bf16, rows * cols), behind(out.codes, rows * cols),
+          behind(out.scales, rows * ((cols + kFp8Group - 1) / kFp8Group))};
+}
+// Rows of a launch of silu_mul_kernel or quantize_rows_kernel.
+int64_t place_rows(int64_t chunks) {
+  return chunks >= kThreads ? kMaxGrid / ((chunks + kThreads - 1) / kThreads) : kMaxGrid * (kThreads / chunks);
+}
 
 }  // namespace
 
 hipError_t launch_add_rmsnorm(const uint16_t* x, const uint16_t* r, int64_t rows, int64_t cols, const uint16_t* weight,
                               float eps, uint16_t* sum, const RowOutputs& out, hipStream_t stream) {
   if (rows <= 0) return hipSuccess;
-  if (rows > kMaxGrid) return hipErrorInvalidValue;
   const bool vec = aligned(cols, {x, r, weight, sum, out.bf16}, out.codes);
   const int64_t passes = (cols + 8 * kThreads - 1) / (8 * kThreads);
   const int lanes = cols <= kFp8Group ? 16 : cols <= 512 ? 64 : kThreads;
@@ -337,19 +352,26 @@ hipError_t launch_add_rmsnorm(const uint16_t* x, const uint16_t* r, int64_t rows
             : passes <= 4 ? (vec ? add_rmsnorm_kernel<kThreads, 4, true> : add_rmsnorm_kernel<kThreads, 4, false>)
                           : (vec ? add_rmsnorm_kernel<kThreads, 0, true> : add_rmsnorm_kernel<kThreads, 0, false>);
   const int64_t per = kThreads / lanes;
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kThreads), 0, stream, x, r, rows, cols,
-                     weight, eps, sum, out);
-  return hipGetLastError();
+  for (int64_t first = 0; first < rows; first += kMaxGrid * per) {
+    const int64_t n = std::min(rows - first, kMaxGrid * per), at = first * cols;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((n + per - 1) / per)), dim3(kThreads), 0, stream, behind(x, at),
+                       behind(r, at), n, cols, weight, eps, behind(sum, at), behind(out, first, cols));
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_silu_mul(const uint16_t* gate_up, int64_t rows, int64_t cols, const RowOutputs& out,
                            hipStream_t stream) {
-  if (rows <= 0) return hipSuccess;
-  const int64_t grid = place_grid(rows, chunks_of(cols));
-  if (grid > kMaxGrid) return hipErrorInvalidValue;
   auto* k = aligned(cols, {gate_up, out.bf16}, out.codes) ? silu_mul_kernel<true> : silu_mul_kernel<false>;
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, gate_up, rows, cols, out);
-  return hipGetLastError();
+  const int64_t chunks = chunks_of(cols), step = place_rows(chunks);
+  for (int64_t first = 0; first < rows; first += step) {
+    const int64_t n = std::min(rows - first, step);
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(place_grid(n, chunks))), dim3(kThreads), 0, stream,
+                       gate_up + first * 2 * cols, n, cols, behind(out, first, cols));
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_fp8_quantize(const uint16_t* x, int64_t rows, int64_t cols, int block_rows, uint8_t* codes,
@@ -358,17 +380,23 @@ hipError_t launch_fp8_quantize(const uint16_t* x, int64_t rows, int64_t cols, in
   const bool vec = aligned(cols, {x}, codes);
   const bool blocks = block_rows == kFp8Group;
   const int64_t across = (cols + kFp8Group - 1) / kFp8Group;
-  const int64_t grid = blocks ? (rows + kFp8Group - 1) / kFp8Group * across : place_grid(rows, chunks_of(cols));
-  if (grid > kMaxGrid) return hipErrorInvalidValue;
-  const dim3 g(static_cast<unsigned>(grid)), t(kThreads);
-  if (blocks) {
-    auto* k = vec ? quantize_blocks_kernel<true> : quantize_blocks_kernel<false>;
-    hipLaunchKernelGGL(k, g, t, 0, stream, x, rows, cols, codes, scales);
-  } else {
-    auto* k = vec ? quantize_rows_kernel<true> : quantize_rows_kernel<false>;
-    hipLaunchKernelGGL(k, g, t, 0, stream, x, rows, cols, RowOutputs{nullptr, codes, scales});
+  const int64_t chunks = chunks_of(cols), step = blocks ? kMaxGrid / across * kFp8Group : place_rows(chunks);
+  if (step == 0) return hipErrorInvalidValue;  // (2^31 - 127 columns or more in blocks)
+  for (int64_t first = 0; first < rows; first += step) {
+    const int64_t n = std::min(rows - first, step), at = first * cols;
+    const dim3 t(kThreads);
+    if (blocks) {
+      const dim3 g(static_cast<unsigned>((n + kFp8Group - 1) / kFp8Group * across));
+      auto* k = vec ? quantize_blocks_kernel<true> : quantize_blocks_kernel<false>;
+      hipLaunchKernelGGL(k, g, t, 0, stream, x + at, n, cols, codes + at, scales + first / kFp8Group * across);
+    } else {
+      auto* k = vec ? quantize_rows_kernel<true> : quantize_rows_kernel<false>;
+      hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(place_grid(n, chunks))), t, 0, stream, x + at, n, cols,
+                         behind(RowOutputs{nullptr, codes, scales}, first, cols));
+    }
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 }  // namespace uqm
