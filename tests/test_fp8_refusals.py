@@ -213,3 +213,33 @@ def test_dense_layers_of_the_host():
         load_fixed_qwen("nowhere", "nothing", model_manifest_sha256="0" * 64, device="cpu", fp8_dense=True)
     with pytest.raises(ContractError, match="HIP device"):
         quantize_dense_fp8(torch.nn.Linear(16, 16))
+
+
+def dense_layer(**changes):
+    """A stand-in for a host's layer, BF16 on the CPU."""
+    from types import SimpleNamespace
+
+    size = {"q_proj": 32, "k_proj": 32, "v_proj": 32, "o_proj": 32, "gate_proj": 32, "up_proj": 32, "down_proj": 48}
+    m = {n: changes.get(n, torch.nn.Linear(k, 32, bias=n in ("q_proj", "k_proj", "v_proj"), dtype=torch.bfloat16)) for n, k in size.items()}
+    attn = SimpleNamespace(**{n: m[n] for n in ("q_proj", "k_proj", "v_proj", "o_proj")})
+    shared = SimpleNamespace(**{n: m[n] for n in ("gate_proj", "up_proj", "down_proj")})
+    return SimpleNamespace(self_attn=attn, mlp=SimpleNamespace(shared_expert=shared, fused_block=changes.get("fused", False)))
+
+
+@pytest.mark.parametrize("changes,words", [
+    ({"fused": True}, "fused_block=False"),
+    ({"o_proj": torch.nn.Identity()}, "BF16 Linear"),
+    ({"q_proj": torch.nn.Linear(32, 32)}, "BF16 Linear"),
+    ({"k_proj": torch.nn.Linear(40, 32, dtype=torch.bfloat16)}, "multiple of 16"),
+    ({"down_proj": torch.nn.Linear(24, 32, bias=False, dtype=torch.bfloat16)}, "multiple of 16"),
+    ({"up_proj": torch.nn.Linear(32, 32, dtype=torch.bfloat16)}, "no bias"),
+    ({"down_proj": torch.nn.Identity()}, "BF16 Linear"),
+])
+def test_dense_layers_that_stay_as_they_are(changes, words):
+    """All layers are looked at before the first is replaced."""
+    from uma_qmoe_amd.formats import ContractError
+    from uma_qmoe_amd.qwen_host import _check_dense
+
+    _check_dense([dense_layer(), dense_layer()])
+    with pytest.raises(ContractError, match=words):
+        _check_dense([dense_layer(), dense_layer(**changes)])

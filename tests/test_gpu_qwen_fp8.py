@@ -10,8 +10,9 @@ import torch
 import fp8_reference as ref
 from qwen_tiny import ARCH, LAYERS, MANIFEST, prompt, write_checkpoint
 from uma_qmoe_amd.custom_op import REGISTRY
+from uma_qmoe_amd.formats import ContractError
 from uma_qmoe_amd.native_backend import install_packed_q4_backend
-from uma_qmoe_amd.qwen_host import DecodeGraph, load_fixed_qwen
+from uma_qmoe_amd.qwen_host import DecodeGraph, load_fixed_qwen, quantize_dense_fp8
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -85,3 +86,13 @@ def test_decode_graph_replays_the_eager_steps(checkpoint):
             torch.cuda.synchronize()
             assert torch.equal(got, want), f"token {i}"
             assert (graph.logits - eager.logits).norm() <= 1e-3 * eager.logits.norm(), f"step {i}"
+
+
+def test_a_second_call_is_refused(checkpoint):
+    print("[case] qwen fp8 twice", flush=True)
+    ids = prompt(3).to(DEV)
+    with load(checkpoint, fp8_dense=True) as host, torch.no_grad():
+        want = host.model(input_ids=ids).logits
+        with pytest.raises(ContractError, match="BF16 Linear"):
+            quantize_dense_fp8(host.model)
+        assert (host.model(input_ids=ids).logits - want).norm() <= 1e-3 * want.norm()

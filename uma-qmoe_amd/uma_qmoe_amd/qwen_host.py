@@ -152,26 +152,49 @@ def _fp8_classes():
 
 
 _FP8_CLASSES = None
+_ATTENTION = ("q_proj", "k_proj", "v_proj", "o_proj")
+
+
+def _check_dense(layers: Any) -> None:
+    """Refuses what ``quantize_dense_fp8`` cannot replace, before anything is."""
+    torch = _torch()
+    from .native_backend import PROJECTIONS
+
+    if any(getattr(layer.mlp, "fused_block", True) for layer in layers):
+        raise ContractError("8-bit dense layers require blocks with fused_block=False")
+    for i, layer in enumerate(layers):
+        shared = layer.mlp.shared_expert
+        modules = [(name, getattr(layer.self_attn, name, None)) for name in _ATTENTION]
+        modules += [(name, getattr(shared, name, None)) for name in PROJECTIONS]
+        for name, module in modules:
+            if not isinstance(module, torch.nn.Linear) or module.weight.dtype is not torch.bfloat16:
+                raise ContractError(f"8-bit dense layers require a BF16 Linear, layer {i}'s {name} is none")
+            if module.in_features % 16:
+                raise ContractError(f"8-bit dense layers require a multiple of 16 input features, layer {i}'s {name} "
+                                    f"has {module.in_features}")
+            if name in PROJECTIONS and module.bias is not None:
+                raise ContractError(f"8-bit shared experts have no bias, layer {i}'s {name} has one")
 
 
 def quantize_dense_fp8(model: Any) -> int:
     """Puts the dense projections of every layer into 8-bit floats: attention's
     q, k, v and o, and the shared expert of its quantized block, which must run
     it as a module of its own (``fused_block=False``). The BF16 weights are
-    dropped. Returns the number of weights replaced. No counterpart in the
+    dropped. Refuses, with the model as it was, projections that are no BF16
+    Linear (a model that is in 8 bits already) or whose input features are no
+    multiple of 16. Returns the number of weights replaced. No counterpart in the
     reference, whose dense layers are BF16."""
     global _FP8_CLASSES
     if next(model.parameters()).device.type != "cuda":
         raise ContractError("8-bit dense layers require a HIP device")
     layers = model.model.layers
-    if any(getattr(layer.mlp, "fused_block", True) for layer in layers):
-        raise ContractError("8-bit dense layers require blocks with fused_block=False")
+    _check_dense(layers)
     if _FP8_CLASSES is None:
         _FP8_CLASSES = _fp8_classes()
     linear, shared = _FP8_CLASSES
     count = 0
     for layer in layers:
-        for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
+        for name in _ATTENTION:
             old = getattr(layer.self_attn, name)
             setattr(layer.self_attn, name, linear(old.weight, old.bias))
         layer.mlp.shared_expert = shared(layer.mlp.shared_expert)
