@@ -341,7 +341,7 @@ def test_linear_of_bf16_and_batches(hip_ext):
 
 
 # ------------------------------------------------------------------- together --
-def ffn(ext, hidden, residual, norm, gate_up, down, fp8=True):
+def ffn(ext, hidden, residual, norm, gate_up, down):
     """The dense gated layer that the operators make together."""
     total, _, q = ext.add_rmsnorm(hidden, residual, 1e-6, norm, bf16=False, fp8=True)
     _, h = ext.silu_mul(ext.fp8_linear(q, gate_up), bf16=False, fp8=True)
