@@ -29,3 +29,11 @@ PLANNED = [
     ((128, 256, 8), 665, 10446, 1344), ((128, 256, 8), 1024, 7680, 1536),
     ((256, 256, 8), 6172, 2433, 272), ((256, 256, 8), 4096, 2304, 256),
 ]
+
+# the last tile has one row and one token, so that its buffers are shorter than the
+# blocks that are loaded ahead, and their scales than a panel of 8
+ONE_ROW = [
+    ((128, 128, 8), 6529, 257, 16), ((128, 128, 8), 6529, 257, 128), ((128, 128, 8), 6529, 257, 144),
+    ((128, 256, 8), 13569, 1025, 1040), ((256, 256, 8), 15105, 1537, 128), ((256, 256, 8), 14081, 513, 144),
+    ((256, 256, 8), 13057, 513, 1040),
+]

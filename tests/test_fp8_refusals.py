@@ -110,7 +110,7 @@ def test_fp8_linear_plan(lib, args, words):
 def test_cases_reach_every_kernel(lib):
     """The GPU tests' sizes (planned for 256 compute units) take the kernels that
     they say, and no size takes another one."""
-    assert all(fp8_cases.plan(t, n, k) == kernel for kernel, t, n, k in fp8_cases.PLANNED)
+    assert all(fp8_cases.plan(t, n, k) == kernel for kernel, t, n, k in fp8_cases.PLANNED + fp8_cases.ONE_ROW)
     known = {kernel for kernel, *_ in fp8_cases.PLANNED}
     sizes = [1, 3, 16, 33, 100, 300, 777, 1500, 4000, 9000, 40000]
     assert {fp8_cases.plan(t, n, 16 * k) for t in sizes for n in sizes for k in (1, 8, 40, 128, 600, 600000)} == known

@@ -291,7 +291,7 @@ def test_linear_leaves_its_surroundings(hip_ext, t, n, k):
     assert torch.equal(shifted.view(t, n), want)
 
 
-@pytest.mark.parametrize("kernel,t,n,k", fp8_cases.PLANNED)
+@pytest.mark.parametrize("kernel,t,n,k", fp8_cases.PLANNED + fp8_cases.ONE_ROW)
 def test_linear_kernels(hip_ext, kernel, t, n, k):
     """Every kernel, at whole and at ragged sizes: the product, again with the
     same bits, with rows lost to NaN that the others must not see, and at an

@@ -41,6 +41,8 @@ __device__ __forceinline__ void dma4_to(const void* src, uint32_t lds_addr) {
 // and the address is a scalar base plus the lane's 32-bit offset plus a scalar
 // one. (Unlike the loads above, which the compiler takes for accesses that also
 // count as LDS reads, so that it waits for all of these where it needs one.)
+// The scalar offset must stay below `bytes`: the lane's is compared with their
+// difference, and nothing says what a negative one means.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t stage_buffer(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
 }
