@@ -67,7 +67,9 @@ constexpr int kScaleBlocks = 8;             // blocks whose scales are loaded to
 // 512 x 2048 x 5632 (13 us) loads 704 KB a CU, at 64 bytes a cycle 5 us; the address
 // unit is busy for half of the time, the waves wait for loads 38% of theirs. The
 // scales come for 8 blocks at a time, 32 bytes of 8 tokens a load: a load per
-// block took 64 cache lines each time (14.5 us). Fewer tokens are bound by what the
+// block took 64 cache lines each time (14.5 us). The way through LDS is only for
+// whole lines: operands straight into registers, where a load takes 64 bytes of 16
+// rows, took 24.9 us (26.8 two blocks ahead). Fewer tokens are bound by what the
 // memory gives: 1 x 11264 x 2048 6.2 us, 23 MB, 3.7 TB/s with the launch.
 template <int TN, int TT, int W>
 struct Split {
@@ -246,7 +248,7 @@ hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
 // * TT tokens in registers. A block of a wave is TN * TT products of 32 cycles and
 // four FMAs each, which run under the products (the two waves of a SIMD in turn
 // reach 4.2 PFLOP/s with nothing else to do).
-// What bounds it: 8191 x 11264 x 2048 takes 194 us (1.95 PFLOP/s; a library product
+// What bounds it: 8191 x 11264 x 2048 takes 196 us (1.93 PFLOP/s; a library product
 // with one scale for a whole matrix 201 us, its best rate, at 8192^3, 2.74; this
 // kernel there 2.40). The matrix cores work 46% of its cycles at 2.05 GHz. Timed
 // with parts left out (8192^3, 458 us): without the operands' loads 384, without
