@@ -52,6 +52,13 @@ def test_add_rmsnorm(lib, args, words):
     refused(lib, "uqm_add_rmsnorm", args, words)
 
 
+@pytest.mark.parametrize("rows", [1, 4])
+def test_add_rmsnorm_keeps_its_weight(lib, rows):
+    """The sum may be written over the input or the residual, never over the
+    weight, which of one row has as many bytes."""
+    refused(lib, "uqm_add_rmsnorm", (A, B, rows, 128, C, 1e-6, C, D, None, None), "overlaps an input")
+
+
 @pytest.mark.parametrize("args,words", [
     ((A, -1, 128, B, None, None), "rows"),
     ((A, 4, 0, B, None, None), "columns"),

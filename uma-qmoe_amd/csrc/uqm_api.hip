@@ -1323,6 +1323,7 @@ bool misaligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintpt
 struct Span {
   const void* p;
   int64_t bytes;
+  bool in_place = false;  // of an input: the sum may be written over it
 };
 int check_rows(const char* what, int64_t rows, int64_t cols, std::initializer_list<Span> inputs, const void* output,
                const void* codes, const float* scales, Span also, int64_t block_rows = 1) {
@@ -1339,8 +1340,8 @@ int check_rows(const char* what, int64_t rows, int64_t cols, std::initializer_li
   for (size_t i = 0; i < sizeof(outs) / sizeof(outs[0]); ++i) {
     for (const Span& in : inputs) {
       if (in.p != nullptr && misaligned(in.p, 2)) return fail(UQM_ERR_ARGUMENT, "%s: inputs must be 2-byte aligned", what);
-      // (the sum may take an input's place element by element)
-      if (i == 3 && in.p == outs[i].p && in.bytes == outs[i].bytes) continue;
+      // (element by element; a weight is as long as one row's sum, but every row reads it)
+      if (i == 3 && in.in_place && in.p == outs[i].p && in.bytes == outs[i].bytes) continue;
       if (overlap(outs[i].p, outs[i].bytes, in.p, in.bytes)) return fail(UQM_ERR_ARGUMENT, "%s: an output overlaps an input", what);
     }
     for (size_t j = 0; j < i; ++j)
@@ -1361,7 +1362,7 @@ int uqm_add_rmsnorm(const void* input, const void* residual, int64_t rows, int64
   if ((residual == nullptr) != (sum == nullptr))
     return fail(UQM_ERR_ARGUMENT, "add_rmsnorm: residual and sum must be given together");
   const int64_t bytes = rows >= 0 && rows <= kMaxExtent && hidden_size > 0 && hidden_size <= kMaxExtent ? 2 * rows * hidden_size : 0;
-  int rc = check_rows("add_rmsnorm", rows, hidden_size, {{input, bytes}, {residual, bytes}, {weight, 2 * hidden_size}},
+  int rc = check_rows("add_rmsnorm", rows, hidden_size, {{input, bytes, true}, {residual, bytes, true}, {weight, 2 * hidden_size}},
                       output, codes, scales, {sum, bytes});
   if (rc) return rc;
   if (misaligned(sum, 2)) return fail(UQM_ERR_ARGUMENT, "add_rmsnorm: outputs must be aligned to their elements");
