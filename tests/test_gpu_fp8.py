@@ -115,6 +115,24 @@ def test_silu_mul_at_the_ends(hip_ext):
     assert q.scales.isnan().all() and q.codes.float().isnan().all()
 
 
+@pytest.mark.parametrize("cols", [16, 48, 130, 384, 648])
+def test_silu_mul_rows_keep_to_themselves(hip_ext, cols):
+    """A wave holds several narrow rows, or parts of two: gates whose exponential
+    overflows, infinities and NaN in every third row change no bit of the others."""
+    note(f"silu_mul rows {cols}")
+    x = normal(gen(cols), 3000, 2 * cols, std=4.0)
+    ends = x.clone()
+    ends[::3, :7] = torch.tensor([-88.0, -100.0, -3e38, float("-inf"), float("inf"), float("nan"), 3e38], dtype=torch.bfloat16)
+    want, q = hip_ext.silu_mul(x.to(DEV), fp8=True)
+    got, p = hip_ext.silu_mul(ends.to(DEV), fp8=True)
+    for rows in (slice(1, None, 3), slice(2, None, 3)):
+        assert torch.equal(p.scales[rows], q.scales[rows])
+        assert torch.equal(p.codes[rows].view(torch.uint8), q.codes[rows].view(torch.uint8))
+        assert torch.equal(got[rows], want[rows])
+    # and the other values of a row in BF16 neither
+    assert torch.equal(got[::3, 7:], want[::3, 7:])
+
+
 @pytest.mark.parametrize("block", [1, 128])
 @pytest.mark.parametrize("rows,offset", [(1, 0), (127, 0), (128, 1), (129, 0), (300, 0)])
 @pytest.mark.parametrize("cols", [1, 8, 120, 128, 129, 136, 1400, 2048, 2056])

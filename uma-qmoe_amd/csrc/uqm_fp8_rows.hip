@@ -235,8 +235,9 @@ int64_t place_grid(int64_t rows, int64_t chunks) {
 __host__ __device__ int64_t chunks_of(int64_t cols) { return (cols + kFp8Group - 1) / kFp8Group * (kFp8Group / 8); }
 
 // g / (1 + exp(-g)): the reciprocal with one Newton step, as near as the division
-// at half its instructions. It flushes subnormal results to 0, so a wave with a
-// gate below -87.3 (1 + exp(-g) from 2^126 on) divides.
+// at half its instructions. It flushes subnormal results to 0, so gates below
+// -87.3 (1 + exp(-g) from 2^126 on) divide, and only they: a wave holds parts of
+// several rows, and a row's result must not depend on its neighbours'.
 __device__ __forceinline__ void silu8(float (&g)[8]) {
   float d[8], most = 0.f;
 #pragma unroll
@@ -244,15 +245,16 @@ __device__ __forceinline__ void silu8(float (&g)[8]) {
     d[j] = 1.0f + __expf(-g[j]);
     most = fmaxf(most, d[j]);
   }
+  auto by_reciprocal = [&](int j) {
+    const float r = __builtin_amdgcn_rcpf(d[j]);
+    return g[j] * fmaf(fmaf(-d[j], r, 1.0f), r, r);
+  };
   if (__builtin_expect(__any(most > 0x1p126f), 0)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] /= d[j];
+    for (int j = 0; j < 8; ++j) g[j] = d[j] > 0x1p126f ? g[j] / d[j] : by_reciprocal(j);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float r = __builtin_amdgcn_rcpf(d[j]);
-      g[j] *= fmaf(fmaf(-d[j], r, 1.0f), r, r);
-    }
+    for (int j = 0; j < 8; ++j) g[j] = by_reciprocal(j);
   }
 }
 
