@@ -300,9 +300,10 @@ int uqm_dequantize(int32_t encoding, const void* data, const float* scales, int6
 /* Residual addition and RMSNorm:
  *   s = bf16(input + residual) -> sum      (residual and sum NULL: s = input)
  *   n = s * rsqrt(mean(s^2) + eps)
- *   output = bf16(weight * bf16(n))        (as uqm_rmsnorm; NULL: not wanted)
- *   codes, scales = weight * n in blocks of 1 x 128, not rounded to BF16
- *                                          in between (both NULL: not wanted)
+ *   output = bf16(weight * n)              (NULL: not wanted)
+ *   codes, scales = weight * n in blocks of 1 x 128 (both NULL: not wanted)
+ * (one rounding; uqm_rmsnorm rounds n to BF16 before the weight, as the models'
+ * own norms do, so its results may be up to three half steps of BF16 away)
  * bf16 [rows, hidden_size], any hidden_size; weight bf16 [hidden_size] or NULL
  * for ones. sum may be input or residual itself; outputs must not overlap
  * otherwise. Rows of a multiple of 8 elements on 16-byte aligned tensors (codes:

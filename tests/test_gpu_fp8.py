@@ -71,6 +71,19 @@ def test_add_rmsnorm(hip_ext, rows, cols, offset, residual):
         assert only[0] is keep and torch.equal(keep, total)
 
 
+@pytest.mark.parametrize("rows,cols", [(9, 120), (5, 512), (64, 2048), (7, 8200), (3, 1401)])
+def test_add_rmsnorm_rounds_its_norm_once(hip_ext, rows, cols):
+    """The BF16 output is the FP32 value of w * n, whose codes the 8-bit output
+    holds, rounded once."""
+    note(f"add_rmsnorm rounds once {rows}x{cols}")
+    g = gen(rows)
+    x, r = normal(g, rows, cols), normal(g, rows, cols, std=4.0)
+    w = (1 + 0.3 * torch.randn(cols, generator=g)).to(torch.bfloat16)
+    total, n, _ = hip_ext.add_rmsnorm(x.to(DEV), r.to(DEV), 1e-6, w.to(DEV), fp8=True)
+    y = ref.rmsnorm64(total.double().cpu(), 1e-6, w.double())
+    assert ((n.double().cpu() - y).abs() <= ((1 + ref.BF16) * (1 + ref.rmsnorm_delta(cols)) - 1) * y.abs()).all()
+
+
 def test_add_rmsnorm_rounds_as_rmsnorm(hip_ext):
     """The BF16 output is uqm_rmsnorm's of the same sum: both divide by the same
     root up to the order of its sum, so at most one step of each rounding."""

@@ -27,7 +27,7 @@ struct RowOutputs {
 };
 
 // s = bf16(x + r) -> sum (r NULL: s = x, nothing written); n = s * rsqrt(mean(s^2) + eps);
-// BF16 output bf16(w * bf16(n)), codes of w * n. weight NULL: ones. sum may be x or r.
+// BF16 output bf16(w * n), codes of the same w * n. weight NULL: ones. sum may be x or r.
 hipError_t launch_add_rmsnorm(const uint16_t* x, const uint16_t* r, int64_t rows, int64_t cols, const uint16_t* weight,
                               float eps, uint16_t* sum, const RowOutputs& out, hipStream_t stream);
 // y = silu(g) * u of rows [g (cols) | u (cols)].

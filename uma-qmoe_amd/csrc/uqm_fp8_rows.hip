@@ -158,16 +158,10 @@ __global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const uint16_t* x
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = 1.0f;
     if (weight != nullptr) load8<VEC>(weight, c, cols, w);
-    if (out.bf16 != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = w[j] * round_bf16(s[j] * rstd);
-      store8_bf16<VEC>(out.bf16 + at, c, cols, y);
-    }
-    if (out.codes != nullptr) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = w[j] * (s[j] * rstd);
-      write_fp8<VEC>(out, row, c, cols, all_cols, y);
-    }
+    for (int j = 0; j < 8; ++j) y[j] = w[j] * (s[j] * rstd);
+    if (out.bf16 != nullptr) store8_bf16<VEC>(out.bf16 + at, c, cols, y);
+    if (out.codes != nullptr) write_fp8<VEC>(out, row, c, cols, all_cols, y);
   };
   float ss = 0.f;
   auto add = [&](const float (&s)[8]) {

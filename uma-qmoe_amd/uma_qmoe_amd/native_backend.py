@@ -464,8 +464,8 @@ class HipExtension:
 
     def add_rmsnorm(self, hidden, residual=None, eps=1e-6, weight=None, *, bf16=True, fp8=False, inplace=False):
         """s = hidden + residual (BF16) and RMSNorm(s): (s, the norm in BF16 or
-        None, the norm as an ``Fp8Matrix`` or None). The BF16 norm rounds as
-        ``rmsnorm`` does; the 8-bit one is taken before any rounding to BF16.
+        None, the norm as an ``Fp8Matrix`` or None). Both round the FP32 norm
+        once; ``rmsnorm`` rounds it to BF16 before the weight's product as well.
         Without a residual s is ``hidden`` itself. ``inplace`` writes s over
         ``residual``."""
         torch = self.torch
