@@ -289,7 +289,9 @@ int uqm_dequantize(int32_t encoding, const void* data, const float* scales, int6
  * smaller. Codes [rows, cols] and scales [ceil(rows / block_rows),
  * ceil(cols / 128)] are row-major and contiguous.
  *   d = max|v| / 448, at least 2^-126; 1 for a block of zeros
- *   code = e4m3(v / d), to nearest even
+ *   code = e4m3(v * r), r = 1 / d rounded to FP32, to nearest even: v / d but for
+ *          two FP32 roundings, so that a v / d within 2^-23 of itself of the middle
+ *          between two codes may get either (their distances differ by no more)
  * A block that holds a NaN or an infinity gets a scale that is one too, and
  * codes that are NaN or 0; a product with it is NaN. None of these entry points
  * needs a workspace, and every result is the same for the same inputs. rows = 0

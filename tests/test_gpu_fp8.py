@@ -166,6 +166,27 @@ def test_quantize_bits(hip_ext, rows, cols, offset, block):
 
 
 @pytest.mark.parametrize("block", [1, 128])
+def test_quantize_takes_a_nearest_code(hip_ext, block):
+    """No e4m3 value is nearer to v / d than the code, but by the roundings of 1 / d
+    and of its product with v (U each). BF16 values are often the middle between
+    two codes, up to them: 0.80859375 beside 1.078125 is 336, between 320 and 352."""
+    note(f"fp8_quantize nearest block={block}")
+    x = normal(gen(12), 256, 512)
+    x[:128, :128] = x[:128, :128].clamp(-1, 1)
+    x[:128, 0] = 1.078125
+    x[:128, 1] = 0.80859375
+    q = hip_ext.fp8_quantize(x.to(DEV), block_rows=block)
+    v = x.double() / ref.each(q.scales.double().cpu(), block, *x.shape)
+    codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    codes = codes[codes.isfinite()].sort().values
+    at = torch.searchsorted(codes, v).clamp(1, len(codes) - 1)
+    nearest = torch.minimum((v - codes[at - 1]).abs(), (v - codes[at]).abs())
+    off = (q.codes.double().cpu() - v).abs()
+    assert (off <= nearest + 2 * 2.001 * ref.U * v.abs()).all()
+    assert q.codes[0, 1].item() in (320, 352)
+
+
+@pytest.mark.parametrize("block", [1, 128])
 def test_quantize_ends(hip_ext, block):
     """Groups of zeros, of the smallest and largest values, with a NaN or an
     infinity; every one beside an ordinary group that is left alone."""

@@ -5,7 +5,12 @@
 // (weights), the last one of a row or of the rows possibly shorter. Its scale is
 //   d = 1                        if every |v| is 0,
 //       max(max|v| / 448, 2^-126) otherwise,
-// and a code is e4m3(v / d), to nearest even. The lower limit keeps 1 / d finite.
+// and a code is e4m3(v * r), r = 1 / d rounded to FP32, to nearest even. That is v / d
+// but for two FP32 roundings: where v / d is the middle between two codes up to
+// 2^-23 of itself, the code may be the other one, as near as the one of the
+// division (1 of 2000 codes of normal BF16 values; d itself is a rounded number, and
+// against v / d in 64 bits the product is off no more often than an FP32 division).
+// The lower limit of d keeps r finite.
 // A group that holds a NaN or an infinity has a scale that is one, too (the
 // maximum is taken over the bits, which keeps a NaN), and its codes are NaN or 0:
 // every product of the row comes out as NaN.

@@ -72,6 +72,7 @@ __device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float 
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
 }
 
+// (inv = 1 / d: one division a group; the codes are defined by the product with it)
 template <bool VEC>
 __device__ __forceinline__ void store8_fp8(uint8_t* row, int64_t c, int64_t cols, const float (&v)[8], float inv) {
   const uint32_t lo = pack_fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
