@@ -356,7 +356,10 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
   // a load takes 8 tokens' 32 bytes. (One float per token and block, straight into
   // registers, were 16 cache lines a load, fetched again for every block: with
   // them 8192 x 8192 x 8192 took 622 us, without any 482.)
-  static_assert((G::kLoadsS & (G::kLoadsS - 1)) == 0 && G::kLoadsS <= kScaleBlocks, "one load a block");
+  // (The last new load of a panel is issued at block kLoadsS - 1 of the panel before
+  // and has landed behind that block's barrier; the panel is first read in the last
+  // block of the panel before, which with as many loads as blocks would issue one itself.)
+  static_assert((G::kLoadsS & (G::kLoadsS - 1)) == 0 && G::kLoadsS < kScaleBlocks, "landed before it is read");
   const auto sbuf = stage_buffer(a.xs + t0 * KB, static_cast<uint32_t>(last_t + 1) * (4 * KB));
   auto s_panel = [&](int slot) { return static_cast<uint32_t>(2 * (G::kPanelN + G::kPanelT) + slot * G::kScalePanel); };
   auto load_scales = [&](int j, int panel) {
@@ -411,7 +414,8 @@ __global__ __launch_bounds__(64 * WN * WT, 1) void fp8_tile_kernel(Fp8LinearArgs
     fw = ws[min(b + 1, KB - 1)];
 #pragma unroll
     for (int n = 0; n < TN; ++n) {
-      // (a panel's loads twice over; the second time they write what is there)
+      // (a panel's loads kScaleBlocks / kLoadsS times over; from the second time on they
+      // write what is there)
       if (n == TN / 2) {
         load_scales(b % G::kLoadsS, b / kScaleBlocks + 1);
         read_scales(min(b + 1, KB - 1));
