@@ -250,3 +250,15 @@ def test_dense_layers_that_stay_as_they_are(changes, words):
     _check_dense([dense_layer(), dense_layer()])
     with pytest.raises(ContractError, match=words):
         _check_dense([dense_layer(), dense_layer(**changes)])
+
+
+def test_dense_layers_with_a_bias_in_fp32():
+    """A BF16 weight with an FP32 bias is refused with the model as it was, not by
+    every product afterwards."""
+    from uma_qmoe_amd.formats import ContractError
+    from uma_qmoe_amd.qwen_host import _check_dense
+
+    q_proj = torch.nn.Linear(32, 32, dtype=torch.bfloat16)
+    q_proj.bias = torch.nn.Parameter(q_proj.bias.detach().float())
+    with pytest.raises(ContractError, match="BF16 bias"):
+        _check_dense([dense_layer(), dense_layer(q_proj=q_proj)])

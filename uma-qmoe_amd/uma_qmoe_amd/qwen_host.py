@@ -172,6 +172,8 @@ def _check_dense(layers: Any) -> None:
             if module.in_features % 16:
                 raise ContractError(f"8-bit dense layers require a multiple of 16 input features, layer {i}'s {name} "
                                     f"has {module.in_features}")
+            if module.bias is not None and module.bias.dtype is not torch.bfloat16:
+                raise ContractError(f"8-bit dense layers require a BF16 bias, layer {i}'s {name} has {module.bias.dtype}")
             if name in PROJECTIONS and module.bias is not None:
                 raise ContractError(f"8-bit shared experts have no bias, layer {i}'s {name} has one")
 
@@ -181,8 +183,8 @@ def quantize_dense_fp8(model: Any) -> int:
     q, k, v and o, and the shared expert of its quantized block, which must run
     it as a module of its own (``fused_block=False``). The BF16 weights are
     dropped. Refuses, with the model as it was, projections that are no BF16
-    Linear (a model that is in 8 bits already) or whose input features are no
-    multiple of 16. Returns the number of weights replaced. No counterpart in the
+    Linear (a model that is in 8 bits already), have a bias that is not BF16, or
+    whose input features are no multiple of 16. Returns the number of weights replaced. No counterpart in the
     reference, whose dense layers are BF16."""
     global _FP8_CLASSES
     if next(model.parameters()).device.type != "cuda":
