@@ -262,3 +262,28 @@ def test_dense_layers_with_a_bias_in_fp32():
     q_proj.bias = torch.nn.Parameter(q_proj.bias.detach().float())
     with pytest.raises(ContractError, match="BF16 bias"):
         _check_dense([dense_layer(), dense_layer(q_proj=q_proj)])
+
+
+def whole_layer(**changes):
+    """A stand-in whose shared expert's projections fit each other."""
+    return dense_layer(**{"down_proj": torch.nn.Linear(32, 32, bias=False, dtype=torch.bfloat16), **changes})
+
+
+def on_hip(*layers):
+    """A stand-in for a model whose first parameter is on a HIP device."""
+    from types import SimpleNamespace
+
+    return SimpleNamespace(parameters=lambda: iter([SimpleNamespace(device=torch.device("cuda:0"))]),
+                           model=SimpleNamespace(layers=layers))
+
+
+def test_dense_layers_on_the_host():
+    """Every projection's device counts, not the first parameter's alone."""
+    from uma_qmoe_amd.formats import ContractError
+    from uma_qmoe_amd.qwen_host import quantize_dense_fp8
+
+    layers = [whole_layer(), whole_layer()]
+    before = [(layer.self_attn.q_proj, layer.mlp.shared_expert) for layer in layers]
+    with pytest.raises(ContractError, match="HIP device, layer 0's q_proj is on cpu"):
+        quantize_dense_fp8(on_hip(*layers))
+    assert all(layer.self_attn.q_proj is q and layer.mlp.shared_expert is s for layer, (q, s) in zip(layers, before))

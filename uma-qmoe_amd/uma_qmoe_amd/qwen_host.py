@@ -155,6 +155,13 @@ _FP8_CLASSES = None
 _ATTENTION = ("q_proj", "k_proj", "v_proj", "o_proj")
 
 
+def _dense_projections(layer: Any) -> list[tuple[str, Any]]:
+    from .native_backend import PROJECTIONS
+
+    return [(name, getattr(layer.self_attn, name, None)) for name in _ATTENTION] + [
+        (name, getattr(layer.mlp.shared_expert, name, None)) for name in PROJECTIONS]
+
+
 def _check_dense(layers: Any) -> None:
     """Refuses what ``quantize_dense_fp8`` cannot replace, before anything is."""
     torch = _torch()
@@ -163,10 +170,7 @@ def _check_dense(layers: Any) -> None:
     if any(getattr(layer.mlp, "fused_block", True) for layer in layers):
         raise ContractError("8-bit dense layers require blocks with fused_block=False")
     for i, layer in enumerate(layers):
-        shared = layer.mlp.shared_expert
-        modules = [(name, getattr(layer.self_attn, name, None)) for name in _ATTENTION]
-        modules += [(name, getattr(shared, name, None)) for name in PROJECTIONS]
-        for name, module in modules:
+        for name, module in _dense_projections(layer):
             if not isinstance(module, torch.nn.Linear) or module.weight.dtype is not torch.bfloat16:
                 raise ContractError(f"8-bit dense layers require a BF16 Linear, layer {i}'s {name} is none")
             if module.in_features % 16:
@@ -178,19 +182,28 @@ def _check_dense(layers: Any) -> None:
                 raise ContractError(f"8-bit shared experts have no bias, layer {i}'s {name} has one")
 
 
+def _check_dense_devices(layers: Any) -> None:
+    for i, layer in enumerate(layers):
+        for name, module in _dense_projections(layer):
+            for t in (module.weight, module.bias):
+                if t is not None and t.device.type != "cuda":
+                    raise ContractError(f"8-bit dense layers require a HIP device, layer {i}'s {name} is on {t.device}")
+
+
 def quantize_dense_fp8(model: Any) -> int:
     """Puts the dense projections of every layer into 8-bit floats: attention's
     q, k, v and o, and the shared expert of its quantized block, which must run
     it as a module of its own (``fused_block=False``). The BF16 weights are
     dropped. Refuses, with the model as it was, projections that are no BF16
-    Linear (a model that is in 8 bits already), have a bias that is not BF16, or
-    whose input features are no multiple of 16. Returns the number of weights replaced. No counterpart in the
+    Linear (a model that is in 8 bits already), are not on a HIP device, have a
+    bias that is not BF16, or whose input features are no multiple of 16. Returns the number of weights replaced. No counterpart in the
     reference, whose dense layers are BF16."""
     global _FP8_CLASSES
     if next(model.parameters()).device.type != "cuda":
         raise ContractError("8-bit dense layers require a HIP device")
     layers = model.model.layers
     _check_dense(layers)
+    _check_dense_devices(layers)
     if _FP8_CLASSES is None:
         _FP8_CLASSES = _fp8_classes()
     linear, shared = _FP8_CLASSES
