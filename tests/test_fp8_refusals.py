@@ -287,3 +287,16 @@ def test_dense_layers_on_the_host():
     with pytest.raises(ContractError, match="HIP device, layer 0's q_proj is on cpu"):
         quantize_dense_fp8(on_hip(*layers))
     assert all(layer.self_attn.q_proj is q and layer.mlp.shared_expert is s for layer, (q, s) in zip(layers, before))
+
+
+@pytest.mark.parametrize("changes", [
+    {"down_proj": torch.nn.Linear(64, 32, bias=False, dtype=torch.bfloat16)},
+    {"gate_proj": torch.nn.Linear(48, 32, bias=False, dtype=torch.bfloat16)},
+    {"up_proj": torch.nn.Linear(32, 48, bias=False, dtype=torch.bfloat16)},
+])
+def test_dense_layers_that_do_not_fit_each_other(changes):
+    from uma_qmoe_amd.formats import ContractError
+    from uma_qmoe_amd.qwen_host import quantize_dense_fp8
+
+    with pytest.raises(ContractError, match="layer 1's shared expert"):
+        quantize_dense_fp8(on_hip(whole_layer(), whole_layer(**changes)))

@@ -182,6 +182,15 @@ def _check_dense(layers: Any) -> None:
                 raise ContractError(f"8-bit shared experts have no bias, layer {i}'s {name} has one")
 
 
+def _check_shared_expert(layers: Any) -> None:
+    for i, layer in enumerate(layers):
+        shared = layer.mlp.shared_expert
+        gate, up, down = shared.gate_proj, shared.up_proj, shared.down_proj
+        if gate.weight.shape != up.weight.shape or down.in_features != gate.out_features:
+            raise ContractError(f"layer {i}'s shared expert has projections that do not fit each other: gate "
+                                f"{tuple(gate.weight.shape)}, up {tuple(up.weight.shape)}, down {tuple(down.weight.shape)}")
+
+
 def _check_dense_devices(layers: Any) -> None:
     for i, layer in enumerate(layers):
         for name, module in _dense_projections(layer):
@@ -196,13 +205,15 @@ def quantize_dense_fp8(model: Any) -> int:
     it as a module of its own (``fused_block=False``). The BF16 weights are
     dropped. Refuses, with the model as it was, projections that are no BF16
     Linear (a model that is in 8 bits already), are not on a HIP device, have a
-    bias that is not BF16, or whose input features are no multiple of 16. Returns the number of weights replaced. No counterpart in the
-    reference, whose dense layers are BF16."""
+    bias that is not BF16 or input features that are no multiple of 16, and a
+    shared expert whose projections do not fit each other. Returns the number of
+    weights replaced. No counterpart in the reference, whose dense layers are BF16."""
     global _FP8_CLASSES
     if next(model.parameters()).device.type != "cuda":
         raise ContractError("8-bit dense layers require a HIP device")
     layers = model.model.layers
     _check_dense(layers)
+    _check_shared_expert(layers)
     _check_dense_devices(layers)
     if _FP8_CLASSES is None:
         _FP8_CLASSES = _fp8_classes()
