@@ -300,3 +300,15 @@ def test_dense_layers_that_do_not_fit_each_other(changes):
 
     with pytest.raises(ContractError, match="layer 1's shared expert"):
         quantize_dense_fp8(on_hip(whole_layer(), whole_layer(**changes)))
+
+
+def test_dense_layers_of_another_activation():
+    """The 8-bit shared expert computes SiLU, whatever the module's own function is."""
+    from uma_qmoe_amd.formats import ContractError
+    from uma_qmoe_amd.qwen_host import quantize_dense_fp8
+
+    layers = [whole_layer(), whole_layer()]
+    layers[0].mlp.shared_expert.act_fn = torch.nn.SiLU()
+    layers[1].mlp.shared_expert.act_fn = torch.nn.GELU()
+    with pytest.raises(ContractError, match="layer 1's shared expert .* SiLU"):
+        quantize_dense_fp8(on_hip(*layers))

@@ -183,12 +183,17 @@ def _check_dense(layers: Any) -> None:
 
 
 def _check_shared_expert(layers: Any) -> None:
+    torch = _torch()
+    probe = torch.linspace(-8.0, 8.0, 33, dtype=torch.float32, device="cpu")
     for i, layer in enumerate(layers):
         shared = layer.mlp.shared_expert
         gate, up, down = shared.gate_proj, shared.up_proj, shared.down_proj
         if gate.weight.shape != up.weight.shape or down.in_features != gate.out_features:
             raise ContractError(f"layer {i}'s shared expert has projections that do not fit each other: gate "
                                 f"{tuple(gate.weight.shape)}, up {tuple(up.weight.shape)}, down {tuple(down.weight.shape)}")
+        act = getattr(shared, "act_fn", None)  # (compared by value: a config's "silu" and "swish" are different classes)
+        if act is not None and not torch.allclose(act(probe), torch.nn.functional.silu(probe), atol=1e-6):
+            raise ContractError(f"layer {i}'s shared expert has another activation than SiLU")
 
 
 def _check_dense_devices(layers: Any) -> None:
@@ -206,8 +211,9 @@ def quantize_dense_fp8(model: Any) -> int:
     dropped. Refuses, with the model as it was, projections that are no BF16
     Linear (a model that is in 8 bits already), are not on a HIP device, have a
     bias that is not BF16 or input features that are no multiple of 16, and a
-    shared expert whose projections do not fit each other. Returns the number of
-    weights replaced. No counterpart in the reference, whose dense layers are BF16."""
+    shared expert whose projections do not fit each other or whose activation is
+    not SiLU. Returns the number of weights replaced. No counterpart in the
+    reference, whose dense layers are BF16."""
     global _FP8_CLASSES
     if next(model.parameters()).device.type != "cuda":
         raise ContractError("8-bit dense layers require a HIP device")
