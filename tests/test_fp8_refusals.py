@@ -312,3 +312,12 @@ def test_dense_layers_of_another_activation():
     layers[1].mlp.shared_expert.act_fn = torch.nn.GELU()
     with pytest.raises(ContractError, match="layer 1's shared expert .* SiLU"):
         quantize_dense_fp8(on_hip(*layers))
+
+
+def test_dense_layers_beside_a_fused_block():
+    """A caller who asks for the fused block does not get the other one unsaid."""
+    from uma_qmoe_amd.formats import ContractError
+    from uma_qmoe_amd.qwen_host import load_fixed_qwen
+
+    with pytest.raises(ContractError, match="fused_block"):
+        load_fixed_qwen("nowhere", "nothing", model_manifest_sha256="0" * 64, device="cuda:0", fp8_dense=True, fused_block=True)

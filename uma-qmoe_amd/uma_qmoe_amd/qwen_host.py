@@ -440,7 +440,7 @@ def _fill_dense(model: Any, index: QwenCheckpointIndex, device: Any) -> tuple[in
 
 def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_manifest_sha256: str,
                     device: str = "cuda:0", performance_mode: bool = False, target_policy_id: str | None = None,
-                    fused_block: bool = True, fp8_dense: bool = False, architecture: tuple = QWEN_ARCHITECTURE,
+                    fused_block: bool | None = None, fp8_dense: bool = False, architecture: tuple = QWEN_ARCHITECTURE,
                     model_id: str = QWEN_MODEL_ID, model_revision: str = QWEN_MODEL_REVISION) -> FixedQwenHost:
     """A Qwen MoE host: the dense BF16 tensors of a local checkpoint directory
     in a Transformers model whose MoE blocks run the HIP operator over one
@@ -448,9 +448,11 @@ def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_mani
     with the same refusals and evidence keys). ``expert_pack`` is a pack file
     or an open reader; ``architecture`` is the (model_type, layers, experts,
     top-k) the checkpoint must have, the fixed model's by default.
-    ``fp8_dense`` puts the attention projections and shared experts into 8-bit
-    floats once they are loaded (``quantize_dense_fp8``; HIP devices only) and
-    runs the blocks with ``fused_block=False``.
+    ``fused_block`` runs each block as one op (``QuantizedQwenMoEBlock``), the
+    default. ``fp8_dense`` puts the attention projections and shared experts into
+    8-bit floats once they are loaded (``quantize_dense_fp8``; HIP devices only);
+    its blocks run the shared expert as a module, so ``fused_block`` is then
+    False, and True is refused.
 
     The pack is checked before anything is built: one mapping (one VMA when
     its file is known) and, for a TargetPack, exactly the model's routed
@@ -464,7 +466,9 @@ def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_mani
     if fp8_dense:
         if not str(device).startswith("cuda"):
             raise ContractError("8-bit dense layers require a HIP device")
-        fused_block = False
+        if fused_block:
+            raise ContractError("8-bit dense layers run the blocks with fused_block=False")
+    fused_block = not fp8_dense if fused_block is None else bool(fused_block)
     from .custom_op import register_expert_pack, register_moe_forward, unregister_expert_pack
     from .packfile import MemoryTargetPack, TargetPackReader
 
