@@ -84,6 +84,33 @@ def test_add_rmsnorm_rounds_its_norm_once(hip_ext, rows, cols):
     assert ((n.double().cpu() - y).abs() <= ((1 + ref.BF16) * (1 + ref.rmsnorm_delta(cols)) - 1) * y.abs()).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 2048), (5, 100), (4, 400), (3, 2047), (2, 8201), (2, 20000)])
+def test_add_rmsnorm_sum_in_an_input(hip_ext, rows, cols):
+    """The sum over the input, over the residual, and over one tensor that is both:
+    the same bits as into a tensor of its own."""
+    note(f"add_rmsnorm sum in an input {rows}x{cols}")
+    g = gen(cols)
+    x, r = normal(g, rows, cols).to(DEV), normal(g, rows, cols).to(DEV)
+    w = (1 + 0.1 * torch.randn(cols, generator=g)).to(torch.bfloat16).to(DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def into(a, b, total):
+        out, codes = torch.empty_like(a), torch.empty(rows, cols, dtype=torch.uint8, device=DEV)
+        scales = torch.empty(rows, -(-cols // 128), device=DEV)
+        assert hip_ext.lib.uqm_add_rmsnorm(a.data_ptr(), b.data_ptr(), rows, cols, w.data_ptr(), 1e-6, total.data_ptr(),
+                                           out.data_ptr(), codes.data_ptr(), scales.data_ptr(), stream) == 0
+        return total, out, codes, scales
+
+    def same(got, want):
+        return all(torch.equal(a, b) for a, b in zip(got, want))
+
+    want = into(x, r, torch.empty_like(x))
+    over_x, over_r = x.clone(), r.clone()
+    assert same(into(over_x, r, over_x), want) and same(into(x, over_r, over_r), want)
+    twice, both = into(x, x, torch.empty_like(x)), x.clone()
+    assert same(into(both, both, both), twice)
+
+
 def test_add_rmsnorm_rounds_as_rmsnorm(hip_ext):
     """The BF16 output is uqm_rmsnorm's of the same sum: both divide by the same
     root up to the order of its sum, so at most one step of each rounding."""
