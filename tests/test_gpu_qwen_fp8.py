@@ -88,6 +88,18 @@ def test_decode_graph_replays_the_eager_steps(checkpoint):
             assert (graph.logits - eager.logits).norm() <= 1e-3 * eager.logits.norm(), f"step {i}"
 
 
+def test_evidence_counts_the_weights_in_8_bits(checkpoint):
+    print("[case] qwen fp8 evidence", flush=True)
+    with load(checkpoint, fp8_dense=True) as host:
+        model = host.model
+        held = sum(p.numel() * p.element_size() for p in model.parameters())
+        for layer in model.model.layers:
+            for m in (*(getattr(layer.self_attn, n) for n in ("q_proj", "k_proj", "v_proj", "o_proj")),
+                      layer.mlp.shared_expert.gate_up, layer.mlp.shared_expert.down):
+                held += m.codes.numel() + 4 * m.scales.numel() + (0 if m.bias is None else 2 * m.bias.numel())
+        assert host.evidence["model_parameter_bytes"] == held
+
+
 def test_a_second_call_is_refused(checkpoint):
     print("[case] qwen fp8 twice", flush=True)
     ids = prompt(3).to(DEV)

@@ -234,6 +234,14 @@ def quantize_dense_fp8(model: Any) -> int:
     return count
 
 
+def _weight_bytes(model: Any) -> int:
+    """Bytes of the parameters and of the 8-bit projections in place of some."""
+    tensors = list(model.parameters())
+    if _FP8_CLASSES is not None:
+        tensors += [b for m in model.modules() if isinstance(m, _FP8_CLASSES[0]) for b in m.buffers()]
+    return sum(t.numel() * t.element_size() for t in tensors)
+
+
 def restore_nonpersistent_buffers(model: Any, config: Any, device: Any) -> None:
     """Rebuilds the rotary embedding, whose frequencies are not in the
     state dict and so are uninitialised after ``to_empty``
@@ -528,7 +536,7 @@ def load_fixed_qwen(model_directory: str | Path, expert_pack: Any, *, model_mani
             "loaded_expert_tensor_count": 0,
             "expert_parameter_count": len(expert_params),
             "quantized_moe_block_count": blocks,
-            "model_parameter_bytes": sum(p.numel() * p.element_size() for p in model.parameters()),
+            "model_parameter_bytes": _weight_bytes(model),
             "expert_pack_mapping_count": reader.mapping_count,
             "expert_pack_vma_count": vmas,
         }
