@@ -290,11 +290,12 @@ int uqm_dequantize(int32_t encoding, const void* data, const float* scales, int6
  * ceil(cols / 128)] are row-major and contiguous.
  *   d = max|v| / 448, at least 2^-126; 1 for a block of zeros
  *   code = e4m3(v * r), r = 1 / d rounded to FP32, to nearest even: v / d but for
- *          two FP32 roundings, so that a v / d within 2^-23 of itself of the middle
- *          between two codes may get either (their distances differ by no more)
+ *          two FP32 roundings, so that a v / d that is the middle between two codes,
+ *          up to 2^-23 of itself, may get either
  * A block that holds a NaN or an infinity gets a scale that is one too, and
  * codes that are NaN or 0; a product with it is NaN. None of these entry points
- * needs a workspace, and every result is the same for the same inputs. rows = 0
+ * needs a workspace, and every result is the same for the same inputs; a row of a
+ * row operator depends on no other row (a block of 128 rows: on that block). rows = 0
  * does nothing. Row operators of more rows than a launch has room for (2^32
  * threads) take several launches; a product of so many outputs (some 2^31 rows
  * or features of one) is refused. No counterpart in the reference, whose dense layers are BF16. */

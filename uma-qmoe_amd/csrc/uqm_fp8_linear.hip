@@ -64,7 +64,7 @@ constexpr int kScaleBlocks = 8;             // blocks whose scales are loaded to
 // blocks split over its W waves. Each wave loads its blocks into a place of its
 // own in LDS, the next one while it multiplies, and waits for nobody until the
 // sums of all waves are added, in wave order.
-// 512 x 2048 x 5632 (13 us) loads 704 KB a CU, at 64 bytes a cycle 5 us; the address
+// 512 x 2048 x 5632 (12.9 us) loads 704 KB a CU, at 64 bytes a cycle 5 us; the address
 // unit is busy for half of the time, the waves wait for loads 38% of theirs. The
 // scales come for 8 blocks at a time, 32 bytes of 8 tokens a load: a load per
 // block took 64 cache lines each time (14.5 us). The way through LDS is only for
@@ -248,7 +248,7 @@ hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
 // * TT tokens in registers. A block of a wave is TN * TT products of 32 cycles and
 // four FMAs each, which run under the products (the two waves of a SIMD in turn
 // reach 4.2 PFLOP/s with nothing else to do).
-// What bounds it: 8191 x 11264 x 2048 takes 196 us (1.93 PFLOP/s; a library product
+// What bounds it: 8191 x 11264 x 2048 takes 193 us (1.96 PFLOP/s; a library product
 // with one scale for a whole matrix 201 us, its best rate, at 8192^3, 2.74; this
 // kernel there 2.40). The matrix cores work 46% of its cycles at 2.05 GHz. Timed
 // with parts left out (8192^3, 458 us): without the operands' loads 384, without
@@ -257,10 +257,10 @@ hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
 // Four operands of the weight in flight instead of two gave nothing. A quarter of
 // the time at K = 2048 is the start and end of a tile (7.6 us of 32, from the fit
 // below); workgroups that walk over their tiles, with the next one's loads under
-// the last one's stores, took 214 us instead of 196.
+// the last one's stores, took 214 us instead of 196 (the build of that day).
 // Steps (8191 x 11264 x 2048, us): one float of scales per token and block straight
 // into registers 251, scales in panels 233, loads in two halves 225, results of two
-// tiles side by side (64-byte stores) 202, loads through buffers 196.
+// tiles side by side (64-byte stores) 202, loads through buffers 196 (193 since).
 constexpr int64_t kFp8TileMaxK = int64_t{1} << 23;  // 256 rows of fewer bytes stay below it
 
 template <int TN, int TT, int WN, int WT>
@@ -515,7 +515,9 @@ hipError_t launch_tiles(const Fp8LinearArgs& a, hipStream_t stream) {
 // best of eighteen that were timed, over 10% in 168 of them (at most 40%, calls of
 // 3 to 7 us). Without one of the ten the best of the others is slower by 1.0, 3.3,
 // 0.6, 0.7, 0.5, 0.7, 0.6, 1.2, 0.2 and 1.1% in the mean (in their order below);
-// some of them (us, launches back to back; 16 x 16 means rows and tokens, W waves):
+// some of them (us, launches back to back as they were timed for the fit; calls on three
+// sets of operands in turn take 12.9 at 512 x 2048 x 5632 and 193 at 8191 x 11264 x 2048
+// today; 16 x 16 means rows and tokens, W waves):
 //   1 x 11264 x 2048       16 x 16 W 4 5.8, W 8 5.9, 32 x 32 W 4 6.5, 64 x 32 6.7
 //   128 x 1408 x 2048      32 x 32 W 8 4.3, 16 x 16 W 4 4.7, 64 x 64 W 8 6.7, 128 x 128 12.5
 //   512 x 2048 x 5632      64 x 64 W 8 13.7, W 4 16.5, 64 x 32 18.0, 128 x 128 35.2

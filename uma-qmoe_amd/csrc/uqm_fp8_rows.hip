@@ -2,11 +2,13 @@
 // and the quantisation itself (definitions in uqm_fp8.h).
 //
 // All of them are bound by memory (3 to 9 bytes per element against some twenty
-// instructions): norm of 4095 x 2048 with a residual and both outputs 14.3 us, 5.3
-// TB/s; blocks of 11264 x 2048 12.2 us, 5.7; gate of 4095 x 5632 22.1 us, 5.3. A lane holds 8 neighbouring columns (one 16-byte load, an 8-byte
-// store of codes), so 16 lanes hold a group and its maximum is four exchanges
-// within a row of the wave; each input is read once and kept in registers
-// between the maximum and the codes.
+// instructions): norm of 4095 x 2048 with a residual and both outputs 13.5 us, 5.6
+// TB/s; blocks of 11264 x 2048 12.2 us, 5.7; gate of 4095 x 5632 21.6 us, 5.4. A lane
+// holds 8 neighbouring columns (one 16-byte load, an 8-byte store of codes), so 16
+// lanes hold a group and its maximum is four exchanges within a row of the wave;
+// each input is read once and kept in registers between the maximum and the codes.
+// A row's results depend on that row alone, to the bit (of blocks of 128 rows: on
+// that block).
 #include "uqm_device.h"
 #include "uqm_fp8.h"
 
@@ -20,8 +22,8 @@ constexpr int kThreads = 256;
 constexpr float kFp8Max = 448.0f;
 
 // 16 and 8 bytes at any alignment of their elements: one access each (the memory
-// takes them at twice the cost or less; one per element was 3 to 4 times slower, 4000
-// rows of 5475 with both outputs 118.6 us).
+// takes them at twice the cost or less; one per element was 3 to 4 times slower: 4000
+// rows of 5475 with both outputs 118.6 us, so 36.9).
 typedef uint32_t loose16_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t loose8_t __attribute__((ext_vector_type(2), aligned(1)));
 

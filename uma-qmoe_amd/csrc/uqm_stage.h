@@ -1,5 +1,5 @@
 // Staging of global memory into LDS, shared by the kernels that keep a ring of
-// stages there (uqm_mfma.hip, uqm_dense.hip, uqm_prefill.hip).
+// stages there (uqm_mfma.hip, uqm_dense.hip, uqm_prefill.hip, uqm_fp8_linear.hip).
 #pragma once
 
 #include "uqm_device.h"
