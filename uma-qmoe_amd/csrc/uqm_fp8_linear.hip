@@ -257,7 +257,7 @@ hipError_t launch_split(const Fp8LinearArgs& a, hipStream_t stream) {
 // Four operands of the weight in flight instead of two gave nothing. A quarter of
 // the time at K = 2048 is the start and end of a tile (7.6 us of 32, from the fit
 // below); workgroups that walk over their tiles, with the next one's loads under
-// the last one's stores, took 214 us instead of 196 (the build of that day).
+// the last one's stores, took 214 us, instead of 196 then.
 // Steps (8191 x 11264 x 2048, us): one float of scales per token and block straight
 // into registers 251, scales in panels 233, loads in two halves 225, results of two
 // tiles side by side (64-byte stores) 202, loads through buffers 196 (193 since).
