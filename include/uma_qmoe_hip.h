@@ -346,6 +346,73 @@ int uqm_fp8_linear(const void* codes, const float* scales, int64_t rows, const v
 int uqm_fp8_linear_plan(int64_t rows, int64_t out_features, int64_t in_features, int32_t* tile_rows,
                         int32_t* tile_tokens, int32_t* waves);
 
+/* ---- Paged key-value cache and the attention of one new token over it ----
+ * Keys and values of one attention layer, each in pages
+ * [pages, kv_heads, page_size, head_dim], contiguous: bf16, or e4m3 codes with one
+ * FP32 scale for the head_dim values of a token's head (value = code * scale; scales
+ * and codes as above with those values for a block). Position p of sequence b is
+ * place p % page_size of page page_table[b * table_stride + p / page_size],
+ * p < max_pages * page_size. An entry outside [0, pages) is no page: nothing is
+ * written there, and what it would hold reads as 0 and is not attended to.
+ * Entries behind a sequence's end are not looked at. The pages of one sequence
+ * may be those of another one (a common beginning), but of the entries that an
+ * append writes none may be written twice in the call: it would hold either's
+ * values, or keys of one beside scales of the other. starts, counts and lengths
+ * are on the device, so that a captured graph follows them. Results are the same
+ * for the same inputs, and a sequence's depend on no other sequence. No counterpart
+ * in the reference, whose hosts use Transformers' caches. */
+typedef struct uqm_kv_cache {
+  void* key;            /* [pages, kv_heads, page_size, head_dim], 16-byte aligned      */
+  void* value;
+  float* key_scales;    /* [pages, kv_heads, page_size], 16-byte aligned; both NULL: the */
+  float* value_scales;  /*   cache is bf16                                                */
+  int64_t pages;        /* below 2^31                                                    */
+  int64_t kv_heads;     /* below 2^16                                                    */
+  int64_t page_size;    /* 16, 32, 64, 128 or 256 tokens                                 */
+  int64_t head_dim;     /* a multiple of 16 up to 256                                    */
+} uqm_kv_cache;
+
+/* Puts new rows into the cache: row j < counts[b] of sequence b at position
+ * starts[b] + j. key and value are bf16; row (b, head h, j) starts at element
+ * b * batch_stride + h * head_stride + j * token_stride and has head_dim
+ * neighbouring elements; data 16-byte aligned, strides multiples of 8 and not
+ * negative. counts NULL: `tokens` rows of every sequence (a count above `tokens`
+ * means `tokens`). Rows whose position has no page (also negative positions)
+ * are dropped; no other place of the cache changes. kv_heads * tokens below 2^31. */
+int uqm_kv_append(const uqm_kv_cache* cache, const void* key, int64_t key_batch_stride, int64_t key_head_stride,
+                  int64_t key_token_stride, const void* value, int64_t value_batch_stride, int64_t value_head_stride,
+                  int64_t value_token_stride, int64_t batch, int64_t tokens, const int32_t* page_table,
+                  int64_t table_stride, int64_t max_pages, const int32_t* starts, const int32_t* counts, void* stream);
+
+/* Reads positions [0, max_length) of every sequence: key and value bf16
+ * [batch, kv_heads, max_length, head_dim], 16-byte aligned, bf16(code * scale) of an
+ * 8-bit cache; zeros from lengths[b] on. kv_heads * max_length below 2^31. */
+int uqm_kv_read(const uqm_kv_cache* cache, int64_t batch, const int32_t* page_table, int64_t table_stride,
+                int64_t max_pages, const int32_t* lengths, int64_t max_length, void* key, void* value, void* stream);
+
+/* Attention of one new token per sequence, output bf16 [batch, heads, head_dim]:
+ *   s_p = scale * sum over i of query[b, h, i] * key[b, g, p, i]
+ *   output[b, h] = sum over p of softmax(s)_p * value[b, g, p],  g = h / (heads / kv_heads)
+ * over the positions max(0, lengths[b] - window) <= p < lengths[b] (window 0: all;
+ * the new token's own key and value are in the cache already, at lengths[b] - 1).
+ * Zeros where no position is seen. query bf16 [batch, heads, head_dim], heads a
+ * multiple of kv_heads, both 16-byte aligned; batch * heads below 2^24.
+ * What places hold that are not seen has no influence, NaN and infinities neither;
+ * a seen NaN gives NaN, a seen infinity NaN or an infinity.
+ * workspace: uqm_paged_attention_workspace_bytes, 16-byte aligned, of any content,
+ * not shared by calls that overlap in time (also those of captured graphs); what
+ * it held is not kept. */
+int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t batch, int64_t heads,
+                        const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                        float scale, int64_t window, void* output, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Bytes of workspace that uqm_paged_attention needs for these sizes on the current
+ * device (0: none; host only, without a device for 256 compute units; 0 as well for
+ * sizes that the call refuses). */
+size_t uqm_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                           int64_t page_size, int64_t max_pages);
+
 #ifdef __cplusplus
 }
 #endif

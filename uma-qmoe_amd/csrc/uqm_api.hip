@@ -15,6 +15,7 @@
 #include "uqm_dense.h"
 #include "uqm_fp8.h"
 #include "uqm_internal.h"
+#include "uqm_kv.h"
 #include "uqm_prefill.h"
 #include "uqm_route.h"
 
@@ -1473,6 +1474,224 @@ int uqm_fp8_linear_plan(int64_t rows, int64_t out_features, int64_t in_features,
   *tile_tokens = p.tokens;
   *waves = p.waves;
   return UQM_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+constexpr int64_t kMaxElements = int64_t{1} << 48;  // of a cache: far beyond the memory, its bytes far below 2^63
+constexpr int64_t kMaxQueryHeads = int64_t{1} << 24;
+
+// Sizes of a cache, before its pointers are looked at.
+int check_kv_sizes(const char* what, int64_t pages, int64_t kv_heads, int64_t page_size, int64_t head_dim) {
+  if (head_dim <= 0 || head_dim % 16 != 0 || head_dim > uqm::kMaxHeadDim)
+    return fail(UQM_ERR_ARGUMENT, "%s: head_dim %lld must be a multiple of 16 up to %d", what, (long long)head_dim, uqm::kMaxHeadDim);
+  if (page_size < uqm::kMinPage || page_size > uqm::kMaxPage || (page_size & (page_size - 1)) != 0)
+    return fail(UQM_ERR_ARGUMENT, "%s: page_size %lld must be a power of two from %d to %d", what, (long long)page_size, uqm::kMinPage, uqm::kMaxPage);
+  if (kv_heads <= 0 || kv_heads >= 65536) return fail(UQM_ERR_ARGUMENT, "%s: kv_heads must be in [1, 2^16)", what);
+  if (pages <= 0 || pages > kMaxExtent || pages > kMaxElements / (kv_heads * page_size * head_dim))
+    return fail(UQM_ERR_ARGUMENT, "%s: pages must be in [1, 2^31), of fewer than 2^48 elements", what);
+  return UQM_OK;
+}
+
+int check_page_table(const char* what, int64_t batch, int64_t page_size, int64_t table_stride, int64_t max_pages) {
+  if (batch < 0 || batch > kMaxExtent) return fail(UQM_ERR_ARGUMENT, "%s: batch must be in [0, 2^31)", what);
+  if (max_pages < 0 || max_pages > kMaxExtent / page_size)
+    return fail(UQM_ERR_ARGUMENT, "%s: max_pages * page_size must be in [0, 2^31)", what);
+  if (table_stride < max_pages || table_stride > kMaxExtent || table_stride * batch > kMaxElements)
+    return fail(UQM_ERR_ARGUMENT, "%s: table_stride must be at least max_pages (a table of fewer than 2^48 entries)", what);
+  return UQM_OK;
+}
+
+int64_t cache_bytes(const uqm_kv_cache* c) {
+  return c->pages * c->kv_heads * c->page_size * c->head_dim * (c->key_scales != nullptr ? 1 : 2);
+}
+int64_t scale_bytes(const uqm_kv_cache* c) { return 4 * c->pages * c->kv_heads * c->page_size; }
+
+int check_cache(const char* what, const uqm_kv_cache* c) {
+  if (c == nullptr) return fail(UQM_ERR_ARGUMENT, "%s: a cache is required", what);
+  const int rc = check_kv_sizes(what, c->pages, c->kv_heads, c->page_size, c->head_dim);
+  if (rc) return rc;
+  if (c->key == nullptr || c->value == nullptr) return fail(UQM_ERR_ARGUMENT, "%s: the cache's key and value are required", what);
+  if ((c->key_scales == nullptr) != (c->value_scales == nullptr))
+    return fail(UQM_ERR_ARGUMENT, "%s: key and value scales must be given together", what);
+  if (!aligned16(c->key) || !aligned16(c->value) || !aligned16(c->key_scales) || !aligned16(c->value_scales))
+    return fail(UQM_ERR_ARGUMENT, "%s: the cache must be 16-byte aligned", what);
+  return UQM_OK;
+}
+
+// Whether [p, p + bytes) lies over a part of the cache.
+bool overlaps_cache(const uqm_kv_cache* c, const void* p, int64_t bytes) {
+  return overlap(p, bytes, c->key, cache_bytes(c)) || overlap(p, bytes, c->value, cache_bytes(c)) ||
+         overlap(p, bytes, c->key_scales, scale_bytes(c)) || overlap(p, bytes, c->value_scales, scale_bytes(c));
+}
+
+uqm::KvPages kv_pages(const uqm_kv_cache* c) {
+  return {c->key, c->value, c->key_scales, c->value_scales, c->pages, static_cast<int>(c->kv_heads),
+          __builtin_ctzll(static_cast<uint64_t>(c->page_size)), static_cast<int>(c->head_dim)};
+}
+
+struct RowStrides {
+  int64_t batch, head, token;
+};
+// Bytes from the first to behind the last element of new rows; -1 for strides that are not taken.
+int64_t rows_extent(const RowStrides& s, int64_t batch, int64_t kv_heads, int64_t tokens, int64_t head_dim) {
+  const int64_t strides[] = {s.batch, s.head, s.token}, counts[] = {batch, kv_heads, tokens};
+  int64_t last = head_dim;
+  for (int i = 0; i < 3; ++i) {
+    if (counts[i] <= 1) continue;  // (the stride of a single item is not used)
+    if (strides[i] < 0 || strides[i] % 8 != 0 || strides[i] > kMaxElements / (counts[i] - 1)) return -1;
+    last += strides[i] * (counts[i] - 1);
+  }
+  return 2 * last;
+}
+
+}  // namespace
+
+extern "C" {
+
+int uqm_kv_append(const uqm_kv_cache* cache, const void* key, int64_t key_batch_stride, int64_t key_head_stride,
+                  int64_t key_token_stride, const void* value, int64_t value_batch_stride, int64_t value_head_stride,
+                  int64_t value_token_stride, int64_t batch, int64_t tokens, const int32_t* page_table,
+                  int64_t table_stride, int64_t max_pages, const int32_t* starts, const int32_t* counts, void* stream) {
+  using namespace uqm;
+  int rc = check_cache("kv_append", cache);
+  if (rc || (rc = check_page_table("kv_append", batch, cache->page_size, table_stride, max_pages))) return rc;
+  if (tokens < 0 || tokens > kMaxExtent / cache->kv_heads)
+    return fail(UQM_ERR_ARGUMENT, "kv_append: kv_heads * tokens must be in [0, 2^31)");
+  const RowStrides ks{key_batch_stride, key_head_stride, key_token_stride}, vs{value_batch_stride, value_head_stride, value_token_stride};
+  const int64_t kbytes = rows_extent(ks, batch, cache->kv_heads, tokens, cache->head_dim);
+  const int64_t vbytes = rows_extent(vs, batch, cache->kv_heads, tokens, cache->head_dim);
+  if (kbytes < 0 || vbytes < 0) return fail(UQM_ERR_ARGUMENT, "kv_append: strides must be multiples of 8 and not negative");
+  if (overlap(cache->key, cache_bytes(cache), cache->value, cache_bytes(cache)) ||
+      overlap(cache->key_scales, scale_bytes(cache), cache->value_scales, scale_bytes(cache)) ||
+      overlap(cache->key_scales, scale_bytes(cache), cache->key, cache_bytes(cache)) ||
+      overlap(cache->key_scales, scale_bytes(cache), cache->value, cache_bytes(cache)) ||
+      overlap(cache->value_scales, scale_bytes(cache), cache->key, cache_bytes(cache)) ||
+      overlap(cache->value_scales, scale_bytes(cache), cache->value, cache_bytes(cache)))
+    return fail(UQM_ERR_ARGUMENT, "kv_append: two parts of the cache overlap");
+  if (batch == 0 || tokens == 0 || max_pages == 0) return UQM_OK;
+  if (key == nullptr || value == nullptr || page_table == nullptr || starts == nullptr)
+    return fail(UQM_ERR_ARGUMENT, "kv_append: key, value, page_table and starts are required");
+  if (!aligned16(key) || !aligned16(value) || misaligned(page_table, 4) || misaligned(starts, 4) || misaligned(counts, 4))
+    return fail(UQM_ERR_ARGUMENT, "kv_append: key and value must be 16-byte aligned, indexes to their elements");
+  if (overlaps_cache(cache, key, kbytes) || overlaps_cache(cache, value, vbytes) ||
+      overlaps_cache(cache, page_table, 4 * (table_stride * (batch - 1) + max_pages)) ||
+      overlaps_cache(cache, starts, 4 * batch) || overlaps_cache(cache, counts, 4 * batch))
+    return fail(UQM_ERR_ARGUMENT, "kv_append: the cache overlaps an input");
+  if ((rc = check_device())) return rc;
+  KvAppendArgs a{};
+  a.cache = kv_pages(cache);
+  a.pages = {page_table, table_stride, static_cast<int32_t>(max_pages)};
+  a.key = {static_cast<const uint16_t*>(key), ks.batch, ks.head, ks.token};
+  a.value = {static_cast<const uint16_t*>(value), vs.batch, vs.head, vs.token};
+  a.batch = batch;
+  a.tokens = static_cast<int32_t>(tokens);
+  a.starts = starts;
+  a.counts = counts;
+  return hip_check(launch_kv_append(a, static_cast<hipStream_t>(stream)), "kv_append launch");
+}
+
+int uqm_kv_read(const uqm_kv_cache* cache, int64_t batch, const int32_t* page_table, int64_t table_stride,
+                int64_t max_pages, const int32_t* lengths, int64_t max_length, void* key, void* value, void* stream) {
+  using namespace uqm;
+  int rc = check_cache("kv_read", cache);
+  if (rc || (rc = check_page_table("kv_read", batch, cache->page_size, table_stride, max_pages))) return rc;
+  if (max_length < 0 || max_length > kMaxExtent / cache->kv_heads || batch * cache->kv_heads > kMaxElements / (max_length * cache->head_dim + 1))
+    return fail(UQM_ERR_ARGUMENT, "kv_read: kv_heads * max_length must be in [0, 2^31)");
+  if (batch == 0 || max_length == 0) return UQM_OK;
+  if (lengths == nullptr || key == nullptr || value == nullptr || (page_table == nullptr && max_pages > 0))
+    return fail(UQM_ERR_ARGUMENT, "kv_read: page_table, lengths, key and value are required");
+  if (!aligned16(key) || !aligned16(value) || misaligned(page_table, 4) || misaligned(lengths, 4))
+    return fail(UQM_ERR_ARGUMENT, "kv_read: key and value must be 16-byte aligned, indexes to their elements");
+  const int64_t bytes = 2 * batch * cache->kv_heads * max_length * cache->head_dim;
+  const int64_t table = max_pages > 0 ? 4 * (table_stride * (batch - 1) + max_pages) : 0;
+  for (const void* out : {key, value})
+    if (overlaps_cache(cache, out, bytes) || overlap(out, bytes, page_table, table) || overlap(out, bytes, lengths, 4 * batch))
+      return fail(UQM_ERR_ARGUMENT, "kv_read: an output overlaps an input");
+  if (overlap(key, bytes, value, bytes)) return fail(UQM_ERR_ARGUMENT, "kv_read: two outputs overlap");
+  if ((rc = check_device())) return rc;
+  KvReadArgs a{};
+  a.cache = kv_pages(cache);
+  a.pages = {page_table, table_stride, static_cast<int32_t>(max_pages)};
+  a.batch = batch;
+  a.length = static_cast<int32_t>(max_length);
+  a.lengths = lengths;
+  a.key = static_cast<uint16_t*>(key);
+  a.value = static_cast<uint16_t*>(value);
+  return hip_check(launch_kv_read(a, static_cast<hipStream_t>(stream)), "kv_read launch");
+}
+
+static int check_attention_sizes(int64_t batch, int64_t heads, int64_t kv_heads) {
+  if (heads <= 0 || heads % kv_heads != 0)
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: %lld heads must be a positive multiple of the %lld key heads", (long long)heads, (long long)kv_heads);
+  if (heads >= kMaxQueryHeads || batch * heads >= kMaxQueryHeads)
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: batch * heads must be below 2^24");
+  return UQM_OK;
+}
+
+static uqm::PagedAttentionArgs attention_sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                               int64_t page_size, int64_t max_pages) {
+  uqm::PagedAttentionArgs a{};
+  a.cache.kv_heads = static_cast<int>(kv_heads);
+  a.cache.dim = static_cast<int>(head_dim);
+  a.cache.page_log2 = __builtin_ctzll(static_cast<uint64_t>(page_size));
+  a.pages.width = static_cast<int32_t>(max_pages);
+  a.batch = batch;
+  a.heads = static_cast<int>(heads);
+  return a;
+}
+
+size_t uqm_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                           int64_t page_size, int64_t max_pages) {
+  if (check_kv_sizes("paged_attention", 1, kv_heads, page_size, head_dim) ||
+      check_page_table("paged_attention", batch, page_size, max_pages, max_pages) ||
+      check_attention_sizes(batch, heads, kv_heads))
+    return 0;
+  return uqm::paged_attention_workspace(attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages), device_cus());
+}
+
+int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t batch, int64_t heads,
+                        const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* lengths,
+                        float scale, int64_t window, void* output, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  using namespace uqm;
+  int rc = check_cache("paged_attention", cache);
+  if (rc || (rc = check_page_table("paged_attention", batch, cache->page_size, table_stride, max_pages)) ||
+      (rc = check_attention_sizes(batch, heads, cache->kv_heads)))
+    return rc;
+  if (!(scale - scale == 0.f)) return fail(UQM_ERR_ARGUMENT, "paged_attention: scale must be finite");
+  if (window < 0) return fail(UQM_ERR_ARGUMENT, "paged_attention: window must be at least 1, or 0 for none");
+  if (batch == 0) return UQM_OK;
+  if (query == nullptr || output == nullptr || lengths == nullptr || (page_table == nullptr && max_pages > 0))
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: query, page_table, lengths and output are required");
+  if (!aligned16(query) || !aligned16(output) || misaligned(page_table, 4) || misaligned(lengths, 4))
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: query and output must be 16-byte aligned, indexes to their elements");
+  PagedAttentionArgs a = attention_sizes(batch, heads, cache->kv_heads, cache->head_dim, cache->page_size, max_pages);
+  const int cus = device_cus();
+  const int64_t need = static_cast<int64_t>(paged_attention_workspace(a, cus));
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < static_cast<size_t>(need)))
+    return fail(UQM_ERR_WORKSPACE, "paged_attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  const int64_t bytes = 2 * batch * heads * cache->head_dim;
+  const int64_t table = max_pages > 0 ? 4 * (table_stride * (batch - 1) + max_pages) : 0;
+  const Span outs[] = {{output, bytes}, {need > 0 ? workspace : nullptr, need}};
+  for (const Span& out : outs)
+    if (overlaps_cache(cache, out.p, out.bytes) || overlap(out.p, out.bytes, query, bytes) ||
+        overlap(out.p, out.bytes, page_table, table) || overlap(out.p, out.bytes, lengths, 4 * batch))
+      return fail(UQM_ERR_ARGUMENT, "paged_attention: the output or the workspace overlaps an input");
+  if (overlap(outs[0].p, outs[0].bytes, outs[1].p, outs[1].bytes))
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: the output overlaps the workspace");
+  if ((rc = check_device())) return rc;
+  a.cache = kv_pages(cache);
+  a.pages = {page_table, table_stride, static_cast<int32_t>(max_pages)};
+  a.query = static_cast<const uint16_t*>(query);
+  a.lengths = lengths;
+  a.window = window > 0 ? window : INT64_MAX;
+  a.scale = scale;
+  a.out = static_cast<uint16_t*>(output);
+  a.workspace = static_cast<float*>(workspace);
+  return hip_check(launch_paged_attention(a, cus, static_cast<hipStream_t>(stream)), "paged_attention launch");
 }
 
 }  // extern "C"

@@ -11,6 +11,7 @@
 // that block).
 #include "uqm_device.h"
 #include "uqm_fp8.h"
+#include "uqm_fp8_codes.h"
 
 #include <algorithm>
 #include <initializer_list>
@@ -19,7 +20,6 @@ namespace uqm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kFp8Max = 448.0f;
 
 // 16 and 8 bytes at any alignment of their elements: one access each (the memory
 // takes them at twice the cost or less; one per element was 3 to 4 times slower: 4000
@@ -68,12 +68,6 @@ __device__ __forceinline__ void store8_bf16(uint16_t* row, int64_t c, int64_t co
   }
 }
 
-// Four values as e4m3 bytes, to nearest even (NaN stays NaN).
-__device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
-}
-
 // (inv = 1 / d: one division a group; the codes are defined by the product with it)
 template <bool VEC>
 __device__ __forceinline__ void store8_fp8(uint8_t* row, int64_t c, int64_t cols, const float (&v)[8], float inv) {
@@ -88,30 +82,6 @@ __device__ __forceinline__ void store8_fp8(uint8_t* row, int64_t c, int64_t cols
     for (int j = 0; j < 7; ++j)
       if (c + j < cols) row[c + j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
   }
-}
-
-// Bits of max|v|: as unsigned numbers magnitudes order like the floats, and a
-// NaN above every other value, which fmaxf would drop.
-__device__ __forceinline__ uint32_t magnitude8(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-  return m;
-}
-template <int O>
-__device__ __forceinline__ uint32_t max_step(uint32_t m) {
-  return max(m, __float_as_uint(xor_partner<O>(__uint_as_float(m))));
-}
-// Maximum over the 16 lanes of a group.
-__device__ __forceinline__ uint32_t group_max(uint32_t m) {
-  m = max_step<8>(m);
-  m = max_step<4>(m);
-  m = max_step<2>(m);
-  return max_step<1>(m);
-}
-__device__ __forceinline__ float scale_of(uint32_t bits) {
-  const float d = __uint_as_float(bits) / kFp8Max;
-  return bits == 0u ? 1.0f : (d < 0x1p-126f ? 0x1p-126f : d);
 }
 
 // Codes and scale of the group that this lane's 8 columns belong to.

@@ -83,6 +83,13 @@ class LayerPlan(ctypes.Structure):
                                           "down_split")]
 
 
+class KVCache(ctypes.Structure):
+    """uqm_kv_cache."""
+
+    _fields_ = [("key", _vp), ("value", _vp), ("key_scales", _vp), ("value_scales", _vp), ("pages", _i64),
+                ("kv_heads", _i64), ("page_size", _i64), ("head_dim", _i64)]
+
+
 class PackTensor(ctypes.Structure):
     """uqm_pack_tensor."""
 
@@ -142,6 +149,20 @@ SIGNATURES = {
     "uqm_fp8_quantize": (ctypes.c_int, (_vp, _i64, _i64, _i64, _vp, _vp, _vp)),
     "uqm_fp8_linear": (ctypes.c_int, (_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp)),
     "uqm_fp8_linear_plan": (ctypes.c_int, (_i64, _i64, _i64, *[ctypes.POINTER(_i32)] * 3)),
+    "uqm_kv_append": (
+        ctypes.c_int,
+        (ctypes.POINTER(KVCache), _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp),
+    ),
+    "uqm_kv_read": (
+        ctypes.c_int,
+        (ctypes.POINTER(KVCache), _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp),
+    ),
+    "uqm_paged_attention": (
+        ctypes.c_int,
+        (ctypes.POINTER(KVCache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, ctypes.c_float, _i64, _vp, _vp,
+         ctypes.c_size_t, _vp),
+    ),
+    "uqm_paged_attention_workspace_bytes": (ctypes.c_size_t, (_i64, _i64, _i64, _i64, _i64, _i64)),
     "uqm_set_option": (ctypes.c_int, (ctypes.c_int, _i64)),
     "uqm_workspace_status": (ctypes.c_int, (_vp, ctypes.c_size_t, _vp)),
     "uqm_noalloc_status": (ctypes.c_int, (_vp,)),

@@ -38,6 +38,7 @@ from .formats import ENCODINGS, ContractError
 EXPERT_NAME = "model.layers.{layer}.mlp.experts.{expert}.{proj}.weight"
 PROJECTIONS = ("gate_proj", "up_proj", "down_proj")
 PLATFORM = "hip_gfx950"
+KV_PAGE_SIZES = (16, 32, 64, 128, 256)
 FP8_GROUP = 128  # columns (and, for weights, rows) that share a scale of an Fp8Matrix
 
 _EXTENSIONS: dict[str, Any] = {}
@@ -161,6 +162,18 @@ class Fp8Matrix(NamedTuple):
         scales = self.scales.reshape(-1, self.scales.shape[-1])
         each = scales.repeat_interleave(self.block_rows, 0)[:rows].repeat_interleave(FP8_GROUP, 1)[:, :cols]
         return self.codes.float() * each.reshape(self.codes.shape)
+
+
+class KVCache(NamedTuple):
+    """Keys and values of one attention layer in pages: ``key`` and ``value``
+    [pages, kv_heads, page_size, head_dim], BF16, or float8_e4m3fn codes with
+    float32 scales [pages, kv_heads, page_size] (value = code * scale).
+    page_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256."""
+
+    key: Any
+    value: Any
+    key_scales: Any = None
+    value_scales: Any = None
 
 
 class HipExtension:
@@ -620,6 +633,159 @@ class HipExtension:
         out = torch.empty(*shape[:-1], n, dtype=torch.bfloat16, device=codes.device)
         self._launch(self.lib.uqm_fp8_linear, index, codes.data_ptr(), scales.data_ptr(), codes.numel() // k,
                      w.data_ptr(), ws.data_ptr(), n, k, bias if bias is None else bias.data_ptr(), out.data_ptr())
+        return out
+
+    # ------------------------------------------- paged key-value cache --
+    # (What a call checks is in one condition, as above.)
+    def new_kv_cache(self, pages, kv_heads, page_size, head_dim, *, fp8=False, device="cuda"):
+        """A ``KVCache`` of zeros in BF16 or (``fp8``) 8-bit floats."""
+        torch = self.torch
+        shape = (pages, kv_heads, page_size, head_dim)
+        if not (pages > 0 and kv_heads > 0 and page_size in KV_PAGE_SIZES and 0 < head_dim <= 256 and head_dim % 16 == 0):
+            raise RuntimeError("new_kv_cache requires at least one page and head, a page size of 16, 32, 64, 128 or 256 and "
+                               f"a head size of a multiple of 16 up to 256, not {shape}")
+        # (codes filled as bytes: 0 is the code of 0)
+        data = [torch.zeros(shape, dtype=torch.uint8 if fp8 else torch.bfloat16, device=device) for _ in range(2)]
+        if not fp8:
+            return KVCache(*data)
+        return KVCache(*(t.view(torch.float8_e4m3fn) for t in data),
+                       *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+
+    def _check_cache(self, cache, what):
+        """The words of a refusal of a ``KVCache`` (or of a tensor beside it)."""
+        torch = self.torch
+        k, v, ks, vs = cache
+        if k.ndim != 4 or k.shape != v.shape or k.dtype is not v.dtype:
+            raise RuntimeError(f"{what} requires key and value [pages, kv_heads, page_size, head_dim] of one shape and type")
+        if k.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise RuntimeError(f"{what} requires a BF16 or float8_e4m3fn cache")
+        scaled = k.dtype is torch.float8_e4m3fn
+        if scaled != (ks is not None) or scaled != (vs is not None):
+            raise RuntimeError(f"{what} requires scales with a float8_e4m3fn cache, and only with one")
+        if scaled and not all(s.dtype is torch.float32 and s.shape == k.shape[:3] for s in (ks, vs)):
+            raise RuntimeError(f"{what} requires float32 scales {tuple(k.shape[:3])}")
+        if not all(t is None or t.is_contiguous() for t in cache):
+            raise RuntimeError(f"{what} requires a contiguous cache")
+        raise RuntimeError(f"{what} requires device tensors, all on one device")
+
+    def _cache(self, cache, what, index):
+        """The descriptor of ``cache`` on device ``index``."""
+        torch = self.torch
+        k, v, ks, vs = cache
+        shape = k.shape
+        scaled = ks is not None
+        if not (len(shape) == 4 and v.shape == shape and k.is_contiguous() and v.is_contiguous() and index >= 0
+                and k.get_device() == index == v.get_device()
+                and ((k.dtype is v.dtype is torch.float8_e4m3fn and vs is not None and ks.dtype is vs.dtype is torch.float32
+                      and ks.shape == vs.shape == shape[:3] and ks.is_contiguous() and vs.is_contiguous()
+                      and ks.get_device() == index == vs.get_device())
+                     if scaled else (k.dtype is v.dtype is torch.bfloat16 and vs is None))):
+            self._check_cache(cache, what)
+        return _native.KVCache(k.data_ptr(), v.data_ptr(), ks.data_ptr() if scaled else None,
+                               vs.data_ptr() if scaled else None, *shape)
+
+    def _indexes(self, what, index, page_table, vector, counts=None):
+        """The page table (rows of neighbouring entries), its row stride and the
+        vectors of one entry per sequence."""
+        i32 = self.torch.int32
+        shape = page_table.shape
+        if len(shape) != 2 or page_table.dtype is not i32:
+            raise RuntimeError(f"{what} requires an int32 page table [batch, pages of a sequence]")
+        if not (vector.shape == shape[:1] and vector.dtype is i32
+                and (counts is None or counts.shape == shape[:1] and counts.dtype is i32)):
+            raise RuntimeError(f"{what} requires an int32 entry for each of the page table's {shape[0]} sequences")
+        if not (page_table.get_device() == index == vector.get_device() and (counts is None or counts.get_device() == index)):
+            raise RuntimeError(f"{what} requires device tensors, all on one device")
+        # (a table by columns, or with one row for all, is laid out row by row; a single entry's stride is not used)
+        if shape[1] > 1 and page_table.stride(1) != 1 or page_table.stride(0) < shape[1]:
+            page_table = page_table.contiguous()
+        return (page_table, max(page_table.stride(0), shape[1]), vector.contiguous(),
+                counts if counts is None else counts.contiguous())
+
+    def _new_rows(self, x, shape, what):
+        """New keys or values with rows that the library takes: neighbouring
+        elements, 16-byte aligned."""
+        if x.dtype is not self.torch.bfloat16 or len(x.shape) != 4 or x.shape[1] != shape[1] or x.shape[3] != shape[3]:
+            raise RuntimeError(f"{what} requires BF16 keys and values [batch, {shape[1]}, tokens, {shape[3]}] (heads and "
+                               "head size as the cache)")
+        b, h, t, d = x.stride()
+        if d != 1 or (b | h | t) & 7 or x.data_ptr() & 15:
+            x = x.clone(memory_format=self.torch.contiguous_format)
+            b, h, t, d = x.stride()
+        return x, b, h, t
+
+    def kv_append(self, cache: KVCache, key, value, page_table, starts, counts=None):
+        """Writes new keys and values (BF16 [batch, kv_heads, tokens, head_dim],
+        any strides) into ``cache``, quantised as they are written if it is in 8
+        bits: token j < ``counts[b]`` (None: every one) of sequence b at position
+        ``starts[b]`` + j, which is in page ``page_table[b, position //
+        page_size]``. Positions without a page (an entry outside [0, pages), or
+        none) are dropped. No place may be written twice in a call.
+        ``page_table``, ``starts`` and ``counts`` int32. Returns ``cache``."""
+        index = key.get_device()
+        desc = self._cache(cache, "kv_append", index)
+        shape = cache.key.shape
+        key, kb, kh, kt = self._new_rows(key, shape, "kv_append")
+        value, vb, vh, vt = self._new_rows(value, shape, "kv_append")
+        batch, _, tokens, _ = key.shape
+        if value.shape != key.shape or value.get_device() != index or page_table.shape[:1] != (batch,):
+            raise RuntimeError("kv_append requires keys and values of one shape on one device, and a row of the page table "
+                               "for each sequence")
+        page_table, stride, starts, counts = self._indexes("kv_append", index, page_table, starts, counts)
+        self._launch(self.lib.uqm_kv_append, index, ctypes.byref(desc), key.data_ptr(), kb, kh, kt, value.data_ptr(), vb, vh,
+                     vt, batch, tokens, page_table.data_ptr(), stride, page_table.shape[1], starts.data_ptr(), _ptr(counts))
+        return cache
+
+    def kv_read(self, cache: KVCache, page_table, lengths, max_length):
+        """(keys, values) of positions [0, ``max_length``) of every sequence in
+        BF16 [batch, kv_heads, max_length, head_dim]; zeros from ``lengths[b]``
+        on, and where the page table has no page."""
+        torch = self.torch
+        index = page_table.get_device()
+        desc = self._cache(cache, "kv_read", index)
+        page_table, stride, lengths, _ = self._indexes("kv_read", index, page_table, lengths)
+        _, kv_heads, _, head_dim = cache.key.shape
+        if not 0 <= max_length * kv_heads < 1 << 31:
+            raise RuntimeError("kv_read requires max_length * kv_heads in [0, 2^31)")
+        batch = page_table.shape[0]
+        shape = (batch, kv_heads, max_length, head_dim)
+        key = torch.empty(shape, dtype=torch.bfloat16, device=page_table.device)
+        value = torch.empty_like(key)
+        self._launch(self.lib.uqm_kv_read, index, ctypes.byref(desc), batch, page_table.data_ptr(), stride,
+                     page_table.shape[1], lengths.data_ptr(), max_length, key.data_ptr(), value.data_ptr())
+        return key, value
+
+    def paged_attention(self, query, cache: KVCache, page_table, lengths, *, scale=None, window=None):
+        """Attention of one new token per sequence, whose key and value are in the
+        cache already: ``query`` BF16 [batch, heads, head_dim] over positions
+        [0, ``lengths[b]``), the last ``window`` of them if that is given; BF16 of
+        ``query``'s shape, zeros where there are none. ``heads`` a multiple of the
+        cache's (neighbouring heads share one); ``scale`` head_dim^-0.5 by
+        default."""
+        torch = self.torch
+        index, shape = query.get_device(), query.shape
+        desc = self._cache(cache, "paged_attention", index)
+        _, kv_heads, page_size, head_dim = cache.key.shape
+        if query.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != head_dim or shape[1] % kv_heads or not shape[1]:
+            raise RuntimeError(f"paged_attention requires a BF16 query [batch, heads, {head_dim}] of a multiple of {kv_heads} "
+                               f"heads, not {query.dtype} {tuple(shape)}")
+        if window is not None and window < 1:
+            raise RuntimeError("paged_attention requires a window of at least 1")
+        batch, heads, _ = shape
+        if page_table.shape[:1] != (batch,):
+            raise RuntimeError("paged_attention requires a row of the page table for each sequence")
+        page_table, stride, lengths, _ = self._indexes("paged_attention", index, page_table, lengths)
+        if not query.is_contiguous() or query.data_ptr() & 15:
+            query = query.clone(memory_format=torch.contiguous_format)
+        out = torch.empty_like(query)
+        width = page_table.shape[1]
+        # (torch's allocator gives memory in stream order, and a captured graph its own)
+        nbytes = self.lib.uqm_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim, page_size, width)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+        self._launch(self.lib.uqm_paged_attention, index, ctypes.byref(desc), query.data_ptr(), batch, heads,
+                     page_table.data_ptr(), stride, width, lengths.data_ptr(),
+                     head_dim ** -0.5 if scale is None else scale, 0 if window is None else min(window, 1 << 31), out.data_ptr(),
+                     _ptr(workspace), nbytes)
         return out
 
     # ------------------------------------- reference binding signatures --
@@ -1117,6 +1283,8 @@ __all__ = [
     "FP8_GROUP",
     "Fp8Matrix",
     "HipExtension",
+    "KVCache",
+    "KV_PAGE_SIZES",
     "MixedTargetNativeBackend",
     "PackedQ4NativeBackend",
     "PinnedStaging",
