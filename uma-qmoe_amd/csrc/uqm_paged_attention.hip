@@ -2,97 +2,571 @@
 // uqm_kv.h):
 //   s_p = scale * sum_i q_i k[p, i],   max(0, length - window) <= p < length
 //   out = sum_p softmax(s)_p v[p]
-// in FP32, with the running maximum and sum of the softmax, so that the cache is
-// read once; zeros where no position is seen.
+// in one pass over the cache with the running maximum m, sum l and output o of the
+// softmax (base 2: s and m carry the factor log2 e).
+//
+// Bound by memory: a key and its value are read for at most 16 query heads, some
+// 4 to 64 operations a byte. What is computed goes to the matrix cores all the same,
+// since the vector unit would be the limit from four query heads a key head on.
+// Everything stays in the wave's registers: no exchange, no shared memory in the
+// loop, but for the maximum over four lanes.
+//   - scores transposed, S^T = K Q^T (16 keys x 16 queries, v_mfma_f32_16x16x32_bf16):
+//     a lane gives 8 neighbouring dimensions of one key, which lie next to each other
+//     in a page, and gets scores of one query (lane % 16) and four keys
+//     (4 (lane / 16) .. + 3). In which order dimensions are summed up is free, so
+//     that 8-bit keys are loaded 16 at a time for two products.
+//   - output transposed, O^T = V^T P^T: the sum over positions is free in its order,
+//     too. So a lane's eight weights, of keys 16 t + 4 (lane / 16) + r, are its operand
+//     as they are, and the other operand needs, of one dimension, the same eight keys:
+//     a lane loads DP / 16 neighbouring dimensions of each of its eight keys (whole
+//     rows of a page, 16 lanes a row), and pairs of keys are put together by one
+//     v_perm each. Product i then holds dimensions lane % 16 * DP / 16 + i.
+//   - e4m3 codes become BF16 exactly (v_cvt_scalef32_pk_bf16_fp8); a key's scale
+//     multiplies its score, a value's scale its weight, both in FP32.
+//   - a weight is split into two BF16 numbers, its rounding and the rest (together off
+//     by 2^-16 of it, where one would be off by 2^-8, as much as the output's own
+//     rounding). Up to 8 query heads, the products' 16 columns hold the rounded
+//     weights in the lower and the rests in the upper half, which costs nothing; with
+//     more of them there is a second product.
+//
+// Work is dealt out in tiles of 128 positions (32 of each of a workgroup's four
+// waves) of one sequence and key head, numbered sequence by sequence, head by head;
+// each workgroup takes the same number of neighbouring tiles, whatever the lengths
+// are, and computes from these where they lie. What it has of a head that other
+// workgroups also work on goes to its two places in the workspace (at most its first
+// and its last head), and a second launch joins these. Without a sequence long
+// enough a workgroup takes whole heads, and there is no second launch.
 #include "uqm_device.h"
 #include "uqm_kv.h"
+
+#include <algorithm>
 
 namespace uqm {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kWavePositions = 32, kTile = kWaves * kWavePositions;
+constexpr int kGroupsPerCu = 4;   // workgroups of the main launch per compute unit
+constexpr int kDirectTiles = 4;   // up to this many tiles a head is one workgroup's
 
-template <bool FP8>
-__device__ __forceinline__ void load4(const void* data, const float* scales, int64_t place, int dim, int c, float (&v)[4]) {
-  if constexpr (FP8) {
-    const uint32_t q = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(data) + place * dim + c);
-    const float d = scales[place];
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(q, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(q, true);
-    v[0] = lo[0] * d, v[1] = lo[1] * d, v[2] = hi[0] * d, v[3] = hi[1] * d;
-  } else {
-    const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(data) + place * dim + c);
-    v[0] = bf16lo(q.x), v[1] = bf16hi(q.x), v[2] = bf16lo(q.y), v[3] = bf16hi(q.y);
+__device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// Codes 0, 1 (hi: 2, 3) of w as a BF16 pair; exact.
+template <bool HI>
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+}
+// The value of lane ^ 8.
+__device__ __forceinline__ float other_half(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));  // row_ror:8
+}
+
+// Where the work lies, from the lengths on the device.
+struct Work {
+  int64_t per;     // units of a workgroup
+  int64_t units;   // of all sequences and heads
+};
+struct Plan {
+  int32_t chunk;        // tiles of a unit
+  int32_t groups;       // workgroups of the launch
+  int32_t query_rows;   // query heads of a unit (at most)
+  int32_t query_tiles;  // units side by side for the query heads of a key head
+};
+
+struct Sequence {
+  int32_t length, first;          // positions seen: first .. length - 1
+  int32_t tile0, tiles, units;    // tiles from tile0 on; units of one head
+};
+__device__ __forceinline__ Sequence sequence_of(const PagedAttentionArgs& a, const Plan& plan, int32_t given) {
+  Sequence s;
+  const int64_t capacity = static_cast<int64_t>(a.pages.width) << a.cache.page_log2;  // below 2^31
+  s.length = min(max(given, 0), static_cast<int32_t>(capacity));
+  s.first = static_cast<int32_t>(max(static_cast<int64_t>(0), s.length - a.window));
+  s.tile0 = s.first / kTile;
+  s.tiles = (s.length + kTile - 1) / kTile - s.tile0;  // (0 at length 0: first is 0, too)
+  s.units = (s.tiles + plan.chunk - 1) / plan.chunk;
+  return s;
+}
+
+// A value that every lane has, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  return static_cast<int64_t>((static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32) | lo);
+}
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return uniform(v);
+}
+
+// Units of one head over sequences [0, end), every lane of the wave the same.
+__device__ __forceinline__ int64_t units_before(const PagedAttentionArgs& a, const Plan& plan, int64_t end) {
+  int64_t sum = 0;
+  for (int64_t b = threadIdx.x & 63; b < end; b += 64) sum += sequence_of(a, plan, a.lengths[b]).units;
+  return wave_sum64(sum);
+}
+__device__ __forceinline__ Work work_of(int64_t head_units, int heads, const Plan& plan) {
+  Work w;
+  w.units = head_units * heads;
+  w.per = max(static_cast<int64_t>(1), (w.units + plan.groups - 1) / plan.groups);
+  return w;
+}
+
+// A workgroup's part of a row: weights relative to 2^most, their sum, the sum of
+// weighted values. most is -inf for a part that saw nothing (sum 0) and for one all
+// of whose scores were -inf (sum NaN: 0 / 0 unless other parts have finite scores).
+__device__ __forceinline__ float part_factor(float most, float all) {
+  return most == -INFINITY ? (all == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(most - all);
+}
+__device__ __forceinline__ float weighted(float f, float v) { return f == 0.0f ? 0.0f : f * v; }
+
+template <int DP, bool FP8, bool DUP, bool PAD>
+__global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
+  constexpr int kRows = DUP ? 8 : 16;      // query heads of a unit
+  constexpr int kVec = DP / 16;            // dimensions of a value row that a lane holds
+  constexpr int kStep = FP8 ? 64 : 32;     // dimensions of one load of 16 keys
+  constexpr int kLoads = DP / kStep;
+  constexpr int kVWords = FP8 ? kVec / 4 : kVec / 2;
+  constexpr int kRowStride = DP + 4;       // (rows of the join four banks apart)
+  __shared__ float part_o[kWaves][kRows][kRowStride];
+  __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
+
+  const KvPages& kv = a.cache;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int dim = PAD ? kv.dim : DP;
+  const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles;
+  const int row_bytes = FP8 ? dim : 2 * dim;
+
+  // Zeros for sequences without a position.
+  for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (sequence_of(a, plan, a.lengths[b]).tiles > 0) continue;
+    uint4* out = reinterpret_cast<uint4*>(a.out + b * a.heads * dim);
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(a.heads) * dim / 8; i += kThreads) out[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+
+  const Work work = work_of(units_before(a, plan, a.batch), heads, plan);
+  const int64_t begin = blockIdx.x * work.per, end = min(begin + work.per, work.units);
+  if (begin >= end) return;
+
+  // The sequence of the first unit, and its own first unit.
+  int64_t b = 0, base = 0;
+  for (int64_t block = 0; block < a.batch; block += 64) {
+    int64_t units = block + lane < a.batch ? sequence_of(a, plan, a.lengths[block + lane]).units : 0;
+    int64_t upto = units;  // inclusive sum over the lanes
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t v = __shfl_up(upto, o);
+      if (lane >= o) upto += v;
+    }
+    const int before = __popcll(__ballot(base + upto * heads <= begin));  // sequences that end at or before `begin`
+    if (before < 64) {
+      b = block + before;
+      if (before > 0) base += __shfl(upto, before - 1) * heads;
+      break;
+    }
+    base += __shfl(upto, 63) * heads;
+  }
+  b = uniform(b);
+  base = uniform(base);
+  int64_t at = begin;
+  Sequence seq = sequence_of(a, plan, a.lengths[b]);
+
+  while (at < end) {
+    while (seq.units == 0 || at - base >= static_cast<int64_t>(seq.units) * heads) {  // (ends: a unit lies in some sequence)
+      base += static_cast<int64_t>(seq.units) * heads;
+      seq = sequence_of(a, plan, a.lengths[++b]);
+    }
+    // This workgroup's units [u0, u1) of head `index`.
+    const int index = static_cast<int>((at - base) / seq.units);
+    const int32_t u0 = static_cast<int32_t>((at - base) - static_cast<int64_t>(index) * seq.units);
+    const int32_t u1 = static_cast<int32_t>(min(static_cast<int64_t>(seq.units), u0 + (end - at)));
+    const int h = index / plan.query_tiles, query0 = (index - h * plan.query_tiles) * plan.query_rows;
+    const int rows = min(plan.query_rows, group - query0);
+    const int64_t query_row = b * a.heads + static_cast<int64_t>(h) * group + query0;
+    const int32_t tile_end = seq.tile0 + min(seq.tiles, u1 * plan.chunk);
+    int32_t tile = seq.tile0 + u0 * plan.chunk;
+
+    // ---- loads of a tile's 32 positions of this wave, as two blocks of 16 ----
+    const int32_t* table = a.pages.table + b * a.pages.stride;
+    auto page_of = [&](int32_t t, int s) -> int32_t {
+      const int32_t p = t * kTile + wave * kWavePositions + 16 * s;
+      const int32_t page = p < seq.length ? table[p >> kv.page_log2] : -1;
+      return page >= 0 && page < kv.pages ? page : -1;
+    };
+    auto place_of = [&](int32_t t, int s, int32_t page) -> int64_t {  // (no page: page 0, whose values are masked)
+      const int32_t slot = (t * kTile + wave * kWavePositions + 16 * s) & ((1 << kv.page_log2) - 1);
+      return (((static_cast<int64_t>(max(page, 0)) * kv.kv_heads + h) << kv.page_log2) | slot);
+    };
+    uint4 k[2][kLoads];
+    float4 ks[2], vs[2];
+    uint32_t v[2][4][kVWords];
+    auto load_keys = [&](int32_t t, const int32_t (&page)[2]) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int64_t place = place_of(t, s, page[s]);
+        const uint8_t* row = static_cast<const uint8_t*>(kv.key) + place * row_bytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          k[s][i] = make_uint4(0u, 0u, 0u, 0u);
+          if (!PAD || i * kStep + g * (kStep / 4) < dim) k[s][i] = ldg16(row + n * row_bytes + i * 64 + g * 16);
+        }
+        if constexpr (FP8) ks[s] = *reinterpret_cast<const float4*>(kv.key_scales + place + 4 * g);
+      }
+    };
+    auto load_values = [&](int32_t t, const int32_t (&page)[2]) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int64_t place = place_of(t, s, page[s]);
+        const uint8_t* row = static_cast<const uint8_t*>(kv.value) + place * row_bytes;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int i = 0; i < kVWords; ++i) v[s][r][i] = 0u;
+          if (!PAD || n * kVec < dim) {
+            const uint8_t* from = row + (4 * g + r) * row_bytes + n * (4 * kVWords);
+            if constexpr (kVWords == 1) {
+              v[s][r][0] = *reinterpret_cast<const uint32_t*>(from);
+            } else if constexpr (kVWords == 2) {
+              const uint2 w = *reinterpret_cast<const uint2*>(from);
+              v[s][r][0] = w.x, v[s][r][1] = w.y;
+            } else {
+#pragma unroll
+              for (int i = 0; i < kVWords / 4; ++i) {
+                const uint4 w = ldg16(from + 16 * i);
+                v[s][r][4 * i] = w.x, v[s][r][4 * i + 1] = w.y, v[s][r][4 * i + 2] = w.z, v[s][r][4 * i + 3] = w.w;
+              }
+            }
+          }
+        }
+        if constexpr (FP8) vs[s] = *reinterpret_cast<const float4*>(kv.value_scales + place + 4 * g);
+      }
+    };
+
+    int32_t page[2], ahead[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      page[s] = page_of(tile, s);
+      ahead[s] = tile + 1 < tile_end ? page_of(tile + 1, s) : -1;
+    }
+    // The queries of column n (of the upper half as of the lower one), in the keys' order of dimensions.
+    uint4 q[DP / 32];
+    const int row = DUP ? n & 7 : n;
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) {
+      const int c = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j % 2) : 32 * j + 8 * g;
+      q[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows && (!PAD || c < dim)) q[j] = ldg16(a.query + (query_row + row) * dim + c);
+    }
+    load_keys(tile, page);
+    load_values(tile, page);
+
+    f32x4_t o[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    bool seen = false;
+    const float scale = a.scale * 1.44269504088896340736f;
+    const uint32_t rest = DUP && n >= 8 ? 0xFFFFFFFFu : 0u;
+
+    for (; tile < tile_end; ++tile) {
+      const bool more = tile + 1 < tile_end;
+      f32x4_t s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          if constexpr (FP8) {
+            const uint4 w = k[t][i];
+            s[t] = mfma(make_uint4(fp8_pair<false>(w.x), fp8_pair<true>(w.x), fp8_pair<false>(w.y), fp8_pair<true>(w.y)), q[2 * i], s[t]);
+            s[t] = mfma(make_uint4(fp8_pair<false>(w.z), fp8_pair<true>(w.z), fp8_pair<false>(w.w), fp8_pair<true>(w.w)), q[2 * i + 1], s[t]);
+          } else {
+            s[t] = mfma(k[t][i], q[i], s[t]);
+          }
+        }
+        if constexpr (FP8) {
+          s[t][0] *= ks[t].x * scale, s[t][1] *= ks[t].y * scale, s[t][2] *= ks[t].z * scale, s[t][3] *= ks[t].w * scale;
+        } else {
+          s[t] *= scale;
+        }
+      }
+      // Positions of this tile that are seen: lo <= place < hi of each block of 16.
+      int lo[2], hi[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int32_t p = tile * kTile + wave * kWavePositions + 16 * t;
+        lo[t] = max(0, seq.first - p);
+        hi[t] = page[t] >= 0 ? min(16, seq.length - p) : 0;
+      }
+      const bool whole = lo[0] <= 0 && lo[1] <= 0 && hi[0] >= 16 && hi[1] >= 16;
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) s[t][r] = -INFINITY;
+      }
+      seen = seen || lo[0] < hi[0] || lo[1] < hi[1];
+      if (more) load_keys(tile + 1, ahead);
+
+      float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      most = fmaxf(most, xor_partner<16>(most));
+      most = fmaxf(most, xor_partner<32>(most));
+      if (__any(most > m)) {  // (seldom after the first tiles)
+        const float next = fmaxf(m, most);
+        const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) o[i] *= keep;
+        m = next;
+      }
+      const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - from);
+          l += s[t][r];
+        }
+      if constexpr (FP8) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t][0] *= vs[t].x, s[t][1] *= vs[t].y, s[t][2] *= vs[t].z, s[t][3] *= vs[t].w;
+      }
+      if (!whole) {  // (what lies in places that are not seen may be NaN)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) {
+              s[t][r] = 0.f;
+#pragma unroll
+              for (int i = 0; i < kVWords; ++i) v[t][r][i] = 0u;
+            }
+      }
+      // Weights as BF16 pairs: rounded (p), and what the rounding left (x).
+      uint32_t p[4], x[4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float y0 = s[t][2 * r], y1 = s[t][2 * r + 1];
+          const uint32_t w = pack_bf16x2(y0, y1);
+          if constexpr (DUP) {
+            const uint32_t z = w & rest;
+            p[2 * t + r] = pack_bf16x2(y0 - bf16lo(z), y1 - bf16hi(z));
+          } else {
+            p[2 * t + r] = w;
+            x[2 * t + r] = pack_bf16x2(y0 - bf16lo(w), y1 - bf16hi(w));
+          }
+        }
+      const uint4 weights = make_uint4(p[0], p[1], p[2], p[3]);
+#pragma unroll
+      for (int i = 0; i < kVec; i += 2) {  // two dimensions: a word of each of the eight keys
+        uint32_t w[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (FP8) w[t][r] = i % 4 == 0 ? fp8_pair<false>(v[t][r][i / 4]) : fp8_pair<true>(v[t][r][i / 4]);
+            else w[t][r] = v[t][r][i / 2];
+          }
+        const uint4 even = make_uint4(perm(w[0][1], w[0][0], 0x05040100u), perm(w[0][3], w[0][2], 0x05040100u),
+                                      perm(w[1][1], w[1][0], 0x05040100u), perm(w[1][3], w[1][2], 0x05040100u));
+        const uint4 odd = make_uint4(perm(w[0][1], w[0][0], 0x07060302u), perm(w[0][3], w[0][2], 0x07060302u),
+                                     perm(w[1][1], w[1][0], 0x07060302u), perm(w[1][3], w[1][2], 0x07060302u));
+        o[i] = mfma(even, weights, o[i]);
+        o[i + 1] = mfma(odd, weights, o[i + 1]);
+        if constexpr (!DUP) {
+          const uint4 rests = make_uint4(x[0], x[1], x[2], x[3]);
+          o[i] = mfma(even, rests, o[i]);
+          o[i + 1] = mfma(odd, rests, o[i + 1]);
+        }
+      }
+      if (more) {
+        load_values(tile + 1, ahead);
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          page[s2] = ahead[s2];
+          ahead[s2] = tile + 2 < tile_end ? page_of(tile + 2, s2) : -1;
+        }
+      }
+    }
+
+    // ---- join of the waves ----
+    l += xor_partner<16>(l);
+    l += xor_partner<32>(l);
+    if (m == -INFINITY && seen) {
+      if (l == 0.f) l = NAN;  // every score -inf
+      else m = 0.f;           // every score -inf or NaN
+    }
+    if constexpr (DUP) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[i][r] += other_half(o[i][r]);
+    }
+    __syncthreads();  // (the last head's join has been read)
+    if (n < rows) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < kVec; i += 4)
+          *reinterpret_cast<float4*>(&part_o[wave][n][kVec * (4 * g + r) + i]) = make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
+      if (g == 0) {
+        part_m[wave][n] = m;
+        part_l[wave][n] = l;
+      }
+    }
+    __syncthreads();
+    const bool complete = u0 == 0 && u1 == seq.units;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at == begin ? 0 : 1);
+    float* part = a.workspace + slot * kRows * (DP + 2);
+    for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads) {
+      const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
+      float all = part_m[0][r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) all = fmaxf(all, part_m[w][r]);
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = part_factor(part_m[w][r], all);
+        const float4 y = *reinterpret_cast<const float4*>(&part_o[w][r][c]);
+        sum += weighted(f, part_l[w][r]);
+        acc.x += weighted(f, y.x), acc.y += weighted(f, y.y), acc.z += weighted(f, y.z), acc.w += weighted(f, y.w);
+      }
+      if (complete) {
+        if (!PAD || c < dim) {
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          *reinterpret_cast<uint2*>(a.out + (query_row + r) * dim + c) =
+              make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        }
+      } else {
+        *reinterpret_cast<float4*>(part + r * DP + c) = acc;
+        if (c == 0) {
+          part[kRows * DP + 2 * r] = all;
+          part[kRows * DP + 2 * r + 1] = sum;
+        }
+      }
+    }
+    at += u1 - u0;
   }
 }
 
-// A workgroup per sequence and query head; each wave takes every fourth position,
-// a lane four of the head's dimensions.
-template <bool FP8>
-__global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentionArgs a) {
-  __shared__ float part_ml[kWaves][2];
-  __shared__ float part_o[kWaves][kMaxHeadDim];
+// Joins the parts of one query head (a workgroup each): 4 dimensions a thread,
+// the parts dealt out over kThreads / (DP / 4) groups of threads.
+template <int DP>
+__global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, Plan plan) {
+  constexpr int kLanes = DP / 4, kSets = kThreads / kLanes;
+  __shared__ float4 sums[kSets][kLanes];
+  __shared__ float parts[kWaves], totals[kSets];
   const KvPages& kv = a.cache;
-  const int wave = threadIdx.x / 64, c = 4 * (threadIdx.x % 64), head = blockIdx.x % a.heads;
+  const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles, rows = plan.query_rows <= 8 ? 8 : 16;
   const int64_t b = blockIdx.x / a.heads;
-  const int h = head / (a.heads / kv.kv_heads);
-  const bool mine = c < kv.dim;
-  const int64_t capacity = static_cast<int64_t>(a.pages.width) << kv.page_log2;
-  const int64_t length = max(static_cast<int64_t>(0), min(static_cast<int64_t>(a.lengths[b]), capacity));
-  float q[4] = {}, o[4] = {};
-  if (mine) {
-    const uint2 w = *reinterpret_cast<const uint2*>(a.query + (b * a.heads + head) * kv.dim + c);
-    q[0] = bf16lo(w.x), q[1] = bf16hi(w.x), q[2] = bf16lo(w.y), q[3] = bf16hi(w.y);
-  }
-  float m = -INFINITY, l = 0.f;
-  bool seen = false;
-  for (int64_t p = max(static_cast<int64_t>(0), length - a.window) + wave; p < length; p += kWaves) {
-    const int32_t page = a.pages.table[b * a.pages.stride + (p >> kv.page_log2)];
-    if (page < 0 || page >= kv.pages) continue;
-    seen = true;
-    const int64_t place = (((static_cast<int64_t>(page) * kv.kv_heads + h) << kv.page_log2) | (p & ((1 << kv.page_log2) - 1)));
-    float k[4] = {}, v[4] = {};
-    if (mine) {
-      load4<FP8>(kv.key, kv.key_scales, place, kv.dim, c, k);
-      load4<FP8>(kv.value, kv.value_scales, place, kv.dim, c, v);
-    }
-    const float s = a.scale * wave_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-    const float m_new = fmaxf(m, s), from = m_new == -INFINITY ? 0.f : m_new;
-    const float keep = __expf(m - from), w = __expf(s - from);
-    m = m_new;
-    l = l * keep + w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + w * v[i];
-  }
-  if (threadIdx.x % 64 == 0) {
-    if (m == -INFINITY && seen) l == 0.f ? l = NAN : m = 0.f;  // every score -inf: 0 / 0, unless another wave has a finite one
-    part_ml[wave][0] = m;
-    part_ml[wave][1] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part_o[wave][c + i] = o[i];
-  __syncthreads();
-  if (static_cast<int>(threadIdx.x) >= kv.dim) return;
+  const int head = static_cast<int>(blockIdx.x - b * a.heads), h = head / group;
+  const int tile = (head - h * group) / plan.query_rows, row = (head - h * group) - tile * plan.query_rows;
+  const Sequence seq = sequence_of(a, plan, a.lengths[b]);
+  if (seq.units == 0) return;
+  const int64_t before = units_before(a, plan, b);
+  const Work work = work_of(units_before(a, plan, a.batch), heads, plan);
+  const int64_t first = before * heads + static_cast<int64_t>(h * plan.query_tiles + tile) * seq.units;
+  const int64_t w0 = first / work.per, w1 = (first + seq.units - 1) / work.per;
+  if (w0 == w1) return;  // one workgroup had it all
+  // (a part is in its workgroup's first place but where another head came before it there)
+  const int64_t stride = static_cast<int64_t>(rows) * (DP + 2);
+  const int64_t first_slot = 2 * w0 + (first % work.per != 0 ? 1 : 0);
+  auto part_of = [&](int64_t w) { return a.workspace + (w == w0 ? first_slot : 2 * w) * stride; };
+
   float most = -INFINITY;
-  for (int w = 0; w < kWaves; ++w) most = fmaxf(most, part_ml[w][0]);
-  float sum = 0.f, acc = 0.f;
-  for (int w = 0; w < kWaves; ++w) {
-    if (most != -INFINITY && part_ml[w][0] == -INFINITY) continue;
-    const float f = most == -INFINITY ? 1.f : __expf(part_ml[w][0] - most);
-    sum += f * part_ml[w][1];
-    acc += f * part_o[w][threadIdx.x];
+  for (int64_t w = w0 + threadIdx.x; w <= w1; w += kThreads) most = fmaxf(most, part_of(w)[rows * DP + 2 * row]);
+  most = wave_max(most);
+  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3]));
+  const int lane = threadIdx.x % kLanes, set = threadIdx.x / kLanes;
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int64_t w = w0 + set; w <= w1; w += kSets) {
+    const float* part = part_of(w);
+    const float f = part_factor(part[rows * DP + 2 * row], most);
+    const float4 y = *reinterpret_cast<const float4*>(part + row * DP + 4 * lane);
+    sum += weighted(f, part[rows * DP + 2 * row + 1]);
+    acc.x += weighted(f, y.x), acc.y += weighted(f, y.y), acc.z += weighted(f, y.z), acc.w += weighted(f, y.w);
   }
-  a.out[(b * a.heads + head) * kv.dim + threadIdx.x] = f32_to_bf16(sum == 0.f ? 0.f : acc / sum);
+  sums[set][lane] = acc;
+  if (lane == 0) totals[set] = sum;
+  __syncthreads();
+  if (set != 0 || 4 * lane >= kv.dim) return;
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < kSets; ++i) {
+    const float4 y = sums[i][lane];
+    sum += totals[i];
+    acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(a.out + blockIdx.x * static_cast<int64_t>(kv.dim) + 4 * lane) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
+int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+// Which sizes the device's lengths may have is known from the table's width alone.
+Plan plan_of(const PagedAttentionArgs& a, int cus) {
+  Plan p;
+  const int group = a.heads / a.cache.kv_heads;
+  p.query_tiles = (group + 15) / 16;
+  p.query_rows = (group + p.query_tiles - 1) / p.query_tiles;
+  const int64_t capacity = static_cast<int64_t>(a.pages.width) << a.cache.page_log2;
+  const int64_t tiles = std::max<int64_t>(1, (capacity + kTile - 1) / kTile);
+  const int64_t heads = a.batch * a.cache.kv_heads * p.query_tiles;
+  p.chunk = static_cast<int32_t>(tiles <= kDirectTiles ? tiles : 1);
+  const int64_t units = heads * ((tiles + p.chunk - 1) / p.chunk);
+  p.groups = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(units, static_cast<int64_t>(kGroupsPerCu) * cus)));
+  return p;
+}
+// Whether a head may be more than one workgroup's.
+bool splits(const PagedAttentionArgs& a, const Plan& p) {
+  return (static_cast<int64_t>(a.pages.width) << a.cache.page_log2) > static_cast<int64_t>(p.chunk) * kTile;
+}
+
+template <int DP, bool FP8, bool DUP>
+void launch_main(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream) {
+  if (a.cache.dim == DP) paged_attention_kernel<DP, FP8, DUP, false><<<p.groups, kThreads, 0, stream>>>(a, p);
+  else paged_attention_kernel<DP, FP8, DUP, true><<<p.groups, kThreads, 0, stream>>>(a, p);
+}
+template <int DP>
+hipError_t launch(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream) {
+  const bool fp8 = a.cache.key_scales != nullptr, dup = p.query_rows <= 8;
+  if (fp8 && dup) launch_main<DP, true, true>(a, p, stream);
+  else if (fp8) launch_main<DP, true, false>(a, p, stream);
+  else if (dup) launch_main<DP, false, true>(a, p, stream);
+  else launch_main<DP, false, false>(a, p, stream);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !splits(a, p)) return e;
+  join_parts_kernel<DP><<<static_cast<unsigned>(a.batch * a.heads), kThreads, 0, stream>>>(a, p);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-size_t paged_attention_workspace(const PagedAttentionArgs&, int) { return 0; }
+size_t paged_attention_workspace(const PagedAttentionArgs& a, int cus) {
+  if (a.batch == 0) return 0;
+  const Plan p = plan_of(a, cus);
+  if (!splits(a, p)) return 0;
+  return 2 * static_cast<size_t>(p.groups) * (p.query_rows <= 8 ? 8 : 16) * (padded_dim(a.cache.dim) + 2) * sizeof(float);
+}
 
-hipError_t launch_paged_attention(const PagedAttentionArgs& a, int, hipStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(a.batch * a.heads);
-  if (a.cache.key_scales != nullptr) paged_attention_kernel<true><<<grid, kThreads, 0, stream>>>(a);
-  else paged_attention_kernel<false><<<grid, kThreads, 0, stream>>>(a);
-  return hipGetLastError();
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, int cus, hipStream_t stream) {
+  const Plan p = plan_of(a, cus);
+  switch (padded_dim(a.cache.dim)) {
+    case 64: return launch<64>(a, p, stream);
+    case 128: return launch<128>(a, p, stream);
+    default: return launch<256>(a, p, stream);
+  }
 }
 
 }  // namespace uqm
