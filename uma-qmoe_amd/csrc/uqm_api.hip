@@ -1623,14 +1623,6 @@ int uqm_kv_read(const uqm_kv_cache* cache, int64_t batch, const int32_t* page_ta
   return hip_check(launch_kv_read(a, static_cast<hipStream_t>(stream)), "kv_read launch");
 }
 
-static int check_attention_sizes(int64_t batch, int64_t heads, int64_t kv_heads) {
-  if (heads <= 0 || heads % kv_heads != 0)
-    return fail(UQM_ERR_ARGUMENT, "paged_attention: %lld heads must be a positive multiple of the %lld key heads", (long long)heads, (long long)kv_heads);
-  if (heads >= kMaxQueryHeads || batch * heads >= kMaxQueryHeads)
-    return fail(UQM_ERR_ARGUMENT, "paged_attention: batch * heads must be below 2^24");
-  return UQM_OK;
-}
-
 static uqm::PagedAttentionArgs attention_sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                int64_t page_size, int64_t max_pages) {
   uqm::PagedAttentionArgs a{};
@@ -1643,11 +1635,22 @@ static uqm::PagedAttentionArgs attention_sizes(int64_t batch, int64_t heads, int
   return a;
 }
 
+static int check_attention_sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                 int64_t max_pages) {
+  if (heads <= 0 || heads % kv_heads != 0)
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: %lld heads must be a positive multiple of the %lld key heads", (long long)heads, (long long)kv_heads);
+  if (heads >= kMaxQueryHeads || batch * heads >= kMaxQueryHeads)
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: batch * heads must be below 2^24");
+  if (!uqm::paged_attention_fits(attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages)))
+    return fail(UQM_ERR_ARGUMENT, "paged_attention: batch * kv_heads * max_pages * page_size is more than a call has room for");
+  return UQM_OK;
+}
+
 size_t uqm_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                            int64_t page_size, int64_t max_pages) {
   if (check_kv_sizes("paged_attention", 1, kv_heads, page_size, head_dim) ||
       check_page_table("paged_attention", batch, page_size, max_pages, max_pages) ||
-      check_attention_sizes(batch, heads, kv_heads))
+      check_attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages))
     return 0;
   return uqm::paged_attention_workspace(attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages), device_cus());
 }
@@ -1659,7 +1662,7 @@ int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t ba
   using namespace uqm;
   int rc = check_cache("paged_attention", cache);
   if (rc || (rc = check_page_table("paged_attention", batch, cache->page_size, table_stride, max_pages)) ||
-      (rc = check_attention_sizes(batch, heads, cache->kv_heads)))
+      (rc = check_attention_sizes(batch, heads, cache->kv_heads, cache->head_dim, cache->page_size, max_pages)))
     return rc;
   if (!(scale - scale == 0.f)) return fail(UQM_ERR_ARGUMENT, "paged_attention: scale must be finite");
   if (window < 0) return fail(UQM_ERR_ARGUMENT, "paged_attention: window must be at least 1, or 0 for none");
@@ -1687,7 +1690,7 @@ int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t ba
   a.pages = {page_table, table_stride, static_cast<int32_t>(max_pages)};
   a.query = static_cast<const uint16_t*>(query);
   a.lengths = lengths;
-  a.window = window > 0 ? window : INT64_MAX;
+  a.window = static_cast<int32_t>(window > 0 && window < INT32_MAX ? window : INT32_MAX);
   a.scale = scale;
   a.out = static_cast<uint16_t*>(output);
   a.workspace = static_cast<float*>(workspace);

@@ -72,11 +72,13 @@ struct PagedAttentionArgs {
   int64_t batch;
   int heads;
   const int32_t* lengths;  // [batch]
-  int64_t window;          // positions seen, from the last one back
+  int32_t window;          // positions seen, from the last one back
   float scale;
   uint16_t* out;           // [batch, heads, dim]
   float* workspace;
 };
+// Whether the work can be numbered (below 2^31 tiles of 128 positions and 16 query heads).
+bool paged_attention_fits(const PagedAttentionArgs& a);
 size_t paged_attention_workspace(const PagedAttentionArgs& a, int cus);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, int cus, hipStream_t stream);
 

@@ -38,6 +38,7 @@
 // enough a workgroup takes whole heads, and there is no second launch.
 #include "uqm_device.h"
 #include "uqm_kv.h"
+#include "uqm_stage.h"
 
 #include <algorithm>
 
@@ -57,60 +58,71 @@ template <bool HI>
 __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
+constexpr uint32_t kOutside = 0x80000000u;  // an offset behind every buffer's bytes
+__device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, 0));
+}
+__device__ __forceinline__ float4 as_float4(uint4 w) {
+  return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+}
 // The value of lane ^ 8.
 __device__ __forceinline__ float other_half(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));  // row_ror:8
 }
 
-// Where the work lies, from the lengths on the device.
-struct Work {
-  int64_t per;     // units of a workgroup
-  int64_t units;   // of all sequences and heads
-};
+// Lengths and page tables are read where all lanes want the same entry: through the
+// scalar cache, so that a wait for an entry is none for the keys and values that are
+// on their way (vector loads arrive in order). Nothing in a launch writes them.
+typedef const __attribute__((address_space(4))) int32_t* Indexes;
+__device__ __forceinline__ Indexes indexes(const int32_t* p) { return reinterpret_cast<Indexes>(reinterpret_cast<uintptr_t>(p)); }
+
 struct Plan {
-  int32_t chunk;        // tiles of a unit
   int32_t groups;       // workgroups of the launch
   int32_t query_rows;   // query heads of a unit (at most)
   int32_t query_tiles;  // units side by side for the query heads of a key head
+  bool whole;           // a sequence's head is one unit, whatever its length
 };
 
 struct Sequence {
-  int32_t length, first;          // positions seen: first .. length - 1
-  int32_t tile0, tiles, units;    // tiles from tile0 on; units of one head
+  int32_t length, first;         // positions seen: first .. length - 1
+  int32_t tile0, tiles, units;   // tiles from tile0 on; units of one head (one at least, which writes the zeros)
 };
 __device__ __forceinline__ Sequence sequence_of(const PagedAttentionArgs& a, const Plan& plan, int32_t given) {
   Sequence s;
-  const int64_t capacity = static_cast<int64_t>(a.pages.width) << a.cache.page_log2;  // below 2^31
-  s.length = min(max(given, 0), static_cast<int32_t>(capacity));
-  s.first = static_cast<int32_t>(max(static_cast<int64_t>(0), s.length - a.window));
+  s.length = min(max(given, 0), a.pages.width << a.cache.page_log2);
+  s.first = s.length > a.window ? s.length - a.window : 0;
   s.tile0 = s.first / kTile;
   s.tiles = (s.length + kTile - 1) / kTile - s.tile0;  // (0 at length 0: first is 0, too)
-  s.units = (s.tiles + plan.chunk - 1) / plan.chunk;
+  s.units = plan.whole ? 1 : max(1, s.tiles);
   return s;
 }
 
-// A value that every lane has, in scalar registers.
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  return static_cast<int64_t>((static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32) | lo);
-}
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return uniform(v);
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int32_t wave_scan(int32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
 }
 
-// Units of one head over sequences [0, end), every lane of the wave the same.
-__device__ __forceinline__ int64_t units_before(const PagedAttentionArgs& a, const Plan& plan, int64_t end) {
-  int64_t sum = 0;
-  for (int64_t b = threadIdx.x & 63; b < end; b += 64) sum += sequence_of(a, plan, a.lengths[b]).units;
-  return wave_sum64(sum);
+// Units of one head of sequences before `end`, and of all (the sums of every head's
+// are below 2^31).
+__device__ __forceinline__ int32_t units_before(const PagedAttentionArgs& a, const Plan& plan, int32_t end, int32_t* all) {
+  int32_t before = 0, total = 0;
+  for (int32_t block = 0; block < a.batch; block += 64) {
+    const int32_t b = block + static_cast<int32_t>(threadIdx.x & 63);
+    const int32_t units = b < a.batch ? sequence_of(a, plan, a.lengths[b]).units : 0;
+    total += __builtin_amdgcn_readlane(wave_scan(units), 63);
+    before += __builtin_amdgcn_readlane(wave_scan(b < end ? units : 0), 63);
+  }
+  *all = total;
+  return before;
 }
-__device__ __forceinline__ Work work_of(int64_t head_units, int heads, const Plan& plan) {
-  Work w;
-  w.units = head_units * heads;
-  w.per = max(static_cast<int64_t>(1), (w.units + plan.groups - 1) / plan.groups);
-  return w;
+__device__ __forceinline__ int32_t units_per_group(int32_t units, const Plan& plan) {
+  return (units + plan.groups - 1) / plan.groups;
 }
 
 // A workgroup's part of a row: weights relative to 2^most, their sum, the sum of
@@ -121,8 +133,11 @@ __device__ __forceinline__ float part_factor(float most, float all) {
 }
 __device__ __forceinline__ float weighted(float f, float v) { return f == 0.0f ? 0.0f : f * v; }
 
+#ifndef MINW
+#define MINW 3
+#endif
 template <int DP, bool FP8, bool DUP, bool PAD>
-__global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
+__global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
   constexpr int kRows = DUP ? 8 : 16;      // query heads of a unit
   constexpr int kVec = DP / 16;            // dimensions of a value row that a lane holds
   constexpr int kStep = FP8 ? 64 : 32;     // dimensions of one load of 16 keys
@@ -139,65 +154,83 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
   const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles;
   const int row_bytes = FP8 ? dim : 2 * dim;
 
-  // Zeros for sequences without a position.
-  for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    if (sequence_of(a, plan, a.lengths[b]).tiles > 0) continue;
-    uint4* out = reinterpret_cast<uint4*>(a.out + b * a.heads * dim);
-    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(a.heads) * dim / 8; i += kThreads) out[i] = make_uint4(0u, 0u, 0u, 0u);
-  }
-
-  const Work work = work_of(units_before(a, plan, a.batch), heads, plan);
-  const int64_t begin = blockIdx.x * work.per, end = min(begin + work.per, work.units);
-  if (begin >= end) return;
-
-  // The sequence of the first unit, and its own first unit.
-  int64_t b = 0, base = 0;
-  for (int64_t block = 0; block < a.batch; block += 64) {
-    int64_t units = block + lane < a.batch ? sequence_of(a, plan, a.lengths[block + lane]).units : 0;
-    int64_t upto = units;  // inclusive sum over the lanes
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(upto, o);
-      if (lane >= o) upto += v;
+  // This workgroup's units [begin, end), the sequence of the first and that sequence's first unit.
+  int32_t b, base = 0, begin, end;
+  Sequence seq;
+  if (plan.whole) {
+    begin = blockIdx.x, end = begin + 1;
+    b = begin / heads;
+    base = b * heads;
+    seq = sequence_of(a, plan, indexes(a.lengths)[b]);
+  } else if (a.batch == 1) {
+    b = 0;
+    seq = sequence_of(a, plan, indexes(a.lengths)[0]);
+    const int32_t per = units_per_group(seq.units * heads, plan);
+    begin = blockIdx.x * per;
+    end = min(begin + per, seq.units * heads);
+    if (begin >= end) return;
+  } else {
+    int32_t units, given = 0;
+    units_before(a, plan, 0, &units);
+    units *= heads;
+    const int32_t per = units_per_group(units, plan);
+    begin = blockIdx.x * per;
+    end = min(begin + per, units);
+    if (begin >= end) return;
+    for (b = 0;; b += 64) {  // (ends: begin is below the sum)
+      const int32_t mine = b + lane < a.batch ? a.lengths[b + lane] : 0;
+      const int32_t upto = wave_scan(b + lane < a.batch ? sequence_of(a, plan, mine).units : 0);
+      const int before = __popcll(__ballot(base + upto * heads <= begin));  // sequences that end at or before `begin`
+      if (before < 64) {
+        if (before > 0) base += __builtin_amdgcn_readlane(upto, before - 1) * heads;
+        given = __builtin_amdgcn_readlane(mine, before);
+        b += before;
+        break;
+      }
+      base += __builtin_amdgcn_readlane(upto, 63) * heads;
     }
-    const int before = __popcll(__ballot(base + upto * heads <= begin));  // sequences that end at or before `begin`
-    if (before < 64) {
-      b = block + before;
-      if (before > 0) base += __shfl(upto, before - 1) * heads;
-      break;
-    }
-    base += __shfl(upto, 63) * heads;
+    seq = sequence_of(a, plan, given);
   }
-  b = uniform(b);
-  base = uniform(base);
-  int64_t at = begin;
-  Sequence seq = sequence_of(a, plan, a.lengths[b]);
+  int32_t at = begin;
 
   while (at < end) {
-    while (seq.units == 0 || at - base >= static_cast<int64_t>(seq.units) * heads) {  // (ends: a unit lies in some sequence)
-      base += static_cast<int64_t>(seq.units) * heads;
-      seq = sequence_of(a, plan, a.lengths[++b]);
+    while (at - base >= seq.units * heads) {  // (ends: a unit lies in some sequence)
+      base += seq.units * heads;
+      seq = sequence_of(a, plan, indexes(a.lengths)[++b]);
     }
     // This workgroup's units [u0, u1) of head `index`.
-    const int index = static_cast<int>((at - base) / seq.units);
-    const int32_t u0 = static_cast<int32_t>((at - base) - static_cast<int64_t>(index) * seq.units);
-    const int32_t u1 = static_cast<int32_t>(min(static_cast<int64_t>(seq.units), u0 + (end - at)));
+    const int32_t index = (at - base) / seq.units, u0 = (at - base) - index * seq.units;
+    const int32_t u1 = min(seq.units, u0 + (end - at));
     const int h = index / plan.query_tiles, query0 = (index - h * plan.query_tiles) * plan.query_rows;
     const int rows = min(plan.query_rows, group - query0);
-    const int64_t query_row = b * a.heads + static_cast<int64_t>(h) * group + query0;
-    const int32_t tile_end = seq.tile0 + min(seq.tiles, u1 * plan.chunk);
-    int32_t tile = seq.tile0 + u0 * plan.chunk;
+    const int64_t query_row = static_cast<int64_t>(b) * a.heads + h * group + query0;
+    const int32_t tile_end = seq.tile0 + (plan.whole ? seq.tiles : min(seq.tiles, u1));
+    int32_t tile = seq.tile0 + u0;
 
     // ---- loads of a tile's 32 positions of this wave, as two blocks of 16 ----
-    const int32_t* table = a.pages.table + b * a.pages.stride;
-    auto page_of = [&](int32_t t, int s) -> int32_t {
-      const int32_t p = t * kTile + wave * kWavePositions + 16 * s;
-      const int32_t page = p < seq.length ? table[p >> kv.page_log2] : -1;
-      return page >= 0 && page < kv.pages ? page : -1;
+    const Indexes table = indexes(a.pages.table + static_cast<int64_t>(b) * a.pages.stride);
+    // (entries of tiles behind the last are asked for, too, and count as none: the loop
+    // has no branch around its loads, behind which a wait could not tell them apart)
+    auto entry_of = [&](int32_t t, int s) -> int32_t {
+      return table[min(t * kTile + wave * kWavePositions + 16 * s, seq.length - 1) >> kv.page_log2];
     };
-    auto place_of = [&](int32_t t, int s, int32_t page) -> int64_t {  // (no page: page 0, whose values are masked)
+    auto page_of = [&](int32_t t, int s, int32_t entry) -> int32_t {
+      const bool there = t < tile_end && t * kTile + wave * kWavePositions + 16 * s < seq.length && entry < kv.pages;
+      return there ? entry : -1;  // (an entry below 0: none, too)
+    };
+    // (no page: page 0, whose values are masked)
+    const int64_t page_rows = static_cast<int64_t>(kv.kv_heads) << kv.page_log2;
+    auto place_of = [&](int32_t t, int s, int32_t page) -> int64_t {
       const int32_t slot = (t * kTile + wave * kWavePositions + 16 * s) & ((1 << kv.page_log2) - 1);
-      return (((static_cast<int64_t>(max(page, 0)) * kv.kv_heads + h) << kv.page_log2) | slot);
+      return max(page, 0) * page_rows + ((h << kv.page_log2) | slot);
+    };
+    const uint32_t key_at = n * row_bytes + 16 * g;
+    const uint32_t value_at = !PAD || n * kVec < dim ? 4 * g * row_bytes + n * (4 * kVWords) : kOutside;
+    // Blocks are read through buffers that end behind their last position that is seen
+    // (at once where there is no page): what lies behind reads as zeros and costs
+    // nothing, as do dimensions behind the last.
+    auto seen_of = [&](int32_t t, int s, int32_t page) -> int32_t {
+      return page >= 0 ? min(16, seq.length - (t * kTile + wave * kWavePositions + 16 * s)) : 0;
     };
     uint4 k[2][kLoads];
     float4 ks[2], vs[2];
@@ -206,49 +239,50 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int64_t place = place_of(t, s, page[s]);
-        const uint8_t* row = static_cast<const uint8_t*>(kv.key) + place * row_bytes;
+        const int32_t rows = seen_of(t, s, page[s]);
+        const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.key) + place * row_bytes, rows * row_bytes);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          k[s][i] = make_uint4(0u, 0u, 0u, 0u);
-          if (!PAD || i * kStep + g * (kStep / 4) < dim) k[s][i] = ldg16(row + n * row_bytes + i * 64 + g * 16);
-        }
-        if constexpr (FP8) ks[s] = *reinterpret_cast<const float4*>(kv.key_scales + place + 4 * g);
+        for (int i = 0; i < kLoads; ++i)
+          k[s][i] = load16(buf, (!PAD || i * kStep + g * (kStep / 4) < dim ? key_at : kOutside) + 64 * i);
+        if constexpr (FP8) ks[s] = as_float4(load16(stage_buffer(kv.key_scales + place, rows > 0 ? 64 : 0), 16u * g));
       }
     };
     auto load_values = [&](int32_t t, const int32_t (&page)[2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int64_t place = place_of(t, s, page[s]);
-        const uint8_t* row = static_cast<const uint8_t*>(kv.value) + place * row_bytes;
+        const int32_t rows = seen_of(t, s, page[s]);
+        const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.value) + place * row_bytes, rows * row_bytes);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+          const uint32_t at = value_at + r * row_bytes;
+          if constexpr (kVWords == 1) {
+            v[s][r][0] = __builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, 0);
+          } else if constexpr (kVWords == 2) {
+            const auto w = __builtin_amdgcn_raw_buffer_load_b64(buf, at, 0, 0);
+            v[s][r][0] = w[0], v[s][r][1] = w[1];
+          } else {
 #pragma unroll
-          for (int i = 0; i < kVWords; ++i) v[s][r][i] = 0u;
-          if (!PAD || n * kVec < dim) {
-            const uint8_t* from = row + (4 * g + r) * row_bytes + n * (4 * kVWords);
-            if constexpr (kVWords == 1) {
-              v[s][r][0] = *reinterpret_cast<const uint32_t*>(from);
-            } else if constexpr (kVWords == 2) {
-              const uint2 w = *reinterpret_cast<const uint2*>(from);
-              v[s][r][0] = w.x, v[s][r][1] = w.y;
-            } else {
-#pragma unroll
-              for (int i = 0; i < kVWords / 4; ++i) {
-                const uint4 w = ldg16(from + 16 * i);
-                v[s][r][4 * i] = w.x, v[s][r][4 * i + 1] = w.y, v[s][r][4 * i + 2] = w.z, v[s][r][4 * i + 3] = w.w;
-              }
+            for (int i = 0; i < kVWords / 4; ++i) {
+              const uint4 w = load16(buf, at + 16 * i);
+              v[s][r][4 * i] = w.x, v[s][r][4 * i + 1] = w.y, v[s][r][4 * i + 2] = w.z, v[s][r][4 * i + 3] = w.w;
             }
           }
         }
-        if constexpr (FP8) vs[s] = *reinterpret_cast<const float4*>(kv.value_scales + place + 4 * g);
+        if constexpr (FP8) vs[s] = as_float4(load16(stage_buffer(kv.value_scales + place, rows > 0 ? 64 : 0), 16u * g));
       }
     };
-
-    int32_t page[2], ahead[2];
+    f32x4_t o[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    bool seen = false;
+    if (tile < tile_end) {  // (a sequence without a position may have no table)
+    int32_t page[2], ahead[2], entry[2];  // pages of this tile and the next one, what the table says of the one behind
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      page[s] = page_of(tile, s);
-      ahead[s] = tile + 1 < tile_end ? page_of(tile + 1, s) : -1;
+      page[s] = page_of(tile, s, entry_of(tile, s));
+      entry[s] = entry_of(tile + 1, s);
     }
     // The queries of column n (of the upper half as of the lower one), in the keys' order of dimensions.
     uint4 q[DP / 32];
@@ -260,32 +294,33 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
       if (row < rows && (!PAD || c < dim)) q[j] = ldg16(a.query + (query_row + row) * dim + c);
     }
     load_keys(tile, page);
+    __builtin_amdgcn_sched_barrier(0);  // (in this order, as in the loop)
     load_values(tile, page);
+    __builtin_amdgcn_sched_barrier(0);
 
-    f32x4_t o[kVec];
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    bool seen = false;
     const float scale = a.scale * 1.44269504088896340736f;
     const uint32_t rest = DUP && n >= 8 ? 0xFFFFFFFFu : 0u;
 
     for (; tile < tile_end; ++tile) {
-      const bool more = tile + 1 < tile_end;
       f32x4_t s[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t) s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          if constexpr (FP8) {
-            const uint4 w = k[t][i];
-            s[t] = mfma(make_uint4(fp8_pair<false>(w.x), fp8_pair<true>(w.x), fp8_pair<false>(w.y), fp8_pair<true>(w.y)), q[2 * i], s[t]);
-            s[t] = mfma(make_uint4(fp8_pair<false>(w.z), fp8_pair<true>(w.z), fp8_pair<false>(w.w), fp8_pair<true>(w.w)), q[2 * i + 1], s[t]);
-          } else {
-            s[t] = mfma(k[t][i], q[i], s[t]);
+      for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+        for (int half = 0; half < (FP8 ? 2 : 1); ++half)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if constexpr (FP8) {
+              const uint32_t lo = half == 0 ? k[t][i].x : k[t][i].z, hi = half == 0 ? k[t][i].y : k[t][i].w;
+              s[t] = mfma(make_uint4(fp8_pair<false>(lo), fp8_pair<true>(lo), fp8_pair<false>(hi), fp8_pair<true>(hi)),
+                          q[2 * i + half], s[t]);
+            } else {
+              s[t] = mfma(k[t][i], q[i], s[t]);
+            }
           }
-        }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         if constexpr (FP8) {
           s[t][0] *= ks[t].x * scale, s[t][1] *= ks[t].y * scale, s[t][2] *= ks[t].z * scale, s[t][3] *= ks[t].w * scale;
         } else {
@@ -298,7 +333,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
       for (int t = 0; t < 2; ++t) {
         const int32_t p = tile * kTile + wave * kWavePositions + 16 * t;
         lo[t] = max(0, seq.first - p);
-        hi[t] = page[t] >= 0 ? min(16, seq.length - p) : 0;
+        hi[t] = seen_of(tile, t, page[t]);
       }
       const bool whole = lo[0] <= 0 && lo[1] <= 0 && hi[0] >= 16 && hi[1] >= 16;
       if (!whole) {
@@ -309,7 +344,14 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
             if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) s[t][r] = -INFINITY;
       }
       seen = seen || lo[0] < hi[0] || lo[1] < hi[1];
-      if (more) load_keys(tile + 1, ahead);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        ahead[t] = page_of(tile + 1, t, entry[t]);
+        entry[t] = entry_of(tile + 2, t);
+      }
+      load_keys(tile + 1, ahead);
+      __builtin_amdgcn_sched_barrier(0);
 
       float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       most = fmaxf(most, xor_partner<16>(most));
@@ -334,16 +376,16 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
 #pragma unroll
         for (int t = 0; t < 2; ++t) s[t][0] *= vs[t].x, s[t][1] *= vs[t].y, s[t][2] *= vs[t].z, s[t][3] *= vs[t].w;
       }
-      if (!whole) {  // (what lies in places that are not seen may be NaN)
+      if (!whole) {  // (what lies in places that are not seen may be NaN; values behind the last read as zeros)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) {
-              s[t][r] = 0.f;
+          for (int r = 0; r < 4; ++r) {
+            if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) s[t][r] = 0.f;
 #pragma unroll
-              for (int i = 0; i < kVWords; ++i) v[t][r][i] = 0u;
-            }
+            for (int i = 0; i < kVWords; ++i)
+              if (4 * g + r < lo[t]) v[t][r][i] = 0u;
+          }
       }
       // Weights as BF16 pairs: rounded (p), and what the rounding left (x).
       uint32_t p[4], x[4];
@@ -384,14 +426,12 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
           o[i + 1] = mfma(odd, rests, o[i + 1]);
         }
       }
-      if (more) {
-        load_values(tile + 1, ahead);
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(tile + 1, ahead);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-          page[s2] = ahead[s2];
-          ahead[s2] = tile + 2 < tile_end ? page_of(tile + 2, s2) : -1;
-        }
-      }
+      for (int t = 0; t < 2; ++t) page[t] = ahead[t];
+    }
     }
 
     // ---- join of the waves ----
@@ -421,7 +461,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
     }
     __syncthreads();
     const bool complete = u0 == 0 && u1 == seq.units;
-    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at == begin ? 0 : 1);
+    const int64_t slot = 2 * blockIdx.x + (at == begin ? 0 : 1);
     float* part = a.workspace + slot * kRows * (DP + 2);
     for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads) {
       const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
@@ -464,23 +504,22 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   __shared__ float parts[kWaves], totals[kSets];
   const KvPages& kv = a.cache;
   const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles, rows = plan.query_rows <= 8 ? 8 : 16;
-  const int64_t b = blockIdx.x / a.heads;
-  const int head = static_cast<int>(blockIdx.x - b * a.heads), h = head / group;
-  const int tile = (head - h * group) / plan.query_rows, row = (head - h * group) - tile * plan.query_rows;
-  const Sequence seq = sequence_of(a, plan, a.lengths[b]);
-  if (seq.units == 0) return;
-  const int64_t before = units_before(a, plan, b);
-  const Work work = work_of(units_before(a, plan, a.batch), heads, plan);
-  const int64_t first = before * heads + static_cast<int64_t>(h * plan.query_tiles + tile) * seq.units;
-  const int64_t w0 = first / work.per, w1 = (first + seq.units - 1) / work.per;
+  const int32_t b = blockIdx.x / a.heads, head = blockIdx.x - b * a.heads, h = head / group;
+  const int32_t tile = (head - h * group) / plan.query_rows, row = (head - h * group) - tile * plan.query_rows;
+  const Sequence seq = sequence_of(a, plan, indexes(a.lengths)[b]);
+  int32_t units = seq.units, before = 0;
+  if (a.batch > 1) before = units_before(a, plan, b, &units);
+  const int32_t per = units_per_group(units * heads, plan);
+  const int32_t first = before * heads + (h * plan.query_tiles + tile) * seq.units;
+  const int32_t w0 = first / per, w1 = (first + seq.units - 1) / per;
   if (w0 == w1) return;  // one workgroup had it all
   // (a part is in its workgroup's first place but where another head came before it there)
   const int64_t stride = static_cast<int64_t>(rows) * (DP + 2);
-  const int64_t first_slot = 2 * w0 + (first % work.per != 0 ? 1 : 0);
-  auto part_of = [&](int64_t w) { return a.workspace + (w == w0 ? first_slot : 2 * w) * stride; };
+  const int32_t first_slot = 2 * w0 + (first != w0 * per ? 1 : 0);
+  auto part_of = [&](int32_t w) { return a.workspace + (w == w0 ? first_slot : 2 * w) * stride; };
 
   float most = -INFINITY;
-  for (int64_t w = w0 + threadIdx.x; w <= w1; w += kThreads) most = fmaxf(most, part_of(w)[rows * DP + 2 * row]);
+  for (int32_t w = w0 + threadIdx.x; w <= w1; w += kThreads) most = fmaxf(most, part_of(w)[rows * DP + 2 * row]);
   most = wave_max(most);
   if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = most;
   __syncthreads();
@@ -489,7 +528,7 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int64_t w = w0 + set; w <= w1; w += kSets) {
+  for (int32_t w = w0 + set; w <= w1; w += kSets) {
     const float* part = part_of(w);
     const float f = part_factor(part[rows * DP + 2 * row], most);
     const float4 y = *reinterpret_cast<const float4*>(part + row * DP + 4 * lane);
@@ -514,23 +553,20 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// Which sizes the device's lengths may have is known from the table's width alone.
+int64_t most_tiles(const PagedAttentionArgs& a) {  // of a sequence, from the table's width alone: lengths are on the device
+  return ((static_cast<int64_t>(a.pages.width) << a.cache.page_log2) + kTile - 1) / kTile;
+}
+int query_tiles(const PagedAttentionArgs& a) { return (a.heads / a.cache.kv_heads + 15) / 16; }
+
 Plan plan_of(const PagedAttentionArgs& a, int cus) {
   Plan p;
   const int group = a.heads / a.cache.kv_heads;
-  p.query_tiles = (group + 15) / 16;
+  p.query_tiles = query_tiles(a);
   p.query_rows = (group + p.query_tiles - 1) / p.query_tiles;
-  const int64_t capacity = static_cast<int64_t>(a.pages.width) << a.cache.page_log2;
-  const int64_t tiles = std::max<int64_t>(1, (capacity + kTile - 1) / kTile);
   const int64_t heads = a.batch * a.cache.kv_heads * p.query_tiles;
-  p.chunk = static_cast<int32_t>(tiles <= kDirectTiles ? tiles : 1);
-  const int64_t units = heads * ((tiles + p.chunk - 1) / p.chunk);
-  p.groups = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(units, static_cast<int64_t>(kGroupsPerCu) * cus)));
+  p.whole = most_tiles(a) <= kDirectTiles;
+  p.groups = static_cast<int32_t>(p.whole ? heads : std::min<int64_t>(heads * most_tiles(a), static_cast<int64_t>(kGroupsPerCu) * cus));
   return p;
-}
-// Whether a head may be more than one workgroup's.
-bool splits(const PagedAttentionArgs& a, const Plan& p) {
-  return (static_cast<int64_t>(a.pages.width) << a.cache.page_log2) > static_cast<int64_t>(p.chunk) * kTile;
 }
 
 template <int DP, bool FP8, bool DUP>
@@ -546,17 +582,21 @@ hipError_t launch(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream
   else if (dup) launch_main<DP, false, true>(a, p, stream);
   else launch_main<DP, false, false>(a, p, stream);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !splits(a, p)) return e;
+  if (e != hipSuccess || p.whole) return e;
   join_parts_kernel<DP><<<static_cast<unsigned>(a.batch * a.heads), kThreads, 0, stream>>>(a, p);
   return hipGetLastError();
 }
 
 }  // namespace
 
+bool paged_attention_fits(const PagedAttentionArgs& a) {
+  return std::max<int64_t>(1, most_tiles(a)) * query_tiles(a) * a.cache.kv_heads < (int64_t{1} << 31) / std::max<int64_t>(1, a.batch);
+}
+
 size_t paged_attention_workspace(const PagedAttentionArgs& a, int cus) {
   if (a.batch == 0) return 0;
   const Plan p = plan_of(a, cus);
-  if (!splits(a, p)) return 0;
+  if (p.whole) return 0;
   return 2 * static_cast<size_t>(p.groups) * (p.query_rows <= 8 ? 8 : 16) * (padded_dim(a.cache.dim) + 2) * sizeof(float);
 }
 
