@@ -47,7 +47,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kWavePositions = 32, kTile = kWaves * kWavePositions;
-constexpr int kGroupsPerCu = 4;   // workgroups of the main launch per compute unit
+constexpr int kGroupsPerCu = 2;   // workgroups of the main launch per compute unit
 constexpr int kDirectTiles = 4;   // up to this many tiles a head is one workgroup's
 
 __device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
@@ -59,8 +59,10 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 constexpr uint32_t kOutside = 0x80000000u;  // an offset behind every buffer's bytes
+constexpr int kOnce = 2;                    // a load whose lines are not kept (nontemporal)
+template <int HINT>
 __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
-  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, 0));
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, HINT));
 }
 __device__ __forceinline__ float4 as_float4(uint4 w) {
   return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
@@ -77,7 +79,7 @@ typedef const __attribute__((address_space(4))) int32_t* Indexes;
 __device__ __forceinline__ Indexes indexes(const int32_t* p) { return reinterpret_cast<Indexes>(reinterpret_cast<uintptr_t>(p)); }
 
 struct Plan {
-  int32_t groups;       // workgroups of the launch
+  int32_t columns;      // shares that the tiles of all sequences are dealt into, each of a workgroup per head
   int32_t query_rows;   // query heads of a unit (at most)
   int32_t query_tiles;  // units side by side for the query heads of a key head
   bool whole;           // a sequence's head is one unit, whatever its length
@@ -108,8 +110,7 @@ __device__ __forceinline__ int32_t wave_scan(int32_t v) {
   return v;
 }
 
-// Units of one head of sequences before `end`, and of all (the sums of every head's
-// are below 2^31).
+// Units of sequences before `end`, and of all (below 2^31).
 __device__ __forceinline__ int32_t units_before(const PagedAttentionArgs& a, const Plan& plan, int32_t end, int32_t* all) {
   int32_t before = 0, total = 0;
   for (int32_t block = 0; block < a.batch; block += 64) {
@@ -121,8 +122,8 @@ __device__ __forceinline__ int32_t units_before(const PagedAttentionArgs& a, con
   *all = total;
   return before;
 }
-__device__ __forceinline__ int32_t units_per_group(int32_t units, const Plan& plan) {
-  return (units + plan.groups - 1) / plan.groups;
+__device__ __forceinline__ int32_t units_per_column(int32_t units, const Plan& plan) {
+  return (units + plan.columns - 1) / plan.columns;
 }
 
 // A workgroup's part of a row: weights relative to 2^most, their sum, the sum of
@@ -154,55 +155,51 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attentio
   const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles;
   const int row_bytes = FP8 ? dim : 2 * dim;
 
-  // This workgroup's units [begin, end), the sequence of the first and that sequence's first unit.
-  int32_t b, base = 0, begin, end;
+  // This workgroup's head, units [begin, end), the sequence of the first and that sequence's first unit.
+  const int32_t column = blockIdx.x / heads, index = blockIdx.x - column * heads;
+  const int h = index / plan.query_tiles, query0 = (index - h * plan.query_tiles) * plan.query_rows;
+  const int rows = min(plan.query_rows, group - query0);
+  int32_t b = 0, base = 0, begin, end;
   Sequence seq;
   if (plan.whole) {
-    begin = blockIdx.x, end = begin + 1;
-    b = begin / heads;
-    base = b * heads;
+    b = base = begin = column;
+    end = begin + 1;
     seq = sequence_of(a, plan, indexes(a.lengths)[b]);
   } else if (a.batch == 1) {
-    b = 0;
     seq = sequence_of(a, plan, indexes(a.lengths)[0]);
-    const int32_t per = units_per_group(seq.units * heads, plan);
-    begin = blockIdx.x * per;
-    end = min(begin + per, seq.units * heads);
+    const int32_t per = units_per_column(seq.units, plan);
+    begin = column * per;
+    end = min(begin + per, seq.units);
     if (begin >= end) return;
   } else {
     int32_t units, given = 0;
     units_before(a, plan, 0, &units);
-    units *= heads;
-    const int32_t per = units_per_group(units, plan);
-    begin = blockIdx.x * per;
+    const int32_t per = units_per_column(units, plan);
+    begin = column * per;
     end = min(begin + per, units);
     if (begin >= end) return;
-    for (b = 0;; b += 64) {  // (ends: begin is below the sum)
+    for (;; b += 64) {  // (ends: begin is below the sum)
       const int32_t mine = b + lane < a.batch ? a.lengths[b + lane] : 0;
       const int32_t upto = wave_scan(b + lane < a.batch ? sequence_of(a, plan, mine).units : 0);
-      const int before = __popcll(__ballot(base + upto * heads <= begin));  // sequences that end at or before `begin`
+      const int before = __popcll(__ballot(base + upto <= begin));  // sequences that end at or before `begin`
       if (before < 64) {
-        if (before > 0) base += __builtin_amdgcn_readlane(upto, before - 1) * heads;
+        if (before > 0) base += __builtin_amdgcn_readlane(upto, before - 1);
         given = __builtin_amdgcn_readlane(mine, before);
         b += before;
         break;
       }
-      base += __builtin_amdgcn_readlane(upto, 63) * heads;
+      base += __builtin_amdgcn_readlane(upto, 63);
     }
     seq = sequence_of(a, plan, given);
   }
   int32_t at = begin;
 
   while (at < end) {
-    while (at - base >= seq.units * heads) {  // (ends: a unit lies in some sequence)
-      base += seq.units * heads;
+    while (at - base >= seq.units) {  // (ends: a unit lies in some sequence)
+      base += seq.units;
       seq = sequence_of(a, plan, indexes(a.lengths)[++b]);
     }
-    // This workgroup's units [u0, u1) of head `index`.
-    const int32_t index = (at - base) / seq.units, u0 = (at - base) - index * seq.units;
-    const int32_t u1 = min(seq.units, u0 + (end - at));
-    const int h = index / plan.query_tiles, query0 = (index - h * plan.query_tiles) * plan.query_rows;
-    const int rows = min(plan.query_rows, group - query0);
+    const int32_t u0 = at - base, u1 = min(seq.units, end - base);  // of this sequence
     const int64_t query_row = static_cast<int64_t>(b) * a.heads + h * group + query0;
     const int32_t tile_end = seq.tile0 + (plan.whole ? seq.tiles : min(seq.tiles, u1));
     int32_t tile = seq.tile0 + u0;
@@ -243,8 +240,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attentio
         const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.key) + place * row_bytes, rows * row_bytes);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
-          k[s][i] = load16(buf, (!PAD || i * kStep + g * (kStep / 4) < dim ? key_at : kOutside) + 64 * i);
-        if constexpr (FP8) ks[s] = as_float4(load16(stage_buffer(kv.key_scales + place, rows > 0 ? 64 : 0), 16u * g));
+          k[s][i] = load16<FP8 ? 0 : kOnce>(buf, (!PAD || i * kStep + g * (kStep / 4) < dim ? key_at : kOutside) + 64 * i);
+        if constexpr (FP8) ks[s] = as_float4(load16<0>(stage_buffer(kv.key_scales + place, rows > 0 ? 64 : 0), 16u * g));
       }
     };
     auto load_values = [&](int32_t t, const int32_t (&page)[2]) {
@@ -257,19 +254,19 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attentio
         for (int r = 0; r < 4; ++r) {
           const uint32_t at = value_at + r * row_bytes;
           if constexpr (kVWords == 1) {
-            v[s][r][0] = __builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, 0);
+            v[s][r][0] = __builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, kOnce);
           } else if constexpr (kVWords == 2) {
-            const auto w = __builtin_amdgcn_raw_buffer_load_b64(buf, at, 0, 0);
+            const auto w = __builtin_amdgcn_raw_buffer_load_b64(buf, at, 0, kOnce);
             v[s][r][0] = w[0], v[s][r][1] = w[1];
           } else {
 #pragma unroll
             for (int i = 0; i < kVWords / 4; ++i) {
-              const uint4 w = load16(buf, at + 16 * i);
+              const uint4 w = load16<kOnce>(buf, at + 16 * i);
               v[s][r][4 * i] = w.x, v[s][r][4 * i + 1] = w.y, v[s][r][4 * i + 2] = w.z, v[s][r][4 * i + 3] = w.w;
             }
           }
         }
-        if constexpr (FP8) vs[s] = as_float4(load16(stage_buffer(kv.value_scales + place, rows > 0 ? 64 : 0), 16u * g));
+        if constexpr (FP8) vs[s] = as_float4(load16<0>(stage_buffer(kv.value_scales + place, rows > 0 ? 64 : 0), 16u * g));
       }
     };
     f32x4_t o[kVec];
@@ -509,14 +506,13 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   const Sequence seq = sequence_of(a, plan, indexes(a.lengths)[b]);
   int32_t units = seq.units, before = 0;
   if (a.batch > 1) before = units_before(a, plan, b, &units);
-  const int32_t per = units_per_group(units * heads, plan);
-  const int32_t first = before * heads + (h * plan.query_tiles + tile) * seq.units;
-  const int32_t w0 = first / per, w1 = (first + seq.units - 1) / per;
+  const int32_t per = units_per_column(units, plan);
+  const int32_t w0 = before / per, w1 = (before + seq.units - 1) / per;
   if (w0 == w1) return;  // one workgroup had it all
   // (a part is in its workgroup's first place but where another head came before it there)
   const int64_t stride = static_cast<int64_t>(rows) * (DP + 2);
-  const int32_t first_slot = 2 * w0 + (first != w0 * per ? 1 : 0);
-  auto part_of = [&](int32_t w) { return a.workspace + (w == w0 ? first_slot : 2 * w) * stride; };
+  const int32_t first_place = before != w0 * per ? 1 : 0, index = h * plan.query_tiles + tile;
+  auto part_of = [&](int32_t w) { return a.workspace + (2 * (w * heads + index) + (w == w0 ? first_place : 0)) * stride; };
 
   float most = -INFINITY;
   for (int32_t w = w0 + threadIdx.x; w <= w1; w += kThreads) most = fmaxf(most, part_of(w)[rows * DP + 2 * row]);
@@ -563,16 +559,17 @@ Plan plan_of(const PagedAttentionArgs& a, int cus) {
   const int group = a.heads / a.cache.kv_heads;
   p.query_tiles = query_tiles(a);
   p.query_rows = (group + p.query_tiles - 1) / p.query_tiles;
-  const int64_t heads = a.batch * a.cache.kv_heads * p.query_tiles;
   p.whole = most_tiles(a) <= kDirectTiles;
-  p.groups = static_cast<int32_t>(p.whole ? heads : std::min<int64_t>(heads * most_tiles(a), static_cast<int64_t>(kGroupsPerCu) * cus));
+  const int64_t wanted = std::max<int64_t>(1, static_cast<int64_t>(kGroupsPerCu) * cus / (a.cache.kv_heads * p.query_tiles));
+  p.columns = static_cast<int32_t>(p.whole ? a.batch : std::min(a.batch * most_tiles(a), wanted));
   return p;
 }
 
 template <int DP, bool FP8, bool DUP>
 void launch_main(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream) {
-  if (a.cache.dim == DP) paged_attention_kernel<DP, FP8, DUP, false><<<p.groups, kThreads, 0, stream>>>(a, p);
-  else paged_attention_kernel<DP, FP8, DUP, true><<<p.groups, kThreads, 0, stream>>>(a, p);
+  const unsigned groups = static_cast<unsigned>(p.columns) * a.cache.kv_heads * p.query_tiles;
+  if (a.cache.dim == DP) paged_attention_kernel<DP, FP8, DUP, false><<<groups, kThreads, 0, stream>>>(a, p);
+  else paged_attention_kernel<DP, FP8, DUP, true><<<groups, kThreads, 0, stream>>>(a, p);
 }
 template <int DP>
 hipError_t launch(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream) {
@@ -597,7 +594,7 @@ size_t paged_attention_workspace(const PagedAttentionArgs& a, int cus) {
   if (a.batch == 0) return 0;
   const Plan p = plan_of(a, cus);
   if (p.whole) return 0;
-  return 2 * static_cast<size_t>(p.groups) * (p.query_rows <= 8 ? 8 : 16) * (padded_dim(a.cache.dim) + 2) * sizeof(float);
+  return 2 * static_cast<size_t>(p.columns) * a.cache.kv_heads * p.query_tiles * (p.query_rows <= 8 ? 8 : 16) * (padded_dim(a.cache.dim) + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, int cus, hipStream_t stream) {
