@@ -134,17 +134,16 @@ __device__ __forceinline__ float part_factor(float most, float all) {
 }
 __device__ __forceinline__ float weighted(float f, float v) { return f == 0.0f ? 0.0f : f * v; }
 
-#ifndef MINW
-#define MINW 3
-#endif
 template <int DP, bool FP8, bool DUP, bool PAD>
-__global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
+__global__ __launch_bounds__(kThreads, DP == 256 ? 2 : 3) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
   constexpr int kRows = DUP ? 8 : 16;      // query heads of a unit
   constexpr int kVec = DP / 16;            // dimensions of a value row that a lane holds
   constexpr int kStep = FP8 ? 64 : 32;     // dimensions of one load of 16 keys
   constexpr int kLoads = DP / kStep;
   constexpr int kVWords = FP8 ? kVec / 4 : kVec / 2;
   constexpr int kRowStride = DP + 4;       // (rows of the join four banks apart)
+  constexpr bool kSharedQuery = DP == 256;  // (there are no registers for them beside keys and values on their way)
+  __shared__ uint4 shared_query[kSharedQuery ? DP / 32 : 1][64];
   __shared__ float part_o[kWaves][kRows][kRowStride];
   __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
 
@@ -282,13 +281,18 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attentio
       entry[s] = entry_of(tile + 1, s);
     }
     // The queries of column n (of the upper half as of the lower one), in the keys' order of dimensions.
-    uint4 q[DP / 32];
     const int row = DUP ? n & 7 : n;
-#pragma unroll
-    for (int j = 0; j < DP / 32; ++j) {
+    auto load_query = [&](int j) {
       const int c = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j % 2) : 32 * j + 8 * g;
-      q[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < rows && (!PAD || c < dim)) q[j] = ldg16(a.query + (query_row + row) * dim + c);
+      return row < rows && (!PAD || c < dim) ? ldg16(a.query + (query_row + row) * dim + c) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    uint4 q[kSharedQuery ? 1 : DP / 32];
+    if constexpr (kSharedQuery) {
+      for (int j = wave; j < DP / 32; j += kWaves) shared_query[j][lane] = load_query(j);
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) q[j] = load_query(j);
     }
     load_keys(tile, page);
     __builtin_amdgcn_sched_barrier(0);  // (in this order, as in the loop)
@@ -299,6 +303,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attentio
     const uint32_t rest = DUP && n >= 8 ? 0xFFFFFFFFu : 0u;
 
     for (; tile < tile_end; ++tile) {
+      auto query = [&](int j) {
+        if constexpr (kSharedQuery) return shared_query[j][lane];
+        else return q[j];
+      };
       f32x4_t s[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -311,9 +319,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : MINW) void paged_attentio
             if constexpr (FP8) {
               const uint32_t lo = half == 0 ? k[t][i].x : k[t][i].z, hi = half == 0 ? k[t][i].y : k[t][i].w;
               s[t] = mfma(make_uint4(fp8_pair<false>(lo), fp8_pair<true>(lo), fp8_pair<false>(hi), fp8_pair<true>(hi)),
-                          q[2 * i + half], s[t]);
+                          query(2 * i + half), s[t]);
             } else {
-              s[t] = mfma(k[t][i], q[i], s[t]);
+              s[t] = mfma(k[t][i], query(i), s[t]);
             }
           }
 #pragma unroll
