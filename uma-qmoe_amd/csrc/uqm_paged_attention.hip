@@ -48,6 +48,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kWavePositions = 32, kTile = kWaves * kWavePositions;
 constexpr int kGroupsPerCu = 2;   // workgroups of the main launch per compute unit
+constexpr int kFewParts = 16;     // up to this many parts a sequence on average a wave joins those of a head
 constexpr int kDirectTiles = 4;   // up to this many tiles a head is one workgroup's
 
 __device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
@@ -500,16 +501,45 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : 3) void paged_attention_k
   }
 }
 
-// Joins the parts of one query head (a workgroup each): 4 dimensions a thread,
-// the parts dealt out over kThreads / (DP / 4) groups of threads.
-template <int DP>
+// Sums of parts: relative to 2^most, the weights' and those of four dimensions.
+struct Joined {
+  float most, sum;
+  float4 acc;
+};
+__device__ __forceinline__ void join(Joined& x, float most, float sum, const float4& acc) {
+  const float all = fmaxf(x.most, most), f = part_factor(x.most, all), h = part_factor(most, all);
+  x.most = all;
+  x.sum = weighted(f, x.sum) + weighted(h, sum);
+  x.acc.x = weighted(f, x.acc.x) + weighted(h, acc.x);
+  x.acc.y = weighted(f, x.acc.y) + weighted(h, acc.y);
+  x.acc.z = weighted(f, x.acc.z) + weighted(h, acc.z);
+  x.acc.w = weighted(f, x.acc.w) + weighted(h, acc.w);
+}
+template <int O>
+__device__ __forceinline__ float lane_xor(float v) {  // (xor_partner<8> would be lane ^ 15)
+  if constexpr (O == 8) return other_half(v);
+  else return xor_partner<O>(v);
+}
+template <int O>
+__device__ __forceinline__ void join_lanes(Joined& x) {
+  static_assert(O >= 8, "xor_partner<4> is lane ^ 7");
+  const float most = lane_xor<O>(x.most), sum = lane_xor<O>(x.sum);
+  join(x, most, sum, make_float4(lane_xor<O>(x.acc.x), lane_xor<O>(x.acc.y), lane_xor<O>(x.acc.z), lane_xor<O>(x.acc.w)));
+}
+
+// Joins the parts of query heads. Of few parts (FEW) a wave has a head, four
+// dimensions a lane; of many a workgroup has 32 dimensions of a head, and 32 sets of
+// 8 lanes share the parts (8 heads in 512 parts of 128: 4 us, with a workgroup a head
+// 12; 4096 heads in 2 to 3 parts: 4 us with a wave a head, with a workgroup 10).
+template <int DP, bool FEW>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, Plan plan) {
-  constexpr int kLanes = DP / 4, kSets = kThreads / kLanes;
-  __shared__ float4 sums[kSets][kLanes];
-  __shared__ float parts[kWaves], totals[kSets];
+  constexpr int kSpan = FEW ? DP : 32, kLanes = kSpan / 4, kSets = (FEW ? 64 : kThreads) / kLanes;
+  constexpr int kSpans = DP / kSpan, kAtOnce = 4;
   const KvPages& kv = a.cache;
   const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles, rows = plan.query_rows <= 8 ? 8 : 16;
-  const int32_t b = blockIdx.x / a.heads, head = blockIdx.x - b * a.heads, h = head / group;
+  const int32_t item = FEW ? blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x / kSpans;
+  if (FEW && item >= a.batch * a.heads) return;
+  const int32_t b = item / a.heads, head = item - b * a.heads, h = head / group;
   const int32_t tile = (head - h * group) / plan.query_rows, row = (head - h * group) - tile * plan.query_rows;
   const Sequence seq = sequence_of(a, plan, indexes(a.lengths)[b]);
   int32_t units = seq.units, before = 0;
@@ -520,39 +550,51 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   // (a part is in its workgroup's first place but where another head came before it there)
   const int64_t stride = static_cast<int64_t>(rows) * (DP + 2);
   const int32_t first_place = before != w0 * per ? 1 : 0, index = h * plan.query_tiles + tile;
-  auto part_of = [&](int32_t w) { return a.workspace + (2 * (w * heads + index) + (w == w0 ? first_place : 0)) * stride; };
-
-  float most = -INFINITY;
-  for (int32_t w = w0 + threadIdx.x; w <= w1; w += kThreads) most = fmaxf(most, part_of(w)[rows * DP + 2 * row]);
-  most = wave_max(most);
-  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = most;
-  __syncthreads();
-  most = fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3]));
-  const int lane = threadIdx.x % kLanes, set = threadIdx.x / kLanes;
-  float sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int32_t w = w0 + set; w <= w1; w += kSets) {
-    const float* part = part_of(w);
-    const float f = part_factor(part[rows * DP + 2 * row], most);
-    const float4 y = *reinterpret_cast<const float4*>(part + row * DP + 4 * lane);
-    sum += weighted(f, part[rows * DP + 2 * row + 1]);
-    acc.x += weighted(f, y.x), acc.y += weighted(f, y.y), acc.z += weighted(f, y.z), acc.w += weighted(f, y.w);
+  const int lane = threadIdx.x % kLanes, set = (FEW ? threadIdx.x & 63 : threadIdx.x) / kLanes;
+  const int c = (FEW ? 0 : (blockIdx.x % kSpans) * kSpan) + 4 * lane;
+  Joined x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int32_t w = w0 + set; w <= w1; w += kAtOnce * kSets) {
+    float most[kAtOnce], sum[kAtOnce];
+    float4 y[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int32_t at = min(w + i * kSets, w1);
+      const float* part = a.workspace + (2 * (at * heads + index) + (at == w0 ? first_place : 0)) * stride;
+      const float2 ml = *reinterpret_cast<const float2*>(part + rows * DP + 2 * row);
+      y[i] = *reinterpret_cast<const float4*>(part + row * DP + c);
+      const bool there = w + i * kSets <= w1;
+      most[i] = there ? ml.x : -INFINITY;
+      sum[i] = there ? ml.y : 0.f;
+    }
+    float all = x.most;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) all = fmaxf(all, most[i]);
+    const float f = part_factor(x.most, all);
+    x.most = all;
+    x.sum = weighted(f, x.sum);
+    x.acc = make_float4(weighted(f, x.acc.x), weighted(f, x.acc.y), weighted(f, x.acc.z), weighted(f, x.acc.w));
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float h = w + i * kSets <= w1 ? part_factor(most[i], all) : 0.f;
+      x.sum += weighted(h, sum[i]);
+      x.acc.x += weighted(h, y[i].x), x.acc.y += weighted(h, y[i].y), x.acc.z += weighted(h, y[i].z), x.acc.w += weighted(h, y[i].w);
+    }
   }
-  sums[set][lane] = acc;
-  if (lane == 0) totals[set] = sum;
-  __syncthreads();
-  if (set != 0 || 4 * lane >= kv.dim) return;
-  sum = 0.f;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < kSets; ++i) {
-    const float4 y = sums[i][lane];
-    sum += totals[i];
-    acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+  if constexpr (kLanes <= 8) join_lanes<8>(x);
+  if constexpr (kLanes <= 16) join_lanes<16>(x);
+  if constexpr (kLanes <= 32) join_lanes<32>(x);
+  if constexpr (!FEW) {
+    __shared__ Joined joined[kWaves][kLanes];
+    if ((threadIdx.x & 63) < kLanes) joined[threadIdx.x >> 6][lane] = x;
+    __syncthreads();
+    if (set != 0) return;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) join(x, joined[i][lane].most, joined[i][lane].sum, joined[i][lane].acc);
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  *reinterpret_cast<uint2*>(a.out + blockIdx.x * static_cast<int64_t>(kv.dim) + 4 * lane) =
-      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (set != 0 || c >= kv.dim) return;
+  const float inv = x.sum == 0.f ? 0.f : 1.0f / x.sum;
+  *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(item) * kv.dim + c) =
+      make_uint2(pack_bf16x2(x.acc.x * inv, x.acc.y * inv), pack_bf16x2(x.acc.z * inv, x.acc.w * inv));
 }
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -588,7 +630,9 @@ hipError_t launch(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream
   else launch_main<DP, false, false>(a, p, stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.whole) return e;
-  join_parts_kernel<DP><<<static_cast<unsigned>(a.batch * a.heads), kThreads, 0, stream>>>(a, p);
+  const unsigned items = static_cast<unsigned>(a.batch * a.heads);
+  if (p.columns <= kFewParts * a.batch) join_parts_kernel<DP, true><<<(items + kWaves - 1) / kWaves, kThreads, 0, stream>>>(a, p);
+  else join_parts_kernel<DP, false><<<items * (DP / 32), kThreads, 0, stream>>>(a, p);
   return hipGetLastError();
 }
 
