@@ -352,15 +352,15 @@ int uqm_fp8_linear_plan(int64_t rows, int64_t out_features, int64_t in_features,
  * FP32 scale for the head_dim values of a token's head (value = code * scale; scales
  * and codes as above with those values for a block). Position p of sequence b is
  * place p % page_size of page page_table[b * table_stride + p / page_size],
- * p < max_pages * page_size. An entry outside [0, pages) is no page: nothing is
+ * p < max_pages * page_size (at most 2^30). An entry outside [0, pages) is no page: nothing is
  * written there, and what it would hold reads as 0 and is not attended to.
  * Entries behind a sequence's end are not looked at. The pages of one sequence
  * may be those of another one (a common beginning), but of the entries that an
  * append writes none may be written twice in the call: it would hold either's
  * values, or keys of one beside scales of the other. starts, counts and lengths
  * are on the device, so that a captured graph follows them. Results are the same
- * for the same inputs, and a sequence's depend on no other sequence. No counterpart
- * in the reference, whose hosts use Transformers' caches. */
+ * for the same inputs. No counterpart in the reference, whose hosts use
+ * Transformers' caches. */
 typedef struct uqm_kv_cache {
   void* key;            /* [pages, kv_heads, page_size, head_dim], 16-byte aligned      */
   void* value;
@@ -398,7 +398,11 @@ int uqm_kv_read(const uqm_kv_cache* cache, int64_t batch, const int32_t* page_ta
  * Zeros where no position is seen. query bf16 [batch, heads, head_dim], heads a
  * multiple of kv_heads, both 16-byte aligned; batch * heads below 2^24.
  * What places hold that are not seen has no influence, NaN and infinities neither;
- * a seen NaN gives NaN, a seen infinity NaN or an infinity.
+ * a seen NaN gives NaN, a seen infinity NaN or an infinity. Sums are in FP32; of
+ * which parts they are joined goes by the table's width and all lengths of the
+ * call, so that a result may differ in its last bit between calls that differ in
+ * these. batch * kv_heads * ceil(heads / kv_heads / 16) * ceil(max_pages * page_size
+ * / 128) below 2^31.
  * workspace: uqm_paged_attention_workspace_bytes, 16-byte aligned, of any content,
  * not shared by calls that overlap in time (also those of captured graphs); what
  * it held is not kept. */

@@ -388,6 +388,18 @@ def test_attention_of_special_scores(hip_ext, fp8):
         assert not special(hip_ext, "value", where, inf, fp8)[0].isfinite().any()
 
 
+def test_attention_without_a_page(hip_ext):
+    """Tables of no column, and no sequence."""
+    print("[case] attention without pages", flush=True)
+    cache = hip_ext.new_kv_cache(2, 2, 16, 64, device=DEV)
+    q = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=DEV)
+    none = torch.zeros(3, 0, dtype=torch.int32, device=DEV)
+    assert hip_ext.paged_attention(q, cache, none, torch.full((3,), 5, dtype=torch.int32, device=DEV)).eq(0).all()
+    hip_ext.kv_append(cache, q[:, :2, None], q[:, :2, None], none, torch.zeros(3, dtype=torch.int32, device=DEV))
+    assert cache.key.eq(0).all()
+    assert hip_ext.paged_attention(q[:0], cache, none[:0], torch.zeros(0, dtype=torch.int32, device=DEV)).shape == (0, 4, 64)
+
+
 def test_attention_takes_views(hip_ext):
     """A query, a table and lengths that are parts of larger tensors, a table by columns or for all sequences."""
     print("[case] attention views", flush=True)
@@ -409,8 +421,7 @@ def test_attention_takes_views(hip_ext):
     ref.check_attention(same, q, cache, table[2:].expand(3, -1), torch.tensor([77] * 3), 32 ** -0.5)
 
 
-def test_attention_is_the_same_each_time_and_in_any_company(hip_ext):
-    """Bits do not change from call to call, nor short sequences' with their neighbours."""
+def test_attention_is_the_same_each_time(hip_ext):
     print("[case] attention repeats", flush=True)
     got, q, cache, table = attend_case(hip_ext, gen(17), [30000, 5, 1200], 8, 2, 16, 128, True)
     n32 = torch.tensor([30000, 5, 1200], dtype=torch.int32, device=DEV)

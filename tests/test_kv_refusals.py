@@ -61,7 +61,7 @@ def test_caches(lib, name):
 @pytest.mark.parametrize("name", CALLS)
 @pytest.mark.parametrize("changed,words", [
     (dict(batch=-1), "batch"), (dict(batch=1 << 31), "batch"), (dict(width=-1), "max_pages"),
-    (dict(width=1 << 27, stride=1 << 27), "max_pages"), (dict(stride=3), "table_stride"), (dict(stride=1 << 31), "table_stride"),
+    (dict(width=(1 << 26) + 1, stride=1 << 27), "max_pages"), (dict(stride=3), "table_stride"), (dict(stride=1 << 31), "table_stride"),
     (dict(stride=1 << 30, batch=1 << 20), "2^48"), (dict(table=None), "required"), (dict(table=E + 2), "aligned"),
 ])
 def test_tables(lib, name, changed, words):
@@ -101,7 +101,8 @@ def test_read(lib, changed, words):
 
 @pytest.mark.parametrize("changed,words", [
     (dict(heads=0), "multiple"), (dict(heads=3), "multiple"), (dict(heads=-2), "multiple"), (dict(heads=1 << 24), "2^24"),
-    (dict(batch=1 << 20, heads=16), "2^24"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
+    (dict(batch=1 << 20, heads=16), "2^24"),
+    (dict(batch=1 << 8, heads=2, width=1 << 26, stride=1 << 26), "room"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
     (dict(window=-1), "window"), (dict(query=None), "required"), (dict(lengths=None), "required"), (dict(out=None), "required"),
     (dict(query=C + 8), "aligned"), (dict(out=D + 2), "aligned"), (dict(lengths=F + 3), "aligned"),
     (dict(out=C + 16), "overlaps"), (dict(out=A), "overlaps"), (dict(out=E), "overlaps"), (dict(out=F), "overlaps"),

@@ -1481,6 +1481,7 @@ int uqm_fp8_linear_plan(int64_t rows, int64_t out_features, int64_t in_features,
 namespace {
 
 constexpr int64_t kMaxElements = int64_t{1} << 48;  // of a cache: far beyond the memory, its bytes far below 2^63
+constexpr int64_t kMaxPositions = int64_t{1} << 30;  // of a sequence, so that a few tiles more are below 2^31, too
 constexpr int64_t kMaxQueryHeads = int64_t{1} << 24;
 
 // Sizes of a cache, before its pointers are looked at.
@@ -1497,8 +1498,8 @@ int check_kv_sizes(const char* what, int64_t pages, int64_t kv_heads, int64_t pa
 
 int check_page_table(const char* what, int64_t batch, int64_t page_size, int64_t table_stride, int64_t max_pages) {
   if (batch < 0 || batch > kMaxExtent) return fail(UQM_ERR_ARGUMENT, "%s: batch must be in [0, 2^31)", what);
-  if (max_pages < 0 || max_pages > kMaxExtent / page_size)
-    return fail(UQM_ERR_ARGUMENT, "%s: max_pages * page_size must be in [0, 2^31)", what);
+  if (max_pages < 0 || max_pages > kMaxPositions / page_size)
+    return fail(UQM_ERR_ARGUMENT, "%s: max_pages * page_size must be in [0, 2^30]", what);
   if (table_stride < max_pages || table_stride > kMaxExtent || table_stride * batch > kMaxElements)
     return fail(UQM_ERR_ARGUMENT, "%s: table_stride must be at least max_pages (a table of fewer than 2^48 entries)", what);
   return UQM_OK;

@@ -68,6 +68,12 @@ __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t buf, uint32_t at)
 __device__ __forceinline__ float4 as_float4(uint4 w) {
   return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
 }
+// A barrier that waits for what the wave has in shared memory, not for its loads.
+__device__ __forceinline__ void local_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 // The value of lane ^ 8.
 __device__ __forceinline__ float other_half(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));  // row_ror:8
@@ -86,21 +92,22 @@ struct Plan {
   bool whole;           // a sequence's head is one unit, whatever its length
 };
 
+// A sequence's tiles from tile0 on are its units, one a head; one without a position
+// has one, too, which writes the zeros.
 struct Sequence {
-  int32_t length, first;         // positions seen: first .. length - 1
-  int32_t tile0, tiles, units;   // tiles from tile0 on; units of one head (one at least, which writes the zeros)
+  int32_t length, first;  // positions seen: first .. length - 1
+  int32_t tile0, units;
 };
-__device__ __forceinline__ Sequence sequence_of(const PagedAttentionArgs& a, const Plan& plan, int32_t given) {
+__device__ __forceinline__ Sequence sequence_of(const PagedAttentionArgs& a, int32_t given) {
   Sequence s;
   s.length = min(max(given, 0), a.pages.width << a.cache.page_log2);
   s.first = s.length > a.window ? s.length - a.window : 0;
-  s.tile0 = s.first / kTile;
-  s.tiles = (s.length + kTile - 1) / kTile - s.tile0;  // (0 at length 0: first is 0, too)
-  s.units = plan.whole ? 1 : max(1, s.tiles);
+  s.tile0 = static_cast<uint32_t>(s.first) / kTile;
+  s.units = max(1, static_cast<int32_t>(static_cast<uint32_t>(s.length + kTile - 1) / kTile) - s.tile0);
   return s;
 }
 
-// Sum over the lanes up to this one.
+// Sum over the lanes up to this one, and over all.
 __device__ __forceinline__ int32_t wave_scan(int32_t v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
@@ -110,22 +117,110 @@ __device__ __forceinline__ int32_t wave_scan(int32_t v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
   return v;
 }
+__device__ __forceinline__ int32_t wave_total(int32_t v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
-// Units of sequences before `end`, and of all (below 2^31).
-__device__ __forceinline__ int32_t units_before(const PagedAttentionArgs& a, const Plan& plan, int32_t end, int32_t* all) {
+// Units of sequences before `end`, and of all (below 2^31): four lengths a lane at once.
+__device__ __forceinline__ int32_t units_before(const PagedAttentionArgs& a, int32_t end, int32_t* all) {
+  constexpr int kAtOnce = 4;
   int32_t before = 0, total = 0;
-  for (int32_t block = 0; block < a.batch; block += 64) {
-    const int32_t b = block + static_cast<int32_t>(threadIdx.x & 63);
-    const int32_t units = b < a.batch ? sequence_of(a, plan, a.lengths[b]).units : 0;
-    total += __builtin_amdgcn_readlane(wave_scan(units), 63);
-    before += __builtin_amdgcn_readlane(wave_scan(b < end ? units : 0), 63);
+  for (int32_t block = static_cast<int32_t>(threadIdx.x & 63); block < a.batch; block += 64 * kAtOnce) {
+    int32_t given[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) given[i] = block + 64 * i < a.batch ? a.lengths[block + 64 * i] : 0;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int32_t units = block + 64 * i < a.batch ? sequence_of(a, given[i]).units : 0;
+      total += units;
+      before += block + 64 * i < end ? units : 0;
+    }
   }
-  *all = total;
-  return before;
+  *all = wave_total(total);
+  return wave_total(before);
 }
 __device__ __forceinline__ int32_t units_per_column(int32_t units, const Plan& plan) {
   return (units + plan.columns - 1) / plan.columns;
 }
+
+// One unit of a workgroup's share, as the loop needs it.
+struct Unit {
+  int32_t b, tile, length, first;
+  bool there, starts, ends;  // whether there is one; whether it is its sequence's first, or last
+};
+
+// A workgroup's share: units [at, end) of the sequences one after the other. Lengths
+// are held 64 at a time, a lane each, so that the next sequence's is at hand.
+template <bool WHOLE>
+struct Share {
+  int32_t at, end;
+  int32_t b, base;       // the sequence of unit `at` (or the one before) and its first unit
+  int32_t block, given;  // this lane's length is that of sequence block + lane
+  Sequence seq;
+
+  __device__ __forceinline__ void load_block(const PagedAttentionArgs& a) {
+    const int32_t mine = block + static_cast<int32_t>(threadIdx.x & 63);
+    given = mine < a.batch ? a.lengths[mine] : 0;
+    asm volatile("" : "+v"(given));  // (the wait for it is here, not with every use, where it would be one for keys and values)
+  }
+  __device__ __forceinline__ void enter(const PagedAttentionArgs& a) {
+    seq = sequence_of(a, __builtin_amdgcn_readlane(given, b - block));
+  }
+  __device__ __forceinline__ int32_t scan_block(const PagedAttentionArgs& a) const {
+    return wave_scan(block + static_cast<int32_t>(threadIdx.x & 63) < a.batch ? sequence_of(a, given).units : 0);
+  }
+  // Column `column`; false: there is nothing for it.
+  __device__ __forceinline__ bool find(const PagedAttentionArgs& a, const Plan& plan, int32_t column) {
+    base = 0;
+    if constexpr (WHOLE) {  // (a sequence to a column)
+      b = column;
+      seq = sequence_of(a, *indexes(a.lengths + b));
+      at = 0;
+      end = seq.units;
+      return true;
+    }
+    block = 0;
+    load_block(a);
+    int32_t upto = scan_block(a), units = __builtin_amdgcn_readlane(upto, 63);
+    if (a.batch > 64) units_before(a, 0, &units);
+    const int32_t per = units_per_column(units, plan);
+    at = column * per;
+    end = min(at + per, units);
+    if (at >= end) return false;
+    int before;  // sequences that end at or before `at`
+    // (`at` is below the sum; should a caller change lengths while the kernel runs, it still ends)
+    while ((before = __popcll(__ballot(base + upto <= at))) == 64) {
+      if (block + 64 >= a.batch) return false;
+      base += __builtin_amdgcn_readlane(upto, 63);
+      block += 64;
+      load_block(a);
+      upto = scan_block(a);
+    }
+    if (before > 0) base += __builtin_amdgcn_readlane(upto, before - 1);
+    b = block + before;
+    enter(a);
+    return b < a.batch;
+  }
+  __device__ __forceinline__ Unit next(const PagedAttentionArgs& a) {
+    Unit u;
+    u.there = at < end;
+    if (!WHOLE && u.there && at - base == seq.units) {  // (every sequence has a unit: `at` is in the next one)
+      base += seq.units;
+      if (++b == block + 64) {
+        block += 64;
+        load_block(a);
+      }
+      enter(a);
+      u.there = b < a.batch;
+    }
+    u.b = b;
+    u.tile = seq.tile0 + (at - base);
+    u.length = u.there ? seq.length : 0;
+    u.first = seq.first;
+    u.starts = WHOLE || at == base;
+    u.ends = at - base == seq.units - 1;
+    ++at;
+    return u;
+  }
+};
 
 // A workgroup's part of a row: weights relative to 2^most, their sum, the sum of
 // weighted values. most is -inf for a part that saw nothing (sum 0) and for one all
@@ -135,8 +230,9 @@ __device__ __forceinline__ float part_factor(float most, float all) {
 }
 __device__ __forceinline__ float weighted(float f, float v) { return f == 0.0f ? 0.0f : f * v; }
 
-template <int DP, bool FP8, bool DUP, bool PAD>
-__global__ __launch_bounds__(kThreads, DP == 256 ? 2 : 3) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
+// (registers for one, two or three workgroups a compute unit, so that none spills)
+template <int DP, bool FP8, bool DUP, bool PAD, bool WHOLE>
+__global__ __launch_bounds__(kThreads, DP == 256 && !FP8 ? 1 : DP == 256 || !FP8 || PAD ? 2 : 3) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
   constexpr int kRows = DUP ? 8 : 16;      // query heads of a unit
   constexpr int kVec = DP / 16;            // dimensions of a value row that a lane holds
   constexpr int kStep = FP8 ? 64 : 32;     // dimensions of one load of 16 keys
@@ -155,349 +251,327 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 2 : 3) void paged_attention_k
   const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles;
   const int row_bytes = FP8 ? dim : 2 * dim;
 
-  // This workgroup's head, units [begin, end), the sequence of the first and that sequence's first unit.
   const int32_t column = blockIdx.x / heads, index = blockIdx.x - column * heads;
   const int h = index / plan.query_tiles, query0 = (index - h * plan.query_tiles) * plan.query_rows;
   const int rows = min(plan.query_rows, group - query0);
-  int32_t b = 0, base = 0, begin, end;
-  Sequence seq;
-  if (plan.whole) {
-    b = base = begin = column;
-    end = begin + 1;
-    seq = sequence_of(a, plan, indexes(a.lengths)[b]);
-  } else if (a.batch == 1) {
-    seq = sequence_of(a, plan, indexes(a.lengths)[0]);
-    const int32_t per = units_per_column(seq.units, plan);
-    begin = column * per;
-    end = min(begin + per, seq.units);
-    if (begin >= end) return;
-  } else {
-    int32_t units, given = 0;
-    units_before(a, plan, 0, &units);
-    const int32_t per = units_per_column(units, plan);
-    begin = column * per;
-    end = min(begin + per, units);
-    if (begin >= end) return;
-    for (;; b += 64) {  // (ends: begin is below the sum)
-      const int32_t mine = b + lane < a.batch ? a.lengths[b + lane] : 0;
-      const int32_t upto = wave_scan(b + lane < a.batch ? sequence_of(a, plan, mine).units : 0);
-      const int before = __popcll(__ballot(base + upto <= begin));  // sequences that end at or before `begin`
-      if (before < 64) {
-        if (before > 0) base += __builtin_amdgcn_readlane(upto, before - 1);
-        given = __builtin_amdgcn_readlane(mine, before);
-        b += before;
-        break;
-      }
-      base += __builtin_amdgcn_readlane(upto, 63);
-    }
-    seq = sequence_of(a, plan, given);
-  }
-  int32_t at = begin;
+  Share<WHOLE> share;
+  if (!share.find(a, plan, column)) return;
 
-  while (at < end) {
-    while (at - base >= seq.units) {  // (ends: a unit lies in some sequence)
-      base += seq.units;
-      seq = sequence_of(a, plan, indexes(a.lengths)[++b]);
-    }
-    const int32_t u0 = at - base, u1 = min(seq.units, end - base);  // of this sequence
-    const int64_t query_row = static_cast<int64_t>(b) * a.heads + h * group + query0;
-    const int32_t tile_end = seq.tile0 + (plan.whole ? seq.tiles : min(seq.tiles, u1));
-    int32_t tile = seq.tile0 + u0;
-
-    // ---- loads of a tile's 32 positions of this wave, as two blocks of 16 ----
-    const Indexes table = indexes(a.pages.table + static_cast<int64_t>(b) * a.pages.stride);
-    // (entries of tiles behind the last are asked for, too, and count as none: the loop
-    // has no branch around its loads, behind which a wait could not tell them apart)
-    auto entry_of = [&](int32_t t, int s) -> int32_t {
-      return table[min(t * kTile + wave * kWavePositions + 16 * s, seq.length - 1) >> kv.page_log2];
-    };
-    auto page_of = [&](int32_t t, int s, int32_t entry) -> int32_t {
-      const bool there = t < tile_end && t * kTile + wave * kWavePositions + 16 * s < seq.length && entry < kv.pages;
-      return there ? entry : -1;  // (an entry below 0: none, too)
-    };
-    // (no page: page 0, whose values are masked)
-    const int64_t page_rows = static_cast<int64_t>(kv.kv_heads) << kv.page_log2;
-    auto place_of = [&](int32_t t, int s, int32_t page) -> int64_t {
-      const int32_t slot = (t * kTile + wave * kWavePositions + 16 * s) & ((1 << kv.page_log2) - 1);
-      return max(page, 0) * page_rows + ((h << kv.page_log2) | slot);
-    };
-    const uint32_t key_at = n * row_bytes + 16 * g;
-    const uint32_t value_at = !PAD || n * kVec < dim ? 4 * g * row_bytes + n * (4 * kVWords) : kOutside;
-    // Blocks are read through buffers that end behind their last position that is seen
-    // (at once where there is no page): what lies behind reads as zeros and costs
-    // nothing, as do dimensions behind the last.
-    auto seen_of = [&](int32_t t, int s, int32_t page) -> int32_t {
-      return page >= 0 ? min(16, seq.length - (t * kTile + wave * kWavePositions + 16 * s)) : 0;
-    };
-    uint4 k[2][kLoads];
-    float4 ks[2], vs[2];
-    uint32_t v[2][4][kVWords];
-    auto load_keys = [&](int32_t t, const int32_t (&page)[2]) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int64_t place = place_of(t, s, page[s]);
-        const int32_t rows = seen_of(t, s, page[s]);
-        const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.key) + place * row_bytes, rows * row_bytes);
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          k[s][i] = load16<FP8 ? 0 : kOnce>(buf, (!PAD || i * kStep + g * (kStep / 4) < dim ? key_at : kOutside) + 64 * i);
-        if constexpr (FP8) ks[s] = as_float4(load16<0>(stage_buffer(kv.key_scales + place, rows > 0 ? 64 : 0), 16u * g));
-      }
-    };
-    auto load_values = [&](int32_t t, const int32_t (&page)[2]) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int64_t place = place_of(t, s, page[s]);
-        const int32_t rows = seen_of(t, s, page[s]);
-        const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.value) + place * row_bytes, rows * row_bytes);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint32_t at = value_at + r * row_bytes;
-          if constexpr (kVWords == 1) {
-            v[s][r][0] = __builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, kOnce);
-          } else if constexpr (kVWords == 2) {
-            const auto w = __builtin_amdgcn_raw_buffer_load_b64(buf, at, 0, kOnce);
-            v[s][r][0] = w[0], v[s][r][1] = w[1];
-          } else {
-#pragma unroll
-            for (int i = 0; i < kVWords / 4; ++i) {
-              const uint4 w = load16<kOnce>(buf, at + 16 * i);
-              v[s][r][4 * i] = w.x, v[s][r][4 * i + 1] = w.y, v[s][r][4 * i + 2] = w.z, v[s][r][4 * i + 3] = w.w;
-            }
-          }
-        }
-        if constexpr (FP8) vs[s] = as_float4(load16<0>(stage_buffer(kv.value_scales + place, rows > 0 ? 64 : 0), 16u * g));
-      }
-    };
-    f32x4_t o[kVec];
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    bool seen = false;
-    if (tile < tile_end) {  // (a sequence without a position may have no table)
-    int32_t page[2], ahead[2], entry[2];  // pages of this tile and the next one, what the table says of the one behind
+  // ---- loads of a unit's 32 positions of this wave, as two blocks of 16 ----
+  // (what lies behind a sequence's end, or behind the share's, counts as no page and
+  // costs no memory; the loop has no branch around its loads, behind which a wait could
+  // not tell them apart)
+  auto entry_of = [&](const Unit& u, int s) -> int32_t {
+    const int32_t p = u.tile * kTile + wave * kWavePositions + 16 * s;
+    const int32_t* table = a.pages.table + u.b * a.pages.stride;
+    return *indexes(u.length > 0 ? table + (min(p, u.length - 1) >> kv.page_log2) : a.lengths);
+  };
+  auto page_of = [&](const Unit& u, int s, int32_t entry) -> int32_t {
+    return u.tile * kTile + wave * kWavePositions + 16 * s < u.length && entry < kv.pages ? entry : -1;  // (below 0: none, too)
+  };
+  // (no page: page 0, whose values are masked)
+  const int64_t page_rows = static_cast<int64_t>(kv.kv_heads) << kv.page_log2;
+  auto place_of = [&](const Unit& u, int s, int32_t page) -> int64_t {
+    const int32_t slot = (u.tile * kTile + wave * kWavePositions + 16 * s) & ((1 << kv.page_log2) - 1);
+    return max(page, 0) * page_rows + ((h << kv.page_log2) | slot);
+  };
+  // What a lane adds to the address of a block of 16 rows, which is the wave's.
+  const uint32_t key_at = n * row_bytes + 16 * g;
+  const uint32_t value_at = !PAD || n * kVec < dim ? 4 * g * row_bytes + n * (4 * kVWords) : kOutside;
+  // Blocks are read through buffers that end behind their last position that is seen
+  // (at once where there is no page): what lies behind reads as zeros and costs
+  // nothing, as do dimensions behind the last.
+  auto seen_of = [&](const Unit& u, int s, int32_t page) -> int32_t {
+    return page >= 0 ? min(16, u.length - (u.tile * kTile + wave * kWavePositions + 16 * s)) : 0;
+  };
+  uint4 k[2][kLoads];
+  float4 ks[2], vs[2];
+  uint32_t v[2][4][kVWords];
+  auto load_keys = [&](const Unit& u, const int32_t (&page)[2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      page[s] = page_of(tile, s, entry_of(tile, s));
-      entry[s] = entry_of(tile + 1, s);
-    }
-    // The queries of column n (of the upper half as of the lower one), in the keys' order of dimensions.
-    const int row = DUP ? n & 7 : n;
-    auto load_query = [&](int j) {
-      const int c = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j % 2) : 32 * j + 8 * g;
-      return row < rows && (!PAD || c < dim) ? ldg16(a.query + (query_row + row) * dim + c) : make_uint4(0u, 0u, 0u, 0u);
-    };
-    uint4 q[kSharedQuery ? 1 : DP / 32];
-    if constexpr (kSharedQuery) {
-      for (int j = wave; j < DP / 32; j += kWaves) shared_query[j][lane] = load_query(j);
-      __syncthreads();
-    } else {
-#pragma unroll
-      for (int j = 0; j < DP / 32; ++j) q[j] = load_query(j);
-    }
-    load_keys(tile, page);
-    __builtin_amdgcn_sched_barrier(0);  // (in this order, as in the loop)
-    load_values(tile, page);
-    __builtin_amdgcn_sched_barrier(0);
-
-    const float scale = a.scale * 1.44269504088896340736f;
-    const uint32_t rest = DUP && n >= 8 ? 0xFFFFFFFFu : 0u;
-
-    for (; tile < tile_end; ++tile) {
-      auto query = [&](int j) {
-        if constexpr (kSharedQuery) return shared_query[j][lane];
-        else return q[j];
-      };
-      f32x4_t s[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      const int64_t place = place_of(u, s, page[s]);
+      const int32_t seen = seen_of(u, s, page[s]);
+      const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.key) + place * row_bytes, seen * row_bytes);
+      // (a load of 8-bit keys takes half of 16 lines, the next one the other half:
+      // these are kept, 310 us against 328 for 64 sequences of 16 heads)
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
+        k[s][i] = load16<FP8 ? 0 : kOnce>(buf, (!PAD || i * kStep + g * (kStep / 4) < dim ? key_at : kOutside) + 64 * i);
+      if constexpr (FP8) ks[s] = as_float4(load16<0>(stage_buffer(kv.key_scales + place, seen > 0 ? 64 : 0), 16u * g));
+    }
+  };
+  auto load_values = [&](const Unit& u, const int32_t (&page)[2]) {
 #pragma unroll
-        for (int half = 0; half < (FP8 ? 2 : 1); ++half)
+    for (int s = 0; s < 2; ++s) {
+      const int64_t place = place_of(u, s, page[s]);
+      const int32_t seen = seen_of(u, s, page[s]);
+      const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.value) + place * row_bytes, seen * row_bytes);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if constexpr (FP8) {
-              const uint32_t lo = half == 0 ? k[t][i].x : k[t][i].z, hi = half == 0 ? k[t][i].y : k[t][i].w;
-              s[t] = mfma(make_uint4(fp8_pair<false>(lo), fp8_pair<true>(lo), fp8_pair<false>(hi), fp8_pair<true>(hi)),
-                          query(2 * i + half), s[t]);
-            } else {
-              s[t] = mfma(k[t][i], query(i), s[t]);
-            }
-          }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if constexpr (FP8) {
-          s[t][0] *= ks[t].x * scale, s[t][1] *= ks[t].y * scale, s[t][2] *= ks[t].z * scale, s[t][3] *= ks[t].w * scale;
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t at = value_at + r * row_bytes;
+        if constexpr (kVWords == 1) {
+          v[s][r][0] = __builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, kOnce);
+        } else if constexpr (kVWords == 2) {
+          const auto w = __builtin_amdgcn_raw_buffer_load_b64(buf, at, 0, kOnce);
+          v[s][r][0] = w[0], v[s][r][1] = w[1];
         } else {
-          s[t] *= scale;
+#pragma unroll
+          for (int i = 0; i < kVWords / 4; ++i) {
+            const uint4 w = load16<kOnce>(buf, at + 16 * i);
+            v[s][r][4 * i] = w.x, v[s][r][4 * i + 1] = w.y, v[s][r][4 * i + 2] = w.z, v[s][r][4 * i + 3] = w.w;
+          }
         }
       }
-      // Positions of this tile that are seen: lo <= place < hi of each block of 16.
-      int lo[2], hi[2];
+      if constexpr (FP8) vs[s] = as_float4(load16<0>(stage_buffer(kv.value_scales + place, seen > 0 ? 64 : 0), 16u * g));
+    }
+  };
+  // The queries of column n (of the upper half as of the lower one), in the keys' order of dimensions.
+  const int row = DUP ? n & 7 : n;
+  auto load_query = [&](int32_t b, int j) {
+    const int c = FP8 ? 64 * (j / 2) + 16 * g + 8 * (j % 2) : 32 * j + 8 * g;
+    const int64_t at = static_cast<int64_t>(b) * a.heads + h * group + query0 + row;
+    return row < rows && (!PAD || c < dim) ? ldg16(a.query + at * dim + c) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  uint4 q[kSharedQuery ? 1 : DP / 32];
+  auto load_queries = [&](int32_t b) {
+    if constexpr (kSharedQuery) {
+      for (int j = wave; j < DP / 32; j += kWaves) shared_query[j][lane] = load_query(b, j);
+    } else {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int32_t p = tile * kTile + wave * kWavePositions + 16 * t;
-        lo[t] = max(0, seq.first - p);
-        hi[t] = seen_of(tile, t, page[t]);
-      }
-      const bool whole = lo[0] <= 0 && lo[1] <= 0 && hi[0] >= 16 && hi[1] >= 16;
-      if (!whole) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) s[t][r] = -INFINITY;
-      }
-      seen = seen || lo[0] < hi[0] || lo[1] < hi[1];
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        ahead[t] = page_of(tile + 1, t, entry[t]);
-        entry[t] = entry_of(tile + 2, t);
-      }
-      load_keys(tile + 1, ahead);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < DP / 32; ++j) q[j] = load_query(b, j);
+    }
+  };
 
-      float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      most = fmaxf(most, xor_partner<16>(most));
-      most = fmaxf(most, xor_partner<32>(most));
-      if (__any(most > m)) {  // (seldom after the first tiles)
-        const float next = fmaxf(m, most);
-        const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-        l *= keep;
+  Unit unit = share.next(a), after = share.next(a);
+  int32_t page[2], ahead[2], entry[2];  // pages of this unit and the next one, what the table says of the one behind
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) o[i] *= keep;
-        m = next;
+  for (int s = 0; s < 2; ++s) {
+    page[s] = page_of(unit, s, entry_of(unit, s));
+    entry[s] = entry_of(after, s);
+  }
+  load_queries(unit.b);
+  if constexpr (kSharedQuery) __syncthreads();
+  load_keys(unit, page);
+  __builtin_amdgcn_sched_barrier(0);  // (in this order, as in the loop)
+  load_values(unit, page);
+  __builtin_amdgcn_sched_barrier(0);
+
+  const float scale = a.scale * 1.44269504088896340736f;
+  const uint32_t rest = DUP && n >= 8 ? 0xFFFFFFFFu : 0u;
+  f32x4_t o[kVec];
+  float m = -INFINITY, l = 0.f;
+  bool seen = false, from_start = unit.starts, first_head = true;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (;;) {
+    const Unit behind = share.next(a);
+    auto query = [&](int j) {
+      if constexpr (kSharedQuery) return shared_query[j][lane];
+      else return q[j];
+    };
+    f32x4_t s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int half = 0; half < (FP8 ? 2 : 1); ++half)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if constexpr (FP8) {
+            const uint32_t lo = half == 0 ? k[t][i].x : k[t][i].z, hi = half == 0 ? k[t][i].y : k[t][i].w;
+            s[t] = mfma(make_uint4(fp8_pair<false>(lo), fp8_pair<true>(lo), fp8_pair<false>(hi), fp8_pair<true>(hi)),
+                        query(2 * i + half), s[t]);
+          } else {
+            s[t] = mfma(k[t][i], query(i), s[t]);
+          }
+        }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if constexpr (FP8) {
+        s[t][0] *= ks[t].x * scale, s[t][1] *= ks[t].y * scale, s[t][2] *= ks[t].z * scale, s[t][3] *= ks[t].w * scale;
+      } else {
+        s[t] *= scale;
       }
-      const float from = m == -INFINITY ? 0.0f : m;
+    }
+    // Positions of this unit that are seen: lo <= place < hi of each block of 16.
+    int lo[2], hi[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      lo[t] = max(0, unit.first - (unit.tile * kTile + wave * kWavePositions + 16 * t));
+      hi[t] = seen_of(unit, t, page[t]);
+    }
+    const bool whole = lo[0] <= 0 && lo[1] <= 0 && hi[0] >= 16 && hi[1] >= 16;
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) s[t][r] = -INFINITY;
+    }
+    seen = seen || lo[0] < hi[0] || lo[1] < hi[1];
+    const bool last = unit.ends || !after.there;  // of this head's part here
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      ahead[t] = page_of(after, t, entry[t]);
+      entry[t] = entry_of(behind, t);
+    }
+    if constexpr (!kSharedQuery && !WHOLE)
+      if (last && after.there) load_queries(after.b);
+    load_keys(after, ahead);
+    __builtin_amdgcn_sched_barrier(0);
+
+    float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    most = fmaxf(most, xor_partner<16>(most));
+    most = fmaxf(most, xor_partner<32>(most));
+    if (__any(most > m)) {  // (seldom after the first tiles)
+      const float next = fmaxf(m, most);
+      const float keep = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+      l *= keep;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) o[i] *= keep;
+      m = next;
+    }
+    const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - from);
+        l += s[t][r];
+      }
+    if constexpr (FP8) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[t][0] *= vs[t].x, s[t][1] *= vs[t].y, s[t][2] *= vs[t].z, s[t][3] *= vs[t].w;
+    }
+    if (!whole) {  // (what lies in places that are not seen may be NaN; values behind the last read as zeros)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - from);
-          l += s[t][r];
+          if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) s[t][r] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kVWords; ++i)
+            if (4 * g + r < lo[t]) v[t][r][i] = 0u;
         }
-      if constexpr (FP8) {
+    }
+    // Weights as BF16 pairs: rounded (p), and what the rounding left (x).
+    uint32_t p[4], x[4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[t][0] *= vs[t].x, s[t][1] *= vs[t].y, s[t][2] *= vs[t].z, s[t][3] *= vs[t].w;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float y0 = s[t][2 * r], y1 = s[t][2 * r + 1];
+        const uint32_t w = pack_bf16x2(y0, y1);
+        if constexpr (DUP) {
+          const uint32_t z = w & rest;
+          p[2 * t + r] = pack_bf16x2(y0 - bf16lo(z), y1 - bf16hi(z));
+        } else {
+          p[2 * t + r] = w;
+          x[2 * t + r] = pack_bf16x2(y0 - bf16lo(w), y1 - bf16hi(w));
+        }
       }
-      if (!whole) {  // (what lies in places that are not seen may be NaN; values behind the last read as zeros)
+    const uint4 weights = make_uint4(p[0], p[1], p[2], p[3]);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if (4 * g + r < lo[t] || 4 * g + r >= hi[t]) s[t][r] = 0.f;
-#pragma unroll
-            for (int i = 0; i < kVWords; ++i)
-              if (4 * g + r < lo[t]) v[t][r][i] = 0u;
-          }
-      }
-      // Weights as BF16 pairs: rounded (p), and what the rounding left (x).
-      uint32_t p[4], x[4];
+    for (int i = 0; i < kVec; i += 2) {  // two dimensions: a word of each of the eight keys
+      uint32_t w[2][4];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float y0 = s[t][2 * r], y1 = s[t][2 * r + 1];
-          const uint32_t w = pack_bf16x2(y0, y1);
-          if constexpr (DUP) {
-            const uint32_t z = w & rest;
-            p[2 * t + r] = pack_bf16x2(y0 - bf16lo(z), y1 - bf16hi(z));
-          } else {
-            p[2 * t + r] = w;
-            x[2 * t + r] = pack_bf16x2(y0 - bf16lo(w), y1 - bf16hi(w));
-          }
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (FP8) w[t][r] = i % 4 == 0 ? fp8_pair<false>(v[t][r][i / 4]) : fp8_pair<true>(v[t][r][i / 4]);
+          else w[t][r] = v[t][r][i / 2];
         }
-      const uint4 weights = make_uint4(p[0], p[1], p[2], p[3]);
-#pragma unroll
-      for (int i = 0; i < kVec; i += 2) {  // two dimensions: a word of each of the eight keys
-        uint32_t w[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if constexpr (FP8) w[t][r] = i % 4 == 0 ? fp8_pair<false>(v[t][r][i / 4]) : fp8_pair<true>(v[t][r][i / 4]);
-            else w[t][r] = v[t][r][i / 2];
-          }
-        const uint4 even = make_uint4(perm(w[0][1], w[0][0], 0x05040100u), perm(w[0][3], w[0][2], 0x05040100u),
-                                      perm(w[1][1], w[1][0], 0x05040100u), perm(w[1][3], w[1][2], 0x05040100u));
-        const uint4 odd = make_uint4(perm(w[0][1], w[0][0], 0x07060302u), perm(w[0][3], w[0][2], 0x07060302u),
-                                     perm(w[1][1], w[1][0], 0x07060302u), perm(w[1][3], w[1][2], 0x07060302u));
-        o[i] = mfma(even, weights, o[i]);
-        o[i + 1] = mfma(odd, weights, o[i + 1]);
-        if constexpr (!DUP) {
-          const uint4 rests = make_uint4(x[0], x[1], x[2], x[3]);
-          o[i] = mfma(even, rests, o[i]);
-          o[i + 1] = mfma(odd, rests, o[i + 1]);
-        }
+      const uint4 even = make_uint4(perm(w[0][1], w[0][0], 0x05040100u), perm(w[0][3], w[0][2], 0x05040100u),
+                                    perm(w[1][1], w[1][0], 0x05040100u), perm(w[1][3], w[1][2], 0x05040100u));
+      const uint4 odd = make_uint4(perm(w[0][1], w[0][0], 0x07060302u), perm(w[0][3], w[0][2], 0x07060302u),
+                                   perm(w[1][1], w[1][0], 0x07060302u), perm(w[1][3], w[1][2], 0x07060302u));
+      o[i] = mfma(even, weights, o[i]);
+      o[i + 1] = mfma(odd, weights, o[i + 1]);
+      if constexpr (!DUP) {
+        const uint4 rests = make_uint4(x[0], x[1], x[2], x[3]);
+        o[i] = mfma(even, rests, o[i]);
+        o[i + 1] = mfma(odd, rests, o[i + 1]);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      load_values(tile + 1, ahead);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) page[t] = ahead[t];
     }
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(after, ahead);
+    __builtin_amdgcn_sched_barrier(0);
 
-    // ---- join of the waves ----
-    l += xor_partner<16>(l);
-    l += xor_partner<32>(l);
-    if (m == -INFINITY && seen) {
-      if (l == 0.f) l = NAN;  // every score -inf
-      else m = 0.f;           // every score -inf or NaN
-    }
-    if constexpr (DUP) {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[i][r] += other_half(o[i][r]);
-    }
-    __syncthreads();  // (the last head's join has been read)
-    if (n < rows) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < kVec; i += 4)
-          *reinterpret_cast<float4*>(&part_o[wave][n][kVec * (4 * g + r) + i]) = make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
-      if (g == 0) {
-        part_m[wave][n] = m;
-        part_l[wave][n] = l;
+    if (last) {
+      // ---- join of the waves; the next head's keys and values are on their way ----
+      l += xor_partner<16>(l);
+      l += xor_partner<32>(l);
+      if (m == -INFINITY && seen) {
+        if (l == 0.f) l = NAN;  // every score -inf
+        else m = 0.f;           // every score -inf or NaN
       }
-    }
-    __syncthreads();
-    const bool complete = u0 == 0 && u1 == seq.units;
-    const int64_t slot = 2 * blockIdx.x + (at == begin ? 0 : 1);
-    float* part = a.workspace + slot * kRows * (DP + 2);
-    for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads) {
-      const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
-      float all = part_m[0][r];
+      if constexpr (DUP) {
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) all = fmaxf(all, part_m[w][r]);
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < kVec; ++i)
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = part_factor(part_m[w][r], all);
-        const float4 y = *reinterpret_cast<const float4*>(&part_o[w][r][c]);
-        sum += weighted(f, part_l[w][r]);
-        acc.x += weighted(f, y.x), acc.y += weighted(f, y.y), acc.z += weighted(f, y.z), acc.w += weighted(f, y.w);
+          for (int r = 0; r < 4; ++r) o[i][r] += other_half(o[i][r]);
       }
-      if (complete) {
-        if (!PAD || c < dim) {
-          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-          *reinterpret_cast<uint2*>(a.out + (query_row + r) * dim + c) =
-              make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        }
-      } else {
-        *reinterpret_cast<float4*>(part + r * DP + c) = acc;
-        if (c == 0) {
-          part[kRows * DP + 2 * r] = all;
-          part[kRows * DP + 2 * r + 1] = sum;
+      local_barrier();  // (the last head's join has been read)
+      if (n < rows) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < kVec; i += 4)
+            *reinterpret_cast<float4*>(&part_o[wave][n][kVec * (4 * g + r) + i]) = make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
+        if (g == 0) {
+          part_m[wave][n] = m;
+          part_l[wave][n] = l;
         }
       }
+      if constexpr (kSharedQuery && !WHOLE)
+        if (after.there) load_queries(after.b);
+      local_barrier();
+      const bool complete = WHOLE || (from_start && unit.ends);
+      const int64_t slot = 2 * blockIdx.x + (first_head ? 0 : 1);
+      float* part = a.workspace + slot * kRows * (DP + 2);
+      const int64_t query_row = static_cast<int64_t>(unit.b) * a.heads + h * group + query0;
+      for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads) {
+        const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
+        float all = part_m[0][r];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) all = fmaxf(all, part_m[w][r]);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float f = part_factor(part_m[w][r], all);
+          const float4 y = *reinterpret_cast<const float4*>(&part_o[w][r][c]);
+          sum += weighted(f, part_l[w][r]);
+          acc.x += weighted(f, y.x), acc.y += weighted(f, y.y), acc.z += weighted(f, y.z), acc.w += weighted(f, y.w);
+        }
+        if (complete) {
+          if (!PAD || c < dim) {
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            *reinterpret_cast<uint2*>(a.out + (query_row + r) * dim + c) =
+                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+          }
+        } else {
+          *reinterpret_cast<float4*>(part + r * DP + c) = acc;
+          if (c == 0) {
+            part[kRows * DP + 2 * r] = all;
+            part[kRows * DP + 2 * r + 1] = sum;
+          }
+        }
+      }
+      if (WHOLE || !after.there) return;
+      m = -INFINITY, l = 0.f;
+      seen = false, from_start = after.starts, first_head = false;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    at += u1 - u0;
+    unit = after;
+    after = behind;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) page[t] = ahead[t];
   }
 }
 
@@ -541,12 +615,12 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   if (FEW && item >= a.batch * a.heads) return;
   const int32_t b = item / a.heads, head = item - b * a.heads, h = head / group;
   const int32_t tile = (head - h * group) / plan.query_rows, row = (head - h * group) - tile * plan.query_rows;
-  const Sequence seq = sequence_of(a, plan, indexes(a.lengths)[b]);
+  const Sequence seq = sequence_of(a, indexes(a.lengths)[b]);
   int32_t units = seq.units, before = 0;
-  if (a.batch > 1) before = units_before(a, plan, b, &units);
+  if (a.batch > 1) before = units_before(a, b, &units);
   const int32_t per = units_per_column(units, plan);
-  const int32_t w0 = before / per, w1 = (before + seq.units - 1) / per;
-  if (w0 == w1) return;  // one workgroup had it all
+  const int32_t w0 = before / per, w1 = min((before + seq.units - 1) / per, plan.columns - 1);
+  if (w0 >= w1) return;  // one workgroup had it all
   // (a part is in its workgroup's first place but where another head came before it there)
   const int64_t stride = static_cast<int64_t>(rows) * (DP + 2);
   const int32_t first_place = before != w0 * per ? 1 : 0, index = h * plan.query_tiles + tile;
@@ -618,8 +692,13 @@ Plan plan_of(const PagedAttentionArgs& a, int cus) {
 template <int DP, bool FP8, bool DUP>
 void launch_main(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream) {
   const unsigned groups = static_cast<unsigned>(p.columns) * a.cache.kv_heads * p.query_tiles;
-  if (a.cache.dim == DP) paged_attention_kernel<DP, FP8, DUP, false><<<groups, kThreads, 0, stream>>>(a, p);
-  else paged_attention_kernel<DP, FP8, DUP, true><<<groups, kThreads, 0, stream>>>(a, p);
+  if (p.whole) {
+    if (a.cache.dim == DP) paged_attention_kernel<DP, FP8, DUP, false, true><<<groups, kThreads, 0, stream>>>(a, p);
+    else paged_attention_kernel<DP, FP8, DUP, true, true><<<groups, kThreads, 0, stream>>>(a, p);
+  } else {
+    if (a.cache.dim == DP) paged_attention_kernel<DP, FP8, DUP, false, false><<<groups, kThreads, 0, stream>>>(a, p);
+    else paged_attention_kernel<DP, FP8, DUP, true, false><<<groups, kThreads, 0, stream>>>(a, p);
+  }
 }
 template <int DP>
 hipError_t launch(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream) {
