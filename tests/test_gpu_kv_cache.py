@@ -304,6 +304,16 @@ def test_attention_over_long_sequences(hip_ext, heads, kv_heads, dim, lengths, f
     attend_case(hip_ext, gen(heads), lengths, heads, kv_heads, 16, dim, fp8)
 
 
+@pytest.mark.parametrize("lengths", [[200, 5, 300], [700, 5, 1300]])  # heads whole, and in parts
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("group", [2, 12])
+@pytest.mark.parametrize("dim", [64, 48, 128, 80, 256, 192])
+def test_every_kernel(hip_ext, dim, group, fp8, lengths):
+    """Whole and ragged head sizes of each width, one and two products a weight, both types, both ways to deal out work."""
+    print(f"[case] attention kernels {dim} {group} {fp8} {lengths}", flush=True)
+    attend_case(hip_ext, gen(dim + group), lengths, 3 * group, 3, 32, dim, fp8)
+
+
 @pytest.mark.parametrize("batch", [63, 64, 65, 129, 300])
 def test_attention_of_many_sequences(hip_ext, batch):
     print(f"[case] attention batch {batch}", flush=True)

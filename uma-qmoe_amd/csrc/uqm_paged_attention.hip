@@ -6,10 +6,15 @@
 // softmax (base 2: s and m carry the factor log2 e).
 //
 // Bound by memory: a key and its value are read for at most 16 query heads, some
-// 4 to 64 operations a byte. What is computed goes to the matrix cores all the same,
-// since the vector unit would be the limit from four query heads a key head on.
-// Everything stays in the wave's registers: no exchange, no shared memory in the
-// loop, but for the maximum over four lanes.
+// 4 to 64 operations a byte. 64 sequences of 4001 to 8191 tokens, 16 heads of 128 in
+// e4m3: 255 us, 6.5 TB/s (290 to 310 once the card throttles, some 3 ms into calls
+// without a pause); 32 heads on 8 over 131071 tokens in BF16 84 us, 6.4 TB/s; 32
+// sequences of up to 2047, 16 heads in BF16, 48 us, 5.6 TB/s. With products and
+// softmax left out the times were the same.
+// What is computed goes to the matrix cores all the same, since the vector unit would
+// be the limit from four query heads a key head on. Everything stays in the wave's
+// registers: no exchange, no shared memory in the loop, but for the maximum over four
+// lanes.
 //   - scores transposed, S^T = K Q^T (16 keys x 16 queries, v_mfma_f32_16x16x32_bf16):
 //     a lane gives 8 neighbouring dimensions of one key, which lie next to each other
 //     in a page, and gets scores of one query (lane % 16) and four keys
@@ -29,13 +34,19 @@
 //     weights in the lower and the rests in the upper half, which costs nothing; with
 //     more of them there is a second product.
 //
-// Work is dealt out in tiles of 128 positions (32 of each of a workgroup's four
-// waves) of one sequence and key head, numbered sequence by sequence, head by head;
-// each workgroup takes the same number of neighbouring tiles, whatever the lengths
-// are, and computes from these where they lie. What it has of a head that other
-// workgroups also work on goes to its two places in the workspace (at most its first
-// and its last head), and a second launch joins these. Without a sequence long
-// enough a workgroup takes whole heads, and there is no second launch.
+// Work is dealt out in tiles of 128 positions, 32 of each of a workgroup's four waves.
+// The tiles of all sequences, one behind the other, are cut into columns of the same
+// number of tiles, whatever the lengths are; a column has a workgroup for each key head,
+// which go through the same positions side by side (that a head's workgroups took its
+// positions one after the other instead cost 5 to 10%). A workgroup finds its column
+// from the lengths on the device. What it has of a sequence that other columns also work
+// on goes to its two places in the workspace (for the first and the last of its
+// sequences), and a second launch joins these. Keys, values and queries of the next tile
+// are on their way while one is computed, also across the end of a sequence (255
+// sequences of 50 to 150 tokens 41 us, with a start of its own for each 50).
+// Where no sequence can have more than four tiles a workgroup takes a sequence's head,
+// without that bookkeeping and without a second launch (one token over 77 positions, 16
+// heads, 4.5 us in a graph; 5.2 with the bookkeeping).
 #include "uqm_device.h"
 #include "uqm_kv.h"
 #include "uqm_stage.h"
@@ -47,9 +58,15 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kWavePositions = 32, kTile = kWaves * kWavePositions;
-constexpr int kGroupsPerCu = 2;   // workgroups of the main launch per compute unit
-constexpr int kFewParts = 16;     // up to this many parts a sequence on average a wave joins those of a head
-constexpr int kDirectTiles = 4;   // up to this many tiles a head is one workgroup's
+// Workgroups of the main launch per compute unit. More of them (3, 4, 6, 8, 12) read no
+// faster, but leave more parts: 131071 tokens 94 us against 96, 106, 118, 119, 124.
+constexpr int kGroupsPerCu = 2;
+// Up to this many parts a sequence on average a wave joins those of a head: 1999 tokens
+// of 13 sequences 12 us, by workgroups 15; 4001 of one the same with either.
+constexpr int kFewParts = 16;
+// Up to this many tiles a head is one workgroup's, a tile 1 us: 4 tiles 7.7 us and in
+// parts 8.4; 8 tiles 12.2 and 8.4.
+constexpr int kDirectTiles = 4;
 
 __device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -60,7 +77,7 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 constexpr uint32_t kOutside = 0x80000000u;  // an offset behind every buffer's bytes
-constexpr int kOnce = 2;                    // a load whose lines are not kept (nontemporal)
+constexpr int kOnce = 2;                    // a load whose lines are not kept (nontemporal): 131071 tokens 94 us, else 106
 template <int HINT>
 __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, HINT));
@@ -603,8 +620,8 @@ __device__ __forceinline__ void join_lanes(Joined& x) {
 
 // Joins the parts of query heads. Of few parts (FEW) a wave has a head, four
 // dimensions a lane; of many a workgroup has 32 dimensions of a head, and 32 sets of
-// 8 lanes share the parts (8 heads in 512 parts of 128: 4 us, with a workgroup a head
-// 12; 4096 heads in 2 to 3 parts: 4 us with a wave a head, with a workgroup 10).
+// 8 lanes share the parts (8 heads of 128 in 512 parts: 5.4 us, with a workgroup a head
+// 12; 4096 heads in 2 to 3 parts: 5.5 us with a wave a head, with a workgroup 10).
 template <int DP, bool FEW>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, Plan plan) {
   constexpr int kSpan = FEW ? DP : 32, kLanes = kSpan / 4, kSets = (FEW ? 64 : kThreads) / kLanes;

@@ -187,6 +187,7 @@ class HipExtension:
         self.lib = _native.library()
         self._ws_lock = threading.Lock()
         self._ws_cache: dict[tuple[int, int], Any] = {}
+        self._bf16, self._e4m3, self._f32, self._i32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32
 
     # ------------------------------------------------------------ helpers --
     def _workspace(self, device, tokens, hidden, inter, shared_inter, experts, top_k):
@@ -669,44 +670,48 @@ class HipExtension:
         raise RuntimeError(f"{what} requires device tensors, all on one device")
 
     def _cache(self, cache, what, index):
-        """The descriptor of ``cache`` on device ``index``."""
-        torch = self.torch
+        """The descriptor of ``cache`` on device ``index``, and its shape."""
         k, v, ks, vs = cache
         shape = k.shape
-        scaled = ks is not None
         if not (len(shape) == 4 and v.shape == shape and k.is_contiguous() and v.is_contiguous() and index >= 0
-                and k.get_device() == index == v.get_device()
-                and ((k.dtype is v.dtype is torch.float8_e4m3fn and vs is not None and ks.dtype is vs.dtype is torch.float32
-                      and ks.shape == vs.shape == shape[:3] and ks.is_contiguous() and vs.is_contiguous()
-                      and ks.get_device() == index == vs.get_device())
-                     if scaled else (k.dtype is v.dtype is torch.bfloat16 and vs is None))):
+                and k.get_device() == index == v.get_device()):
             self._check_cache(cache, what)
-        return _native.KVCache(k.data_ptr(), v.data_ptr(), ks.data_ptr() if scaled else None,
-                               vs.data_ptr() if scaled else None, *shape)
+        dtype = k.dtype
+        if ks is None:
+            if not (vs is None and dtype is self._bf16 and v.dtype is dtype):
+                self._check_cache(cache, what)
+            return _native.KVCache(k.data_ptr(), v.data_ptr(), None, None, *shape), shape
+        if not (vs is not None and dtype is self._e4m3 and v.dtype is dtype and ks.dtype is self._f32 and vs.dtype is self._f32
+                and ks.shape == shape[:3] and vs.shape == ks.shape and ks.is_contiguous() and vs.is_contiguous()
+                and ks.get_device() == index == vs.get_device()):
+            self._check_cache(cache, what)
+        return _native.KVCache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *shape), shape
 
     def _indexes(self, what, index, page_table, vector, counts=None):
-        """The page table (rows of neighbouring entries), its row stride and the
-        vectors of one entry per sequence."""
-        i32 = self.torch.int32
-        shape = page_table.shape
-        if len(shape) != 2 or page_table.dtype is not i32:
+        """The page table (rows of neighbouring entries), its row stride, its width
+        and the vectors of one entry per sequence."""
+        i32 = self._i32
+        if page_table.ndim != 2 or page_table.dtype is not i32:
             raise RuntimeError(f"{what} requires an int32 page table [batch, pages of a sequence]")
-        if not (vector.shape == shape[:1] and vector.dtype is i32
-                and (counts is None or counts.shape == shape[:1] and counts.dtype is i32)):
-            raise RuntimeError(f"{what} requires an int32 entry for each of the page table's {shape[0]} sequences")
+        batch, width = page_table.shape
+        if not (vector.ndim == 1 and vector.numel() == batch and vector.dtype is i32
+                and (counts is None or counts.ndim == 1 and counts.numel() == batch and counts.dtype is i32)):
+            raise RuntimeError(f"{what} requires an int32 entry for each of the page table's {batch} sequences")
         if not (page_table.get_device() == index == vector.get_device() and (counts is None or counts.get_device() == index)):
             raise RuntimeError(f"{what} requires device tensors, all on one device")
+        stride, step = page_table.stride()
         # (a table by columns, or with one row for all, is laid out row by row; a single entry's stride is not used)
-        if shape[1] > 1 and page_table.stride(1) != 1 or page_table.stride(0) < shape[1]:
+        if width > 1 and step != 1 or stride < width:
             page_table = page_table.contiguous()
-        return (page_table, max(page_table.stride(0), shape[1]), vector.contiguous(),
-                counts if counts is None else counts.contiguous())
+            stride = max(page_table.stride(0), width)
+        return (page_table, stride, width, vector if vector.is_contiguous() else vector.contiguous(),
+                counts if counts is None or counts.is_contiguous() else counts.contiguous())
 
-    def _new_rows(self, x, shape, what):
-        """New keys or values with rows that the library takes: neighbouring
-        elements, 16-byte aligned."""
-        if x.dtype is not self.torch.bfloat16 or len(x.shape) != 4 or x.shape[1] != shape[1] or x.shape[3] != shape[3]:
-            raise RuntimeError(f"{what} requires BF16 keys and values [batch, {shape[1]}, tokens, {shape[3]}] (heads and "
+    def _new_rows(self, x, kv_heads, head_dim, what):
+        """New keys or values with rows that the library takes (neighbouring
+        elements, 16-byte aligned), and their strides."""
+        if x.dtype is not self._bf16 or x.ndim != 4 or x.size(1) != kv_heads or x.size(3) != head_dim:
+            raise RuntimeError(f"{what} requires BF16 keys and values [batch, {kv_heads}, tokens, {head_dim}] (heads and "
                                "head size as the cache)")
         b, h, t, d = x.stride()
         if d != 1 or (b | h | t) & 7 or x.data_ptr() & 15:
@@ -723,17 +728,18 @@ class HipExtension:
         none) are dropped. No place may be written twice in a call.
         ``page_table``, ``starts`` and ``counts`` int32. Returns ``cache``."""
         index = key.get_device()
-        desc = self._cache(cache, "kv_append", index)
-        shape = cache.key.shape
-        key, kb, kh, kt = self._new_rows(key, shape, "kv_append")
-        value, vb, vh, vt = self._new_rows(value, shape, "kv_append")
-        batch, _, tokens, _ = key.shape
-        if value.shape != key.shape or value.get_device() != index or page_table.shape[:1] != (batch,):
+        desc, (_, kv_heads, _, head_dim) = self._cache(cache, "kv_append", index)
+        key, kb, kh, kt = self._new_rows(key, kv_heads, head_dim, "kv_append")
+        value, vb, vh, vt = self._new_rows(value, kv_heads, head_dim, "kv_append")
+        shape = key.shape
+        batch, _, tokens, _ = shape
+        page_table, stride, width, starts, counts = self._indexes("kv_append", index, page_table, starts, counts)
+        if value.shape != shape or value.get_device() != index or page_table.size(0) != batch:
             raise RuntimeError("kv_append requires keys and values of one shape on one device, and a row of the page table "
                                "for each sequence")
-        page_table, stride, starts, counts = self._indexes("kv_append", index, page_table, starts, counts)
         self._launch(self.lib.uqm_kv_append, index, ctypes.byref(desc), key.data_ptr(), kb, kh, kt, value.data_ptr(), vb, vh,
-                     vt, batch, tokens, page_table.data_ptr(), stride, page_table.shape[1], starts.data_ptr(), _ptr(counts))
+                     vt, batch, tokens, page_table.data_ptr(), stride, width, starts.data_ptr(),
+                     None if counts is None else counts.data_ptr())
         return cache
 
     def kv_read(self, cache: KVCache, page_table, lengths, max_length):
@@ -742,17 +748,14 @@ class HipExtension:
         on, and where the page table has no page."""
         torch = self.torch
         index = page_table.get_device()
-        desc = self._cache(cache, "kv_read", index)
-        page_table, stride, lengths, _ = self._indexes("kv_read", index, page_table, lengths)
-        _, kv_heads, _, head_dim = cache.key.shape
+        desc, (_, kv_heads, _, head_dim) = self._cache(cache, "kv_read", index)
+        page_table, stride, width, lengths, _ = self._indexes("kv_read", index, page_table, lengths)
         if not 0 <= max_length * kv_heads < 1 << 31:
             raise RuntimeError("kv_read requires max_length * kv_heads in [0, 2^31)")
-        batch = page_table.shape[0]
-        shape = (batch, kv_heads, max_length, head_dim)
-        key = torch.empty(shape, dtype=torch.bfloat16, device=page_table.device)
+        batch = page_table.size(0)
+        key = torch.empty((batch, kv_heads, max_length, head_dim), dtype=self._bf16, device=page_table.device)
         value = torch.empty_like(key)
-        self._launch(self.lib.uqm_kv_read, index, ctypes.byref(desc), batch, page_table.data_ptr(), stride,
-                     page_table.shape[1], lengths.data_ptr(), max_length, key.data_ptr(), value.data_ptr())
+        self._launch(self.lib.uqm_kv_read, index, ctypes.byref(desc), batch, page_table.data_ptr(), stride, width, lengths.data_ptr(), max_length, key.data_ptr(), value.data_ptr())
         return key, value
 
     def paged_attention(self, query, cache: KVCache, page_table, lengths, *, scale=None, window=None):
@@ -764,28 +767,26 @@ class HipExtension:
         default."""
         torch = self.torch
         index, shape = query.get_device(), query.shape
-        desc = self._cache(cache, "paged_attention", index)
-        _, kv_heads, page_size, head_dim = cache.key.shape
-        if query.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != head_dim or shape[1] % kv_heads or not shape[1]:
+        desc, (_, kv_heads, page_size, head_dim) = self._cache(cache, "paged_attention", index)
+        if query.dtype is not self._bf16 or len(shape) != 3 or shape[2] != head_dim or shape[1] % kv_heads or not shape[1]:
             raise RuntimeError(f"paged_attention requires a BF16 query [batch, heads, {head_dim}] of a multiple of {kv_heads} "
                                f"heads, not {query.dtype} {tuple(shape)}")
         if window is not None and window < 1:
             raise RuntimeError("paged_attention requires a window of at least 1")
         batch, heads, _ = shape
-        if page_table.shape[:1] != (batch,):
+        page_table, stride, width, lengths, _ = self._indexes("paged_attention", index, page_table, lengths)
+        if page_table.size(0) != batch:
             raise RuntimeError("paged_attention requires a row of the page table for each sequence")
-        page_table, stride, lengths, _ = self._indexes("paged_attention", index, page_table, lengths)
         if not query.is_contiguous() or query.data_ptr() & 15:
             query = query.clone(memory_format=torch.contiguous_format)
         out = torch.empty_like(query)
-        width = page_table.shape[1]
         # (torch's allocator gives memory in stream order, and a captured graph its own)
         nbytes = self.lib.uqm_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim, page_size, width)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
         self._launch(self.lib.uqm_paged_attention, index, ctypes.byref(desc), query.data_ptr(), batch, heads,
                      page_table.data_ptr(), stride, width, lengths.data_ptr(),
                      head_dim ** -0.5 if scale is None else scale, 0 if window is None else min(window, 1 << 31), out.data_ptr(),
-                     _ptr(workspace), nbytes)
+                     None if workspace is None else workspace.data_ptr(), nbytes)
         return out
 
     # ------------------------------------- reference binding signatures --
