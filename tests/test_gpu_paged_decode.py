@@ -95,6 +95,22 @@ def test_replays_are_the_eager_steps(checkpoint, fp8):
         assert graph.next_positions == eager.next_positions == [15 + 9, 15 + 20, 2 + 14]
 
 
+def test_with_dense_layers_in_8_bits(checkpoint):
+    """A host whose projections are 8-bit modules: replays are the eager steps."""
+    print("[case] paged fp8 dense", flush=True)
+    with load(checkpoint, fp8_dense=True) as host:
+        eager, graph = (PagedDecodeGraph(host.model, batch=2, max_len=40, page_size=16, fp8_cache=True) for _ in range(2))
+        for dg in (eager, graph):
+            dg.prefill(0, prompt(5, seed=1).to(DEV))
+            dg.prefill(1, prompt(17, seed=2).to(DEV))
+        graph.capture()
+        for step in range(8):
+            want, got = eager.step_eager(), graph.replay().clone()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), f"step {step}"
+            assert (graph.logits - eager.logits).norm() <= 1e-3 * eager.logits.norm(), f"step {step}"
+
+
 def test_one_sequence_is_the_one_sequence_graph(checkpoint):
     """The same logits as DecodeGraph's, from a captured step each, as long as both
     choose the same tokens. Either is within 2e-2 of the sequence run again without a
@@ -136,6 +152,32 @@ def test_a_conversation_goes_on(checkpoint, fp8):
             assert om.rel_l2(dg.logits[1].cpu(), want.cpu()) <= LIMIT[fp8], f"step {step}"
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_layer_with_a_window(checkpoint, fp8):
+    """A layer that sees the last 8 positions only: in prefill, in steps and when a conversation goes on."""
+    print(f"[case] paged window {fp8}", flush=True)
+    with load(checkpoint) as host:
+        host.model.config.layer_types = ["full_attention", "sliding_attention"]
+        host.model.config.sliding_window = 8
+        host.model.model.layers[1].self_attn.sliding_window = 8
+        dg = PagedDecodeGraph(host.model, batch=1, max_len=96, page_size=16, fp8_cache=fp8)
+        ids = prompt(21, seed=5).to(DEV)
+        seq = torch.cat([ids, dg.prefill(0, ids)], 1)
+        for step in range(6):
+            want = uncached(host.model, seq)
+            seq = torch.cat([seq, dg.step_eager()], 1)
+            assert om.rel_l2(dg.logits[0].cpu(), want.cpu()) <= LIMIT[fp8], f"step {step}"
+        seq = torch.cat([seq, prompt(9, seed=6).to(DEV)], 1)
+        dg.extend(0, seq[:, dg.next_positions[0]:])  # (the last choice and what follows)
+        seq = torch.cat([seq, dg.token], 1)
+        want = uncached(host.model, seq)
+        dg.step_eager()
+        assert om.rel_l2(dg.logits[0].cpu(), want.cpu()) <= LIMIT[fp8]
+        # (the window matters: a model without it gives other logits)
+        host.model.config.layer_types = ["full_attention", "full_attention"]
+        assert om.rel_l2(want.cpu(), uncached(host.model, seq).cpu()) > LIMIT[fp8]
+
+
 def test_refusals_change_nothing(checkpoint):
     print("[case] paged refusals", flush=True)
     ids = prompt(10).to(DEV)
@@ -144,6 +186,10 @@ def test_refusals_change_nothing(checkpoint):
                               (dict(batch=1, max_len=8, page_size=24), "pages of")):
             with pytest.raises(ContractError, match=words):
                 PagedDecodeGraph(host.model, **kwargs)
+        host.model.config.model_type = "olmoe"
+        with pytest.raises(ContractError, match="Qwen2MoE"):
+            PagedDecodeGraph(host.model, batch=1, max_len=8)
+        host.model.config.model_type = "qwen2_moe"
         dg = PagedDecodeGraph(host.model, batch=2, max_len=20, page_size=16, pages=2)
         with pytest.raises(ContractError, match="no sequence"):
             dg.step_eager()
@@ -172,5 +218,5 @@ def test_refusals_change_nothing(checkpoint):
         dg.finish(0)
         for _ in range(4):
             dg.step_eager()  # with the page that the other sequence had
-        with pytest.raises(ContractError, match="filled its places"):
+        with pytest.raises(ContractError, match=r"sequences \[1\] have filled their places"):
             dg.step_eager()

@@ -38,7 +38,7 @@
 // The tiles of all sequences, one behind the other, are cut into columns of the same
 // number of tiles, whatever the lengths are; a column has a workgroup for each key head,
 // which go through the same positions side by side (that a head's workgroups took its
-// positions one after the other instead cost 5 to 10%). A workgroup finds its column
+// positions one after the other instead cost 2 to 8%). A workgroup finds its column
 // from the lengths on the device. What it has of a sequence that other columns also work
 // on goes to its two places in the workspace (for the first and the last of its
 // sequences), and a second launch joins these. Keys, values and queries of the next tile
@@ -58,14 +58,15 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kWavePositions = 32, kTile = kWaves * kWavePositions;
-// Workgroups of the main launch per compute unit. More of them (3, 4, 6, 8, 12) read no
-// faster, but leave more parts: 131071 tokens 94 us against 96, 106, 118, 119, 124.
+// Workgroups of the main launch per compute unit. More of them read no faster, but
+// leave more parts: 2, 3, 4 and 8 for 131071 tokens 94, 97, 96 and 102 us, for 32
+// sequences of up to 2047 in BF16 52, 53, 56 and 55.
 constexpr int kGroupsPerCu = 2;
-// Up to this many parts a sequence on average a wave joins those of a head: 1999 tokens
-// of 13 sequences 12 us, by workgroups 15; 4001 of one the same with either.
+// Up to this many parts a sequence on average a wave joins those of a head: 13 sequences
+// (10 parts) 12.5 us, by workgroups 15.4; one of 4001 tokens (32) 13.7, by workgroups 12.0.
 constexpr int kFewParts = 16;
 // Up to this many tiles a head is one workgroup's, a tile 1 us: 4 tiles 7.7 us and in
-// parts 8.4; 8 tiles 12.2 and 8.4.
+// parts 8.4; 8 tiles 11.6 and 8.5.
 constexpr int kDirectTiles = 4;
 
 __device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
@@ -77,7 +78,7 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 constexpr uint32_t kOutside = 0x80000000u;  // an offset behind every buffer's bytes
-constexpr int kOnce = 2;                    // a load whose lines are not kept (nontemporal): 131071 tokens 94 us, else 106
+constexpr int kOnce = 2;                    // a load whose lines are not kept (nontemporal): 131071 tokens 94 us, kept 106
 template <int HINT>
 __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, HINT));

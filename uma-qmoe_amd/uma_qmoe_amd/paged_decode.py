@@ -72,6 +72,8 @@ class PagedDecodeGraph:
         self.device = next(model.parameters()).device
         if self.device.type != "cuda":
             raise ContractError("a paged cache requires a HIP device")
+        if getattr(model.config, "model_type", None) != "qwen2_moe":  # (others have norms of queries and keys, too)
+            raise ContractError("a paged cache requires a Qwen2MoE model")
         if batch < 1 or max_len < 1:
             raise ContractError("a paged cache requires at least one sequence and one position")
         if page_size not in KV_PAGE_SIZES:
@@ -221,8 +223,9 @@ class PagedDecodeGraph:
         """Pages for every sequence's next position, or a refusal with nothing changed."""
         if all(p is None for p in self.next_positions):
             raise ContractError("no sequence to decode")
-        if any(p is not None and p >= self.max_len for p in self.next_positions):
-            raise ContractError("a sequence has filled its places in the cache")
+        full = [i for i, p in enumerate(self.next_positions) if p is not None and p >= self.max_len]
+        if full:
+            raise ContractError(f"sequences {full} have filled their places in the cache: finish() them first")
         self._enter(self.pool.reserve((i, p + 1) for i, p in enumerate(self.next_positions) if p is not None))
 
     def _advance(self) -> None:
