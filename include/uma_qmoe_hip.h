@@ -402,7 +402,7 @@ int uqm_kv_read(const uqm_kv_cache* cache, int64_t batch, const int32_t* page_ta
  * which parts they are joined goes by the table's width and all lengths of the
  * call, so that a result may differ in its last bit between calls that differ in
  * these. batch * kv_heads * ceil(heads / kv_heads / 16) * ceil(max_pages * page_size
- * / 128) below 2^31.
+ * / 128) below 2^30.
  * workspace: uqm_paged_attention_workspace_bytes, 16-byte aligned, of any content,
  * not shared by calls that overlap in time (also those of captured graphs); what
  * it held is not kept. */

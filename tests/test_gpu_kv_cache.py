@@ -318,7 +318,10 @@ def test_every_kernel(hip_ext, dim, group, fp8, lengths):
 def test_attention_of_many_sequences(hip_ext, batch):
     print(f"[case] attention batch {batch}", flush=True)
     attend_case(hip_ext, gen(batch), [(37 * i) % 71 for i in range(batch)], 2, 2, 16, 32, True)
+    attend_case(hip_ext, gen(batch), [(37 * i) % 71 for i in range(batch)], 2, 2, 16, 32, True, width=40)
+    attend_case(hip_ext, gen(batch), [(211 * i) % 900 for i in range(batch)], 2, 2, 16, 32, False)
     attend_case(hip_ext, gen(batch), [0] * (batch - 1) + [1500], 2, 1, 16, 32, False)
+    attend_case(hip_ext, gen(batch), [1500] + [0] * (batch - 1), 2, 1, 16, 32, False)
 
 
 @pytest.mark.parametrize("fp8", [False, True])

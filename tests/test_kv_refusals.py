@@ -102,7 +102,7 @@ def test_read(lib, changed, words):
 @pytest.mark.parametrize("changed,words", [
     (dict(heads=0), "multiple"), (dict(heads=3), "multiple"), (dict(heads=-2), "multiple"), (dict(heads=1 << 24), "2^24"),
     (dict(batch=1 << 20, heads=16), "2^24"),
-    (dict(batch=1 << 8, heads=2, width=1 << 26, stride=1 << 26), "room"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
+    (dict(batch=1 << 6, heads=2, width=1 << 26, stride=1 << 26), "room"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"),
     (dict(window=-1), "window"), (dict(query=None), "required"), (dict(lengths=None), "required"), (dict(out=None), "required"),
     (dict(query=C + 8), "aligned"), (dict(out=D + 2), "aligned"), (dict(lengths=F + 3), "aligned"),
     (dict(out=C + 16), "overlaps"), (dict(out=A), "overlaps"), (dict(out=E), "overlaps"), (dict(out=F), "overlaps"),
@@ -225,6 +225,7 @@ GOOD = KVCache(dev(bf(4, 2, 16, 64)), dev(bf(4, 2, 16, 64)))
     (lambda e: e.kv_read(GOOD, dev(i32(1, 4)), dev(i32(1)), -1), "max_length"),
     (lambda e: e.kv_read(GOOD, dev(i32(1, 4)), dev(i32(1)), 1 << 30), "max_length"),
     (lambda e: e.paged_attention(dev(bf(1, 3, 64)), GOOD, dev(i32(1, 4)), dev(i32(1))), "BF16 query"),
+    (lambda e: e.paged_attention(dev(bf(1, 4, 64)), KVCache(dev(bf(4, 0, 16, 64)), dev(bf(4, 0, 16, 64))), dev(i32(1, 4)), dev(i32(1))), "BF16 query"),
     (lambda e: e.paged_attention(dev(bf(1, 0, 64)), GOOD, dev(i32(1, 4)), dev(i32(1))), "BF16 query"),
     (lambda e: e.paged_attention(dev(bf(1, 4, 32)), GOOD, dev(i32(1, 4)), dev(i32(1))), "BF16 query"),
     (lambda e: e.paged_attention(dev(bf(1, 4, 1, 64)), GOOD, dev(i32(1, 4)), dev(i32(1))), "BF16 query"),

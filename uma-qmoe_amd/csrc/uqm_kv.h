@@ -77,7 +77,7 @@ struct PagedAttentionArgs {
   uint16_t* out;           // [batch, heads, dim]
   float* workspace;
 };
-// Whether the work can be numbered (below 2^31 tiles of 128 positions and 16 query heads).
+// Whether the work can be numbered (below 2^30 tiles of 128 positions and 16 query heads).
 bool paged_attention_fits(const PagedAttentionArgs& a);
 size_t paged_attention_workspace(const PagedAttentionArgs& a, int cus);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, int cus, hipStream_t stream);

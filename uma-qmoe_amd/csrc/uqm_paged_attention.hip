@@ -104,14 +104,14 @@ typedef const __attribute__((address_space(4))) int32_t* Indexes;
 __device__ __forceinline__ Indexes indexes(const int32_t* p) { return reinterpret_cast<Indexes>(reinterpret_cast<uintptr_t>(p)); }
 
 struct Plan {
-  int32_t columns;      // shares that the tiles of all sequences are dealt into, each of a workgroup per head
-  int32_t query_rows;   // query heads of a unit (at most)
-  int32_t query_tiles;  // units side by side for the query heads of a key head
-  bool whole;           // a sequence's head is one unit, whatever its length
+  int32_t columns;      // shares that the tiles of all sequences are cut into, each of a workgroup per head
+  int32_t query_rows;   // query heads of a workgroup (at most)
+  int32_t query_tiles;  // workgroups side by side for the query heads of a key head
+  bool whole;           // a sequence is a column, whatever its length
 };
 
-// A sequence's tiles from tile0 on are its units, one a head; one without a position
-// has one, too, which writes the zeros.
+// A sequence's units are its tiles from tile0 on; one without a position has one, too,
+// which writes the zeros.
 struct Sequence {
   int32_t length, first;  // positions seen: first .. length - 1
   int32_t tile0, units;
@@ -125,7 +125,7 @@ __device__ __forceinline__ Sequence sequence_of(const PagedAttentionArgs& a, int
   return s;
 }
 
-// Sum over the lanes up to this one, and over all.
+// Sum over the lanes up to this one; over all.
 __device__ __forceinline__ int32_t wave_scan(int32_t v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
@@ -251,7 +251,7 @@ __device__ __forceinline__ float weighted(float f, float v) { return f == 0.0f ?
 // (registers for one, two or three workgroups a compute unit, so that none spills)
 template <int DP, bool FP8, bool DUP, bool PAD, bool WHOLE>
 __global__ __launch_bounds__(kThreads, DP == 256 && !FP8 ? 1 : DP == 256 || !FP8 || PAD ? 2 : 3) void paged_attention_kernel(PagedAttentionArgs a, Plan plan) {
-  constexpr int kRows = DUP ? 8 : 16;      // query heads of a unit
+  constexpr int kRows = DUP ? 8 : 16;      // query heads that there is room for
   constexpr int kVec = DP / 16;            // dimensions of a value row that a lane holds
   constexpr int kStep = FP8 ? 64 : 32;     // dimensions of one load of 16 keys
   constexpr int kLoads = DP / kStep;
@@ -736,7 +736,7 @@ hipError_t launch(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream
 }  // namespace
 
 bool paged_attention_fits(const PagedAttentionArgs& a) {
-  return std::max<int64_t>(1, most_tiles(a)) * query_tiles(a) * a.cache.kv_heads < (int64_t{1} << 31) / std::max<int64_t>(1, a.batch);
+  return std::max<int64_t>(1, most_tiles(a)) * query_tiles(a) * a.cache.kv_heads < (int64_t{1} << 30) / std::max<int64_t>(1, a.batch);
 }
 
 size_t paged_attention_workspace(const PagedAttentionArgs& a, int cus) {

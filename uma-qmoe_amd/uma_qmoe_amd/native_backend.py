@@ -755,7 +755,8 @@ class HipExtension:
         batch = page_table.size(0)
         key = torch.empty((batch, kv_heads, max_length, head_dim), dtype=self._bf16, device=page_table.device)
         value = torch.empty_like(key)
-        self._launch(self.lib.uqm_kv_read, index, ctypes.byref(desc), batch, page_table.data_ptr(), stride, width, lengths.data_ptr(), max_length, key.data_ptr(), value.data_ptr())
+        self._launch(self.lib.uqm_kv_read, index, ctypes.byref(desc), batch, page_table.data_ptr(), stride, width,
+                     lengths.data_ptr(), max_length, key.data_ptr(), value.data_ptr())
         return key, value
 
     def paged_attention(self, query, cache: KVCache, page_table, lengths, *, scale=None, window=None):
@@ -768,7 +769,8 @@ class HipExtension:
         torch = self.torch
         index, shape = query.get_device(), query.shape
         desc, (_, kv_heads, page_size, head_dim) = self._cache(cache, "paged_attention", index)
-        if query.dtype is not self._bf16 or len(shape) != 3 or shape[2] != head_dim or shape[1] % kv_heads or not shape[1]:
+        if (query.dtype is not self._bf16 or len(shape) != 3 or shape[2] != head_dim or not kv_heads or not shape[1]
+                or shape[1] % kv_heads):
             raise RuntimeError(f"paged_attention requires a BF16 query [batch, heads, {head_dim}] of a multiple of {kv_heads} "
                                f"heads, not {query.dtype} {tuple(shape)}")
         if window is not None and window < 1:
