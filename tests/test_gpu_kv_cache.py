@@ -518,6 +518,69 @@ def test_decode_steps_together(hip_ext, fp8):
         assert a is None or torch.equal(bits(a), bits(b))
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_captured_call_follows_lengths_and_pages(hip_ext, fp8):
+    """One graph, replayed with other lengths, tables and queries in its buffers: other
+    sequences are short, long and empty each time, and lie in other columns."""
+    print(f"[case] captured lengths {fp8}", flush=True)
+    g = gen(22)
+    most = [9000, 700, 4000, 130, 2500]
+    cache, table = filled(g, most, 2, 32, 64, fp8)
+    kv = to(cache)
+    dtable, n32, q = table.to(DEV), torch.zeros(5, dtype=torch.int32, device=DEV), torch.zeros(5, 6, 64, dtype=torch.bfloat16, device=DEV)
+    hip_ext.paged_attention(q, kv, dtable, n32)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hip_ext.paged_attention(q, kv, dtable, n32)
+    for share in ([1, 1, 1, 1, 1], [0, 0, 1, 0.5, 0], [0.01, 1, 0, 0, 0.9], [0, 0, 0, 0, 0], [0.5, 0.3, 0.2, 1, 0.1], [1, 0, 0, 0, 0]):
+        lengths = torch.tensor([int(n * f) for n, f in zip(most, share)], dtype=torch.int32)
+        query = normal(g, 5, 6, 64).to(torch.bfloat16)
+        n32.copy_(lengths)
+        q.copy_(query)
+        graph.replay()
+        want = hip_ext.paged_attention(q, kv, dtable, n32)  # eager work between the replays
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        ref.check_attention(out, query, cache, table, lengths, 0.125)
+
+
+def test_every_code_is_its_value(hip_ext):
+    """Each of the 256 codes as a value, attended to alone, and read back: exact (both NaN codes NaN)."""
+    print("[case] codes", flush=True)
+    codes = torch.arange(256, dtype=torch.int32).to(torch.uint8)
+    cache = hip_ext.new_kv_cache(1, 1, 16, 256, fp8=True, device=DEV)
+    bits(cache.value)[0, 0, 0] = codes.to(DEV)
+    cache.value_scales[0, 0, 0] = 0.5
+    one = torch.ones(1, dtype=torch.int32, device=DEV)
+    out = hip_ext.paged_attention(torch.ones(1, 2, 256, dtype=torch.bfloat16, device=DEV), cache, one.view(1, 1) - 1, one)
+    read = hip_ext.kv_read(cache, one.view(1, 1) - 1, one, 1)[1]
+    want = codes.view(F8).float() * 0.5
+    assert want.isnan().sum() == 2
+    for got in (out[0, 0], out[0, 1], read[0, 0, 0]):
+        assert torch.equal(got.float().cpu().nan_to_num(1e9), want.nan_to_num(1e9))
+
+
+def test_another_stream_than_the_tensors(hip_ext):
+    """Written on one stream, attended to on another one behind it."""
+    print("[case] other stream", flush=True)
+    g = gen(23)
+    rows = [normal(g, 2, 4, 900, 64).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    q = normal(g, 2, 8, 64).to(torch.bfloat16).to(DEV)
+    cache = hip_ext.new_kv_cache(60, 4, 32, 64, fp8=True, device=DEV)
+    table = torch.randperm(60, generator=g)[:58].view(2, 29).to(torch.int32).to(DEV)
+    starts, n32 = torch.zeros(2, dtype=torch.int32, device=DEV), torch.tensor([900, 41], dtype=torch.int32, device=DEV)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        hip_ext.kv_append(cache, *rows, table, starts, n32)
+    streams[1].wait_stream(streams[0])
+    with torch.cuda.stream(streams[1]):
+        out = hip_ext.paged_attention(q, cache, table, n32)
+    torch.cuda.synchronize()
+    ref.check_attention(out, q, to(cache, "cpu"), table, n32, 0.125)
+
+
 def test_calls_on_two_streams_at_once(hip_ext):
     print("[case] two streams", flush=True)
     g = gen(20)

@@ -782,8 +782,13 @@ class HipExtension:
         if not query.is_contiguous() or query.data_ptr() & 15:
             query = query.clone(memory_format=torch.contiguous_format)
         out = torch.empty_like(query)
+        sizes = (batch, heads, kv_heads, head_dim, page_size, width)
+        if torch._C._cuda_getDevice() == index:
+            nbytes = self.lib.uqm_paged_attention_workspace_bytes(*sizes)
+        else:
+            with torch.cuda.device(index):
+                nbytes = self.lib.uqm_paged_attention_workspace_bytes(*sizes)
         # (torch's allocator gives memory in stream order, and a captured graph its own)
-        nbytes = self.lib.uqm_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim, page_size, width)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
         self._launch(self.lib.uqm_paged_attention, index, ctypes.byref(desc), query.data_ptr(), batch, heads,
                      page_table.data_ptr(), stride, width, lengths.data_ptr(),
