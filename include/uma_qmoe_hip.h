@@ -415,7 +415,7 @@ int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t ba
  * device (0: none; host only, without a device for 256 compute units; 0 as well for
  * sizes that the call refuses). */
 size_t uqm_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                           int64_t page_size, int64_t max_pages);
+                                           int64_t page_size, int64_t max_pages, int64_t window);
 
 #ifdef __cplusplus
 }

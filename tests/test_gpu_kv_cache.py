@@ -349,6 +349,13 @@ def test_attention_clamps_lengths(hip_ext):
     attend_case(hip_ext, gen(12), [0, 640, 640, 5], 2, 1, 16, 32, True, given=[-2147483648, 10000, 2147483647, 5])
 
 
+@pytest.mark.parametrize("window", [1, 128, 129, 130, 384, 385, 386, 387, 500])
+def test_windows_over_long_tables(hip_ext, window):
+    """Windows whose tiles are one workgroup's, and the first that are not, at every offset within a tile."""
+    print(f"[case] attention window of a long table {window}", flush=True)
+    attend_case(hip_ext, gen(window), [5000 + 37 * i for i in range(9)] + [0, 1, window, window + 1], 2, 1, 16, 32, True, window=window)
+
+
 @pytest.mark.parametrize("scale", [1.0, -0.3, 0.0, 3.0])
 def test_attention_of_a_scale(hip_ext, scale):
     print(f"[case] attention scale {scale}", flush=True)

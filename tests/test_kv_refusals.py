@@ -121,7 +121,10 @@ def test_no_work(lib):
 
 
 def test_workspace_of_refused_sizes(lib):
-    for sizes in ((-1, 4, 2, 64, 16, 4), (3, 3, 2, 64, 16, 4), (3, 4, 0, 64, 16, 4), (3, 4, 2, 60, 16, 4), (3, 4, 2, 64, 15, 4), (3, 4, 2, 64, 16, -1)):
+    good = (3, 4, 2, 64, 16, 400, 0)
+    assert lib.uqm_paged_attention_workspace_bytes(*good) > 0
+    for i, bad in enumerate((-1, 3, 0, 60, 15, -1, -1)):
+        sizes = (*good[:i], bad, *good[i + 1:])
         assert lib.uqm_paged_attention_workspace_bytes(*sizes) == 0
 
 

@@ -1633,8 +1633,13 @@ static uqm::PagedAttentionArgs attention_sizes(int64_t batch, int64_t heads, int
   a.pages.width = static_cast<int32_t>(max_pages);
   a.batch = batch;
   a.heads = static_cast<int>(heads);
+  a.window = INT32_MAX;
   return a;
 }
+static int check_window(int64_t window) {
+  return window < 0 ? fail(UQM_ERR_ARGUMENT, "paged_attention: window must be at least 1, or 0 for none") : UQM_OK;
+}
+static int32_t window_of(int64_t window) { return static_cast<int32_t>(window > 0 && window < INT32_MAX ? window : INT32_MAX); }
 
 static int check_attention_sizes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                                  int64_t max_pages) {
@@ -1648,12 +1653,14 @@ static int check_attention_sizes(int64_t batch, int64_t heads, int64_t kv_heads,
 }
 
 size_t uqm_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                           int64_t page_size, int64_t max_pages) {
+                                           int64_t page_size, int64_t max_pages, int64_t window) {
   if (check_kv_sizes("paged_attention", 1, kv_heads, page_size, head_dim) ||
       check_page_table("paged_attention", batch, page_size, max_pages, max_pages) ||
-      check_attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages))
+      check_attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages) || check_window(window))
     return 0;
-  return uqm::paged_attention_workspace(attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages), device_cus());
+  uqm::PagedAttentionArgs a = attention_sizes(batch, heads, kv_heads, head_dim, page_size, max_pages);
+  a.window = window_of(window);
+  return uqm::paged_attention_workspace(a, device_cus());
 }
 
 int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t batch, int64_t heads,
@@ -1666,13 +1673,14 @@ int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t ba
       (rc = check_attention_sizes(batch, heads, cache->kv_heads, cache->head_dim, cache->page_size, max_pages)))
     return rc;
   if (!(scale - scale == 0.f)) return fail(UQM_ERR_ARGUMENT, "paged_attention: scale must be finite");
-  if (window < 0) return fail(UQM_ERR_ARGUMENT, "paged_attention: window must be at least 1, or 0 for none");
+  if ((rc = check_window(window))) return rc;
   if (batch == 0) return UQM_OK;
   if (query == nullptr || output == nullptr || lengths == nullptr || (page_table == nullptr && max_pages > 0))
     return fail(UQM_ERR_ARGUMENT, "paged_attention: query, page_table, lengths and output are required");
   if (!aligned16(query) || !aligned16(output) || misaligned(page_table, 4) || misaligned(lengths, 4))
     return fail(UQM_ERR_ARGUMENT, "paged_attention: query and output must be 16-byte aligned, indexes to their elements");
   PagedAttentionArgs a = attention_sizes(batch, heads, cache->kv_heads, cache->head_dim, cache->page_size, max_pages);
+  a.window = window_of(window);
   const int cus = device_cus();
   const int64_t need = static_cast<int64_t>(paged_attention_workspace(a, cus));
   if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < static_cast<size_t>(need)))
@@ -1691,7 +1699,6 @@ int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t ba
   a.pages = {page_table, table_stride, static_cast<int32_t>(max_pages)};
   a.query = static_cast<const uint16_t*>(query);
   a.lengths = lengths;
-  a.window = static_cast<int32_t>(window > 0 && window < INT32_MAX ? window : INT32_MAX);
   a.scale = scale;
   a.out = static_cast<uint16_t*>(output);
   a.workspace = static_cast<float*>(workspace);

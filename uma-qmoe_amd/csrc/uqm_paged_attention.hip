@@ -66,7 +66,8 @@ constexpr int kGroupsPerCu = 2;
 // (10 parts) 12.5 us, by workgroups 15.4; one of 4001 tokens (32) 13.7, by workgroups 12.0.
 constexpr int kFewParts = 16;
 // Up to this many tiles a head is one workgroup's, a tile 1 us: 4 tiles 7.7 us and in
-// parts 8.4; 8 tiles 11.6 and 8.5.
+// parts 8.4; 8 tiles 11.6 and 8.5. (What a compute unit alone can load: with eight waves
+// instead of four on it, 1000 positions 11.8 us.)
 constexpr int kDirectTiles = 4;
 
 __device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
@@ -691,8 +692,10 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-int64_t most_tiles(const PagedAttentionArgs& a) {  // of a sequence, from the table's width alone: lengths are on the device
-  return ((static_cast<int64_t>(a.pages.width) << a.cache.page_log2) + kTile - 1) / kTile;
+// Most tiles of a sequence, from the table's width and the window: lengths are on the device.
+int64_t most_tiles(const PagedAttentionArgs& a) {
+  const int64_t capacity = static_cast<int64_t>(a.pages.width) << a.cache.page_log2, tiles = (capacity + kTile - 1) / kTile;
+  return a.window < capacity ? std::min<int64_t>(tiles, (a.window + kTile - 2) / kTile + 1) : tiles;  // (a window begins anywhere in a tile)
 }
 int query_tiles(const PagedAttentionArgs& a) { return (a.heads / a.cache.kv_heads + 15) / 16; }
 

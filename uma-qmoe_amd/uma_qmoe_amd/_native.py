@@ -162,7 +162,7 @@ SIGNATURES = {
         (ctypes.POINTER(KVCache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, ctypes.c_float, _i64, _vp, _vp,
          ctypes.c_size_t, _vp),
     ),
-    "uqm_paged_attention_workspace_bytes": (ctypes.c_size_t, (_i64, _i64, _i64, _i64, _i64, _i64)),
+    "uqm_paged_attention_workspace_bytes": (ctypes.c_size_t, (_i64,) * 7),
     "uqm_set_option": (ctypes.c_int, (ctypes.c_int, _i64)),
     "uqm_workspace_status": (ctypes.c_int, (_vp, ctypes.c_size_t, _vp)),
     "uqm_noalloc_status": (ctypes.c_int, (_vp,)),

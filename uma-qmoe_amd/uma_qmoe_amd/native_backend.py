@@ -773,8 +773,12 @@ class HipExtension:
                 or shape[1] % kv_heads):
             raise RuntimeError(f"paged_attention requires a BF16 query [batch, heads, {head_dim}] of a multiple of {kv_heads} "
                                f"heads, not {query.dtype} {tuple(shape)}")
-        if window is not None and window < 1:
+        if window is None:
+            window = 0
+        elif window < 1:
             raise RuntimeError("paged_attention requires a window of at least 1")
+        else:
+            window = min(window, 1 << 31)
         batch, heads, _ = shape
         page_table, stride, width, lengths, _ = self._indexes("paged_attention", index, page_table, lengths)
         if page_table.size(0) != batch:
@@ -782,7 +786,7 @@ class HipExtension:
         if not query.is_contiguous() or query.data_ptr() & 15:
             query = query.clone(memory_format=torch.contiguous_format)
         out = torch.empty_like(query)
-        sizes = (batch, heads, kv_heads, head_dim, page_size, width)
+        sizes = (batch, heads, kv_heads, head_dim, page_size, width, window)
         if torch._C._cuda_getDevice() == index:
             nbytes = self.lib.uqm_paged_attention_workspace_bytes(*sizes)
         else:
@@ -792,7 +796,7 @@ class HipExtension:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
         self._launch(self.lib.uqm_paged_attention, index, ctypes.byref(desc), query.data_ptr(), batch, heads,
                      page_table.data_ptr(), stride, width, lengths.data_ptr(),
-                     head_dim ** -0.5 if scale is None else scale, 0 if window is None else min(window, 1 << 31), out.data_ptr(),
+                     head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
                      None if workspace is None else workspace.data_ptr(), nbytes)
         return out
 
