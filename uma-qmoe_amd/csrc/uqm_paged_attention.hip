@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
 }
 constexpr uint32_t kOutside = 0x80000000u;  // an offset behind every buffer's bytes
-constexpr int kOnce = 2;                    // a load whose lines are not kept (nontemporal): 131071 tokens 94 us, kept 106
+constexpr int kOnce = 2;                    // a load whose lines are not kept (nontemporal)
 template <int HINT>
 __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t buf, uint32_t at) {
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buf, at, 0, HINT));
@@ -257,6 +257,12 @@ __global__ __launch_bounds__(kThreads, DP == 256 && !FP8 ? 1 : DP == 256 || !FP8
   constexpr int kStep = FP8 ? 64 : 32;     // dimensions of one load of 16 keys
   constexpr int kLoads = DP / kStep;
   constexpr int kVWords = FP8 ? kVec / 4 : kVec / 2;
+  // Lines that another load of the same rows takes a part of are kept: 8-bit keys (two
+  // loads to a line; 64 sequences 310 us, not kept 328), keys of rows that do not begin
+  // with a line (heads of 80 in BF16 130 and 148), values of 32 bytes a lane (heads of
+  // 256 in BF16 411 and 435). BF16 keys, two loads to a line as well, are faster not kept
+  // all the same (131071 tokens 94 us, kept 97).
+  constexpr int kKeyHint = FP8 || PAD ? 0 : kOnce, kValueHint = kVWords > 4 ? 0 : kOnce;
   constexpr int kRowStride = DP + 4;       // (rows of the join four banks apart)
   constexpr bool kSharedQuery = DP == 256;  // (there are no registers for them beside keys and values on their way)
   __shared__ uint4 shared_query[kSharedQuery ? DP / 32 : 1][64];
@@ -312,11 +318,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 && !FP8 ? 1 : DP == 256 || !FP8
       const int64_t place = place_of(u, s, page[s]);
       const int32_t seen = seen_of(u, s, page[s]);
       const auto buf = stage_buffer(static_cast<const uint8_t*>(kv.key) + place * row_bytes, seen * row_bytes);
-      // (a load of 8-bit keys takes half of 16 lines, the next one the other half:
-      // these are kept, 310 us against 328 for 64 sequences of 16 heads)
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        k[s][i] = load16<FP8 ? 0 : kOnce>(buf, (!PAD || i * kStep + g * (kStep / 4) < dim ? key_at : kOutside) + 64 * i);
+        k[s][i] = load16<kKeyHint>(buf, (!PAD || i * kStep + g * (kStep / 4) < dim ? key_at : kOutside) + 64 * i);
       if constexpr (FP8) ks[s] = as_float4(load16<0>(stage_buffer(kv.key_scales + place, seen > 0 ? 64 : 0), 16u * g));
     }
   };
@@ -330,14 +334,14 @@ __global__ __launch_bounds__(kThreads, DP == 256 && !FP8 ? 1 : DP == 256 || !FP8
       for (int r = 0; r < 4; ++r) {
         const uint32_t at = value_at + r * row_bytes;
         if constexpr (kVWords == 1) {
-          v[s][r][0] = __builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, kOnce);
+          v[s][r][0] = __builtin_amdgcn_raw_buffer_load_b32(buf, at, 0, kValueHint);
         } else if constexpr (kVWords == 2) {
-          const auto w = __builtin_amdgcn_raw_buffer_load_b64(buf, at, 0, kOnce);
+          const auto w = __builtin_amdgcn_raw_buffer_load_b64(buf, at, 0, kValueHint);
           v[s][r][0] = w[0], v[s][r][1] = w[1];
         } else {
 #pragma unroll
           for (int i = 0; i < kVWords / 4; ++i) {
-            const uint4 w = load16<kOnce>(buf, at + 16 * i);
+            const uint4 w = load16<kValueHint>(buf, at + 16 * i);
             v[s][r][4 * i] = w.x, v[s][r][4 * i + 1] = w.y, v[s][r][4 * i + 2] = w.z, v[s][r][4 * i + 3] = w.w;
           }
         }
