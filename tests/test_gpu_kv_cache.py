@@ -356,6 +356,19 @@ def test_windows_over_long_tables(hip_ext, window):
     attend_case(hip_ext, gen(window), [5000 + 37 * i for i in range(9)] + [0, 1, window, window + 1], 2, 1, 16, 32, True, window=window)
 
 
+@pytest.mark.parametrize("window", [None, 896, 897, 898, 899])
+@pytest.mark.parametrize("width", [64, 65])  # pages of 16: eight tiles, and the first page of a ninth
+@pytest.mark.parametrize("batch,heads,kv_heads", [(7, 16, 16), (9, 16, 16), (18, 40, 4)])
+def test_tables_of_eight_tiles(hip_ext, batch, heads, kv_heads, width, window):
+    """Sequences of up to eight tiles are one workgroup's a head where there are many of them;
+    fewer sequences, one page more and longer windows are in parts."""
+    print(f"[case] attention eight tiles {batch} {heads} {kv_heads} {width} {window}", flush=True)
+    most = 16 * width
+    lengths = ([most, 0, 1, most - 1, 513, 640, 897] * 3)[:batch]
+    lengths[-1] = 1023
+    attend_case(hip_ext, gen(width + batch), lengths, heads, kv_heads, 16, 32, batch % 2 == 0, window=window, width=width + (0 if window is None else 300))
+
+
 @pytest.mark.parametrize("scale", [1.0, -0.3, 0.0, 3.0])
 def test_attention_of_a_scale(hip_ext, scale):
     print(f"[case] attention scale {scale}", flush=True)

@@ -44,9 +44,10 @@
 // sequences), and a second launch joins these. Keys, values and queries of the next tile
 // are on their way while one is computed, also across the end of a sequence (255
 // sequences of 50 to 150 tokens 41 us, with a start of its own for each 50).
-// Where no sequence can have more than four tiles a workgroup takes a sequence's head,
-// without that bookkeeping and without a second launch (one token over 77 positions, 16
-// heads, 4.5 us in a graph; 5.2 with the bookkeeping).
+// Where no sequence can have more than four tiles (eight, where there are workgroups for
+// half of the compute units all the same) a workgroup takes a sequence's head, without
+// that bookkeeping and without a second launch (one token over 77 positions, 16 heads,
+// 4.5 us in a graph; 5.2 with the bookkeeping).
 #include "uqm_device.h"
 #include "uqm_kv.h"
 #include "uqm_stage.h"
@@ -69,6 +70,15 @@ constexpr int kFewParts = 16;
 // parts 8.4; 8 tiles 11.6 and 8.5. (What a compute unit alone can load: with eight waves
 // instead of four on it, 1000 positions 11.8 us.)
 constexpr int kDirectTiles = 4;
+// The same where that makes a workgroup for half of the compute units or more, so that
+// parts would only add their joins. Heads of 128, sequences of 10 to 100% and of 90 to
+// 100% of six tiles, whole and in parts: 32 of 28 heads on 4 in e4m3 10.1 and 10.6 us, in
+// parts 12.5 and 15.7; 8 of 16 heads in BF16 14.5 and 14.9, in parts 13.0 and 16.9. Of
+// eight tiles: 12.2 and 12.7 against 15.4 and 15.2; 18.1 and 19.0 against 16.9 and 17.9;
+// 64 of 16 heads in BF16 64.8 and 89.5 against 57.8 and 92.2. Heads of 64: a quarter less
+// than in parts on average. Of 16 tiles the longest sequence is waited for: 32 of 32
+// heads on 8 in BF16 37.2 and 49.4, in parts 32.6 and 55.2.
+constexpr int kManyDirectTiles = 8;
 
 __device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -708,7 +718,8 @@ Plan plan_of(const PagedAttentionArgs& a, int cus) {
   const int group = a.heads / a.cache.kv_heads;
   p.query_tiles = query_tiles(a);
   p.query_rows = (group + p.query_tiles - 1) / p.query_tiles;
-  p.whole = most_tiles(a) <= kDirectTiles;
+  const bool many = 2 * static_cast<int64_t>(a.batch) * a.cache.kv_heads * p.query_tiles >= cus;
+  p.whole = most_tiles(a) <= (many ? kManyDirectTiles : kDirectTiles);
   const int64_t wanted = std::max<int64_t>(1, static_cast<int64_t>(kGroupsPerCu) * cus / (a.cache.kv_heads * p.query_tiles));
   p.columns = static_cast<int32_t>(p.whole ? a.batch : std::min(a.batch * most_tiles(a), wanted));
   return p;
