@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+import functools
 import hashlib
 from pathlib import Path
 import threading
@@ -43,6 +44,16 @@ FP8_GROUP = 128  # columns (and, for weights, rows) that share a scale of an Fp8
 
 _EXTENSIONS: dict[str, Any] = {}
 _BUILD_LOCK = threading.Lock()
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_attention_workspace_bytes(index: int, *sizes: int) -> int:
+    """What a call of these sizes needs on device ``index`` (0 for sizes that are
+    refused). It depends on nothing else; asking anew costs 0.6 of a call's 10 us."""
+    import torch
+
+    with torch.cuda.device(index):
+        return _native.library().uqm_paged_attention_workspace_bytes(*sizes)
 
 
 def native_kernel_source_sha256() -> str:
@@ -753,7 +764,7 @@ class HipExtension:
         if not 0 <= max_length * kv_heads < 1 << 31:
             raise RuntimeError("kv_read requires max_length * kv_heads in [0, 2^31)")
         batch = page_table.size(0)
-        key = torch.empty((batch, kv_heads, max_length, head_dim), dtype=self._bf16, device=page_table.device)
+        key = page_table.new_empty((batch, kv_heads, max_length, head_dim), dtype=self._bf16)
         value = torch.empty_like(key)
         self._launch(self.lib.uqm_kv_read, index, ctypes.byref(desc), batch, page_table.data_ptr(), stride, width,
                      lengths.data_ptr(), max_length, key.data_ptr(), value.data_ptr())
@@ -786,12 +797,7 @@ class HipExtension:
         if not query.is_contiguous() or query.data_ptr() & 15:
             query = query.clone(memory_format=torch.contiguous_format)
         out = torch.empty_like(query)
-        sizes = (batch, heads, kv_heads, head_dim, page_size, width, window)
-        if torch._C._cuda_getDevice() == index:
-            nbytes = self.lib.uqm_paged_attention_workspace_bytes(*sizes)
-        else:
-            with torch.cuda.device(index):
-                nbytes = self.lib.uqm_paged_attention_workspace_bytes(*sizes)
+        nbytes = _paged_attention_workspace_bytes(index, batch, heads, kv_heads, head_dim, page_size, width, window)
         # (torch's allocator gives memory in stream order, and a captured graph its own)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
         self._launch(self.lib.uqm_paged_attention, index, ctypes.byref(desc), query.data_ptr(), batch, heads,
