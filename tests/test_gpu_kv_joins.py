@@ -1,0 +1,129 @@
+"""What the attention over a paged cache puts together from its parts (waves of a
+workgroup, workgroups of a sequence): values that are not finite stay in the result
+however small their part's weight is."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import kv_reference as ref
+from test_gpu_kv_cache import bits, filled, gen, to
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+INF, NAN = float("inf"), float("nan")
+TILE, WAVE = 128, 32  # positions that a workgroup, and a wave of it, take at a time
+
+
+def places(cache, table, b, positions):
+    p = torch.as_tensor(positions)
+    return table[b, p // cache.key.shape[2]].long(), p % cache.key.shape[2]
+
+
+def scored(g, lengths, heads, kv_heads, dim, fp8, scores):
+    """A cache, a table and queries whose scores at scale 1 are those of ``scores``
+    ({sequence: [length]}): the queries' first dimension is 1 and a key is its score
+    there and 0 elsewhere."""
+    cache, table = filled(g, lengths, kv_heads, 16, dim, fp8)
+    for b, s in scores.items():
+        page, slot = places(cache, table, b, range(lengths[b]))
+        bits(cache.key)[page, :, slot] = 0
+        if fp8:
+            bits(cache.key)[page, :, slot, 0] = torch.where(s < 0, 0xB8, 0x38).to(torch.uint8)[:, None]  # -1, 1
+            cache.key_scales[page, :, slot] = s.abs()[:, None]
+        else:
+            cache.key[page, :, slot, 0] = s.to(torch.bfloat16)[:, None]
+    q = torch.zeros(len(lengths), heads, dim, dtype=torch.bfloat16)
+    q[:, :, 0] = 1
+    return cache, table, q
+
+
+def attend(ext, cache, table, q, lengths):
+    n32 = torch.tensor(lengths, dtype=torch.int32)
+    out = ext.paged_attention(q.to(DEV), to(cache), table.to(DEV), n32.to(DEV), scale=1.0)
+    torch.cuda.synchronize()
+    return out.float().cpu()
+
+
+# One workgroup's; in parts that a wave joins, and that a workgroup joins.
+SPREAD = {"whole": 500, "few": 1300, "many": 20000}
+
+
+@pytest.mark.parametrize("heads", [2, 24])  # one product a weight, and two
+@pytest.mark.parametrize("dim", [64, 128, 192])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("spread", list(SPREAD))
+@pytest.mark.parametrize("low", [WAVE, TILE])  # positions whose scores are far below all others'
+def test_what_is_not_finite_stays(hip_ext, spread, low, fp8, dim, heads):
+    """A NaN key, a NaN value, an infinite value, and a NaN value behind a score of -inf,
+    at a position whose neighbours' scores lie 200 below all others (a factor that
+    underflows to 0)."""
+    print(f"[case] not finite {spread} {low} {fp8} {dim} {heads}", flush=True)
+    n = SPREAD[spread]
+    at = 2 * TILE + 2 * WAVE + 5
+    first = at // low * low
+    s = torch.zeros(n)
+    s[first:first + low] = -200.0
+    cache, table, q = scored(gen(dim), [n, 40], heads, 2, dim, fp8, {0: s, 1: torch.zeros(40)})
+    page, slot = places(cache, table, 0, [at])
+
+    def with_(fill, value, score=None):
+        k = to(cache, "cpu")._replace(**{f: getattr(cache, f).clone() for f in ("key", "value")},
+                                      **({f: getattr(cache, f).clone() for f in ("key_scales", "value_scales")} if fp8 else {}))
+        if score is not None:
+            if fp8:
+                k.key_scales[page, :, slot] = abs(score)  # (the code is -1)
+            else:
+                k.key[page, :, slot, 0] = score
+        if fill == "key":
+            (k.key_scales if fp8 else k.key)[page, :, slot] = value
+        elif fp8 and value != value:
+            bits(k.value)[page, :, slot, 3] = 0x7F
+        elif fp8:
+            k.value_scales[page, :, slot] = value
+        else:
+            k.value[page, :, slot, 3] = value
+        out = attend(hip_ext, k, table, q, [n, 40])
+        assert out[1].isfinite().all()
+        return out[0]
+
+    assert attend(hip_ext, cache, table, q, [n, 40]).isfinite().all()
+    assert with_("key", NAN).isnan().all()
+    for score in (None, -INF):
+        got = with_("value", NAN, score)
+        assert got[:, 3].isnan().all() and got[:, 4:].isfinite().all()
+    got = with_("value", INF)
+    assert not got[:, 3].isfinite().any() and (fp8 or got[:, 4:].isfinite().all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", [100, 3 * TILE + 4, 10 * TILE + 4, 156 * TILE + 4])
+def test_a_part_of_nothing_but_nan(hip_ext, n, fp8):
+    """The last four positions, which are their wave's only ones, have NaN keys; all
+    other scores are 200 (a part without a finite score counts as one whose maximum is 0)."""
+    print(f"[case] nan part {n} {fp8}", flush=True)
+    cache, table, q = scored(gen(n), [n, 40], 4, 2, 64, fp8, {0: torch.full((n,), 200.0), 1: torch.zeros(40)})
+    page, slot = places(cache, table, 0, range(n - 4, n))
+    (cache.key_scales if fp8 else cache.key)[page, :, slot] = NAN
+    got = attend(hip_ext, cache, table, q, [n, 40])
+    assert got[0].isnan().all() and got[1].isfinite().all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", [100, 3 * TILE + 4, 10 * TILE + 4, 156 * TILE + 4])
+def test_a_part_of_scores_without_weight(hip_ext, n, fp8):
+    """Scores of -inf in a part of their own take no weight, and a sequence of nothing else is NaN."""
+    print(f"[case] -inf part {n} {fp8}", flush=True)
+    s = torch.zeros(n)
+    s[n - 4:] = -INF
+    cache, table, q = scored(gen(n), [n, 40], 4, 2, 64, fp8, {0: s, 1: torch.full((40,), -INF)})
+    if not fp8:  # (a query's 0 times an infinity would be a NaN; here only the first dimension is one)
+        assert cache.key[..., 1:].isinf().sum() == 0
+    got = attend(hip_ext, cache, table, q, [n, 40])
+    assert got[1].isnan().all()
+    v, _ = ref.position_rows(cache.value, cache.value_scales, table[0], torch.arange(n - 4))
+    want = v.mean(0).repeat_interleave(2, 0)
+    # (n FP32 sums and the two numbers of a weight beside the output's rounding)
+    off = (2.0 ** -16 + 4 * n * ref.U) * v.abs().mean(0).repeat_interleave(2, 0)
+    assert ((got[0].double() - want).abs() <= off * (1 + ref.BF16) + ref.BF16 * want.abs()).all()

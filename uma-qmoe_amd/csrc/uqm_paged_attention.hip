@@ -251,13 +251,18 @@ struct Share {
   }
 };
 
-// A workgroup's part of a row: weights relative to 2^most, their sum, the sum of
-// weighted values. most is -inf for a part that saw nothing (sum 0) and for one all
-// of whose scores were -inf (sum NaN: 0 / 0 unless other parts have finite scores).
+// A part of a row, a wave's or a workgroup's: weights relative to 2^most, their sum, the
+// sum of weighted values. most is -inf for a part that saw nothing (sum 0, values 0) and
+// for one all of whose scores were -inf (sum NaN: 0 / 0 unless other parts have finite
+// scores). A factor that underflows to 0 multiplies like any other, so that a NaN or an
+// infinity of a part far below the others stays one, as it does within a wave.
 __device__ __forceinline__ float part_factor(float most, float all) {
   return most == -INFINITY ? (all == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(most - all);
 }
-__device__ __forceinline__ float weighted(float f, float v) { return f == 0.0f ? 0.0f : f * v; }
+// A part's sum relative to 2^all, f its factor: what has no weight is left out.
+__device__ __forceinline__ float part_sum(float most, float all, float f, float sum) {
+  return most == -INFINITY && all != -INFINITY ? 0.0f : f * sum;
+}
 
 // (registers for one, two or three workgroups a compute unit, so that none spills)
 template <int DP, bool FP8, bool DUP, bool PAD, bool WHOLE>
@@ -578,8 +583,8 @@ __global__ __launch_bounds__(kThreads, DP == 256 && !FP8 ? 1 : DP == 256 || !FP8
         for (int w = 0; w < kWaves; ++w) {
           const float f = part_factor(part_m[w][r], all);
           const float4 y = *reinterpret_cast<const float4*>(&part_o[w][r][c]);
-          sum += weighted(f, part_l[w][r]);
-          acc.x += weighted(f, y.x), acc.y += weighted(f, y.y), acc.z += weighted(f, y.z), acc.w += weighted(f, y.w);
+          sum += part_sum(part_m[w][r], all, f, part_l[w][r]);
+          acc.x += f * y.x, acc.y += f * y.y, acc.z += f * y.z, acc.w += f * y.w;
         }
         if (complete) {
           if (!PAD || c < dim) {
@@ -615,12 +620,9 @@ struct Joined {
 };
 __device__ __forceinline__ void join(Joined& x, float most, float sum, const float4& acc) {
   const float all = fmaxf(x.most, most), f = part_factor(x.most, all), h = part_factor(most, all);
+  x.sum = part_sum(x.most, all, f, x.sum) + part_sum(most, all, h, sum);
+  x.acc = make_float4(f * x.acc.x + h * acc.x, f * x.acc.y + h * acc.y, f * x.acc.z + h * acc.z, f * x.acc.w + h * acc.w);
   x.most = all;
-  x.sum = weighted(f, x.sum) + weighted(h, sum);
-  x.acc.x = weighted(f, x.acc.x) + weighted(h, acc.x);
-  x.acc.y = weighted(f, x.acc.y) + weighted(h, acc.y);
-  x.acc.z = weighted(f, x.acc.z) + weighted(h, acc.z);
-  x.acc.w = weighted(f, x.acc.w) + weighted(h, acc.w);
 }
 template <int O>
 __device__ __forceinline__ float lane_xor(float v) {  // (xor_partner<8> would be lane ^ 15)
@@ -669,22 +671,23 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
       const float* part = a.workspace + (2 * (at * heads + index) + (at == w0 ? first_place : 0)) * stride;
       const float2 ml = *reinterpret_cast<const float2*>(part + rows * DP + 2 * row);
       y[i] = *reinterpret_cast<const float4*>(part + row * DP + c);
-      const bool there = w + i * kSets <= w1;
+      const bool there = w + i * kSets <= w1;  // (else a part that saw nothing)
       most[i] = there ? ml.x : -INFINITY;
       sum[i] = there ? ml.y : 0.f;
+      y[i] = there ? y[i] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float all = x.most;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) all = fmaxf(all, most[i]);
     const float f = part_factor(x.most, all);
+    x.sum = part_sum(x.most, all, f, x.sum);
+    x.acc = make_float4(f * x.acc.x, f * x.acc.y, f * x.acc.z, f * x.acc.w);
     x.most = all;
-    x.sum = weighted(f, x.sum);
-    x.acc = make_float4(weighted(f, x.acc.x), weighted(f, x.acc.y), weighted(f, x.acc.z), weighted(f, x.acc.w));
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const float h = w + i * kSets <= w1 ? part_factor(most[i], all) : 0.f;
-      x.sum += weighted(h, sum[i]);
-      x.acc.x += weighted(h, y[i].x), x.acc.y += weighted(h, y[i].y), x.acc.z += weighted(h, y[i].z), x.acc.w += weighted(h, y[i].w);
+      const float h = part_factor(most[i], all);
+      x.sum += part_sum(most[i], all, h, sum[i]);
+      x.acc.x += h * y[i].x, x.acc.y += h * y[i].y, x.acc.z += h * y[i].z, x.acc.w += h * y[i].w;
     }
   }
   if constexpr (kLanes <= 8) join_lanes<8>(x);
