@@ -54,7 +54,7 @@ SPREAD = {"whole": 500, "few": 1300, "many": 20000}
 @pytest.mark.parametrize("dim", [64, 128, 192])
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("spread", list(SPREAD))
-@pytest.mark.parametrize("low", [WAVE, TILE])  # positions whose scores are far below all others'
+@pytest.mark.parametrize("low", [WAVE, TILE])  # whose scores are far below all others': a wave's of every tile, a tile's
 def test_what_is_not_finite_stays(hip_ext, spread, low, fp8, dim, heads):
     """A NaN key, a NaN value, an infinite value, and a NaN value behind a score of -inf,
     at a position whose neighbours' scores lie 200 below all others (a factor that
@@ -62,9 +62,8 @@ def test_what_is_not_finite_stays(hip_ext, spread, low, fp8, dim, heads):
     print(f"[case] not finite {spread} {low} {fp8} {dim} {heads}", flush=True)
     n = SPREAD[spread]
     at = 2 * TILE + 2 * WAVE + 5
-    first = at // low * low
-    s = torch.zeros(n)
-    s[first:first + low] = -200.0
+    p = torch.arange(n)
+    s = torch.where(p // TILE == at // TILE if low == TILE else p % TILE // WAVE == at % TILE // WAVE, -200.0, 0.0)
     cache, table, q = scored(gen(dim), [n, 40], heads, 2, dim, fp8, {0: s, 1: torch.zeros(40)})
     page, slot = places(cache, table, 0, [at])
 
