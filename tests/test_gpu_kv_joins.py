@@ -1,6 +1,6 @@
 """What the attention over a paged cache puts together from its parts (waves of a
 workgroup, workgroups of a sequence): values that are not finite stay in the result
-however small their part's weight is."""
+however small their part's weight is, and no part is lost or counted twice."""
 
 from __future__ import annotations
 
@@ -126,3 +126,50 @@ def test_a_part_of_scores_without_weight(hip_ext, n, fp8):
     # (n FP32 sums and the two numbers of a weight beside the output's rounding)
     off = (2.0 ** -16 + 4 * n * ref.U) * v.abs().mean(0).repeat_interleave(2, 0)
     assert ((got[0].double() - want).abs() <= off * (1 + ref.BF16) + ref.BF16 * want.abs()).all()
+
+
+# Lengths that go over columns of one and of several tiles, joins by waves and by
+# workgroups, more sequences than columns.
+MARKED = [
+    (4, 4, 128, [20000], None), (8, 1, 64, [40001], None), (2, 1, 256, [9999, 3], None), (16, 4, 128, [1, 0, 8191, 30, 4097], None),
+    (3, 3, 80, [1000 + 37 * i for i in range(70)], None), (32, 2, 96, [5000, 77], None), (1, 1, 64, [65001], None),
+    (1, 1, 256, [131071], None), (20, 1, 128, [60001, 700], None), (4, 2, 64, [300 * i for i in range(17)], None),
+    (16, 16, 48, [(211 * i) % 1500 for i in range(40)], None), (2, 1, 64, [9000, 700, 20001], 5003),
+    (6, 2, 96, [(977 * i) % 4000 for i in range(33)], 1234),
+]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths,window", MARKED)
+def test_every_position_counts_once(hip_ext, heads, kv_heads, dim, lengths, window, fp8):
+    """Queries of 0 weigh all positions alike, and the values of 16 positions are 1 in one
+    dimension, which goes by their place, sequence and head. An output is then the part of
+    the positions that mark its dimension: whole numbers below 2^24 are exact in FP32, so
+    that the quotient is off by the reciprocal's, the product's and the output's rounding.
+    Sixteen positions lost or doubled change it by dim / (positions / 16), four such
+    roundings or more."""
+    print(f"[case] marks {heads} {kv_heads} {dim} {lengths[:5]} {window} {fp8}", flush=True)
+    longest = max(min(n, window or n) for n in lengths)
+    assert 16 * dim >= 4 * ref.BF16 * longest
+    g = gen(dim + heads)
+    cache, table = filled(g, lengths, kv_heads, 16, dim, fp8)
+    want = torch.zeros(len(lengths), kv_heads, dim, dtype=torch.float64)
+    for b, n in enumerate(lengths):
+        if n == 0:
+            continue
+        p = torch.arange(n)
+        mark = (p[:, None] // 16 + 7 * b + 3 * torch.arange(kv_heads)) % dim  # [positions, kv_heads]
+        rows = torch.nn.functional.one_hot(mark, dim)
+        page, slot = places(cache, table, b, p)
+        if fp8:
+            bits(cache.value)[page, :, slot] = (0x38 * rows).to(torch.uint8)
+            cache.value_scales[page, :, slot] = 0.5
+        else:
+            cache.value[page, :, slot] = (0.5 * rows).to(torch.bfloat16)
+        first = max(0, n - window) if window else 0
+        want[b] = rows[first:].sum(0).double() / (2 * (n - first))
+    n32 = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    q = torch.zeros(len(lengths), heads, dim, dtype=torch.bfloat16, device=DEV)
+    got = hip_ext.paged_attention(q, to(cache), table.to(DEV), n32, window=window).double().cpu()
+    want = want.repeat_interleave(heads // kv_heads, 1)
+    assert ((got - want).abs() <= (ref.BF16 + 4 * ref.U) * want).all()
