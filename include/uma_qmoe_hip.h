@@ -397,8 +397,10 @@ int uqm_kv_read(const uqm_kv_cache* cache, int64_t batch, const int32_t* page_ta
  * the new token's own key and value are in the cache already, at lengths[b] - 1).
  * Zeros where no position is seen. query bf16 [batch, heads, head_dim], heads a
  * multiple of kv_heads, both 16-byte aligned; batch * heads below 2^24.
- * What places hold that are not seen has no influence, NaN and infinities neither;
- * a seen NaN gives NaN, a seen infinity NaN or an infinity. Sums are in FP32; of
+ * What places hold that are not seen has no influence, NaN and infinities neither.
+ * Of those seen, however little they weigh: a score of NaN or +inf gives NaN, one of
+ * -inf takes no weight (NaN where every seen score is -inf), a NaN value gives NaN and
+ * an infinite one NaN or an infinity, each in its dimension. Sums are in FP32; of
  * which parts they are joined goes by the table's width and all lengths of the
  * call, so that a result may differ in its last bit between calls that differ in
  * these. batch * kv_heads * ceil(heads / kv_heads / 16) * ceil(max_pages * page_size

@@ -128,11 +128,24 @@ def test_a_part_of_scores_without_weight(hip_ext, n, fp8):
     assert ((got[0].double() - want).abs() <= off * (1 + ref.BF16) + ref.BF16 * want.abs()).all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", [100, 3 * TILE + 4, 10 * TILE + 4, 156 * TILE + 4])
+def test_an_infinite_score(hip_ext, n, fp8):
+    """One score of +inf: NaN (inf - inf), wherever it lies."""
+    print(f"[case] +inf {n} {fp8}", flush=True)
+    for at in (0, n // 2, n - 1):
+        s = torch.zeros(n)
+        s[at] = INF
+        cache, table, q = scored(gen(n), [n, 40], 4, 2, 64, fp8, {0: s, 1: torch.zeros(40)})
+        got = attend(hip_ext, cache, table, q, [n, 40])
+        assert got[0].isnan().all() and got[1].isfinite().all()
+
+
 # Lengths that go over columns of one and of several tiles, joins by waves and by
 # workgroups, more sequences than columns.
 MARKED = [
     (4, 4, 128, [20000], None), (8, 1, 64, [40001], None), (2, 1, 256, [9999, 3], None), (16, 4, 128, [1, 0, 8191, 30, 4097], None),
-    (3, 3, 80, [1000 + 37 * i for i in range(70)], None), (32, 2, 96, [5000, 77], None), (1, 1, 64, [65001], None),
+    (3, 3, 80, [1000 + 38 * i for i in range(70)], None), (32, 2, 96, [5000, 77], None), (1, 1, 64, [65001], None),
     (1, 1, 256, [131071], None), (20, 1, 128, [60001, 700], None), (4, 2, 64, [300 * i for i in range(17)], None),
     (16, 16, 48, [(211 * i) % 1500 for i in range(40)], None), (2, 1, 64, [9000, 700, 20001], 5003),
     (6, 2, 96, [(977 * i) % 4000 for i in range(33)], 1234),
