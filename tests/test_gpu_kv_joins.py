@@ -141,6 +141,47 @@ def test_an_infinite_score(hip_ext, n, fp8):
         assert got[0].isnan().all() and got[1].isfinite().all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads", [32, 36])
+def test_what_is_not_finite_stays_among_many_sequences(hip_ext, heads, fp8):
+    """The same where parts are joined column by column (more heads than the card has waves)."""
+    print(f"[case] not finite, columns {heads} {fp8}", flush=True)
+    n, at, lengths = 3000, 1500, [40] * 150 + [3000] + [40] * 150
+    s = torch.where(torch.arange(n) // TILE == at // TILE, -200.0, 0.0)
+    zeros = {b: torch.zeros(m) for b, m in enumerate(lengths)}
+    for fill, where in (("key", (0,)), ("value", (3,))):
+        cache, table, q = scored(gen(heads), lengths, heads, 2, 64, fp8, {**zeros, 150: s})
+        page, slot = places(cache, table, 150, [at])
+        if fp8:
+            bits(getattr(cache, fill))[page, :, slot, where[0]] = 0x7F
+        else:
+            getattr(cache, fill)[page, :, slot, where[0]] = NAN
+        got = attend(hip_ext, cache, table, q, lengths)
+        assert got[150, :, 3].isnan().all() and got[150, :, 4:].isnan().all().item() == (fill == "key")
+        assert got[:150].isfinite().all() and got[151:].isfinite().all()
+
+
+def test_many_sequences_cost_no_more_each(hip_ext):
+    """Four times as many sequences in a wide table take some four times as long, not sixteen."""
+    print("[case] cost of many sequences", flush=True)
+    cache = hip_ext.new_kv_cache(8, 1, 16, 64, device=DEV)
+    took = []
+    for batch in (16384, 65536):
+        table = torch.arange(72, dtype=torch.int32, device=DEV).remainder(8).expand(batch, -1).contiguous()
+        lengths = torch.full((batch,), 50, dtype=torch.int32, device=DEV)
+        query = torch.ones(batch, 8, 64, dtype=torch.bfloat16, device=DEV)
+        times = []
+        for _ in range(4):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            hip_ext.paged_attention(query, cache, table, lengths)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        took.append(min(times))
+    assert took[1] < 8 * took[0], took
+
+
 # Lengths that go over columns of one and of several tiles, joins by waves and by
 # workgroups, more sequences than columns.
 MARKED = [
@@ -149,6 +190,10 @@ MARKED = [
     (1, 1, 256, [131071], None), (20, 1, 128, [60001, 700], None), (4, 2, 64, [300 * i for i in range(17)], None),
     (16, 16, 48, [(211 * i) % 1500 for i in range(40)], None), (2, 1, 64, [9000, 700, 20001], 5003),
     (6, 2, 96, [(977 * i) % 4000 for i in range(33)], 1234),
+    # (more heads than waves: joined column by column)
+    (64, 4, 64, [(211 * i) % 1500 for i in range(140)], None), (40, 40, 16, [(101 * i) % 1100 for i in range(220)], None),
+    (160, 10, 80, [0] * 30 + [20000] + [5] * 30 + [1], None), (256, 16, 144, [900] * 17 + [7000] * 17, 3000),
+    (288, 288, 16, [1500, 0, 30] * 10, None),
 ]
 
 

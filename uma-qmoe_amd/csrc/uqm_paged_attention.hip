@@ -66,6 +66,7 @@ constexpr int kGroupsPerCu = 2;
 // Up to this many parts a sequence on average a wave joins those of a head: 13 sequences
 // (10 parts) 12.5 us, by workgroups 15.4; one of 4001 tokens (32) 13.7, by workgroups 12.0.
 constexpr int kFewParts = 16;
+constexpr int kWavesPerCu = 32;  // that there is room for
 // Up to this many tiles a head is one workgroup's, a tile 1 us: 4 tiles 7.7 us and in
 // parts 8.4; 8 tiles 11.6 and 8.5. (What a compute unit alone can load: with eight waves
 // instead of four on it, 1000 positions 11.8 us.)
@@ -636,26 +637,50 @@ __device__ __forceinline__ void join_lanes(Joined& x) {
   join(x, most, sum, make_float4(lane_xor<O>(x.acc.x), lane_xor<O>(x.acc.y), lane_xor<O>(x.acc.z), lane_xor<O>(x.acc.w)));
 }
 
-// Joins the parts of query heads. Of few parts (FEW) a wave has a head, four
-// dimensions a lane; of many a workgroup has 32 dimensions of a head, and 32 sets of
-// 8 lanes share the parts (8 heads of 128 in 512 parts: 5.4 us, with a workgroup a head
-// 12; 4096 heads in 2 to 3 parts: 5.5 us with a wave a head, with a workgroup 10).
-template <int DP, bool FEW>
+// Joins the parts of query heads. Of few parts a wave has a head, four dimensions a lane;
+// of many (kMany) a workgroup has 32 dimensions of a head, and 32 sets of 8 lanes share the
+// parts (8 heads of 128 in 512 parts: 5.4 us, with a workgroup a head 12; 4096 heads in 2 to
+// 3 parts: 5.5 us with a wave a head, with a workgroup 10).
+// More heads than the card has room for waves (kColumns): a wave has a head of the sequence
+// that a column begins within, where that is the sequence's second one, since a wave for each
+// head of each sequence goes through all lengths as many times as there are sequences. Calls
+// of 50 positions in wide tables: 65536 sequences of 8 heads 1.3 ms, a wave a head 14.4; 4096
+// of 16 heads 93 us and 187; 300 of 28 heads 35.5 and 37.0. Below that a wave a head: 4096 of
+// one head 60 us, by columns 71.
+enum class Join { kFew, kMany, kColumns };
+template <int DP, Join JOIN>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs a, Plan plan) {
+  constexpr bool FEW = JOIN != Join::kMany;
   constexpr int kSpan = FEW ? DP : 32, kLanes = kSpan / 4, kSets = (FEW ? 64 : kThreads) / kLanes;
   constexpr int kSpans = DP / kSpan, kAtOnce = 4;
   const KvPages& kv = a.cache;
   const int group = a.heads / kv.kv_heads, heads = kv.kv_heads * plan.query_tiles, rows = plan.query_rows <= 8 ? 8 : 16;
   const int32_t item = FEW ? blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x / kSpans;
-  if (FEW && item >= a.batch * a.heads) return;
-  const int32_t b = item / a.heads, head = item - b * a.heads, h = head / group;
+  int32_t b = item / a.heads;
+  const int32_t head = item - b * a.heads, h = head / group;
   const int32_t tile = (head - h * group) / plan.query_rows, row = (head - h * group) - tile * plan.query_rows;
-  const Sequence seq = sequence_of(a, indexes(a.lengths)[b]);
-  int32_t units = seq.units, before = 0;
-  if (a.batch > 1) before = units_before(a, b, &units);
-  const int32_t per = units_per_column(units, plan);
-  const int32_t w0 = before / per, w1 = min((before + seq.units - 1) / per, plan.columns - 1);
-  if (w0 >= w1) return;  // one workgroup had it all
+  int32_t before, per, w0, w1;
+  if constexpr (JOIN == Join::kColumns) {
+    const int32_t column = b + 1;
+    Share<false> share;
+    if (column >= plan.columns || !share.find(a, plan, column)) return;
+    b = share.b;
+    before = share.base;
+    per = share.at / column;
+    w0 = before / per;
+    if (w0 != column - 1) return;  // (it begins with this column, or further back)
+    w1 = min((before + share.seq.units - 1) / per, plan.columns - 1);
+  } else {
+    if (FEW && b >= a.batch) return;
+    const Sequence seq = sequence_of(a, indexes(a.lengths)[b]);
+    int32_t units = seq.units;
+    before = 0;
+    if (a.batch > 1) before = units_before(a, b, &units);
+    per = units_per_column(units, plan);
+    w0 = before / per;
+    w1 = min((before + seq.units - 1) / per, plan.columns - 1);
+    if (w0 >= w1) return;  // one workgroup had it all
+  }
   // (a part is in its workgroup's first place but where another head came before it there)
   const int64_t stride = static_cast<int64_t>(rows) * (DP + 2);
   const int32_t first_place = before != w0 * per ? 1 : 0, index = h * plan.query_tiles + tile;
@@ -703,7 +728,7 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(PagedAttentionArgs
   }
   if (set != 0 || c >= kv.dim) return;
   const float inv = x.sum == 0.f ? 0.f : 1.0f / x.sum;
-  *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(item) * kv.dim + c) =
+  *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(b) * a.heads + head) * kv.dim + c) =
       make_uint2(pack_bf16x2(x.acc.x * inv, x.acc.y * inv), pack_bf16x2(x.acc.z * inv, x.acc.w * inv));
 }
 
@@ -740,17 +765,19 @@ void launch_main(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream)
   }
 }
 template <int DP>
-hipError_t launch(const PagedAttentionArgs& a, const Plan& p, hipStream_t stream) {
+hipError_t launch(const PagedAttentionArgs& a, const Plan& p, int cus, hipStream_t stream) {
   const bool fp8 = a.cache.key_scales != nullptr, dup = p.query_rows <= 8;
   if (fp8 && dup) launch_main<DP, true, true>(a, p, stream);
   else if (fp8) launch_main<DP, true, false>(a, p, stream);
   else if (dup) launch_main<DP, false, true>(a, p, stream);
   else launch_main<DP, false, false>(a, p, stream);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.whole) return e;
-  const unsigned items = static_cast<unsigned>(a.batch * a.heads);
-  if (p.columns <= kFewParts * a.batch) join_parts_kernel<DP, true><<<(items + kWaves - 1) / kWaves, kThreads, 0, stream>>>(a, p);
-  else join_parts_kernel<DP, false><<<items * (DP / 32), kThreads, 0, stream>>>(a, p);
+  if (e != hipSuccess || p.whole || p.columns == 1) return e;
+  const bool by_columns = a.batch * a.heads > static_cast<int64_t>(kWavesPerCu) * cus;  // (there are fewer columns than sequences then)
+  const unsigned items = static_cast<unsigned>(by_columns ? p.columns - 1 : a.batch) * a.heads, groups = (items + kWaves - 1) / kWaves;
+  if (by_columns) join_parts_kernel<DP, Join::kColumns><<<groups, kThreads, 0, stream>>>(a, p);
+  else if (p.columns <= kFewParts * a.batch) join_parts_kernel<DP, Join::kFew><<<groups, kThreads, 0, stream>>>(a, p);
+  else join_parts_kernel<DP, Join::kMany><<<items * (DP / 32), kThreads, 0, stream>>>(a, p);
   return hipGetLastError();
 }
 
@@ -770,9 +797,9 @@ size_t paged_attention_workspace(const PagedAttentionArgs& a, int cus) {
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, int cus, hipStream_t stream) {
   const Plan p = plan_of(a, cus);
   switch (padded_dim(a.cache.dim)) {
-    case 64: return launch<64>(a, p, stream);
-    case 128: return launch<128>(a, p, stream);
-    default: return launch<256>(a, p, stream);
+    case 64: return launch<64>(a, p, cus, stream);
+    case 128: return launch<128>(a, p, cus, stream);
+    default: return launch<256>(a, p, cus, stream);
   }
 }
 
