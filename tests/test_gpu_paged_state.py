@@ -1,0 +1,61 @@
+"""What a decode object holds between its calls: eager steps and replays mixed on one
+object, and calls that fail or are refused with the sequences left as they were."""
+
+from __future__ import annotations
+
+import sys
+
+import pytest
+import torch
+
+from oracle import moe as om
+from qwen_tiny import prompt
+from test_gpu_paged_decode import DEV, _backend, checkpoint, load  # noqa: F401 (fixtures)
+from uma_qmoe_amd.formats import ContractError
+from uma_qmoe_amd.paged_decode import PagedDecodeGraph
+from uma_qmoe_amd.qwen_host import DecodeGraph
+
+pytestmark = pytest.mark.gpu
+
+
+def same(a, b, what):
+    assert torch.equal(a.token, b.token), what
+    assert (a.logits - b.logits).norm() <= 1e-3 * b.logits.norm(), what
+
+
+def mixed_steps(mixed, eager):
+    """Eager steps, a capture and replays on one object, eager steps on the other."""
+    for step, kind in enumerate(["step_eager", "step_eager", "capture", "replay", "replay", "step_eager", "replay", "capture",
+                                 "replay", "step_eager", "step_eager", "capture", "step_eager", "replay", "replay"]):
+        if kind == "capture":
+            held = mixed.logits.clone()
+            mixed.capture()
+            torch.cuda.synchronize()
+            assert torch.equal(mixed.logits, held), "capturing is no step"
+            continue
+        getattr(mixed, kind)()
+        eager.step_eager()
+        torch.cuda.synchronize()
+        same(mixed, eager, f"{kind} {step}")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_logits_are_the_last_steps(checkpoint, fp8):
+    print(f"[case] paged logits {fp8}", flush=True)
+    with load(checkpoint) as host:
+        mixed, eager = (PagedDecodeGraph(host.model, batch=2, max_len=64, page_size=16, fp8_cache=fp8) for _ in range(2))
+        for dg in (mixed, eager):
+            dg.prefill(0, prompt(5, seed=1).to(DEV))
+            dg.prefill(1, prompt(17, seed=2).to(DEV))
+        mixed_steps(mixed, eager)
+
+
+def test_logits_of_a_capture_before_the_first_step(checkpoint):
+    print("[case] paged logits before a step", flush=True)
+    with load(checkpoint) as host:
+        dg = PagedDecodeGraph(host.model, batch=1, max_len=32)
+        dg.prefill(0, prompt(5, seed=1).to(DEV))
+        dg.capture()
+        assert dg.logits is None
+        dg.replay()
+        assert dg.logits.isfinite().all()

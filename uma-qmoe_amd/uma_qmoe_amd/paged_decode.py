@@ -54,8 +54,8 @@ class PagedDecodeGraph:
     between steps, also after ``capture``, which records one step of the batch;
     every ``replay`` then decodes one token of each sequence. ``token`` [batch, 1]
     holds what they chose last (of places without a sequence: whatever was there),
-    ``logits`` [batch, vocab] (fp32) the last step's. A token is in the cache from
-    the step on that reads it.
+    ``logits`` [batch, vocab] (fp32) the last step's (a replay's until the next one).
+    A token is in the cache from the step on that reads it.
 
     Calls are made on one stream (replays of several objects, too: the library's
     workspace for the MoE blocks is one per capture stream, which objects may share).
@@ -98,6 +98,7 @@ class PagedDecodeGraph:
         self.next_positions: list[int | None] = [None] * self.batch  # host copy of ``positions``
         self.logits = None
         self.graph = None
+        self._graph_logits = None  # what a replay writes
         self.stream = torch.cuda.Stream(device=self.device)  # warm-up and capture, as DecodeGraph
 
     # ------------------------------------------------------------- the model --
@@ -244,7 +245,8 @@ class PagedDecodeGraph:
     def capture(self) -> None:
         """Records one step. A warm-up step runs before it on the capture's stream
         (it writes the sequences' next positions, which the next step writes
-        again); the tokens and positions are put back afterwards."""
+        again); the tokens and positions are put back afterwards. ``logits`` stay
+        those of the last step: recording computes none."""
         import torch
 
         self._prepare_step()
@@ -258,10 +260,10 @@ class PagedDecodeGraph:
         torch.cuda.current_stream().wait_stream(self.stream)
         graph = torch.cuda.CUDAGraph()
         with torch.no_grad(), torch.cuda.graph(graph, stream=self.stream):
-            self.logits = self._step()
+            logits = self._step()
         # (a larger call on the capture's stream gets the extension another workspace; the graph keeps this one)
         self._workspaces = list(self.extension._ws_cache.values())
-        self.graph = graph
+        self.graph, self._graph_logits = graph, logits
 
     def replay(self) -> Any:
         """One token of each sequence: the token buffer (device, [batch, 1]) after the step."""
@@ -269,6 +271,7 @@ class PagedDecodeGraph:
             raise ContractError("capture() a decode step first")
         self._prepare_step()
         self.graph.replay()
+        self.logits = self._graph_logits
         self._advance()
         return self.token
 
