@@ -59,3 +59,12 @@ def test_logits_of_a_capture_before_the_first_step(checkpoint):
         assert dg.logits is None
         dg.replay()
         assert dg.logits.isfinite().all()
+
+
+def test_logits_of_the_one_sequence_graph_are_the_last_steps(checkpoint):
+    print("[case] static logits", flush=True)
+    with load(checkpoint) as host:
+        mixed, eager = (DecodeGraph(host.model, max_len=64) for _ in range(2))
+        for dg in (mixed, eager):
+            dg.prefill(prompt(9).to(DEV))
+        mixed_steps(mixed, eager)

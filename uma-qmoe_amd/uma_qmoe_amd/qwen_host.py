@@ -562,7 +562,7 @@ class DecodeGraph:
     the current position, the argmax of the last logits written back into the
     token buffer, the position advanced — so every ``replay`` produces the
     next token with no host work. ``logits`` holds the last step's logits
-    (fp32 [vocab]) and ``token`` the token it chose."""
+    (fp32 [vocab], a replay's until the next one) and ``token`` the token it chose."""
 
     def __init__(self, model: Any, *, max_len: int) -> None:
         torch = _torch()
@@ -577,6 +577,7 @@ class DecodeGraph:
         self.next_position = 0  # host copy of ``position`` (no sync per token)
         self.logits = None
         self.graph = None
+        self._graph_logits = None  # what a replay writes
         # the stream the warm-up and the capture run on: the library's
         # per-stream workspace is then allocated (and zero-filled) by the
         # warm-up, outside the graph
@@ -651,9 +652,9 @@ class DecodeGraph:
         torch.cuda.current_stream().wait_stream(self.stream)
         graph = torch.cuda.CUDAGraph()
         with torch.no_grad(), torch.cuda.graph(graph, stream=self.stream):
-            self.logits = self._step()
+            logits = self._step()
         # capture ran nothing: the buffers still hold the prefilled state
-        self.graph = graph
+        self.graph, self._graph_logits = graph, logits
 
     def replay(self) -> Any:
         """One token: returns the token buffer (device, [1, 1]) after the step."""
@@ -662,6 +663,7 @@ class DecodeGraph:
         if self.next_position >= self.max_len:
             raise ContractError("the static cache is full")
         self.graph.replay()
+        self.logits = self._graph_logits
         self.next_position += 1
         return self.token
 
