@@ -68,3 +68,45 @@ def test_logits_of_the_one_sequence_graph_are_the_last_steps(checkpoint):
         for dg in (mixed, eager):
             dg.prefill(prompt(9).to(DEV))
         mixed_steps(mixed, eager)
+
+
+def state(dg):
+    return (dg.page_table.tolist(), dg.positions.tolist(), dg.lengths.tolist(), dg.active.tolist(), dg.token.tolist(),
+            list(dg.next_positions), [list(o) for o in dg.pool.owned], list(dg.pool.free))
+
+
+def pair(host, **kwargs):
+    """Two objects with the same two sequences of three places."""
+    objects = [PagedDecodeGraph(host.model, batch=3, max_len=64, page_size=16, **kwargs) for _ in range(2)]
+    for dg in objects:
+        dg.prefill(0, prompt(5, seed=1).to(DEV))
+        dg.prefill(2, prompt(15, seed=2).to(DEV))
+        for _ in range(3):
+            dg.step_eager()
+    return objects
+
+
+@pytest.mark.parametrize("bad", [
+    torch.ones(2, 4, dtype=torch.long), torch.ones(4, dtype=torch.long), torch.ones(1, 2, 2, dtype=torch.long),
+    torch.ones(1, 4), torch.ones(1, 4, dtype=torch.bool)])
+def test_tokens_of_another_form_are_refused(checkpoint, bad):
+    """Before anything of the sequence is given up."""
+    print(f"[case] paged tokens {tuple(bad.shape)} {bad.dtype}", flush=True)
+    with load(checkpoint) as host:
+        dg, twin = pair(host)
+        before = state(dg)
+        for call in (dg.prefill, dg.extend):
+            for ids in (bad.to(DEV), torch.ones(1, 4, dtype=torch.long)):  # (also on the host)
+                with pytest.raises(ContractError, match="token ids"):
+                    call(2, ids)
+                assert state(dg) == before
+        for _ in range(3):
+            dg.step_eager()
+            twin.step_eager()
+            same_sequences(dg, twin)
+
+
+def same_sequences(a, b, live=(0, 2)):
+    live = list(live)
+    assert torch.equal(a.token[live], b.token[live])
+    assert (a.logits[live] - b.logits[live]).norm() <= 1e-3 * b.logits[live].norm()

@@ -148,6 +148,16 @@ class PagedDecodeGraph:
             raise ContractError(f"no place {index} in a batch of {self.batch}")
         return index
 
+    def _count(self, ids: Any) -> int:
+        """How many tokens ``ids`` has, which must be [1, n] ids on the device."""
+        import torch
+
+        if not torch.is_tensor(ids) or ids.ndim != 2 or ids.shape[0] != 1 or ids.dtype not in (torch.long, torch.int32):
+            raise ContractError("a sequence takes a tensor of [1, n] token ids (int64 or int32)")
+        if ids.device != self.device:
+            raise ContractError(f"a sequence takes token ids on {self.device}, not on {ids.device}")
+        return int(ids.shape[1])
+
     def _enter(self, given: list[tuple[int, int, int]]) -> None:
         for i, entry, page in given:
             self.page_table[i, entry] = page
@@ -164,8 +174,8 @@ class PagedDecodeGraph:
     def prefill(self, index: int, prompt_ids: Any) -> Any:
         """Starts a sequence at ``index`` (ending the one there) with a prompt of
         [1, n] token ids on the device; returns its first new token [1, 1]."""
-        n = int(prompt_ids.shape[1])
         self._place(index)
+        n = self._count(prompt_ids)
         if n < 1 or n >= self.max_len:
             raise ContractError("prompt must be non-empty and shorter than the cache")
         missing = -(-n // self.pool.page_size) - len(self.pool.owned[index])
@@ -181,7 +191,7 @@ class PagedDecodeGraph:
         the first of ``ids``, or not at all."""
         import torch
 
-        start, n = self.next_positions[self._place(index)] or 0, int(ids.shape[1])
+        start, n = self.next_positions[self._place(index)] or 0, self._count(ids)
         if n < 1 or start + n >= self.max_len:
             raise ContractError("a sequence must grow by at least one token and stay shorter than the cache")
         self._enter(self.pool.reserve([(index, start + n)]))
