@@ -110,3 +110,58 @@ def same_sequences(a, b, live=(0, 2)):
     live = list(live)
     assert torch.equal(a.token[live], b.token[live])
     assert (a.logits[live] - b.logits[live]).norm() <= 1e-3 * b.logits[live].norm()
+
+
+def failing(host, layer):
+    """A model whose ``layer`` runs out of memory."""
+    def fail(*_):
+        raise RuntimeError("out of memory")
+    return host.model.model.layers[layer].mlp.register_forward_pre_hook(fail)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("layer", [0, 1])
+def test_tokens_that_could_not_be_added(checkpoint, layer, fp8):
+    """The model fails: the sequence is as it was, and its pages are those it had."""
+    print(f"[case] paged extend fails {layer} {fp8}", flush=True)
+    more = prompt(20, seed=3).to(DEV)
+    with load(checkpoint) as host:
+        dg, twin = pair(host, fp8_cache=fp8)
+        before = state(dg)
+        hook = failing(host, layer)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            dg.extend(2, more)
+        hook.remove()
+        assert state(dg) == before
+        for _ in range(3):
+            dg.step_eager()
+            twin.step_eager()
+            same_sequences(dg, twin)
+        for x in (dg, twin):
+            x.extend(2, more)
+            x.step_eager()
+        same_sequences(dg, twin)
+
+
+def test_a_prompt_that_could_not_be_put_in(checkpoint):
+    """The model fails: the place is empty, and the pool has all of its pages."""
+    print("[case] paged prefill fails", flush=True)
+    ids = prompt(20, seed=3).to(DEV)
+    with load(checkpoint) as host:
+        dg, twin = pair(host)
+        for place in (1, 2):  # an empty one, and one with a sequence (which ends)
+            hook = failing(host, 1)
+            with pytest.raises(RuntimeError, match="out of memory"):
+                dg.prefill(place, ids)
+            hook.remove()
+            assert dg.pool.owned[place] == [] and dg.next_positions[place] is None
+            assert sorted(dg.pool.free + dg.pool.owned[0] + dg.pool.owned[2]) == list(range(12))
+            assert dg.page_table[place].eq(-1).all() and dg.lengths[place] == 0 and dg.active[place] == 0
+        twin.finish(2)
+        dg.step_eager()
+        twin.step_eager()
+        same_sequences(dg, twin, [0])
+        for x in (dg, twin):
+            x.prefill(2, ids)
+            x.step_eager()
+        same_sequences(dg, twin)

@@ -38,3 +38,15 @@ def test_pool_takes_pages_back():
 def test_a_model_on_the_host_is_refused():
     with pytest.raises(ContractError, match="HIP device"):
         PagedDecodeGraph(torch.nn.Linear(2, 2), batch=1, max_len=8)
+
+
+def test_pool_takes_back_what_it_gave_last():
+    pool = PagePool(8, 16, 2)
+    pool.reserve([(0, 20), (1, 3)])
+    before = ([list(o) for o in pool.owned], list(pool.free))
+    given = pool.reserve([(0, 50), (1, 17)])
+    assert given == [(0, 2, 3), (0, 3, 4), (1, 1, 5)]
+    pool.give_back(given)
+    assert (pool.owned, pool.free) == before
+    pool.give_back([])
+    assert (pool.owned, pool.free) == before

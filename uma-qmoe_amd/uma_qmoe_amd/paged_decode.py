@@ -38,6 +38,13 @@ class PagePool:
             self.owned[i].append(page)
         return given
 
+    def give_back(self, given: list[tuple[int, int, int]]) -> None:
+        """Takes back what the last ``reserve`` gave."""
+        for i, _e, page in reversed(given):
+            self.owned[i].remove(page)
+            self.free.append(page)
+        self.free.sort(reverse=True)
+
     def release(self, index: int) -> None:
         self.free.extend(self.owned[index])
         self.free.sort(reverse=True)
@@ -173,7 +180,8 @@ class PagedDecodeGraph:
 
     def prefill(self, index: int, prompt_ids: Any) -> Any:
         """Starts a sequence at ``index`` (ending the one there) with a prompt of
-        [1, n] token ids on the device; returns its first new token [1, 1]."""
+        [1, n] token ids on the device; returns its first new token [1, 1]. If the
+        model fails the place is empty."""
         self._place(index)
         n = self._count(prompt_ids)
         if n < 1 or n >= self.max_len:
@@ -188,15 +196,15 @@ class PagedDecodeGraph:
         """Adds tokens ([1, n] ids on the device) behind those that the cache holds
         of the sequence at ``index``, and chooses the next one [1, 1]. The token
         that was chosen last is not in the cache yet: it stays in the sequence as
-        the first of ``ids``, or not at all."""
+        the first of ``ids``, or not at all. If the model fails the sequence is as
+        it was."""
         import torch
 
         start, n = self.next_positions[self._place(index)] or 0, self._count(ids)
         if n < 1 or start + n >= self.max_len:
             raise ContractError("a sequence must grow by at least one token and stay shorter than the cache")
-        self._enter(self.pool.reserve([(index, start + n)]))
+        given = self.pool.reserve([(index, start + n)])
         table = self.page_table[index:index + 1]
-        starts = torch.full((1,), start, dtype=torch.int32, device=self.device)
 
         def attend(i: int, attn: Any, q: Any, k: Any, v: Any) -> Any:
             past = self.extension.kv_read(self.caches[i], table, starts, start) if start else None
@@ -205,9 +213,17 @@ class PagedDecodeGraph:
                 k, v = torch.cat([past[0], k], 2), torch.cat([past[1], v], 2)
             return self._dense(attn, q, k, v, start, getattr(attn, "sliding_window", None))
 
-        with torch.no_grad():
-            logits = self._forward(ids, torch.arange(start, start + n, device=self.device)[None], attend)
-            self.token[index] = logits[0].argmax()
+        try:
+            self._enter(given)
+            starts = torch.full((1,), start, dtype=torch.int32, device=self.device)
+            with torch.no_grad():
+                logits = self._forward(ids, torch.arange(start, start + n, device=self.device)[None], attend)
+                self.token[index] = logits[0].argmax()
+        except BaseException:
+            # (what was written lies behind the sequence's end, where nothing is read)
+            table[0, len(self.pool.owned[index]) - len(given):] = -1
+            self.pool.give_back(given)
+            raise
         self.positions[index] = start + n
         self.lengths[index] = start + n + 1
         self.active[index] = 1
