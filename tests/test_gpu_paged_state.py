@@ -165,3 +165,16 @@ def test_a_prompt_that_could_not_be_put_in(checkpoint):
             x.prefill(2, ids)
             x.step_eager()
         same_sequences(dg, twin)
+
+
+def test_tokens_for_no_sequence_are_refused(checkpoint):
+    """A sequence that has ended does not go on as a new one."""
+    print("[case] paged extend of nothing", flush=True)
+    with load(checkpoint) as host:
+        dg, _ = pair(host)
+        dg.finish(2)
+        before = state(dg)
+        for place in (1, 2):
+            with pytest.raises(ContractError, match=f"no sequence at {place}"):
+                dg.extend(place, prompt(4).to(DEV))
+            assert state(dg) == before

@@ -190,7 +190,7 @@ class PagedDecodeGraph:
         if missing > len(self.pool.free):
             raise ContractError(f"the cache has {len(self.pool.free)} free pages, {missing} are needed")
         self.finish(index)
-        return self.extend(index, prompt_ids)
+        return self._grow(index, 0, prompt_ids)
 
     def extend(self, index: int, ids: Any) -> Any:
         """Adds tokens ([1, n] ids on the device) behind those that the cache holds
@@ -198,11 +198,18 @@ class PagedDecodeGraph:
         that was chosen last is not in the cache yet: it stays in the sequence as
         the first of ``ids``, or not at all. If the model fails the sequence is as
         it was."""
-        import torch
-
-        start, n = self.next_positions[self._place(index)] or 0, self._count(ids)
+        start, n = self.next_positions[self._place(index)], self._count(ids)
+        if start is None:
+            raise ContractError(f"no sequence at {index} to add tokens to: prefill() one")
         if n < 1 or start + n >= self.max_len:
             raise ContractError("a sequence must grow by at least one token and stay shorter than the cache")
+        return self._grow(index, start, ids)
+
+    def _grow(self, index: int, start: int, ids: Any) -> Any:
+        """Tokens at positions ``start`` on of the sequence at ``index``, and the next choice."""
+        import torch
+
+        n = ids.shape[1]
         given = self.pool.reserve([(index, start + n)])
         table = self.page_table[index:index + 1]
 
