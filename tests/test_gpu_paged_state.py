@@ -178,3 +178,26 @@ def test_tokens_for_no_sequence_are_refused(checkpoint):
             with pytest.raises(ContractError, match=f"no sequence at {place}"):
                 dg.extend(place, prompt(4).to(DEV))
             assert state(dg) == before
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_capture_waits_for_its_own_device(checkpoint, monkeypatch, paged):
+    """The work before a capture is on the model's device, whichever is the current one."""
+    print(f"[case] capture's stream {paged}", flush=True)
+    asked, current = [], torch.cuda.current_stream
+
+    def recorded(device=None):
+        if sys._getframe(1).f_code.co_filename.endswith(("paged_decode.py", "qwen_host.py")):
+            asked.append(device)
+        return current(device)
+
+    with load(checkpoint) as host:
+        if paged:
+            dg = PagedDecodeGraph(host.model, batch=1, max_len=32)
+            dg.prefill(0, prompt(5).to(DEV))
+        else:
+            dg = DecodeGraph(host.model, max_len=32)
+            dg.prefill(prompt(5).to(DEV))
+        monkeypatch.setattr(torch.cuda, "current_stream", recorded)
+        dg.capture()
+        assert asked and all(d == dg.device for d in asked)

@@ -285,12 +285,12 @@ class PagedDecodeGraph:
         self._prepare_step()
         counters = (self.token, self.positions, self.lengths)
         saved = [c.clone() for c in counters]
-        self.stream.wait_stream(torch.cuda.current_stream())
+        self.stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.no_grad(), torch.cuda.stream(self.stream):
             self._step()
             for c, v in zip(counters, saved):
                 c.copy_(v)
-        torch.cuda.current_stream().wait_stream(self.stream)
+        torch.cuda.current_stream(self.device).wait_stream(self.stream)
         graph = torch.cuda.CUDAGraph()
         with torch.no_grad(), torch.cuda.graph(graph, stream=self.stream):
             logits = self._step()

@@ -642,14 +642,14 @@ class DecodeGraph:
             raise ContractError("no room in the cache to capture a decode step")
         counters = self._counters()
         saved = [c.clone() for c in counters]
-        self.stream.wait_stream(torch.cuda.current_stream())
+        self.stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.no_grad(), torch.cuda.stream(self.stream):
             self._step()
             if [c.data_ptr() for c in self._counters()] != [c.data_ptr() for c in counters]:
                 raise ContractError("the decode step replaced a cache counter instead of advancing it in place")
             for c, v in zip(counters, saved):
                 c.copy_(v)
-        torch.cuda.current_stream().wait_stream(self.stream)
+        torch.cuda.current_stream(self.device).wait_stream(self.stream)
         graph = torch.cuda.CUDAGraph()
         with torch.no_grad(), torch.cuda.graph(graph, stream=self.stream):
             logits = self._step()
