@@ -201,3 +201,29 @@ def test_a_capture_waits_for_its_own_device(checkpoint, monkeypatch, paged):
         monkeypatch.setattr(torch.cuda, "current_stream", recorded)
         dg.capture()
         assert asked and all(d == dg.device for d in asked)
+
+
+def test_the_same_tokens_in_both_caches(checkpoint):
+    """Every step of DecodeGraph and PagedDecodeGraph on the same tokens: either's logits are
+    within 2e-2 of the sequence run again without a cache, so within 2 * 2e-2 / (1 - 2e-2) of
+    each other, and a choice differs only where the two best logits are closer than that."""
+    print("[case] paged and static cache, same tokens", flush=True)
+    limit = 4.1e-2
+    ids = prompt(9).to(DEV)
+    with load(checkpoint) as host:
+        a, b = DecodeGraph(host.model, max_len=40), PagedDecodeGraph(host.model, batch=1, max_len=40, page_size=16)
+        a.prefill(ids)
+        b.prefill(0, ids)
+        b.token.copy_(a.token)
+        a.capture()
+        b.capture()
+        for step in range(24):
+            a.replay()
+            b.replay()
+            torch.cuda.synchronize()
+            x, y = a.logits.double().cpu(), b.logits[0].double().cpu()
+            assert om.rel_l2(y, x) <= limit, f"step {step}"
+            if not torch.equal(a.token, b.token):
+                # (each logit is off by no more than the whole difference's norm)
+                assert x.max() - x[int(b.token)] <= 2 * (y - x).norm(), f"step {step}"
+            b.token.copy_(a.token)
