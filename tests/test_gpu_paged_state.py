@@ -12,6 +12,7 @@ from oracle import moe as om
 from qwen_tiny import prompt
 from test_gpu_paged_decode import DEV, _backend, checkpoint, load  # noqa: F401 (fixtures)
 from uma_qmoe_amd.formats import ContractError
+from uma_qmoe_amd.native_backend import load_native_extension
 from uma_qmoe_amd.paged_decode import PagedDecodeGraph
 from uma_qmoe_amd.qwen_host import DecodeGraph
 
@@ -227,3 +228,30 @@ def test_the_same_tokens_in_both_caches(checkpoint):
                 # (each logit is off by no more than the whole difference's norm)
                 assert x.max() - x[int(b.token)] <= 2 * (y - x).norm(), f"step {step}"
             b.token.copy_(a.token)
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_graph_keeps_its_workspace(checkpoint, paged):
+    """A larger call on the capture's stream between replays, and memory that is filled
+    afterwards: replays are the eager steps."""
+    print(f"[case] captured workspace {paged}", flush=True)
+    with load(checkpoint) as host:
+        graph, eager = ((PagedDecodeGraph(host.model, batch=1, max_len=64, page_size=16) if paged else
+                         DecodeGraph(host.model, max_len=64)) for _ in range(2))
+        for dg in (graph, eager):
+            dg.prefill(*((0, prompt(9).to(DEV)) if paged else (prompt(9).to(DEV),)))
+        graph.capture()
+        for n in (30, 100):
+            graph.replay()
+            eager.step_eager()
+            graph.stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(graph.stream), torch.no_grad():
+                host.model(input_ids=prompt(n).to(DEV))
+                filled = [torch.full((m,), 255, dtype=torch.uint8, device=DEV) for m in (1 << 12, 1 << 16, 1 << 18, 1 << 20) for _ in range(8)]
+            torch.cuda.current_stream().wait_stream(graph.stream)
+            graph.replay()
+            eager.step_eager()
+            torch.cuda.synchronize()
+            same(graph, eager, f"{n}")
+            assert all(t.eq(255).all() for t in filled)
+        load_native_extension()[1].status()

@@ -198,6 +198,7 @@ class HipExtension:
         self.lib = _native.library()
         self._ws_lock = threading.Lock()
         self._ws_cache: dict[tuple[int, int], Any] = {}
+        self._ws_captured: list[Any] = []  # those that captured graphs have, which may be replayed at any time
         self._bf16, self._e4m3, self._f32, self._i32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32
 
     # ------------------------------------------------------------ helpers --
@@ -205,7 +206,8 @@ class HipExtension:
         """A zero-filled workspace of the size the library asks for, reused by
         later calls on the same device and stream (stream order keeps them
         from overlapping; the fused single-token kernel leaves its sync words
-        ready for the next call). It grows when a call needs more."""
+        ready for the next call). It grows when a call needs more; one that
+        a graph was captured with stays beside the larger one."""
         n = self.lib.uqm_moe_workspace_bytes(tokens, hidden, inter, shared_inter, experts, top_k)
         if n == 0:
             raise RuntimeError("invalid workspace shape")
@@ -214,15 +216,18 @@ class HipExtension:
         key = (dev.index if dev.index is not None else torch.cuda.current_device(), _stream_handle(torch, dev))
         with self._ws_lock:
             ws = self._ws_cache.get(key)
+            capturing = key[1] != 0 and torch.cuda.is_current_stream_capturing()  # (the default stream cannot be)
             if ws is None or ws.numel() < n:
                 # Zero-filling inside a HIP-graph capture would record the
                 # fill, and every replay would reset the fused kernel's launch
                 # epochs (stale hand-offs would then look current).
-                if torch.cuda.is_current_stream_capturing():
+                if capturing:
                     raise RuntimeError("uma_qmoe workspace would be allocated inside a HIP-graph capture: run one "
                                        "call of this shape on the capture stream before capturing")
                 ws = torch.zeros(n, dtype=torch.uint8, device=dev)
                 self._ws_cache[key] = ws
+            elif capturing and not any(w is ws for w in self._ws_captured):
+                self._ws_captured.append(ws)
             return ws
 
     def new_workspace(self, device, tokens, hidden, inter, shared_inter, experts, top_k):
@@ -839,6 +844,7 @@ class HipExtension:
         its wait budget (synchronises each workspace's stream)."""
         with self._ws_lock:
             spaces = list(self._ws_cache.values())
+            spaces += [w for w in self._ws_captured if not any(w is ws for ws in spaces)]
         for ws in spaces:
             self.workspace_status(ws)
 

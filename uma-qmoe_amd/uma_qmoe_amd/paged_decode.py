@@ -294,8 +294,6 @@ class PagedDecodeGraph:
         graph = torch.cuda.CUDAGraph()
         with torch.no_grad(), torch.cuda.graph(graph, stream=self.stream):
             logits = self._step()
-        # (a larger call on the capture's stream gets the extension another workspace; the graph keeps this one)
-        self._workspaces = list(self.extension._ws_cache.values())
         self.graph, self._graph_logits = graph, logits
 
     def replay(self) -> Any:
