@@ -51,6 +51,9 @@ def parse_args():
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-batch32", dest="batch32", action="store_false",
                     help="skip the batch-32 decode measurement reported beside the batch-1 value")
+    ap.add_argument("--paged", action="store_true",
+                    help="with --config qwen: also times a step over the static and the paged cache (BF16 and 8-bit "
+                         "floats) at several lengths, and of 32 sequences")
     ap.add_argument("--multi-kernel", action="store_true",
                     help="one- and two-token calls take the multi-launch path (UQM_OPT_FUSED_DECODE = 0) "
                          "instead of the fused kernel")
@@ -539,6 +542,51 @@ def qwen_config():
                           tie_word_embeddings=False, decoder_sparse_step=1, mlp_only_layers=[])
 
 
+def cached_decode_steps(torch, model, vocab, gen) -> list[dict]:
+    """A captured step of ``model`` over the static cache (one sequence) and the
+    paged ones: ms a step (4 untimed replays, the median of 3 x 32) and the
+    memory of the object, its cache included."""
+    from uma_qmoe_amd.paged_decode import PagedDecodeGraph
+    from uma_qmoe_amd.qwen_host import DecodeGraph
+
+    caches = {"static bf16": lambda n: DecodeGraph(model, max_len=n),
+              "paged bf16": lambda n, batch=1: PagedDecodeGraph(model, batch=batch, max_len=n),
+              "paged e4m3": lambda n, batch=1: PagedDecodeGraph(model, batch=batch, max_len=n, fp8_cache=True)}
+    out = []
+
+    def measure(cache, max_len, lengths):
+        before = torch.cuda.memory_allocated()
+        dg = caches[cache](max_len) if len(lengths) == 1 else caches[cache](max_len, len(lengths))
+        for i, n in enumerate(lengths):
+            ids = torch.randint(0, vocab, (1, n), generator=gen, device=dg.device)
+            dg.prefill(*((ids,) if cache.startswith("static") else (i, ids)))
+        dg.capture()
+        held = torch.cuda.memory_allocated() - before
+        for _ in range(4):
+            dg.replay()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        times = []
+        for _ in range(3):
+            torch.cuda.synchronize()
+            e0.record()
+            for _ in range(32):
+                dg.replay()
+            e1.record()
+            torch.cuda.synchronize()
+            times.append(e0.elapsed_time(e1) / 32)
+        ms = sorted(times)[1]
+        out.append({"cache": cache, "sequences": len(lengths), "positions": [min(lengths), max(lengths)], "max_len": max_len,
+                    "ms_per_step": round(ms, 3), "tokens_per_s": round(1000.0 * len(lengths) / ms), "gb": round(held / 1e9, 2)})
+        progress(f"qwen: {out[-1]}")
+
+    for max_len, n in ((512, 200), (4096, 2000), (8192, 7900)):
+        for cache in caches:
+            measure(cache, max_len, [n])
+    for cache in ("paged bf16", "paged e4m3"):
+        measure(cache, 4096, [100 + 60 * i for i in range(32)])
+    return out
+
+
 def main_qwen(args, torch, syn, ext) -> int:
     """Greedy decode of a Qwen1.5-MoE-A2.7B-shaped model with synthetic
     weights (dense BF16 tensors N(0, 0.02), norms 1; routed experts the
@@ -626,6 +674,9 @@ def main_qwen(args, torch, syn, ext) -> int:
             "timing": {**stats, "steps_per_sample": per_sample},
             "reference_tpot_ms": {"value": 94.6, "hardware": "gfx1151 (the reference's eager host, real weights)"},
         }
+        if args.paged:
+            del dg
+            line["caches"] = cached_decode_steps(torch, model, config.vocab_size, gen)
         progress("done")
         print(json.dumps(line), flush=True)
         return 0
