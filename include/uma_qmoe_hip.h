@@ -396,7 +396,8 @@ int uqm_kv_read(const uqm_kv_cache* cache, int64_t batch, const int32_t* page_ta
  * over the positions max(0, lengths[b] - window) <= p < lengths[b] (window 0: all;
  * the new token's own key and value are in the cache already, at lengths[b] - 1).
  * Zeros where no position is seen. query bf16 [batch, heads, head_dim], heads a
- * multiple of kv_heads, both 16-byte aligned; batch * heads below 2^24.
+ * multiple of kv_heads, both 16-byte aligned; batch * heads below 2^24; scale below
+ * 2^127 in magnitude.
  * What places hold that are not seen has no influence, NaN and infinities neither.
  * Of those seen, however little they weigh: a score of NaN or +inf gives NaN, one of
  * -inf takes no weight (NaN where every seen score is -inf), a NaN value gives NaN and

@@ -240,3 +240,9 @@ GOOD = KVCache(dev(bf(4, 2, 16, 64)), dev(bf(4, 2, 16, 64)))
 def test_wrappers(ext, call, words):
     with pytest.raises(RuntimeError, match=words):
         call(ext)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, -3e38])
+def test_scales_that_overflow(lib, scale):
+    """Times log2 e, as scores are scaled, these are infinite, and a score of 0 would be NaN."""
+    refused(lib, "uqm_paged_attention", cache(), "2^127", scale=scale)

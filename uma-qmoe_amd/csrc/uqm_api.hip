@@ -1672,7 +1672,8 @@ int uqm_paged_attention(const uqm_kv_cache* cache, const void* query, int64_t ba
   if (rc || (rc = check_page_table("paged_attention", batch, cache->page_size, table_stride, max_pages)) ||
       (rc = check_attention_sizes(batch, heads, cache->kv_heads, cache->head_dim, cache->page_size, max_pages)))
     return rc;
-  if (!(scale - scale == 0.f)) return fail(UQM_ERR_ARGUMENT, "paged_attention: scale must be finite");
+  // (the kernel's scores carry the factor log2 e, too)
+  if (!(scale > -0x1p127f && scale < 0x1p127f)) return fail(UQM_ERR_ARGUMENT, "paged_attention: scale must be finite, below 2^127 in magnitude");
   if ((rc = check_window(window))) return rc;
   if (batch == 0) return UQM_OK;
   if (query == nullptr || output == nullptr || lengths == nullptr || (page_table == nullptr && max_pages > 0))
