@@ -7,10 +7,11 @@
 //
 // Bound by memory: a key and its value are read for at most 16 query heads, some
 // 4 to 64 operations a byte. 64 sequences of 4001 to 8191 tokens, 16 heads of 128 in
-// e4m3: 255 us, 6.5 TB/s (290 to 310 once the card throttles, some 3 ms into calls
-// without a pause); 32 heads on 8 over 131071 tokens in BF16 84 us, 6.4 TB/s; 32
-// sequences of up to 2047, 16 heads in BF16, 48 us, 5.6 TB/s. With products and
-// softmax left out the times were the same.
+// e4m3: 254 us, 6.5 TB/s; 32 heads on 8 over 131071 tokens in BF16 84 us, 6.4 TB/s; 32
+// sequences of up to 2047, 16 heads in BF16, 48 us, 5.6 TB/s. Those are calls that begin
+// from rest; without a pause the card throttles after some 3 ms, and they take 310, 91 to
+// 94 and 51 to 53. Times of variants, further below, are of calls without a pause. With
+// products and softmax left out the times were the same.
 // What is computed goes to the matrix cores all the same, since the vector unit would
 // be the limit from four query heads a key head on. Everything stays in the wave's
 // registers: no exchange, no shared memory in the loop, but for the maximum over four
@@ -41,9 +42,11 @@
 // positions one after the other instead cost 2 to 8%). A workgroup finds its column
 // from the lengths on the device. What it has of a sequence that other columns also work
 // on goes to its two places in the workspace (for the first and the last of its
-// sequences), and a second launch joins these. Keys, values and queries of the next tile
-// are on their way while one is computed, also across the end of a sequence (255
-// sequences of 50 to 150 tokens 41 us, with a start of its own for each 50).
+// sequences), and a second launch joins these (a wave or a workgroup has a head of a
+// sequence, or, where there are many, a wave a head of a column). Keys, values and
+// queries of the next tile are on their way while one is computed, also across the end
+// of a sequence (255 sequences of 50 to 150 tokens 41 us, with a start of its own for
+// each 50).
 // Where no sequence can have more than four tiles (eight, where there are workgroups for
 // half of the compute units all the same) a workgroup takes a sequence's head, without
 // that bookkeeping and without a second launch (one token over 77 positions, 16 heads,
@@ -79,6 +82,7 @@ constexpr int kDirectTiles = 4;
 // 64 of 16 heads in BF16 64.8 and 89.5 against 57.8 and 92.2. Heads of 64: a quarter less
 // than in parts on average. Of 16 tiles the longest sequence is waited for: 32 of 32
 // heads on 8 in BF16 37.2 and 49.4, in parts 32.6 and 55.2.
+// (It goes by tiles alone: the BF16 pairs that are slower whole lose 6 to 12%.)
 constexpr int kManyDirectTiles = 8;
 
 __device__ __forceinline__ f32x4_t mfma(const uint4 a, const uint4 b, f32x4_t c) {
@@ -275,9 +279,10 @@ __global__ __launch_bounds__(kThreads, DP == 256 && !FP8 ? 1 : DP == 256 || !FP8
   constexpr int kVWords = FP8 ? kVec / 4 : kVec / 2;
   // Lines that another load of the same rows takes a part of are kept: 8-bit keys (two
   // loads to a line; 64 sequences 310 us, not kept 328), keys of rows that do not begin
-  // with a line (heads of 80 in BF16 130 and 148), values of 32 bytes a lane (heads of
-  // 256 in BF16 411 and 435). BF16 keys, two loads to a line as well, are faster not kept
-  // all the same (131071 tokens 94 us, kept 97).
+  // with a line (32 sequences of 2001 to 6001, heads of 80 in BF16 135 and 151), values of
+  // 32 bytes a lane (the same with heads of 256 411 and 432; heads of 192, whose rows end
+  // within a line, 307 and 280). BF16 keys, two loads to a line as well, are faster not
+  // kept all the same (131071 tokens 91 to 94 us, kept 95 to 100).
   constexpr int kKeyHint = FP8 || PAD ? 0 : kOnce, kValueHint = kVWords > 4 ? 0 : kOnce;
   constexpr int kRowStride = DP + 4;       // (rows of the join four banks apart)
   constexpr bool kSharedQuery = DP == 256;  // (there are no registers for them beside keys and values on their way)
